@@ -590,6 +590,142 @@ int mvsd_topk_scores(int32_t* ids, float* scores, int32_t* ranks, const float* l
                      int64_t logits_stride, const int32_t* token_ids, int64_t num_rows,
                      int64_t vocab_size, int64_t k, int logits_mode, mvsd_stream_t stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* Beam search.  No counterpart in the reference.  A group is one request with W beams;     */
+/* G groups in a batch, 1 <= W <= 64.  Every array is contiguous.                           */
+/*                                                                                          */
+/* beam_select — each group's num_candidates (1..256) best continuations:                   */
+/*   total(b, v) = scores[g, b] + (x_bv - log sum_u exp(x_bu))                              */
+/* in the order (total descending, beam ascending, logit descending, token ascending), the  */
+/* totals formed and compared in 64 bits, written as fp32.  Row of beam (g, b): logits +    */
+/* target_rows[g * W + b] * stride (clamped to [0, num_rows)), or g * W + b without         */
+/* target_rows; dtype MVSD_F32 / MVSD_BF16 / MVSD_F16, any alignment.  A beam whose score or */
+/* whose row's log-sum is not finite (no beam, a row of -inf, a NaN or +inf) proposes        */
+/* nothing, and its row is not read where the score says so; -inf entries are no candidates. */
+/* Places without a candidate: token and parent -1, score -inf.                             */
+/* workspace: mvsd_beam_workspace_bytes() bytes, 16-byte aligned, no initial contents needed */
+/* (0: more rows and columns than one call takes, MVSD_E_RANGE); one per call in flight.    */
+/* ------------------------------------------------------------------------------------ */
+int64_t mvsd_beam_workspace_bytes(int64_t num_groups, int64_t beam_width, int64_t vocab_size,
+                                  int64_t num_candidates);
+int mvsd_beam_select(int32_t* token_ids, int32_t* parents, float* out_scores, const void* logits,
+                     int dtype, int64_t stride, int64_t num_rows, const int32_t* target_rows,
+                     const float* scores, int64_t num_groups, int64_t beam_width,
+                     int64_t vocab_size, int64_t num_candidates, void* workspace,
+                     int64_t workspace_bytes, mvsd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* beam_step — one decoding step.  For every group with done 0 and 0 <= length < max_length, */
+/* with the candidates of beam_select (W (1 + num_stop_ids) of them, at most 256) and        */
+/* L = length + 1:                                                                          */
+/*   - stop tokens among the W best candidates end a hypothesis of score                     */
+/*     fl32(fl32(total) / L^length_penalty); finished_* keep the W best old and new ones,    */
+/*     best first (the old first where they are equal; none: -inf, -1, -1, 0);               */
+/*   - the W best candidates that are no stop tokens are the next beams: out_scores,         */
+/*     token_ids, parents (none: -inf, -1, -1), also recorded at token_history and           */
+/*     parent_history [g, length, :] of [G, max_length, W];                                  */
+/*   - length becomes L; done becomes 1 when no beam is left, or W hypotheses are finished   */
+/*     and early_stopping != 0 or the worst of them is at least the best running             */
+/*     fl32(score / L^length_penalty).                                                       */
+/* Other groups stay as they are, their token_ids and parents are -1.  out_* may be the      */
+/* arrays they follow.  finished_beams: the beam the last token (finished_token_ids) was     */
+/* appended to; finished_lengths count that token.                                          */
+/* workspace: as beam_select with num_candidates = W (1 + num_stop_ids).                     */
+/* ------------------------------------------------------------------------------------ */
+typedef struct mvsd_beam_step_args {
+  const void* logits;
+  int64_t stride;
+  int64_t num_rows;
+  const int32_t* target_rows;
+  int64_t num_groups;
+  int64_t beam_width;
+  int64_t vocab_size;
+  int64_t max_length;
+  const int32_t* stop_token_ids; /* [num_stop_ids] */
+  int64_t num_stop_ids;
+  double length_penalty;
+  int dtype;
+  int early_stopping;
+  const float* scores;         /* [G, W] */
+  const int32_t* lengths;      /* [G] */
+  const uint8_t* done;         /* [G] */
+  const float* finished_scores;       /* [G, W], as the next three */
+  const int32_t* finished_beams;
+  const int32_t* finished_token_ids;
+  const int32_t* finished_lengths;
+  float* out_scores;
+  int32_t* out_lengths;
+  uint8_t* out_done;
+  float* out_finished_scores;
+  int32_t* out_finished_beams;
+  int32_t* out_finished_token_ids;
+  int32_t* out_finished_lengths;
+  int32_t* token_history;      /* [G, max_length, W] */
+  int32_t* parent_history;
+  int32_t* token_ids;          /* [G, W] */
+  int32_t* parents;
+  void* workspace;
+  int64_t workspace_bytes;
+} mvsd_beam_step_args;
+
+int mvsd_beam_step(const mvsd_beam_step_args* args, mvsd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* beam_reorder — the rows of num_states state tensors follow the beams' parents: entries    */
+/* [starts[g], lengths[g]) (0 and the whole length without them, clamped to the tensor's     */
+/* length) of every one of a row's `outer` pieces of `length` entries of `inner` bytes       */
+/* become those of the parent's row before the call.  Row of beam (g, w): slots[g * W + w],  */
+/* or g * W + w; a row outside [0, num_rows) is neither read nor written.  A parent outside  */
+/* [0, W) is the beam itself.  dst == src in every state (with equal strides) reorders in    */
+/* place; else none of the dst may overlap a src, and rows that keep their beam are copied   */
+/* too.  Slots of one call are distinct.  Everything else is left as it was.                 */
+/* ------------------------------------------------------------------------------------ */
+typedef struct mvsd_beam_state {
+  const void* src;
+  void* dst;
+  int64_t src_stride; /* bytes between rows */
+  int64_t dst_stride;
+  int64_t num_rows;
+  int64_t outer;
+  int64_t length;
+  int64_t inner;
+} mvsd_beam_state;
+
+int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const int32_t* parents,
+                      const int32_t* starts, const int32_t* lengths, const int32_t* slots,
+                      int64_t num_groups, int64_t beam_width, mvsd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* beam_finish — the num_return (1..W) best answers of every group: its finished hypotheses  */
+/* and, where done is 0, its running beams at fl32(score / length^length_penalty), best      */
+/* first, the finished ones first where they are equal.  token_ids [G, num_return,           */
+/* max_length] (-1 behind a sequence), lengths and scores [G, num_return] (none: 0, -inf).   */
+/* The tokens of a hypothesis of L tokens are its last token at L - 1 and, from t = L - 2     */
+/* down, token_history[g, t, b] with b the beam at step t: the hypothesis' own, then          */
+/* parent_history[g, t, b] (outside [0, W): b itself).                                        */
+/* ------------------------------------------------------------------------------------ */
+typedef struct mvsd_beam_finish_args {
+  int64_t num_groups;
+  int64_t beam_width;
+  int64_t max_length;
+  int64_t num_return;
+  double length_penalty;
+  const float* scores; /* the state, as in mvsd_beam_step_args */
+  const int32_t* lengths;
+  const uint8_t* done;
+  const float* finished_scores;
+  const int32_t* finished_beams;
+  const int32_t* finished_token_ids;
+  const int32_t* finished_lengths;
+  const int32_t* token_history;
+  const int32_t* parent_history;
+  int32_t* out_token_ids;
+  int32_t* out_lengths;
+  float* out_scores;
+} mvsd_beam_finish_args;
+
+int mvsd_beam_finish(const mvsd_beam_finish_args* args, mvsd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,670 @@
+"""Beam search on the device against the 64-bit oracle (oracle/beam.py).
+
+Token ids, parents, lengths and flags are exact.  Scores: a total is formed in 64 bits from the
+row's lse and rounded once (2^-24 relative).  The lse carries the error of its fp32 sums: a term's
+exponent is the rounded product of a rounded difference, 2.2 * 2^-24 relative, at most 40 in
+magnitude where the term counts, times ln 2; v_exp_f32 is good to 2^-23; a lane adds up to 32 terms,
+then ten more additions.  (2.2 * 40 * 0.7 + 2 + 42) * 2^-24 = 6.3e-6 at most."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mvsd.sample import (BeamSearch, BeamState, beam_search_finish, beam_search_select,
+                         beam_search_step, reorder_beams)
+from oracle import beam as oracle
+
+pytestmark = pytest.mark.gpu
+
+LSE_ERROR = 6.3e-6
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def close(got, want, scale=1.0):
+    got, want = got.double().cpu().numpy(), np.asarray(want, np.float64)
+    fine = np.isfinite(want)
+    assert np.array_equal(fine, np.isfinite(got))
+    assert np.array_equal(got[~fine], want[~fine])
+    bar = LSE_ERROR * scale + 2.0 ** -22 * np.abs(want[fine])
+    assert (np.abs(got[fine] - want[fine]) <= bar).all()
+
+
+def rows_of(x, W, rows=None):
+    host = x.double().cpu().numpy()
+    return lambda g, w: host[g * W + w if rows is None else int(rows[g, w])]
+
+
+def make_scores(device, G, W, seed, alive=None):
+    s = -20 - np.cumsum(np.random.default_rng(seed).exponential(0.4, (G, W)), axis=1)
+    if alive is not None:
+        s[:, alive:] = -np.inf
+    return torch.tensor(s, dtype=torch.float32, device=device)
+
+
+def check_select(x, scores, C, rows=None):
+    got = beam_search_select(x, scores, C, target_rows=rows)
+    W = scores.shape[1]
+    ids, parents, want = oracle.select(rows_of(x, W, rows), scores.cpu().numpy(), C)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    assert np.array_equal(got.parents.cpu().numpy(), parents)
+    close(got.scores, want)
+    return got
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [1, 3, 7, 9, 63, 500, 2047, 2049, 8191, 8193, 50257])
+@pytest.mark.parametrize("G,W,C", [(1, 1, 1), (2, 4, 8), (1, 5, 256), (3, 17, 40)])
+def test_select_edges(device, dtype, V, G, W, C):
+    gen = torch.Generator(device=device).manual_seed(V * 7 + W)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2.5).to(DTYPES[dtype])
+    check_select(x, make_scores(device, G, W, V), C)
+    if V > 2:  # a view: rows start at an odd element and are not adjacent
+        check_select(x[:, 1:], make_scores(device, G, W, V), C)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("alive", [1, 3, 8])
+def test_select_long_chunks(device, dtype, alive):
+    """Enough rows for the long chunks, a full vocabulary, beams that do not run."""
+    G, W, V = 16, 8, 151936
+    gen = torch.Generator(device=device).manual_seed(alive)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2.5).to(DTYPES[dtype])
+    scores = make_scores(device, G, W, alive, alive)
+    x[alive:W] = math.nan  # rows of absent beams are not looked at
+    check_select(x, scores, 16)
+
+
+def test_select_64_beams(device):
+    G, W, V = 2, 64, 3001
+    x = torch.randn(G * W, V, device=device, generator=torch.Generator(device=device).manual_seed(0))
+    check_select(x, make_scores(device, G, W, 1), 256)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_select_masked_rows(device, dtype):
+    """Rows of -inf, of the type's lowest value, with NaN or infinities; whole groups of them."""
+    G, W, V, C = 6, 4, 9000, 8
+    t = DTYPES[dtype]
+    low = torch.finfo(t).min
+    gen = torch.Generator(device=device).manual_seed(3)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2).to(t)
+    x[0] = -math.inf
+    x[1, :8999] = -math.inf          # one token allowed
+    x[2, 17] = math.nan
+    x[3, 8998] = math.inf
+    x[4:8] = -math.inf               # a group that cannot go on
+    x[8:12, 5:] = -math.inf          # five tokens a beam
+    x[12:16] = low                   # masked by the lowest value, one token allowed
+    x[12:16, 77] = 1.0
+    x[16] = low                      # nothing but the lowest value
+    x[17:20] = 0.0                   # uniform rows
+    x[20:24] = x[20:24].float().round().to(t)  # long runs of equal values
+    got = check_select(x, make_scores(device, G, W, 2), C)
+    assert (got.parents[1] == -1).all()
+    check_select(x, make_scores(device, G, W, 4), 33)
+    scores = make_scores(device, G, W, 2)
+    scores[0, 0], scores[2, 1], scores[3, 2] = math.nan, math.inf, -math.inf
+    check_select(x, scores, C)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [4000, 151936])
+@pytest.mark.parametrize("C", [8, 256])
+def test_select_runs_of_equal_values(device, dtype, V, C):
+    """More entries at the bound than the gather holds: the lowest beams and tokens win."""
+    G, W = 2, 4
+    x = torch.zeros(G * W, V, device=device, dtype=DTYPES[dtype])
+    x[5, V // 2:] = 3.0
+    x[6, V - 3] = 9.0
+    scores = torch.zeros(G, W, device=device)
+    scores[1] = torch.tensor([-1.0, -1.0, -0.5, 0.0], device=device)
+    check_select(x, scores, C)
+    x[:] = torch.finfo(x.dtype).min
+    check_select(x, scores, C)
+    x[:, ::2] = -math.inf
+    check_select(x, scores, C)
+
+
+def test_negative_zero_ties_with_zero(device):
+    x = torch.full((2, 700), -5.0, device=device)
+    x[0, [3, 600]] = torch.tensor([-0.0, 0.0], device=device)
+    x[1, [2, 5, 9]] = torch.tensor([0.0, -0.0, 0.0], device=device)
+    got = check_select(x, torch.zeros(1, 2, device=device), 5)
+    assert got.token_ids.tolist() == [[3, 600, 2, 5, 9]] or \
+        got.token_ids.tolist() == [[2, 5, 9, 3, 600]]
+
+
+def test_select_reads_rows_by_index(device):
+    G, W, V = 3, 4, 4099
+    gen = torch.Generator(device=device).manual_seed(9)
+    big = torch.randn(40, V + 5, device=device, generator=gen).to(torch.bfloat16)[:, 3:3 + V]
+    rows = torch.randperm(40, device=device, generator=gen)[:G * W].view(G, W).to(torch.int32)
+    scores = make_scores(device, G, W, 0)
+    check_select(big, scores, 8, rows)
+    # indices outside the tensor read its nearest row
+    out = rows.clone()
+    out[0, 0], out[1, 1], out[2, 2] = -5, 40, 2 ** 31 - 1
+    inside = out.clamp(0, 39)
+    a, b = (beam_search_select(big, scores, 8, target_rows=r) for r in (out, inside))
+    assert torch.equal(a.token_ids, b.token_ids) and torch.equal(a.scores, b.scores)
+    # the same row for every beam: beams differ by their scores only
+    check_select(big, scores, 8, torch.zeros_like(rows))
+    check_select(big[:1].expand(G * W, V), scores, 8)
+
+
+def test_order_of_two_beams_is_that_of_the_64_bit_totals(device):
+    """Totals of two beams one fp32 rounding apart keep their order."""
+    V = 5000
+    row = torch.randn(V, device=device, generator=torch.Generator(device=device).manual_seed(4))
+    x = row.repeat(2, 1)
+    for ulps in (1, 2, 40):
+        s = torch.tensor([[-20.0, -20.0]], device=device)
+        s[0, 1] += ulps * 2.0 ** -19  # an ulp of 20 is 2^-19
+        got = check_select(x, s, 6)
+        assert got.parents[0].tolist() == [1, 0, 1, 0, 1, 0]
+
+
+def test_huge_offsets(device):
+    """Rows whose element offsets pass 2^31 (bf16, a row stride of 2^29)."""
+    V, stride = 1500, 2 ** 29
+    base = torch.zeros(5 * stride + V, device=device, dtype=torch.bfloat16)
+    x = base.as_strided((6, V), (stride, 1))
+    x.copy_(torch.randn(6, V, device=device, generator=torch.Generator(device=device).manual_seed(8)))
+    check_select(x, make_scores(device, 2, 3, 5), 6)
+
+
+def test_empty_batch(device):
+    got = beam_search_select(torch.zeros(0, 10, device=device), torch.zeros(0, 4, device=device), 8)
+    assert got.token_ids.shape == (0, 8)
+    state = BeamState.new(0, 4, 8, device)
+    assert beam_search_step(torch.zeros(0, 10, device=device), state).parents.shape == (0, 4)
+    assert beam_search_finish(state).token_ids.shape == (0, 4, 8)
+    assert reorder_beams([], torch.zeros(2, 4, dtype=torch.int32, device=device)) == []
+
+
+# ----------------------------------------------------------------- step
+
+
+def host(state):
+    return {k: v.cpu().numpy() for k, v in vars(state).items()}
+
+
+def random_state(device, G, W, T, seed, done=(), full=()):
+    r = np.random.default_rng(seed)
+    s = BeamState.new(G, W, T, device)
+    s.scores = make_scores(device, G, W, seed)
+    lengths = r.integers(0, T, G)
+    lengths[list(full)] = T
+    s.lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
+    s.done[list(done)] = True
+    fs = -np.sort(r.exponential(2.0, (G, W)), axis=1)
+    none = np.arange(W)[None] >= r.integers(0, W + 1, G)[:, None]
+    fs[none] = -np.inf
+    fb, ft, fl = r.integers(0, W, (G, W)), r.integers(0, 99, (G, W)), r.integers(1, T + 1, (G, W))
+    fb[none], ft[none], fl[none] = -1, -1, 0
+
+    def put(v, dtype=torch.int32):
+        return torch.tensor(v, dtype=dtype, device=device)
+
+    s.finished_scores = put(fs, torch.float32)
+    s.finished_beams, s.finished_token_ids, s.finished_lengths = put(fb), put(ft), put(fl)
+    s.token_history = put(r.integers(0, 99, (G, T, W)))
+    s.parent_history = put(r.integers(0, W, (G, T, W)))
+    return s
+
+
+def clone(state):
+    return BeamState(**{k: v.clone() for k, v in vars(state).items()})
+
+
+def check_state(got, want):
+    for k, v in vars(got).items():
+        if k.endswith("scores"):
+            close(v, want[k])
+        else:
+            assert np.array_equal(v.cpu().numpy(), want[k]), k
+
+
+def check_step(x, state, stops, alpha=1.0, early=False, rows=None):
+    want = oracle.step(rows_of(x, state.scores.shape[1], rows), host(state), stops, alpha, early)
+    ids = torch.tensor(stops, dtype=torch.int32, device=x.device)
+    out = clone(state)  # separate arrays for the new state, the histories shared
+    mine = clone(state)
+    out.token_history, out.parent_history = mine.token_history, mine.parent_history
+    before = {k: v.clone() for k, v in vars(mine).items() if not k.endswith("history")}
+    got = beam_search_step(x, mine, stop_token_ids=ids, length_penalty=alpha,
+                           early_stopping=early, target_rows=rows, out=out)
+    check_state(got.state, want)
+    assert np.array_equal(got.token_ids.cpu().numpy(), want["token_ids"])
+    assert np.array_equal(got.parents.cpu().numpy(), want["parents"])
+    for k, v in before.items():  # the old state is left as it was
+        assert torch.equal(getattr(mine, k), v), k
+    # and in place
+    inside = clone(state)
+    here = beam_search_step(x, inside, stop_token_ids=ids, length_penalty=alpha,
+                            early_stopping=early, target_rows=rows)
+    assert here.state is inside
+    for k, v in vars(out).items():
+        assert torch.equal(v, getattr(inside, k)), k
+    assert torch.equal(here.token_ids, got.token_ids)
+    return got, want
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("G,W,V,E", [(1, 1, 50, 1), (9, 4, 700, 2), (5, 8, 2100, 0), (3, 12, 9001, 5),
+                                     (2, 64, 4100, 3), (1, 128 // 2, 40, 1)])
+@pytest.mark.parametrize("alpha,early", [(1.0, False), (0.0, True), (0.6, False)])
+def test_step(device, dtype, G, W, V, E, alpha, early):
+    gen = torch.Generator(device=device).manual_seed(G * 100 + W)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2.5).to(DTYPES[dtype])
+    stops = np.random.default_rng(W).permutation(V)[:E].tolist()
+    if E:  # a third of the rows want to stop
+        want = torch.rand(G * W, 1, device=device, generator=gen) < 0.33
+        at = torch.tensor(stops, device=device)
+        x[:, at] = torch.where(want, torch.full_like(x[:, at], 9.0), x[:, at])
+    state = random_state(device, G, W, 20, W, done=[1] if G > 2 else [], full=[2] if G > 2 else [])
+    check_step(x, state, stops, alpha, early)
+
+
+def test_step_groups_that_rest(device):
+    """Done and full groups, lengths outside the histories, a group whose rows are masked."""
+    G, W, V, T = 6, 3, 600, 5
+    x = torch.randn(G * W, V, device=device, generator=torch.Generator(device=device).manual_seed(1))
+    state = random_state(device, G, W, T, 3, done=[0], full=[1])
+    state.lengths[2] = -4
+    state.lengths[3] = 2 ** 31 - 1
+    x[4 * W:5 * W] = -math.inf
+    state.done[4] = state.done[5] = False
+    state.lengths[4:] = 2
+    got, _ = check_step(x, state, [7])
+    assert got.token_ids[:5].eq(-1).all() and got.state.done[4] and not got.state.done[5]
+    # resting groups' rows are not looked at
+    y = x.clone()
+    y[:4 * W] = math.nan
+    again = beam_search_step(y, clone(state), stop_token_ids=torch.tensor([7], dtype=torch.int32,
+                                                                          device=device))
+    assert torch.equal(again.token_ids, got.token_ids)
+
+
+def test_step_all_candidates_stop(device):
+    """Only stop tokens are allowed: nothing runs on, the group is done."""
+    W, V = 4, 300
+    x = torch.full((W, V), -math.inf, device=device)
+    x[:, 5], x[:, 9] = 1.0, 0.5
+    state = BeamState.new(1, W, 6, device)
+    state.scores = make_scores(device, 1, W, 0)
+    got, want = check_step(x, state, [9, 5])
+    assert bool(got.state.done[0]) and torch.isneginf(got.state.scores).all()
+    assert want["finished_scores"][0, 0] > -np.inf
+
+
+def test_equal_hypotheses_keep_the_earlier_one(device):
+    W, V = 2, 64
+    x = torch.zeros(W, V, device=device)
+    state = BeamState.new(1, W, 8, device)
+    lp = -math.log(64.0)
+    state.scores = torch.tensor([[0.0, 0.0]], device=device)
+    state.finished_scores = torch.tensor([[lp, lp]], dtype=torch.float32, device=device)
+    state.finished_beams = torch.tensor([[1, 0]], dtype=torch.int32, device=device)
+    state.finished_token_ids = torch.tensor([[40, 41]], dtype=torch.int32, device=device)
+    state.finished_lengths = torch.tensor([[1, 1]], dtype=torch.int32, device=device)
+    # a sum of 64 ones is exact, and so is what follows from it in 64 bits
+    stop = torch.tensor([0, 1], dtype=torch.int32, device=device)
+    got = beam_search_step(x, state, stop_token_ids=stop)
+    assert got.state.finished_token_ids.tolist() == [[40, 41]]
+    assert bool(got.state.done[0]) and got.token_ids.tolist() == [[2, 3]]
+    assert got.parents.tolist() == [[0, 0]]
+
+
+# ----------------------------------------------------------------- reorder
+
+
+def values(device, shape, dtype, seed):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    if dtype.is_floating_point:
+        return torch.randn(shape, device=device, generator=gen).to(dtype)
+    most = 2 if dtype == torch.bool else 200
+    return torch.randint(0, most, shape, device=device, generator=gen).to(dtype)
+
+
+def as_bytes(x):
+    return x.contiguous().view(torch.uint8).cpu().numpy().reshape(x.shape + (-1,))
+
+
+def check_reorder(x, parents, length_dim=1, **kw):
+    """In place and out of place against the oracle, byte for byte."""
+    args = {k: None if v is None else v.cpu().numpy() for k, v in kw.items()}
+    raw = as_bytes(x)
+    want = oracle.reorder(raw, parents.cpu().numpy(), length_dim=length_dim, **args)
+    out = values(x.device, x.shape, x.dtype, 77)
+    want_out = oracle.reorder(raw, parents.cpu().numpy(), length_dim=length_dim, out=as_bytes(out),
+                              **args)
+    assert reorder_beams(x, parents, length_dim=length_dim, out=out, **kw) is out
+    assert np.array_equal(as_bytes(out), want_out)
+    assert np.array_equal(as_bytes(x), raw)  # the states are left alone
+    assert reorder_beams(x, parents, length_dim=length_dim, **kw) is x
+    assert np.array_equal(as_bytes(x), want)
+
+
+def make_parents(device, G, W, seed):
+    r = np.random.default_rng(seed)
+    p = r.integers(0, W, (G, W))
+    p[0] = np.roll(np.arange(W), 1)  # a cycle through every row
+    if G > 1:
+        p[1] = W - 1                 # one heir of all
+    if G > 2:
+        p[2] = -1                    # a group that rests
+    if G > 3:
+        p[3, 0], p[3, -1] = W, 2 ** 31 - 1  # outside: kept
+    return torch.tensor(p, dtype=torch.int32, device=device)
+
+
+def counts(device, G, T, seed):
+    n = np.random.default_rng(seed).integers(0, T + 1, G)
+    n[0] = T
+    if G > 1:
+        n[1] = 1
+    if G > 4:
+        n[3], n[4] = 0, T + 100      # nothing; past the end: the tensor's length
+    return torch.tensor(n, dtype=torch.int32, device=device)
+
+
+@pytest.mark.parametrize("W", [1, 2, 5, 8, 9, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("shape,dim,dtype", [
+    ((37,), 1, torch.int32), ((1,), 1, torch.int64), ((3, 19, 5), 2, torch.float16),
+    ((70, 2, 3), 1, torch.bfloat16), ((2, 3, 13, 1), 3, torch.uint8), ((259,), 1, torch.bool),
+    ((33, 16), 1, torch.float32)])
+def test_reorder(device, W, shape, dim, dtype):
+    G = 6
+    x = values(device, (G * W, *shape), dtype, W)
+    T = shape[dim - 1]
+    check_reorder(x, make_parents(device, G, W, W), dim)
+    check_reorder(x, make_parents(device, G, W, W), dim, lengths=counts(device, G, T, W))
+    starts = torch.tensor([0, 1, T // 2, T + 5, -3, T // 3], dtype=torch.int32, device=device)
+    check_reorder(x, make_parents(device, G, W, 2 * W), dim, starts=starts)
+    check_reorder(x, make_parents(device, G, W, 3 * W), dim, starts=starts,
+                  lengths=counts(device, G, T, 2 * W))
+
+
+@pytest.mark.parametrize("W", [2, 4, 20])
+def test_reorder_pages_through_slots(device, W):
+    """The last pages of the beams in a pool; slots outside it are left alone, and so is the rest."""
+    G, pages = 5, 300
+    x = values(device, (pages, 16, 3, 8), torch.bfloat16, W)
+    order = np.random.default_rng(W).permutation(pages)[:G * W].reshape(G, W)
+    slots = torch.tensor(order, dtype=torch.int32, device=device)
+    slots[0, 0], slots[1, 1] = -1, pages
+    check_reorder(x, make_parents(device, G, W, 1), 1, slots=slots,
+                  lengths=counts(device, G, 16, 3))
+
+
+def test_reorder_views(device):
+    """Rows apart from each other, off a vector's alignment, keys and values in one tensor."""
+    G, W = 3, 4
+    parents = make_parents(device, G, W, 5)
+    base = values(device, (G * W, 2, 9, 7), torch.float16, 0)
+    want = np.stack([oracle.reorder(as_bytes(base[:, k]), parents.cpu().numpy())
+                     for k in range(2)], axis=1)
+    reorder_beams([base[:, 0], base[:, 1]], parents)
+    assert np.array_equal(as_bytes(base), want)
+    wide = values(device, (G * W, 50), torch.uint8, 1)
+    keep = wide.clone()
+    part = wide[:, 3:44]
+    want = oracle.reorder(as_bytes(part), parents.cpu().numpy())
+    reorder_beams(part, parents)
+    assert np.array_equal(as_bytes(part), want)
+    assert torch.equal(wide[:, :3], keep[:, :3]) and torch.equal(wide[:, 44:], keep[:, 44:])
+    # more rows than beams: those behind the last are left as they were
+    more = values(device, (G * W + 3, 20), torch.int32, 2)
+    tail = more[G * W:].clone()
+    reorder_beams(more, parents)
+    assert torch.equal(more[G * W:], tail)
+
+
+def test_reorder_many_tensors(device):
+    """More states than one launch takes, of different shapes and types, empty ones among them."""
+    G, W = 4, 3
+    parents = make_parents(device, G, W, 2)
+    shapes = [(G * W, 11), (G * W, 0), (G * W, 40, 2), (G * W, 11, 0), (G * W + 5, 200)]
+    states = [values(device, shapes[k % 5], [torch.int32, torch.bfloat16][k % 2], k)
+              for k in range(60)]
+    want = [oracle.reorder(as_bytes(x), parents.cpu().numpy()) if x.numel() else None
+            for x in states]
+    got = reorder_beams(states, parents)
+    for x, y, w in zip(states, got, want):
+        assert y is x
+        if w is not None:
+            assert np.array_equal(as_bytes(x), w)
+
+
+def test_reorder_many_groups(device):
+    """More (group, state) pairs than one grid has rows."""
+    G, W = 3000, 2
+    r = np.random.default_rng(0)
+    parents = torch.tensor(r.integers(0, W, (G, W)), dtype=torch.int32, device=device)
+    states = [values(device, (G * W, 5), torch.int32, k) for k in range(24)]
+    src = (torch.arange(G, device=device)[:, None] * W + parents).view(-1).long()
+    want = [x[src] for x in states]
+    reorder_beams(states, parents)
+    assert all(torch.equal(x, w) for x, w in zip(states, want))
+
+
+def test_reorder_huge_offsets(device):
+    """Rows beyond 4 GiB."""
+    W, T, D = 3, 1_000_000, 800
+    x = torch.empty((2 * W, T, D), dtype=torch.uint8, device=device)
+    for r in range(2 * W):
+        x[r] = r + 1
+    parents = torch.tensor([[1, 2, 0], [0, 0, 1]], dtype=torch.int32, device=device)
+    n = torch.tensor([T, 999_999], dtype=torch.int32, device=device)
+    reorder_beams(x, parents, lengths=n)
+    assert [int(x[r, T - 2, D - 1]) for r in range(6)] == [2, 3, 1, 4, 4, 5]
+    assert [int(x[r, T - 1, 0]) for r in range(6)] == [2, 3, 1, 4, 5, 6]
+    assert [int(x[r, 0, 0]) for r in range(6)] == [2, 3, 1, 4, 4, 5]
+
+
+def test_reorder_refusals(device):
+    x = torch.zeros(8, 10, device=device)
+    parents = torch.zeros(2, 4, dtype=torch.int32, device=device)
+    for bad in (dict(out=x[:, :].view(8, 10)), dict(out=torch.zeros(8, 11, device=device)),
+                dict(out=[x, x]), dict(length_dim=2), dict(length_dim=0),
+                dict(lengths=torch.zeros(3, dtype=torch.int32, device=device)),
+                dict(slots=torch.zeros(8, dtype=torch.int32, device=device)),
+                dict(lengths=torch.zeros(2, dtype=torch.int32))):
+        if "out" in bad and isinstance(bad["out"], torch.Tensor) and bad["out"].shape == x.shape:
+            assert reorder_beams(x, parents, **bad) is bad["out"]  # the same memory: in place
+            continue
+        with pytest.raises((ValueError, NotImplementedError)):
+            reorder_beams(x, parents, **bad)
+    with pytest.raises(TypeError):
+        reorder_beams(x, parents.long())
+    with pytest.raises(ValueError):
+        reorder_beams(x[:7], parents)
+    with pytest.raises(ValueError):
+        reorder_beams(x.t(), torch.zeros(1, 4, dtype=torch.int32, device=device))
+    with pytest.raises(ValueError, match="share memory"):
+        reorder_beams([x, x], parents)
+    with pytest.raises(ValueError, match="share memory"):
+        reorder_beams(x[:4], parents[:1], out=x[2:6])
+    with pytest.raises(ValueError):
+        reorder_beams(x.expand(2, 8, 10).transpose(0, 1), parents)
+
+
+# ----------------------------------------------------------------- finish
+
+
+@pytest.mark.parametrize("G,W,T,n", [(1, 1, 1, 1), (1, 4, 2, 4), (7, 3, 33, 2), (5, 8, 300, 8),
+                                     (2, 64, 130, 64), (3, 5, 4097, 1), (1, 2, 20000, 2)])
+@pytest.mark.parametrize("alpha", [0.0, 1.0])
+def test_finish(device, G, W, T, n, alpha):
+    state = random_state(device, G, W, T, T + W, done=[1] if G > 2 else [],
+                         full=[0])
+    before = {k: v.clone() for k, v in vars(state).items()}
+    got = beam_search_finish(state, n, length_penalty=alpha)
+    ids, lengths, scores = oracle.finish(host(state), n, alpha)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    assert np.array_equal(got.lengths.cpu().numpy(), lengths)
+    close(got.scores, scores)
+    for k, v in before.items():
+        assert torch.equal(getattr(state, k), v)
+
+
+def test_finish_of_odd_histories(device):
+    """Parents outside the group, lengths outside the histories, beams that are none."""
+    G, W, T = 4, 3, 50
+    state = random_state(device, G, W, T, 11)
+    r = np.random.default_rng(1)
+    state.parent_history = torch.tensor(r.integers(-2, W + 3, (G, T, W)), dtype=torch.int32,
+                                        device=device)
+    state.lengths = torch.tensor([0, -7, 2 ** 31 - 1, 9], dtype=torch.int32, device=device)
+    state.finished_lengths[0, 0] = 2 ** 31 - 1
+    state.finished_scores[0, 0], state.finished_beams[0, 0] = -0.5, 99
+    state.scores[3] = torch.tensor([-1.0, math.nan, -math.inf], device=device)
+    got = beam_search_finish(state)
+    ids, lengths, scores = oracle.finish(host(state), W, 1.0)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    assert np.array_equal(got.lengths.cpu().numpy(), lengths)
+    close(got.scores, scores)
+
+
+# ----------------------------------------------------------------- together
+
+
+class Chain:
+    """A tiny model with a state: the next row depends on the sum of the beam's cached tokens."""
+
+    def __init__(self, device, V, seed):
+        gen = torch.Generator(device=device).manual_seed(seed)
+        self.V, self.table = V, torch.randn(V, V, device=device, generator=gen) * 2
+
+    def rows(self, cache, length):
+        return self.table[(cache[:, :length].sum(dim=1) % self.V)]
+
+
+@pytest.mark.parametrize("G,W,alpha,early", [(1, 4, 1.0, False), (5, 3, 0.6, True)])
+def test_a_whole_search(device, G, W, alpha, early):
+    """step, reorder and finish together, as a server runs them, against the oracle's own search."""
+    V, T = 23, 12
+    model = Chain(device, V, 0)
+    table = model.table.double().cpu().numpy()
+    search = BeamSearch(G, W, T, device, stop_token_ids=[0, 4], length_penalty=alpha,
+                        early_stopping=early)
+    cache = torch.zeros(G * W, T + 1, dtype=torch.int64, device=device)
+    cache[:, 0] = torch.arange(G, device=device).repeat_interleave(W) * 5 + 1
+    mine = {k: v.copy() for k, v in host(search.state).items()}
+    prefix = [[[g * 5 + 1]] * W for g in range(G)]
+    for t in range(T):
+        step = search.step(model.rows(cache, t + 1))
+        search.reorder(cache, lengths=torch.full((G,), t + 1, dtype=torch.int32, device=device))
+        cache[:, t + 1] = step.token_ids.view(-1).clamp(min=0)
+        want = oracle.step(lambda g, w: table[sum(prefix[g][w]) % V], mine, [0, 4], alpha, early)
+        assert np.array_equal(step.token_ids.cpu().numpy(), want["token_ids"])
+        assert np.array_equal(step.parents.cpu().numpy(), want["parents"])
+        prefix = [[prefix[g][max(want["parents"][g, w], 0)] + [max(int(want["token_ids"][g, w]), 0)]
+                   if want["parents"][g, w] >= 0 else prefix[g][w] + [0]
+                   for w in range(W)] for g in range(G)]
+        mine = {k: want[k] for k in mine}
+    got = search.finish()
+    ids, lengths, scores = oracle.finish(mine, W, alpha)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    assert np.array_equal(got.lengths.cpu().numpy(), lengths)
+    close(got.scores, scores, scale=T)
+
+
+def test_streams_and_graphs(device):
+    """Two captured steps, replayed several times and beside eager work, share no scratch."""
+    G, W, V, T = 3, 4, 5003, 6
+    gen = torch.Generator(device=device).manual_seed(0)
+    rows = [torch.randn(G * W, V, device=device, generator=gen) for _ in range(2)]
+    states = [random_state(device, G, W, T, k) for k in range(2)]
+    for s in states:
+        s.lengths.fill_(2)
+        s.done.fill_(False)
+    caches = [values(device, (G * W, 77), torch.int32, k) for k in range(2)]
+    stop = torch.tensor([3], dtype=torch.int32, device=device)
+
+    def work(k, state, cache, out):
+        step = beam_search_step(rows[k], state, stop_token_ids=stop, out=out)
+        return step, reorder_beams(cache, step.parents, out=torch.zeros_like(cache)), \
+            beam_search_finish(out)
+
+    def separate(state):
+        out = clone(state)
+        out.token_history, out.parent_history = state.token_history, state.parent_history
+        return out
+
+    want = []
+    for k in range(2):
+        s = clone(states[k])
+        want.append(work(k, s, caches[k], separate(s)))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    graphs, got, inputs = [], [], []
+    for k in range(2):
+        s = clone(states[k])
+        o = separate(s)
+        inputs.append(s)  # a graph reads its inputs' memory at every replay
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            work(k, s, caches[k], o)  # warm
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(work(k, s, caches[k], o))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for graph, stream in zip(graphs, streams):  # both in flight
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                graph.replay()
+        beam_search_select(rows[0], states[0].scores, 8)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0].token_ids, b[0].token_ids)
+            assert torch.equal(a[0].parents, b[0].parents)
+            assert torch.equal(a[0].state.scores, b[0].state.scores)
+            assert torch.equal(a[1], b[1])
+            assert torch.equal(a[2].token_ids, b[2].token_ids)
+
+
+def test_same_results_twice(device):
+    G, W, V = 16, 8, 32000
+    gen = torch.Generator(device=device).manual_seed(0)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2).to(torch.bfloat16)
+    s = make_scores(device, G, W, 0)
+    a = [beam_search_select(x, s, 16) for _ in range(4)]
+    for b in a[1:]:
+        assert torch.equal(a[0].scores, b.scores) and torch.equal(a[0].token_ids, b.token_ids)
+
+
+def test_refusals(device):
+    x = torch.zeros(8, 100, device=device)
+    s = torch.zeros(2, 4, device=device)
+    i32 = dict(dtype=torch.int32, device=device)
+    for bad in (lambda: beam_search_select(x, s, 0), lambda: beam_search_select(x, s, 257),
+                lambda: beam_search_select(x[:7], s, 8), lambda: beam_search_select(x.t(), s[:1], 8),
+                lambda: beam_search_select(x, s[0], 8), lambda: beam_search_select(x, s[:, ::2], 4),
+                lambda: beam_search_select(x, torch.zeros(1, 65, device=device), 4),
+                lambda: beam_search_select(x, torch.zeros(1, 0, device=device), 4),
+                lambda: beam_search_select(x[:, :0], s, 4),
+                lambda: beam_search_select(x, s, 8, target_rows=torch.zeros(3, **i32)),
+                lambda: beam_search_finish(BeamState.new(2, 4, 8, device), 5),
+                lambda: beam_search_finish(BeamState.new(2, 4, 8, device), 0),
+                lambda: beam_search_step(x, BeamState.new(2, 4, 8, device),
+                                         stop_token_ids=torch.zeros(64, **i32)),
+                lambda: beam_search_step(x, BeamState.new(2, 4, 8, device),
+                                         out=BeamState.new(2, 4, 8, device)),
+                lambda: beam_search_step(x[:7], BeamState.new(2, 4, 8, device))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: beam_search_select(x.double(), s, 8),
+                lambda: beam_search_select(x, s.double(), 8),
+                lambda: beam_search_select(x, s, 8, target_rows=torch.zeros(2, 4, dtype=torch.int64,
+                                                                            device=device))):
+        with pytest.raises(TypeError):
+            bad()
+    with pytest.raises(NotImplementedError):
+        beam_search_select(x, s.cpu(), 8)

@@ -1,0 +1,609 @@
+// Beam search: the selection over beams and vocabulary, and a decoding step around it.
+//
+// A group is one request with W beams.  Beam b has the summed log-probability s_b and a row of
+// logits x_b over V tokens:
+//   lse_b       = log sum_v exp(x_bv)
+//   total(b, v) = s_b + (x_bv - lse_b)
+// and the group's candidates are its C largest totals, in the order (total descending, beam
+// ascending, logit descending, token ascending).  A beam whose score or lse is not finite (no beam,
+// a row masked everywhere, a NaN or +inf) proposes nothing; entries of -inf are no candidates.
+//
+//   beam_scan_kernel    one 256-thread workgroup per (beam, chunk of columns) reads the chunk once,
+//                       into registers, and leaves its maximum, its sum of exp(x - maximum) and the
+//                       largest entry of every 16 lanes (a "top": 16 of them a chunk).
+//   beam_finish_kernel  one 512-thread workgroup per group:
+//     - lse_b in 64 bits from the chunks' sums;
+//     - theta, the C-th largest of the maxima of 512 disjoint unions of tops, as totals: at least C
+//       entries of the group reach it, so the candidates are among the entries that do, and these lie
+//       under the tops that do (a few more than C);
+//     - per beam the logit that theta stands for (rounded down), so that tops and entries are compared
+//       as they are; the entries under the tops that reach it are gathered into LDS, their totals
+//       formed in 64 bits, and ranked by counting;
+//     - more entries than LDS holds (long runs of one value: masks of the type's lowest value, a
+//       uniform row): the beams one after the other, each one's C largest by a radix selection.
+//   A step goes on in the same workgroup: stop tokens, finished hypotheses, histories.
+//
+// The sums of a chunk are fp32 (each of 32 or fewer terms of a lane, then a tree over the lanes), the
+// chunks are combined in fp64: lse is within about 1e-7 of the 64-bit value, and the totals are formed
+// and compared in 64 bits, so the order of two candidates of one beam is exact and that of candidates
+// of two beams is the 64-bit order unless they are closer than that.
+#include "beam.h"
+#include "mvsd_device.h"
+
+namespace mvsd {
+
+constexpr int kTops = 16;          // of a chunk, 16 lanes each
+constexpr int kFThreads = 512;
+constexpr int kFWaves = kFThreads / kWave;
+constexpr int kListCap = 2048;     // tops that reach theta
+constexpr int kCandCap = 1024;     // gathered entries
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Columns per chunk: long ones, unless they leave compute units idle (fewer than 4 workgroups each)
+// or give a row fewer than two tops per candidate (a group may have one beam only), so that theta is
+// a poor bound or none.
+constexpr int kBeamLong = 8192, kBeamShort = 2048;
+
+static int beam_chunk(int64_t rows, int64_t V, int64_t C) {
+  const int64_t chunks = (V + kBeamLong - 1) / kBeamLong;
+  return rows * chunks < 1024 || chunks * kTops < 2 * C ? kBeamShort : kBeamLong;
+}
+
+__device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Whether a step leaves the group as it is.
+__device__ inline bool group_rests(const BeamScanParams& p, int g) {
+  if (!p.lengths) return false;
+  const int len = p.lengths[g];
+  return p.done[g] != 0 || len < 0 || len >= p.max_length;
+}
+
+template <typename S>
+__device__ inline const S* beam_row(const BeamScanParams& p, int64_t r) {
+  int64_t row = r;
+  if (p.rows) row = min(max((int64_t)p.rows[r], (int64_t)0), p.num_rows - 1);
+  return static_cast<const S*>(p.logits) + row * p.stride;
+}
+
+template <int DT, int NV>
+__global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
+  using S = typename Elem<DT>::storage;
+  constexpr int VEC = Elem<DT>::kVec;
+  constexpr int CH = NV * kThreads * VEC;
+  __shared__ float s_m[kWaves], s_s[kWaves];
+  const int r = blockIdx.x / p.nchunks, c = blockIdx.x - r * p.nchunks;
+  if (!finite(p.scores[r]) || group_rests(p, r / p.W)) return;  // the finish does the same test
+  const S* row = beam_row<S>(p, r);
+  const int tid = threadIdx.x;
+  const int64_t base = (int64_t)c * CH;
+  const int left = (int)min((int64_t)p.V - base, (int64_t)CH);  // columns of the chunk
+  row += base;
+  u32x4 q[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) q[j] = load_vec_inside<DT>(row, (j * kThreads + tid) * VEC, left);
+  float v[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      v[j][e] = vec_elem<DT>(q[j], e);
+      if (left < CH)
+        v[j][e] = inside_col<DT>((j * kThreads + tid) * VEC, e, left) < 0 ? -INFINITY : v[j][e];
+    }
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = fmaxf(m, v[j][e]);
+  const float top = max16(m);
+  const float wm = fmaxf(fmaxf(readlane_f32(top, 0), readlane_f32(top, 16)),
+                         fmaxf(readlane_f32(top, 32), readlane_f32(top, 48)));
+  float s = 0.f;
+  if (wm != -INFINITY) {  // +inf gives a NaN sum, as a NaN does
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += __builtin_amdgcn_exp2f((v[j][e] - wm) * kLog2e);
+  } else {  // every entry is -inf or NaN
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s += v[j][e] != v[j][e] ? NAN : 0.f;
+  }
+  s = wave_sum(s);
+  const int64_t slot = (int64_t)r * p.nchunks + c;
+  if ((tid & 15) == 0) p.tops[slot * kTops + tid / 16] = top;
+  if (lane_id() == 0) {
+    s_m[wave_id()] = wm;
+    s_s[wave_id()] = s;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float M = s_m[0], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+      sum += s_m[w] == -INFINITY ? s_s[w]
+                                 : s_s[w] * __builtin_amdgcn_exp2f((s_m[w] - M) * kLog2e);
+    p.stats[slot] = make_float2(M, sum);
+  }
+}
+
+// ------------------------------------------------------------------ finish -----------
+
+struct Candidate {
+  double total;
+  float x;
+  int token, beam;
+};
+
+__device__ inline bool better(const Candidate& a, const Candidate& b) {
+  if (a.total != b.total) return a.total > b.total;
+  if (a.beam != b.beam) return a.beam < b.beam;
+  if (a.x != b.x) return a.x > b.x;
+  return a.token < b.token;
+}
+
+struct BeamSmem {
+  Candidate cand[kCandCap];
+  Candidate best[kMaxCandidates];  // the group's candidates in order
+  int list[kListCap];
+  __align__(16) float key[kFThreads];
+  double lse[kMaxBeams];
+  float score[kMaxBeams];
+  float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
+  int hist[256];
+  int wave_cnt[kFWaves];
+  uint64_t stop_mask[kMaxCandidates / kWave], on_mask[kMaxCandidates / kWave];
+  float pool[2 * kMaxBeams];
+  int listed, count, above, digit;
+  uint32_t theta_key;
+  float worst;
+};
+
+__device__ inline double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// The C largest entries of one row, by (value desc, token asc), into cand[at ..]; returns how many.
+// Radix selection of the C-th largest key, eight bits at a time, then one pass for the entries
+// above it and one, from the first column, for as many equal ones as are missing.
+template <int DT>
+__device__ inline int row_largest(const typename Elem<DT>::storage* row, int V, int C, int beam,
+                                  BeamSmem& sm, int at) {
+  const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
+  constexpr uint32_t kNinf = 0x007fffffu;  // ordered_bits(-inf): not a candidate
+  uint32_t prefix = 0, mask = 0;
+  int want = C;
+  bool all = false;  // fewer than C entries: take every one
+  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
+    for (int i = tid; i < 256; i += kFThreads) sm.hist[i] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < V; i += kFThreads) {
+      const uint32_t key = ordered_bits(Elem<DT>::cvt(row[i]));
+      const bool in = key > kNinf && (key & mask) == prefix;
+      const uint32_t digit = (key >> shift) & 255u;
+      const uint64_t live = __ballot(in);
+      if (live == 0) continue;
+      // one addition for the lanes that share the first one's digit, the rest one each
+      const int leader = __ffsll((long long)live) - 1;
+      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
+      const uint64_t same = __ballot(in && digit == first);
+      if (lane == leader) atomicAdd(&sm.hist[first], __popcll(same));
+      if (in && digit != first) atomicAdd(&sm.hist[digit], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int above = 0, d = 255;
+      while (d > 0 && above + sm.hist[d] < want) above += sm.hist[d--];
+      sm.digit = above + sm.hist[d] < want ? -1 : d;
+      sm.above = above;
+    }
+    __syncthreads();
+    if (sm.digit < 0) {
+      all = true;  // only in the first round: later ones count what the round before found
+    } else {
+      want -= sm.above;
+      prefix |= (uint32_t)sm.digit << shift;
+      mask |= 255u << shift;
+    }
+    __syncthreads();
+  }
+  const uint32_t kth = all ? kNinf : prefix;  // entries above it are taken, equal ones as wanted
+  if (tid == 0) sm.count = 0;
+  __syncthreads();
+  for (int64_t i = tid; i < V; i += kFThreads) {
+    const float x = Elem<DT>::cvt(row[i]);
+    if (ordered_bits(x) > kth) {
+      const int pos = atomicAdd(&sm.count, 1);
+      if (pos < C) {
+        Candidate& o = sm.cand[at + pos];
+        o.x = x;
+        o.token = (int)i;
+        o.beam = beam;
+      }
+    }
+  }
+  __syncthreads();
+  int found = min(sm.count, C);
+  __syncthreads();
+  if (all) return found;
+  for (int64_t b = 0; b < V && found < C; b += kFThreads) {
+    const int64_t i = b + tid;
+    const float x = i < V ? Elem<DT>::cvt(row[i]) : -INFINITY;
+    const bool eq = i < V && ordered_bits(x) == kth;
+    const uint64_t hit = __ballot(eq);
+    if (lane == 0) sm.wave_cnt[wid] = __popcll(hit);
+    __syncthreads();
+    int pos = found, total = 0;
+    for (int w = 0; w < kFWaves; ++w) {
+      pos += w < wid ? sm.wave_cnt[w] : 0;
+      total += sm.wave_cnt[w];
+    }
+    pos += __popcll(hit & ((1ull << lane) - 1ull));
+    if (eq && pos < C) {
+      Candidate& o = sm.cand[at + pos];
+      o.x = x;
+      o.token = (int)i;
+      o.beam = beam;
+    }
+    found = min(found + total, C);
+    __syncthreads();
+  }
+  return found;
+}
+
+// The group's candidates, in order, in sm.best; returns how many.
+template <int DT, int NV>
+__device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem& sm) {
+  using S = typename Elem<DT>::storage;
+  constexpr int VEC = Elem<DT>::kVec;
+  constexpr int CH = NV * kThreads * VEC;
+  const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
+  const int W = p.W, C = p.C, nch = p.nchunks;
+  const int64_t first = (int64_t)g * W;
+  // ---- lse of every beam, one wave each ----
+  for (int w = wid; w < W; w += kFWaves) {
+    const float score = p.scores[first + w];
+    double lse = NAN;
+    if (finite(score)) {
+      const float2* st = p.stats + (first + w) * nch;
+      float m = -INFINITY;
+      for (int c = lane; c < nch; c += kWave) m = fmaxf(m, st[c].x);
+      const float M = wave_max(m);
+      double s = 0.0;
+      for (int c = lane; c < nch; c += kWave) {
+        const float2 v = st[c];
+        // a chunk of -inf alone adds its sum, 0 (NaN where it holds a NaN)
+        s += v.x == -INFINITY ? (double)v.y : (double)v.y * exp((double)v.x - (double)M);
+      }
+      s = wave_sum_f64(s);
+      lse = (double)M + log(s);
+    }
+    if (lane == 0) {
+      const bool live = fabs(lse) < (double)INFINITY;
+      sm.lse[w] = live ? lse : 0.0;
+      sm.score[w] = live ? score : -INFINITY;
+    }
+  }
+  if (tid == 0) sm.listed = sm.count = 0;
+  if (tid == 0) sm.theta_key = 0xffffffffu;
+  __syncthreads();
+  // ---- theta ----
+  const int per_row = nch * kTops;
+  const int tops = W * per_row;
+  const float* top = p.tops + first * per_row;
+  float own = -INFINITY;
+  for (int i = tid; i < tops; i += kFThreads) {
+    const int w = i / per_row;
+    if (sm.score[w] == -INFINITY) continue;
+    own = fmaxf(own, (float)((double)sm.score[w] + ((double)top[i] - sm.lse[w])));
+  }
+  sm.key[tid] = own;
+  __syncthreads();
+  {
+    int above = 0;
+    const float4* keys = reinterpret_cast<const float4*>(sm.key);
+#pragma unroll 8
+    for (int j = 0; j < kFThreads / 4; ++j) {
+      const float4 o = keys[j];
+      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+    }
+    if (above < C) atomicMin(&sm.theta_key, ordered_bits(own));
+  }
+  __syncthreads();
+  const float theta = key_float(sm.theta_key);
+  // ---- the least logit of each beam that can reach theta, rounded down ----
+  for (int w = tid; w < W; w += kFThreads) {
+    float f = INFINITY;
+    if (sm.score[w] != -INFINITY) {
+      f = -3.402823466e38f;  // -inf is no candidate
+      if (theta != -INFINITY) {
+        // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
+        const double t = (double)theta - fabs((double)theta) * 0x1p-23;
+        f = fmaxf(f, __double2float_rd(t - (double)sm.score[w] + sm.lse[w]));
+      }
+    }
+    sm.floor[w] = f;
+  }
+  __syncthreads();
+  for (int i = tid; i < tops; i += kFThreads) {
+    const int w = i / per_row;
+    const float f = sm.floor[w];
+    if (f < INFINITY && top[i] >= f) {
+      const int pos = atomicAdd(&sm.listed, 1);
+      if (pos < kListCap) sm.list[pos] = i;
+    }
+  }
+  __syncthreads();
+  const int listed = sm.listed;
+  int found = 0;
+  if (listed <= kListCap) {
+    // ---- the entries under the listed tops, 16 lanes each ----
+    for (int b = 0; b < listed; b += kFThreads / 16) {
+      const int li = b + tid / 16;
+      if (li >= listed) continue;
+      const int i = sm.list[li];
+      const int w = i / per_row, rest = i - w * per_row;
+      const int c = rest / kTops, lanes = rest - c * kTops;
+      const int64_t base = (int64_t)c * CH;
+      const int left = (int)min((int64_t)p.V - base, (int64_t)CH);
+      const S* row = beam_row<S>(p, first + w) + base;
+      const float f = sm.floor[w];
+      u32x4 q[NV];
+      const int col0 = (lanes * 16 + (tid & 15)) * VEC;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) q[j] = load_vec_inside<DT>(row, col0 + j * kThreads * VEC, left);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float x = vec_elem<DT>(q[j], e);
+          if (!(x >= f)) continue;
+          const int col = inside_col<DT>(col0 + j * kThreads * VEC, e, left);
+          if (col < 0) continue;
+          const int pos = atomicAdd(&sm.count, 1);
+          if (pos < kCandCap) {
+            Candidate& o = sm.cand[pos];
+            o.total = (double)sm.score[w] + ((double)x - sm.lse[w]);
+            o.x = x;
+            o.token = (int)(base + col);
+            o.beam = w;
+          }
+        }
+    }
+    __syncthreads();
+    found = sm.count;
+  }
+  if (listed <= kListCap && found <= kCandCap) {
+    for (int i = tid; i < found; i += kFThreads) {
+      const Candidate mine = sm.cand[i];
+      int rank = 0;
+      for (int j = 0; j < found; ++j) rank += better(sm.cand[j], mine);
+      if (rank < C) sm.best[rank] = mine;
+    }
+    __syncthreads();
+    return min(found, C);
+  }
+  // ---- too many: the beams one after the other ----
+  found = 0;
+  for (int w = 0; w < W; ++w) {
+    __syncthreads();
+    if (sm.floor[w] == INFINITY) continue;
+    const int got = row_largest<DT>(beam_row<S>(p, first + w), p.V, C, w, sm, 0);
+    __syncthreads();
+    // the best so far and the beam's own: at most 2 C = 512, one a thread
+    Candidate mine;
+    const bool have = tid < found + got;
+    if (have) {
+      mine = tid < found ? sm.best[tid] : sm.cand[tid - found];
+      if (tid >= found) mine.total = (double)sm.score[w] + ((double)mine.x - sm.lse[w]);
+    }
+    __syncthreads();
+    if (have) sm.cand[tid] = mine;
+    __syncthreads();
+    int rank = 0;
+    if (have)
+      for (int j = 0; j < found + got; ++j) rank += better(sm.cand[j], mine);
+    if (have && rank < C) sm.best[rank] = mine;
+    found = min(found + got, C);
+  }
+  __syncthreads();
+  return found;
+}
+
+template <int DT, int NV>
+__global__ __launch_bounds__(kFThreads) void beam_select_kernel(BeamScanParams p,
+                                                                 BeamSelectOut o) {
+  __shared__ BeamSmem sm;
+  const int g = blockIdx.x;
+  const int found = group_candidates<DT, NV>(p, g, sm);
+  for (int i = threadIdx.x; i < p.C; i += kFThreads) {
+    const int64_t at = (int64_t)g * p.C + i;
+    const bool on = i < found;
+    o.token_ids[at] = on ? sm.best[i].token : -1;
+    o.parents[at] = on ? sm.best[i].beam : -1;
+    o.scores[at] = on ? (float)sm.best[i].total : -INFINITY;
+  }
+}
+
+// ------------------------------------------------------------------ step -------------
+// Candidates in order; those of rank below W that are stop tokens end a hypothesis of
+// length + 1 tokens with the normalised score fl32(fl32(total) / (length + 1)^alpha); the first W
+// that are no stop tokens are the next beams.  W (1 + E) candidates always hold W of the latter if
+// there are as many.  Finished hypotheses: the W best of the old and the new ones, the old first
+// where they are equal.
+template <int DT, int NV>
+__global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
+                                                               mvsd_beam_step_args a) {
+  __shared__ BeamSmem sm;
+  const int g = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wid = wave_id();
+  const int W = p.W, C = p.C;
+  const int64_t first = (int64_t)g * W;
+  const int len = p.lengths[g];
+  if (group_rests(p, g)) {  // block-uniform
+    if (tid < W) {
+      a.token_ids[first + tid] = -1;
+      a.parents[first + tid] = -1;
+      a.out_scores[first + tid] = a.scores[first + tid];
+      a.out_finished_scores[first + tid] = a.finished_scores[first + tid];
+      a.out_finished_beams[first + tid] = a.finished_beams[first + tid];
+      a.out_finished_token_ids[first + tid] = a.finished_token_ids[first + tid];
+      a.out_finished_lengths[first + tid] = a.finished_lengths[first + tid];
+    }
+    if (tid == 0) {
+      const uint8_t was = a.done[g];
+      a.out_lengths[g] = len;
+      a.out_done[g] = was;
+    }
+    return;
+  }
+  const int found = group_candidates<DT, NV>(p, g, sm);
+  const int new_len = len + 1;
+  const double power = pow((double)new_len, a.length_penalty);
+  if (wid < kMaxCandidates / kWave) {
+    bool stop = false;
+    if (tid < found)
+      for (int64_t e = 0; e < a.num_stop_ids; ++e)
+        stop |= sm.best[tid].token == a.stop_token_ids[e];
+    const uint64_t sb = __ballot(stop), ob = __ballot(tid < found && !stop);
+    if (lane == 0) {
+      sm.stop_mask[wid] = sb;
+      sm.on_mask[wid] = ob;
+    }
+  }
+  // the old hypotheses, and what they hold, before anything is written (outputs may be inputs)
+  float hyp = -INFINITY;
+  int hyp_beam = -1, hyp_token = -1, hyp_len = 0;
+  if (tid < W) {
+    hyp = a.finished_scores[first + tid];
+    if (!(hyp > -INFINITY)) hyp = -INFINITY;
+    else {
+      hyp_beam = a.finished_beams[first + tid];
+      hyp_token = a.finished_token_ids[first + tid];
+      hyp_len = a.finished_lengths[first + tid];
+    }
+  }
+  __syncthreads();
+  // ---- next beams ----
+  int going = 0;
+  for (int k = 0; k < kMaxCandidates / kWave; ++k) going += __popcll(sm.on_mask[k]);
+  going = min(going, W);
+  float next_best = -INFINITY;
+  {
+    // the first candidate that goes on is the best running beam
+    for (int k = kMaxCandidates / kWave - 1; k >= 0; --k)
+      if (sm.on_mask[k])
+        next_best = (float)sm.best[k * kWave + __ffsll((long long)sm.on_mask[k]) - 1].total;
+  }
+  const int64_t hist = ((int64_t)g * a.max_length + len) * W;
+  auto put = [&](int w, float score, int token, int parent) {
+    a.out_scores[first + w] = score;
+    a.token_ids[first + w] = token;
+    a.parents[first + w] = parent;
+    a.token_history[hist + w] = token;
+    a.parent_history[hist + w] = parent;
+  };
+  if (wid < kMaxCandidates / kWave && ((sm.on_mask[wid] >> lane) & 1)) {
+    int place = __popcll(sm.on_mask[wid] & ((1ull << lane) - 1ull));
+    for (int k = 0; k < wid; ++k) place += __popcll(sm.on_mask[k]);
+    if (place < W) put(place, (float)sm.best[tid].total, sm.best[tid].token, sm.best[tid].beam);
+  }
+  if (tid >= going && tid < W) put(tid, -INFINITY, -1, -1);
+  // ---- finished hypotheses: entries [0, W) are the old ones, [W, 2 W) the candidates of rank < W ----
+  if (tid >= W && tid < 2 * W) {
+    const int r = tid - W;
+    if (r < found && ((sm.stop_mask[r / kWave] >> (r % kWave)) & 1)) {
+      hyp = (float)((double)(float)sm.best[r].total / power);
+      if (!(hyp > -INFINITY)) hyp = -INFINITY;
+      hyp_beam = sm.best[r].beam;
+      hyp_token = sm.best[r].token;
+      hyp_len = new_len;
+    }
+  }
+  if (tid < 2 * W) sm.pool[tid] = hyp;
+  __syncthreads();
+  if (tid < 2 * W) {
+    int rank = 0;
+    for (int j = 0; j < 2 * W; ++j) {
+      const float o = sm.pool[j];
+      rank += o > hyp || (o == hyp && j < tid);
+    }
+    if (rank < W) {
+      const bool any = hyp > -INFINITY;
+      a.out_finished_scores[first + rank] = hyp;
+      a.out_finished_beams[first + rank] = any ? hyp_beam : -1;
+      a.out_finished_token_ids[first + rank] = any ? hyp_token : -1;
+      a.out_finished_lengths[first + rank] = any ? hyp_len : 0;
+      if (rank == W - 1) sm.worst = hyp;  // the worst one kept
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const float worst = sm.worst;
+    const bool full = worst > -INFINITY;
+    const float reach = (float)((double)next_best / power);
+    const bool over = going == 0 || (full && (a.early_stopping || worst >= reach));
+    a.out_lengths[g] = new_len;
+    a.out_done[g] = over ? 1 : 0;
+  }
+}
+
+// ------------------------------------------------------------------ launches ---------
+
+int64_t beam_workspace_bytes(int64_t G, int64_t W, int64_t V, int64_t C) {
+  if (G <= 0 || W <= 0 || V <= 0) return 0;
+  const int64_t rows = G * W;
+  const int64_t chunk = beam_chunk(rows, V, C), nch = (V + chunk - 1) / chunk;
+  // the scan's threads stay below 2^32
+  if (rows * nch >= (1ll << 24)) return 0;
+  return rows * nch * (int64_t)(sizeof(float2) + kTops * sizeof(float));
+}
+
+template <int DT>
+static void launch_dt(const BeamScanParams& p, const BeamSelectOut* o,
+                      const mvsd_beam_step_args* a, int chunk, hipStream_t stream) {
+  constexpr int kLong = kBeamLong / (kThreads * Elem<DT>::kVec);
+  constexpr int kShort = kBeamShort / (kThreads * Elem<DT>::kVec);
+  const dim3 scan((unsigned)(p.G * p.W) * (unsigned)p.nchunks), groups(p.G);
+  if (chunk == kBeamLong) {
+    hipLaunchKernelGGL((beam_scan_kernel<DT, kLong>), scan, dim3(kThreads), 0, stream, p);
+    if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *o);
+    else hipLaunchKernelGGL((beam_step_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *a);
+  } else {
+    hipLaunchKernelGGL((beam_scan_kernel<DT, kShort>), scan, dim3(kThreads), 0, stream, p);
+    if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *o);
+    else hipLaunchKernelGGL((beam_step_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *a);
+  }
+}
+
+static hipError_t launch(BeamScanParams p, const BeamSelectOut* o, const mvsd_beam_step_args* a,
+                         int dtype, void* workspace, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.G * p.W;
+  const int chunk = beam_chunk(rows, p.V, p.C);
+  p.nchunks = (int)(((int64_t)p.V + chunk - 1) / chunk);
+  p.stats = static_cast<float2*>(workspace);
+  p.tops = reinterpret_cast<float*>(p.stats + rows * p.nchunks);
+  switch (dtype) {
+    case MVSD_F32: launch_dt<MVSD_F32>(p, o, a, chunk, stream); break;
+    case MVSD_BF16: launch_dt<MVSD_BF16>(p, o, a, chunk, stream); break;
+    case MVSD_F16: launch_dt<MVSD_F16>(p, o, a, chunk, stream); break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_beam_select(BeamScanParams p, const BeamSelectOut& out, int dtype,
+                              void* workspace, hipStream_t stream) {
+  return launch(p, &out, nullptr, dtype, workspace, stream);
+}
+
+hipError_t launch_beam_step(BeamScanParams p, const mvsd_beam_step_args& a, void* workspace,
+                            hipStream_t stream) {
+  return launch(p, nullptr, &a, a.dtype, workspace, stream);
+}
+
+}  // namespace mvsd

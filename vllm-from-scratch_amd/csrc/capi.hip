@@ -6,9 +6,11 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
+#include "beam.h"
 #include "mvsd_device.h"
 #include "rows.h"
 #include "sampler.h"
@@ -412,6 +414,79 @@ int static_scratch_for_current_device(void** out, hipStream_t stream) {
     st.ptr[device] = ptr;
   }
   *out = st.ptr[device];
+  return MVSD_OK;
+}
+
+// State tensors of one mvsd_beam_reorder call.
+constexpr int64_t kMaxStatesPerCall = 512;
+
+// The bytes [lo, hi) that one side of a state spans: rows of `row` bytes, `stride` apart.
+struct StateSpan {
+  uintptr_t lo, hi;
+  int64_t row, stride;
+  bool written;
+};
+
+StateSpan state_span(const void* p, const mvsd_beam_state& s, int64_t stride, bool written) {
+  const int64_t row = s.outer * s.length * s.inner;
+  const uintptr_t lo = (uintptr_t)p;
+  return {lo, lo + (uintptr_t)((s.num_rows - 1) * stride + row), row, stride, written};
+}
+
+// Rows of equal strides may interleave (keys and values of one tensor); others that span common
+// bytes count as overlapping.
+bool spans_overlap(const StateSpan& a, const StateSpan& b) {
+  if (a.row == 0 || b.row == 0 || a.hi <= b.lo || b.hi <= a.lo) return false;
+  if (a.stride != b.stride || a.stride <= 0) return true;
+  const uintptr_t d = (a.lo >= b.lo ? a.lo - b.lo : b.lo - a.lo) % (uintptr_t)a.stride;
+  const int64_t early = a.lo >= b.lo ? b.row : a.row, late = a.lo >= b.lo ? a.row : b.row;
+  return !((int64_t)d >= early && (int64_t)d + late <= a.stride);
+}
+
+// Whether what one thread writes is what another reads or writes: sorted by their first byte, only
+// spans that begin before an earlier one ends are compared.
+bool states_overlap(const mvsd_beam_state* states, int n, bool in_place) {
+  StateSpan span[2 * kMaxStatesPerCall];
+  int m = 0;
+  for (int k = 0; k < n; ++k) {
+    span[m++] = state_span(states[k].dst, states[k], states[k].dst_stride, true);
+    if (!in_place) span[m++] = state_span(states[k].src, states[k], states[k].src_stride, false);
+  }
+  std::sort(span, span + m, [](const StateSpan& a, const StateSpan& b) { return a.lo < b.lo; });
+  for (int i = 0; i < m; ++i)
+    for (int j = i + 1; j < m && span[j].lo < span[i].hi; ++j)
+      if ((span[i].written || span[j].written) && spans_overlap(span[i], span[j])) return true;
+  return false;
+}
+
+// The arguments that beam_select and beam_step share, checked.
+int beam_scan_params(mvsd::BeamScanParams* p, const void* logits, int dtype, int64_t stride,
+                     int64_t num_rows, const int32_t* target_rows, const float* scores,
+                     int64_t num_groups, int64_t beam_width, int64_t vocab_size,
+                     int64_t num_candidates, const void* workspace, int64_t workspace_bytes) {
+  if (num_groups < 0 || beam_width < 1 || vocab_size < 1 || num_candidates < 1)
+    return MVSD_E_INVALID;
+  if (beam_width > mvsd::kMaxBeams || num_candidates > mvsd::kMaxCandidates ||
+      vocab_size > 0x7fffffff || num_groups > 0x7fffffff / mvsd::kMaxBeams)
+    return MVSD_E_RANGE;
+  if (dtype != MVSD_F32 && dtype != MVSD_BF16 && dtype != MVSD_F16) return MVSD_E_INVALID;
+  if (num_groups == 0) return MVSD_OK;
+  if (!logits || !scores || num_rows < 1 || stride < 0) return MVSD_E_INVALID;
+  if (!target_rows && num_rows < num_groups * beam_width) return MVSD_E_INVALID;
+  const int64_t need =
+      mvsd::beam_workspace_bytes(num_groups, beam_width, vocab_size, num_candidates);
+  if (need == 0) return MVSD_E_RANGE;
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
+    return MVSD_E_WORKSPACE;
+  p->logits = logits;
+  p->stride = stride;
+  p->num_rows = num_rows;
+  p->rows = target_rows;
+  p->scores = scores;
+  p->G = (int)num_groups;
+  p->W = (int)beam_width;
+  p->V = (int)vocab_size;
+  p->C = (int)num_candidates;
   return MVSD_OK;
 }
 
@@ -965,6 +1040,118 @@ int mvsd_ngram_propose_split(int32_t* drafts, int32_t* num_valid, int32_t* token
   p.cap_by_model_len = cap_by_model_len ? 1 : 0;
   p.max_model_len = max_model_len;
   return hip_status(mvsd::launch_ngram(p, num_reqs, workspace, (hipStream_t)stream));
+}
+
+int64_t mvsd_beam_workspace_bytes(int64_t num_groups, int64_t beam_width, int64_t vocab_size,
+                                  int64_t num_candidates) {
+  if (num_groups < 0 || beam_width < 1 || beam_width > mvsd::kMaxBeams || vocab_size < 1 ||
+      vocab_size > 0x7fffffff || num_candidates < 1 || num_candidates > mvsd::kMaxCandidates ||
+      num_groups > 0x7fffffff / mvsd::kMaxBeams)
+    return 0;
+  return mvsd::beam_workspace_bytes(num_groups, beam_width, vocab_size, num_candidates);
+}
+
+int mvsd_beam_select(int32_t* token_ids, int32_t* parents, float* out_scores, const void* logits,
+                     int dtype, int64_t stride, int64_t num_rows, const int32_t* target_rows,
+                     const float* scores, int64_t num_groups, int64_t beam_width,
+                     int64_t vocab_size, int64_t num_candidates, void* workspace,
+                     int64_t workspace_bytes, mvsd_stream_t stream) {
+  mvsd::BeamScanParams p{};
+  const int status = beam_scan_params(&p, logits, dtype, stride, num_rows, target_rows, scores,
+                                      num_groups, beam_width, vocab_size, num_candidates,
+                                      workspace, workspace_bytes);
+  if (status != MVSD_OK || num_groups == 0) return status;
+  if (!token_ids || !parents || !out_scores) return MVSD_E_INVALID;
+  const mvsd::BeamSelectOut o{token_ids, parents, out_scores};
+  return hip_status(mvsd::launch_beam_select(p, o, dtype, workspace, (hipStream_t)stream));
+}
+
+int mvsd_beam_step(const mvsd_beam_step_args* a, mvsd_stream_t stream) {
+  if (!a || a->max_length < 1 || a->num_stop_ids < 0) return MVSD_E_INVALID;
+  if (a->max_length > 0x7fffffff || a->num_stop_ids >= mvsd::kMaxCandidates) return MVSD_E_RANGE;
+  mvsd::BeamScanParams p{};
+  const int status = beam_scan_params(&p, a->logits, a->dtype, a->stride, a->num_rows,
+                                      a->target_rows, a->scores, a->num_groups, a->beam_width,
+                                      a->vocab_size, a->beam_width * (1 + a->num_stop_ids),
+                                      a->workspace, a->workspace_bytes);
+  if (status != MVSD_OK || a->num_groups == 0) return status;
+  if (!a->lengths || !a->done || !a->finished_scores || !a->finished_beams ||
+      !a->finished_token_ids || !a->finished_lengths || !a->out_scores || !a->out_lengths ||
+      !a->out_done || !a->out_finished_scores || !a->out_finished_beams ||
+      !a->out_finished_token_ids || !a->out_finished_lengths || !a->token_history ||
+      !a->parent_history || !a->token_ids || !a->parents ||
+      (a->num_stop_ids > 0 && !a->stop_token_ids))
+    return MVSD_E_INVALID;
+  p.lengths = a->lengths;
+  p.done = a->done;
+  p.max_length = (int)a->max_length;
+  return hip_status(mvsd::launch_beam_step(p, *a, a->workspace, (hipStream_t)stream));
+}
+
+int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const int32_t* parents,
+                      const int32_t* starts, const int32_t* lengths, const int32_t* slots,
+                      int64_t num_groups, int64_t beam_width, mvsd_stream_t stream) {
+  if (num_states < 0 || num_groups < 0 || beam_width < 1) return MVSD_E_INVALID;
+  if (beam_width > mvsd::kMaxBeams || num_groups > 0x7fffffff / mvsd::kMaxBeams)
+    return MVSD_E_RANGE;
+  if (num_states == 0 || num_groups == 0) return MVSD_OK;
+  if (!states || !parents) return MVSD_E_INVALID;
+  if (num_states > kMaxStatesPerCall) return MVSD_E_RANGE;
+  const bool in_place = states[0].src == states[0].dst;
+  for (int64_t k = 0; k < num_states; ++k) {
+    const mvsd_beam_state& s = states[k];
+    if (!s.src || !s.dst || s.num_rows < 1 || s.outer < 0 || s.length < 0 || s.inner < 0)
+      return MVSD_E_INVALID;
+    // a row stays below 2^31 sixteen-byte units (sizes first, so that the products cannot overflow)
+    const int64_t most = 1ll << 35;
+    if (s.num_rows > 0x7fffffff || s.length > 0x7fffffff || s.inner > most || s.outer > most ||
+        (s.inner > 0 && s.length > most / s.inner) ||
+        (s.inner * s.length > 0 && s.outer > most / (s.inner * s.length)))
+      return MVSD_E_RANGE;
+    const int64_t row = s.outer * s.length * s.inner;
+    if (s.num_rows > 1 && (s.src_stride < row || s.dst_stride < row)) return MVSD_E_INVALID;
+    if (s.src_stride > (1ll << 32) * 64 || s.dst_stride > (1ll << 32) * 64) return MVSD_E_RANGE;
+    if (!slots && s.num_rows < num_groups * beam_width) return MVSD_E_INVALID;
+    if (in_place != (s.src == s.dst) || (in_place && s.src_stride != s.dst_stride))
+      return MVSD_E_INVALID;
+  }
+  if (states_overlap(states, (int)num_states, in_place)) return MVSD_E_INVALID;
+  mvsd::BeamStatesParams p{};
+  p.parents = parents;
+  p.starts = starts;
+  p.lengths = lengths;
+  p.slots = slots;
+  p.W = (int)beam_width;
+  // blocks: one row of the grid per (group, state), at most 65535 rows
+  const int64_t groups = 65535 / mvsd::kMaxBeamStates;
+  for (int64_t k = 0; k < num_states; k += mvsd::kMaxBeamStates) {
+    p.n = 0;
+    for (int64_t j = k; j < num_states && p.n < mvsd::kMaxBeamStates; ++j)
+      if (states[j].outer * states[j].length * states[j].inner > 0) p.state[p.n++] = states[j];
+    if (p.n == 0) continue;
+    for (int64_t g = 0; g < num_groups; g += groups) {
+      p.first_group = g;
+      p.G = (int)(num_groups - g < groups ? num_groups - g : groups);
+      const int status = hip_status(mvsd::launch_beam_reorder(p, in_place, (hipStream_t)stream));
+      if (status != MVSD_OK) return status;
+    }
+  }
+  return MVSD_OK;
+}
+
+int mvsd_beam_finish(const mvsd_beam_finish_args* a, mvsd_stream_t stream) {
+  if (!a || a->num_groups < 0 || a->beam_width < 1 || a->max_length < 1 || a->num_return < 1 ||
+      a->num_return > a->beam_width)
+    return MVSD_E_INVALID;
+  if (a->beam_width > mvsd::kMaxBeams || a->max_length > 0x7fffffff / mvsd::kMaxBeams ||
+      a->num_groups > 0x7fffffff / mvsd::kMaxBeams)
+    return MVSD_E_RANGE;
+  if (a->num_groups == 0) return MVSD_OK;
+  if (!a->scores || !a->lengths || !a->done || !a->finished_scores || !a->finished_beams ||
+      !a->finished_token_ids || !a->finished_lengths || !a->token_history ||
+      !a->parent_history || !a->out_token_ids || !a->out_lengths || !a->out_scores)
+    return MVSD_E_INVALID;
+  return hip_status(mvsd::launch_beam_finish(*a, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -75,6 +75,70 @@ class RejectionArgs(ctypes.Structure):
     ]
 
 
+class BeamStepArgs(ctypes.Structure):
+    """Mirror of ``mvsd_beam_step_args``."""
+
+    _fields_ = [
+        ("logits", c_void_p),
+        ("stride", c_int64),
+        ("num_rows", c_int64),
+        ("target_rows", c_void_p),
+        ("num_groups", c_int64),
+        ("beam_width", c_int64),
+        ("vocab_size", c_int64),
+        ("max_length", c_int64),
+        ("stop_token_ids", c_void_p),
+        ("num_stop_ids", c_int64),
+        ("length_penalty", c_double),
+        ("dtype", c_int),
+        ("early_stopping", c_int),
+        ("scores", c_void_p),
+        ("lengths", c_void_p),
+        ("done", c_void_p),
+        ("finished_scores", c_void_p),
+        ("finished_beams", c_void_p),
+        ("finished_token_ids", c_void_p),
+        ("finished_lengths", c_void_p),
+        ("out_scores", c_void_p),
+        ("out_lengths", c_void_p),
+        ("out_done", c_void_p),
+        ("out_finished_scores", c_void_p),
+        ("out_finished_beams", c_void_p),
+        ("out_finished_token_ids", c_void_p),
+        ("out_finished_lengths", c_void_p),
+        ("token_history", c_void_p),
+        ("parent_history", c_void_p),
+        ("token_ids", c_void_p),
+        ("parents", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
+class BeamFinishArgs(ctypes.Structure):
+    """Mirror of ``mvsd_beam_finish_args``."""
+
+    _fields_ = [
+        ("num_groups", c_int64),
+        ("beam_width", c_int64),
+        ("max_length", c_int64),
+        ("num_return", c_int64),
+        ("length_penalty", c_double),
+        ("scores", c_void_p),
+        ("lengths", c_void_p),
+        ("done", c_void_p),
+        ("finished_scores", c_void_p),
+        ("finished_beams", c_void_p),
+        ("finished_token_ids", c_void_p),
+        ("finished_lengths", c_void_p),
+        ("token_history", c_void_p),
+        ("parent_history", c_void_p),
+        ("out_token_ids", c_void_p),
+        ("out_lengths", c_void_p),
+        ("out_scores", c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/mvsd.h declares
 SIGNATURES = {
     "mvsd_version": (c_int, []),
@@ -163,6 +227,15 @@ SIGNATURES = {
     "mvsd_topk_scores_split": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
                                        c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p,
                                        c_int64, c_void_p]),
+    "mvsd_beam_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
+    "mvsd_beam_select": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,
+                                 c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                 c_void_p, c_int64, c_void_p]),
+    "mvsd_beam_step": (c_int, [ctypes.POINTER(BeamStepArgs), c_void_p]),
+    # the states: an array of mvsd_beam_state, eight int64 each
+    "mvsd_beam_reorder": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_int64, c_int64, c_void_p]),
+    "mvsd_beam_finish": (c_int, [ctypes.POINTER(BeamFinishArgs), c_void_p]),
     "mvsd_ngram_valid_sampled": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                          c_int64, c_int64, c_void_p, c_void_p, c_int64,
                                          c_void_p, c_int64, c_int64, c_void_p]),

@@ -1,0 +1,431 @@
+"""Beam search on the device: selection over beams and vocabulary, a whole decoding step, the
+reordering of the beams' states and the answers (csrc/beam.hip, csrc/beam_states.hip; C ABI
+``mvsd_beam_select``, ``mvsd_beam_step``, ``mvsd_beam_reorder``, ``mvsd_beam_finish``).
+
+The reference has no beam search; this stands beside ``Sampler`` for requests that want the most
+probable sequences.  A group is one request with W beams (1..64), G groups a batch, the rows of a
+group's beams in the order g * W + w.
+
+    search = BeamSearch(G, W, max_length, device, stop_token_ids=[eos])
+    logits = prefill(...)                       # a row a beam (the first beam's counts)
+    while not all_done:
+        step = search.step(logits)              # step.token_ids, step.parents [G, W]
+        search.reorder(caches, lengths=...)     # the beams' states follow their parents
+        logits = decode(step.token_ids, caches)
+    answers = search.finish(n)                  # token ids, lengths and scores of the n best
+
+Nothing here synchronises the host.  Work is enqueued on the current stream of the logits' (or
+states') device; scratch comes from torch's allocator within the call, so calls on several streams
+and captured graphs share nothing.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, fields
+
+import torch
+
+from .. import _native as nat
+
+PLACEHOLDER_TOKEN_ID = -1
+MAX_BEAMS = 64
+MAX_CANDIDATES = 256
+
+_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+@dataclass
+class BeamCandidates:
+    """The best continuations of every group, best first; [G, C] each.  Places without one:
+    token and parent -1, score -inf."""
+
+    token_ids: torch.Tensor  # int32
+    parents: torch.Tensor    # int32, the beam (0..W-1) that each continues
+    scores: torch.Tensor     # fp32, summed log-probabilities
+
+
+@dataclass
+class BeamState:
+    """A search under way.  ``finished_*`` hold each group's W best finished hypotheses, best first
+    (none: score -inf, -1, -1, 0): a hypothesis is its last token (``finished_token_ids``) appended
+    to a beam (``finished_beams``) of the step before, ``finished_lengths`` tokens in all.
+    ``token_history`` and ``parent_history`` hold what every step gave each beam."""
+
+    scores: torch.Tensor              # fp32 [G, W], -inf: no beam
+    lengths: torch.Tensor             # int32 [G], steps taken = tokens of the running beams
+    done: torch.Tensor                # bool [G]
+    finished_scores: torch.Tensor     # fp32 [G, W], divided by length ** length_penalty
+    finished_beams: torch.Tensor      # int32 [G, W]
+    finished_token_ids: torch.Tensor  # int32 [G, W]
+    finished_lengths: torch.Tensor    # int32 [G, W]
+    token_history: torch.Tensor       # int32 [G, max_length, W]
+    parent_history: torch.Tensor      # int32 [G, max_length, W]
+
+    @classmethod
+    def new(cls, num_groups: int, beam_width: int, max_length: int, device) -> "BeamState":
+        """Before the first step: beam 0 of every group holds the prompt."""
+        G, W = num_groups, beam_width
+
+        def full(value, dtype, *shape):
+            return torch.full(shape, value, dtype=dtype, device=device)
+
+        scores = full(-float("inf"), torch.float32, G, W)
+        scores[:, 0] = 0.0
+        return cls(scores, full(0, torch.int32, G), full(False, torch.bool, G),
+                   full(-float("inf"), torch.float32, G, W), full(-1, torch.int32, G, W),
+                   full(-1, torch.int32, G, W), full(0, torch.int32, G, W),
+                   full(-1, torch.int32, G, max_length, W),
+                   full(-1, torch.int32, G, max_length, W))
+
+
+@dataclass
+class BeamStep:
+    """What the model runs next: [G, W] each, -1 where a group rests or has no such beam."""
+
+    token_ids: torch.Tensor  # int32
+    parents: torch.Tensor    # int32, the beam of the step before that each one continues
+    state: BeamState
+
+
+@dataclass
+class BeamHypotheses:
+    """The best answers of every group, best first."""
+
+    token_ids: torch.Tensor  # int32 [G, n, max_length], -1 behind a sequence
+    lengths: torch.Tensor    # int32 [G, n], 0: no such answer
+    scores: torch.Tensor     # fp32 [G, n], -inf: no such answer
+
+
+_STATE_FIELDS = tuple(f.name for f in fields(BeamState))
+_STATE_DTYPES = {"scores": torch.float32, "done": torch.bool, "finished_scores": torch.float32}
+_HISTORIES = ("token_history", "parent_history")
+
+
+def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}, {dtype} expected")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, {tuple(shape)} expected")
+    if t.device != device:
+        nat.require_device_tensor(t, name)
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+
+
+def _check_state(state: BeamState, name: str, device) -> tuple[int, int, int]:
+    """(G, W, max_length) of a state whose every tensor fits them."""
+    history = state.token_history
+    if history.ndim != 3:
+        raise ValueError(f"{name}.token_history is not [G, max_length, W]")
+    G, T, W = history.shape
+    if T < 1:
+        raise ValueError(f"{name} has max_length 0")
+    shapes = {"lengths": (G,), "done": (G,), "token_history": (G, T, W),
+              "parent_history": (G, T, W)}
+    for field in _STATE_FIELDS:
+        _check_array(getattr(state, field), f"{name}.{field}",
+                     _STATE_DTYPES.get(field, torch.int32), shapes.get(field, (G, W)), device)
+    return G, W, T
+
+
+def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.device:
+    nat.require_device_tensor(logits, "logits")
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"{W} beams: 1 to {MAX_BEAMS} are supported")
+    if logits.ndim != 2 or logits.dtype not in _ROW_DTYPES:
+        raise TypeError("logits are 2-D fp32, bf16 or fp16 rows")
+    V = logits.shape[1]
+    if V < 1:
+        raise ValueError("logits without columns")
+    if logits.stride(1) != 1 and V > 1:
+        raise ValueError("logits need rows with unit stride")
+    device = logits.device
+    if target_rows is None:
+        if logits.shape[0] < G * W:
+            raise ValueError(f"{logits.shape[0]} logits rows for {G} groups of {W} beams")
+    else:
+        if target_rows.numel() != G * W:
+            raise ValueError(f"{target_rows.numel()} row indices for {G} groups of {W} beams")
+        _check_array(target_rows, "target_rows", torch.int32, target_rows.shape, device)
+        if logits.shape[0] < 1 and G > 0:
+            raise ValueError("row indices into logits without rows")
+    return device
+
+
+def _workspace(G: int, W: int, V: int, C: int, device) -> torch.Tensor:
+    size = nat.lib().mvsd_beam_workspace_bytes(G, W, V, C)
+    if size <= 0:
+        raise ValueError(f"{G} groups of {W} beams over {V} tokens are more than one call takes")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+class _on:
+    """Makes `device` the current one where it is not (launches go to the current device)."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
+def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int, *,
+                       target_rows: torch.Tensor | None = None) -> BeamCandidates:
+    """The ``num_candidates`` (1..256) best continuations of every group.
+
+    ``scores [G, W]`` fp32 are the beams' summed log-probabilities, ``logits`` their rows (fp32,
+    bf16 or fp16, any row stride): row g * W + w, or ``target_rows [G, W]`` (int32) into a larger
+    tensor (indices outside it read its nearest row).  Candidate (beam, token) has the score
+    ``scores[beam] + log_softmax(row)[token]``, formed and compared in 64 bits and returned in fp32;
+    the order is score descending, beam ascending, logit descending, token ascending.  A beam whose
+    score is not finite, or whose row is -inf throughout or holds a NaN or +inf, proposes nothing;
+    tokens at -inf are no candidates.
+    """
+    if scores.ndim != 2:
+        raise ValueError("scores are [G, W]")
+    G, W = scores.shape
+    device = _check_rows(logits, G, W, target_rows)
+    _check_array(scores, "scores", torch.float32, scores.shape, device)
+    C = int(num_candidates)
+    if not 1 <= C <= MAX_CANDIDATES:
+        raise ValueError(f"num_candidates={C}: 1 to {MAX_CANDIDATES} are supported")
+    with _on(device):
+        ids = torch.empty((3, G, C), dtype=torch.int32, device=device)
+        out = BeamCandidates(ids[0], ids[1], ids[2].view(torch.float32))
+        if G == 0:
+            return out
+        V = logits.shape[1]
+        ws = _workspace(G, W, V, C, device)
+        base = ids.data_ptr()
+        nat.check(nat.lib().mvsd_beam_select(
+            base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
+            nat.dtype_code(logits.dtype), logits.stride(0), logits.shape[0],
+            nat.ptr(target_rows), scores.data_ptr(), G, W, V, C, ws.data_ptr(), ws.numel(),
+            nat.stream_of(device)), "mvsd_beam_select")
+    return out
+
+
+def beam_search_step(logits: torch.Tensor, state: BeamState, *,
+                     stop_token_ids: torch.Tensor | None = None, length_penalty: float = 1.0,
+                     early_stopping: bool = False, target_rows: torch.Tensor | None = None,
+                     out: BeamState | None = None) -> BeamStep:
+    """One decoding step of every group that is not done and has fewer than ``max_length`` tokens.
+
+    With the candidates of :func:`beam_search_select` and L = length + 1:
+
+    * stop tokens (``stop_token_ids``, int32 on the device, W * (1 + their number) <= 256) among the
+      W best candidates end a hypothesis with score ``sum / L ** length_penalty``; each group keeps
+      its W best, an earlier one first where they are equal;
+    * the W best candidates that are no stop tokens are the next beams, also recorded in the
+      histories;
+    * the group is done when no beam is left, or when W hypotheses are finished and, unless
+      ``early_stopping``, the worst of them is at least the best running sum / L ** length_penalty.
+
+    Other groups stay as they are (token_ids and parents -1).  The new state is written to ``out``
+    (another :class:`BeamState` with the same histories), or to ``state`` itself.
+    """
+    device = logits.device
+    nat.require_device_tensor(logits, "logits")
+    G, W, T = _check_state(state, "state", device)
+    _check_rows(logits, G, W, target_rows)
+    if out is None:
+        out = state
+    elif out is not state:
+        _check_state(out, "out", device)
+        for name in _HISTORIES:
+            if getattr(out, name).data_ptr() != getattr(state, name).data_ptr():
+                raise ValueError(f"out.{name} is another tensor than state.{name}")
+        if out.scores.shape != state.scores.shape:
+            raise ValueError("out has another shape than state")
+    E = 0
+    if stop_token_ids is not None:
+        E = stop_token_ids.numel()
+        _check_array(stop_token_ids, "stop_token_ids", torch.int32, (E,), device)
+    C = W * (1 + E)
+    if C > MAX_CANDIDATES:
+        raise ValueError(f"{W} beams with {E} stop tokens: W * (1 + E) is over {MAX_CANDIDATES}")
+    with _on(device):
+        ids = torch.empty((2, G, W), dtype=torch.int32, device=device)
+        step = BeamStep(ids[0], ids[1], out)
+        if G == 0:
+            return step
+        V = logits.shape[1]
+        ws = _workspace(G, W, V, C, device)
+        base = ids.data_ptr()
+        args = nat.BeamStepArgs(
+            logits.data_ptr(), logits.stride(0), logits.shape[0], nat.ptr(target_rows), G, W, V,
+            T, nat.ptr(stop_token_ids), E, float(length_penalty), nat.dtype_code(logits.dtype),
+            int(bool(early_stopping)), state.scores.data_ptr(), state.lengths.data_ptr(),
+            state.done.data_ptr(), state.finished_scores.data_ptr(),
+            state.finished_beams.data_ptr(), state.finished_token_ids.data_ptr(),
+            state.finished_lengths.data_ptr(), out.scores.data_ptr(), out.lengths.data_ptr(),
+            out.done.data_ptr(), out.finished_scores.data_ptr(), out.finished_beams.data_ptr(),
+            out.finished_token_ids.data_ptr(), out.finished_lengths.data_ptr(),
+            state.token_history.data_ptr(), state.parent_history.data_ptr(), base,
+            base + 4 * G * W, ws.data_ptr(), ws.numel())
+        nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), nat.stream_of(device)),
+                  "mvsd_beam_step")
+    return step
+
+
+def beam_search_finish(state: BeamState, num_return: int | None = None, *,
+                       length_penalty: float = 1.0) -> BeamHypotheses:
+    """The ``num_return`` (default W) best answers of every group: its finished hypotheses and, unless
+    the group is done, its running beams (sum / length ** length_penalty); finished ones first where
+    they are equal.  The sequences are read back from the histories; the state is left as it is."""
+    device = state.scores.device
+    nat.require_device_tensor(state.scores, "state.scores")
+    G, W, T = _check_state(state, "state", device)
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"{W} beams: 1 to {MAX_BEAMS} are supported")
+    n = W if num_return is None else int(num_return)
+    if not 1 <= n <= W:
+        raise ValueError(f"num_return={n}: 1 to {W} (the beams) are kept")
+    with _on(device):
+        ids = torch.empty((G, n, T), dtype=torch.int32, device=device)
+        two = torch.empty((2, G, n), dtype=torch.int32, device=device)
+        out = BeamHypotheses(ids, two[0], two[1].view(torch.float32))
+        if G == 0:
+            return out
+        args = nat.BeamFinishArgs(
+            G, W, T, n, float(length_penalty), state.scores.data_ptr(), state.lengths.data_ptr(),
+            state.done.data_ptr(), state.finished_scores.data_ptr(),
+            state.finished_beams.data_ptr(), state.finished_token_ids.data_ptr(),
+            state.finished_lengths.data_ptr(), state.token_history.data_ptr(),
+            state.parent_history.data_ptr(), ids.data_ptr(), two.data_ptr(),
+            two.data_ptr() + 4 * G * n)
+        nat.check(nat.lib().mvsd_beam_finish(ctypes.byref(args), nat.stream_of(device)),
+                  "mvsd_beam_finish")
+    return out
+
+
+def _state_rows(x: torch.Tensor, name: str, length_dim: int, device) -> tuple:
+    """(row stride in bytes, rows, pieces, length, bytes of an entry) of a state tensor."""
+    if x.device != device:
+        nat.require_device_tensor(x, name)
+        raise ValueError(f"{name} is on {x.device}, parents on {device}")
+    shape = x.shape
+    if not 1 <= length_dim < len(shape):
+        raise ValueError(f"{name} has no dimension {length_dim} behind its rows")
+    stride, expect = x.stride(), 1
+    for d in range(len(shape) - 1, 0, -1):
+        if stride[d] != expect and shape[d] > 1 and expect:
+            raise ValueError(f"{name} is not contiguous within a row")
+        expect *= shape[d]
+    if shape[0] > 1 and stride[0] < expect:
+        raise ValueError(f"{name} has overlapping rows")
+    outer = inner = 1
+    for d in range(1, length_dim):
+        outer *= shape[d]
+    for d in range(length_dim + 1, len(shape)):
+        inner *= shape[d]
+    size = x.element_size()
+    return stride[0] * size, shape[0], outer, shape[length_dim], inner * size
+
+
+def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None = None,
+                  lengths: torch.Tensor | None = None, length_dim: int = 1,
+                  slots: torch.Tensor | None = None, out=None):
+    """The states of the beams follow their parents: the row of beam (g, w) becomes what the row of
+    beam (g, ``parents[g, w]``) was before the call.
+
+    ``states`` is a tensor or a sequence of tensors (caches, token tables; any dtype), one row a
+    beam along dimension 0 -- row g * W + w, or ``slots [G, W]`` (int32, distinct) into a pool of
+    rows -- contiguous within a row, any row stride.  ``length_dim`` is the dimension of the
+    positions in all of them; only positions ``starts[g] <= t < lengths[g]`` (int32 [G]; default:
+    all) move, so a prompt that the beams of a group share can stay where it is.  A parent outside
+    0..W-1 (the -1 of a resting group) keeps the beam's own row; a slot outside the pool is left
+    alone.
+
+    Without ``out`` the states are reordered in place, in one pass and without a second buffer; with
+    ``out`` (tensors of the same shapes that share no memory with the states) the rows are written
+    there.  Returns the tensors written.  Nothing else is touched.
+    """
+    if parents.ndim != 2:
+        raise ValueError("parents are [G, W]")
+    nat.require_device_tensor(parents, "parents")
+    device = parents.device
+    G, W = parents.shape
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"{W} beams: 1 to {MAX_BEAMS} are supported")
+    _check_array(parents, "parents", torch.int32, (G, W), device)
+    if starts is not None:
+        _check_array(starts, "starts", torch.int32, (G,), device)
+    if lengths is not None:
+        _check_array(lengths, "lengths", torch.int32, (G,), device)
+    if slots is not None:
+        _check_array(slots, "slots", torch.int32, (G, W), device)
+    single = isinstance(states, torch.Tensor)
+    tensors = [states] if single else list(states)
+    targets = tensors if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    if len(targets) != len(tensors):
+        raise ValueError(f"{len(targets)} out tensors for {len(tensors)} states")
+    flat = []
+    for k, (x, to) in enumerate(zip(tensors, targets)):
+        stride, rows, outer, length, inner = _state_rows(x, f"states[{k}]", length_dim, device)
+        to_stride = stride
+        if to is not x:
+            if to.shape != x.shape or to.dtype != x.dtype:
+                raise ValueError(f"out[{k}] has another shape or dtype than states[{k}]")
+            to_stride = _state_rows(to, f"out[{k}]", length_dim, device)[0]
+        if slots is None and rows < G * W:
+            raise ValueError(f"states[{k}] has {rows} rows for {G} groups of {W} beams")
+        if rows and outer * length * inner:
+            flat += (x.data_ptr(), to.data_ptr(), stride, to_stride, rows, outer, length, inner)
+    n = len(flat) // 8
+    if n and G:
+        with _on(device):
+            status = nat.lib().mvsd_beam_reorder(
+                (ctypes.c_int64 * len(flat))(*flat), n, parents.data_ptr(), nat.ptr(starts),
+                nat.ptr(lengths), nat.ptr(slots), G, W, nat.stream_of(device))
+        if status == -1:
+            raise ValueError("the states (or out) share memory with each other")
+        nat.check(status, "mvsd_beam_reorder")
+    return targets[0] if single else targets
+
+
+class BeamSearch:
+    """A beam search of G requests: its state, step by step (see the module's example)."""
+
+    def __init__(self, num_groups: int, beam_width: int, max_length: int, device, *,
+                 stop_token_ids=(), length_penalty: float = 1.0, early_stopping: bool = False):
+        if not 1 <= beam_width <= MAX_BEAMS:
+            raise ValueError(f"{beam_width} beams: 1 to {MAX_BEAMS} are supported")
+        if max_length < 1:
+            raise ValueError("max_length is at least 1")
+        if beam_width * (1 + len(stop_token_ids)) > MAX_CANDIDATES:
+            raise ValueError(f"{beam_width} beams with {len(stop_token_ids)} stop tokens: "
+                             f"W * (1 + E) is over {MAX_CANDIDATES}")
+        self.state = BeamState.new(num_groups, beam_width, max_length, device)
+        self.stop_token_ids = torch.tensor(list(stop_token_ids), dtype=torch.int32, device=device)
+        self.length_penalty = float(length_penalty)
+        self.early_stopping = bool(early_stopping)
+        self.parents: torch.Tensor | None = None
+
+    def step(self, logits: torch.Tensor, target_rows: torch.Tensor | None = None) -> BeamStep:
+        """One step on the beams' logits (:func:`beam_search_step`); the state is updated."""
+        step = beam_search_step(logits, self.state, stop_token_ids=self.stop_token_ids,
+                                length_penalty=self.length_penalty,
+                                early_stopping=self.early_stopping, target_rows=target_rows)
+        self.parents = step.parents
+        return step
+
+    def reorder(self, states, **where):
+        """The states of the beams follow the last step's parents (:func:`reorder_beams`)."""
+        if self.parents is None:
+            raise RuntimeError("no step has been taken")
+        return reorder_beams(states, self.parents, **where)
+
+    def finish(self, num_return: int | None = None) -> BeamHypotheses:
+        """The best answers so far (:func:`beam_search_finish`)."""
+        return beam_search_finish(self.state, num_return, length_penalty=self.length_penalty)
