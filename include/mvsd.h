@@ -703,6 +703,8 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
 /* The tokens of a hypothesis of L tokens are its last token at L - 1 and, from t = L - 2     */
 /* down, token_history[g, t, b] with b the beam at step t: the hypothesis' own, then          */
 /* parent_history[g, t, b] (outside [0, W): b itself).                                        */
+/* workspace: mvsd_beam_finish_workspace_bytes() bytes (0: none needed), no initial contents  */
+/* needed; one per call in flight.                                                            */
 /* ------------------------------------------------------------------------------------ */
 typedef struct mvsd_beam_finish_args {
   int64_t num_groups;
@@ -722,8 +724,13 @@ typedef struct mvsd_beam_finish_args {
   int32_t* out_token_ids;
   int32_t* out_lengths;
   float* out_scores;
+  void* workspace;
+  int64_t workspace_bytes;
 } mvsd_beam_finish_args;
 
+
+int64_t mvsd_beam_finish_workspace_bytes(int64_t num_groups, int64_t beam_width,
+                                         int64_t max_length, int64_t num_return);
 int mvsd_beam_finish(const mvsd_beam_finish_args* args, mvsd_stream_t stream);
 
 #ifdef __cplusplus

@@ -104,6 +104,7 @@ def finish_args(**change):
         if kind is ctypes.c_void_p:
             setattr(a, name, P)
     a.num_groups, a.beam_width, a.max_length, a.num_return = 2, 4, 16, 4
+    a.workspace_bytes = 1 << 20
     for k, v in change.items():
         setattr(a, k, v)
     return a
@@ -113,8 +114,11 @@ def finish_args(**change):
     ({"num_groups": -1}, INVALID), ({"beam_width": 0}, INVALID), ({"num_return": 0}, INVALID),
     ({"num_return": 5}, INVALID), ({"max_length": 0}, INVALID), ({"max_length": 2 ** 31}, RANGE),
     ({"beam_width": 65}, RANGE), ({"num_groups": 2 ** 40}, RANGE), ({"num_groups": 0}, 0)]
+    + [({"max_length": 9000, "workspace": None}, WORKSPACE),
+       ({"max_length": 9000, "workspace_bytes": 9}, WORKSPACE),
+       ({"num_groups": 2 ** 23}, RANGE), ({"num_groups": 2 ** 12, "max_length": 2 ** 22}, RANGE)]
     + [({f: None}, INVALID) for f, kind in nat.BeamFinishArgs._fields_
-       if kind is ctypes.c_void_p])
+       if kind is ctypes.c_void_p and f != "workspace"])
 def test_finish_refusals(change, status):
     assert nat.lib().mvsd_beam_finish(ctypes.byref(finish_args(**change)), None) == status
     assert nat.lib().mvsd_beam_finish(None, None) == INVALID

@@ -50,6 +50,7 @@ struct BeamStatesParams {
 };
 
 hipError_t launch_beam_reorder(const BeamStatesParams& p, bool in_place, hipStream_t stream);
+int64_t beam_finish_workspace_bytes(int64_t G, int64_t W, int64_t T, int64_t n);
 hipError_t launch_beam_finish(const mvsd_beam_finish_args& a, hipStream_t stream);
 
 }  // namespace mvsd

@@ -126,23 +126,71 @@ hipError_t launch_beam_reorder(const BeamStatesParams& p, bool in_place, hipStre
 // running beam is its last token appended to its parent), the finished ones first where they are
 // equal; then each one's tokens, from the last step back: the token and the parent recorded in the
 // beam's place.  A parent outside [0, W) is the beam itself.
+//
+// With b_t the beam at step t, b_(t-1) = parent_t(b_t): a chain of T dependent reads.  The steps'
+// maps are composed instead.  A workgroup holds the parents of a chunk of steps in LDS, a byte each;
+//   - the chunk's sub-chunks of kSub steps are walked from every beam at once, which gives their maps;
+//   - the hypotheses go through the sub-chunks' maps, which gives their beam at the top of each;
+//   - every sub-chunk is walked again from there, all at once, and leaves the beam of each step, by
+//     which the tokens are gathered and the sequences written, coalesced.
+// Histories of one chunk take one launch.  Longer ones take two: the first leaves every chunk's map
+// and, for a hypothesis that ends in the chunk, its beam below it; the second starts from those.
 
-__global__ __launch_bounds__(kThreads) void beam_finish_hyps_kernel(mvsd_beam_finish_args a) {
+constexpr int kTThreads = 512;
+constexpr int kSub = 32;
+constexpr int kTraceLds = 56 * 1024;
+constexpr int kMapPiece = 4096;  // bytes of chunk maps held at a time
+enum { kTraceWhole, kTraceMaps, kTraceEmit };
+
+// Steps per chunk: the whole history where it fits LDS and is short, else 1024 steps or fewer.
+static int trace_chunk(int64_t W, int64_t n, int64_t T) {
+  if (T <= 4096 && T * (W + n) <= kTraceLds) return (int)T;
+  return W + n <= 48 ? 1024 : 384;
+}
+
+// Dynamic LDS: parents [S, W], beams [n, S], sub-chunk maps [nsub, W], tops [n, nsub] in bytes.
+static int trace_lds(int64_t W, int64_t n, int64_t S) {
+  const int64_t nsub = (S + kSub - 1) / kSub;
+  return (int)(((S + 3) / 4 * 4) * W + n * S + nsub * (W + n));
+}
+
+int64_t beam_finish_workspace_bytes(int64_t G, int64_t W, int64_t T, int64_t n) {
+  const int64_t S = trace_chunk(W, n, T), chunks = (T + S - 1) / S;
+  return chunks > 1 ? G * (chunks * W + n) : 0;
+}
+
+template <int MODE>
+__global__ __launch_bounds__(kTThreads) void beam_trace_kernel(mvsd_beam_finish_args a, int S,
+                                                                int chunks, uint8_t* maps,
+                                                                uint8_t* exits) {
   __shared__ float s_key[2 * kMaxBeams];
-  __shared__ int s_beam[kMaxBeams], s_token[kMaxBeams], s_len[kMaxBeams];
-  const int g = blockIdx.x, tid = threadIdx.x, W = (int)a.beam_width, n = (int)a.num_return;
-  const int64_t first = (int64_t)g * W, T = a.max_length;
+  __shared__ int s_token[kMaxBeams], s_len[kMaxBeams];
+  __shared__ uint8_t s_beam[kMaxBeams];
+  __shared__ int s_longest;
+  __shared__ uint8_t s_maps[MODE == kTraceEmit ? kMapPiece : 1];
+  extern __shared__ __align__(16) uint8_t lds[];
+  const int tid = threadIdx.x, W = (int)a.beam_width, n = (int)a.num_return;
+  const int64_t T = a.max_length;
+  const int64_t g = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - g * chunks);
+  const int64_t first = g * W;
+  const int nsub = (S + kSub - 1) / kSub;
+  uint8_t* parent = lds;
+  uint8_t* sub_map = parent + (int64_t)((S + 3) / 4 * 4) * W;
+  uint8_t* tops = sub_map + nsub * W;
+  uint8_t* beams = tops + n * nsub;
+  // ---- the n best hypotheses ----
   const int len = (int)min(max((int64_t)a.lengths[g], (int64_t)0), T);
-  if (tid < 2 * W) {
-    float v = -INFINITY;
-    if (tid < W) v = a.finished_scores[first + tid];
-    else if (a.done[g] == 0 && len > 0 && fabsf(a.scores[first + tid - W]) < INFINITY)
-      v = (float)((double)a.scores[first + tid - W] / pow((double)len, a.length_penalty));
-    s_key[tid] = v > -INFINITY ? v : -INFINITY;
-  }
+  if (tid == 0) s_longest = 0;
+  float v = -INFINITY;
+  if (tid < W) v = a.finished_scores[first + tid];
+  else if (tid < 2 * W && a.done[g] == 0 && len > 0 &&
+           fabsf(a.scores[first + tid - W]) < INFINITY)
+    v = (float)((double)a.scores[first + tid - W] / pow((double)len, a.length_penalty));
+  if (!(v > -INFINITY)) v = -INFINITY;
+  if (tid < 2 * W) s_key[tid] = v;
   __syncthreads();
   if (tid < 2 * W) {
-    const float v = s_key[tid];
     int rank = 0;
     for (int j = 0; j < 2 * W; ++j) rank += s_key[j] > v || (s_key[j] == v && j < tid);
     if (rank < n) {
@@ -153,41 +201,157 @@ __global__ __launch_bounds__(kThreads) void beam_finish_hyps_kernel(mvsd_beam_fi
           token = a.finished_token_ids[first + tid];
           l = (int)min(max((int64_t)a.finished_lengths[first + tid], (int64_t)0), T);
         } else {
-          const int64_t at = ((int64_t)g * T + len - 1) * W + tid - W;
+          const int64_t at = (g * T + len - 1) * W + tid - W;
           beam = a.parent_history[at];
           token = a.token_history[at];
           l = len;
         }
       }
-      a.out_scores[(int64_t)g * n + rank] = v;
-      a.out_lengths[(int64_t)g * n + rank] = l;
-      s_beam[rank] = beam >= 0 && beam < W ? beam : 0;
+      if (MODE != kTraceMaps && chunk == 0) {
+        a.out_scores[g * n + rank] = v;
+        a.out_lengths[g * n + rank] = l;
+      }
+      s_beam[rank] = (uint8_t)(beam >= 0 && beam < W ? beam : 0);
       s_token[rank] = token;
       s_len[rank] = l;
+      atomicMax(&s_longest, l);
     }
   }
   __syncthreads();
-  for (int h = 0; h < n; ++h) {
-    int32_t* out = a.out_token_ids + ((int64_t)g * n + h) * T;
-    for (int64_t t = s_len[h] + tid; t < T; t += kThreads) out[t] = -1;
+  // ---- the parents of the steps [c0, c0 + steps) that some hypothesis goes through ----
+  const int64_t c0 = (int64_t)chunk * S;
+  const int steps = (int)min(max((int64_t)s_longest - 1 - c0, (int64_t)0), (int64_t)S);
+  if (MODE == kTraceMaps && steps == 0) return;
+  {
+    const int32_t* from = a.parent_history + (g * T + c0) * W;
+    const int count = steps * W;
+    for (int i = tid * 4; i < count; i += kTThreads * 4) {
+      uint32_t four = 0;
+      int p[4];
+      if (i + 4 <= count) {
+        const u32x4 q = *reinterpret_cast<const u32x4_align4*>(from + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = (int)q[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = i + e < count ? from[i + e] : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((unsigned)p[e] >= (unsigned)W) p[e] = (i + e) % W;
+        four |= (uint32_t)p[e] << (8 * e);
+      }
+      *reinterpret_cast<uint32_t*>(parent + i) = four;
+    }
   }
+  __syncthreads();
+  // ---- the sub-chunks' maps ----
+  const int subs = (steps + kSub - 1) / kSub;
+  for (int i = tid; i < subs * W; i += kTThreads) {
+    const int s = i / W;
+    int b = i - s * W;
+    for (int t = min(steps, (s + 1) * kSub) - 1; t >= s * kSub; --t) b = parent[t * W + b];
+    sub_map[i] = (uint8_t)b;
+  }
+  __syncthreads();
+  if (MODE == kTraceMaps) {
+    // the whole chunk's map, and the hypotheses that end in it (at step len - 2)
+    if (tid < W) {
+      int b = tid;
+      for (int s = subs - 1; s >= 0; --s) b = sub_map[s * W + b];
+      maps[(g * chunks + chunk) * W + tid] = (uint8_t)b;
+    } else if (tid >= kTThreads / 2 && tid < kTThreads / 2 + n) {
+      const int h = tid - kTThreads / 2;
+      const int64_t end = (int64_t)s_len[h] - 2 - c0;
+      if (end >= 0 && end < S) {
+        int b = s_beam[h], t = (int)end;
+        for (; t >= 0 && (t + 1) % kSub != 0; --t) b = parent[t * W + b];
+        for (int s = (t + 1) / kSub - 1; s >= 0; --s) b = sub_map[s * W + b];
+        exits[g * n + h] = (uint8_t)b;
+      }
+    }
+    return;
+  }
+  // ---- each hypothesis' beam at the top of every sub-chunk ----
+  int b = 0;
+  int64_t end = -1;  // its last step, from c0
   if (tid < n) {
-    int32_t* out = a.out_token_ids + ((int64_t)g * n + tid) * T;
-    const int l = s_len[tid];
-    int slot = s_beam[tid];
-    if (l > 0) out[l - 1] = s_token[tid];
-    for (int t = l - 2; t >= 0; --t) {
-      const int64_t at = ((int64_t)g * T + t) * W + slot;
-      out[t] = a.token_history[at];
-      const int parent = a.parent_history[at];
-      if (parent >= 0 && parent < W) slot = parent;
+    b = s_beam[tid];
+    end = (int64_t)s_len[tid] - 2 - c0;
+    if (MODE == kTraceEmit && end >= S) b = exits[g * n + tid];
+  }
+  if (MODE == kTraceEmit) {
+    // down through the chunks above this one, a piece of their maps at a time
+    const int per = kMapPiece / W;
+    const int last = (int)((max((int64_t)s_longest - 2, (int64_t)0)) / S);  // uniform
+    for (int hi = last; hi > chunk; hi -= per) {
+      const int lo = max(chunk + 1, hi - per + 1);
+      const uint8_t* from = maps + (g * chunks + lo) * W;
+      for (int i = tid; i < (hi - lo + 1) * W; i += kTThreads) s_maps[i] = from[i];
+      __syncthreads();
+      if (tid < n && end >= S) {
+        const int mine = (int)((int64_t)(s_len[tid] - 2) / S) - 1;  // the first one below its own
+        for (int c = min(hi, mine); c >= lo; --c) b = s_maps[(c - lo) * W + b];
+      }
+      __syncthreads();
+    }
+  }
+  if (tid < n && end >= 0) {
+    int s = (int)(min(end, (int64_t)steps - 1) / kSub);
+    tops[tid * nsub + s] = (uint8_t)b;
+    if (s > 0) {
+      // the first one from the hypothesis' own last step
+      for (int t = (int)min(end, (int64_t)steps - 1); t >= s * kSub; --t) b = parent[t * W + b];
+      for (--s; s >= 0; --s) {
+        tops[tid * nsub + s] = (uint8_t)b;
+        b = sub_map[s * W + b];
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the beam of every step ----
+  for (int i = tid; i < subs * n; i += kTThreads) {
+    const int h = i / subs, s = i - h * subs;
+    const int64_t top = min((int64_t)s_len[h] - 2 - c0, (int64_t)(s + 1) * kSub - 1);
+    if (top < s * kSub) continue;
+    int at = tops[h * nsub + s];
+    for (int t = (int)min(top, (int64_t)steps - 1); t >= s * kSub; --t) {
+      beams[h * S + t] = (uint8_t)at;
+      at = parent[t * W + at];
+    }
+  }
+  __syncthreads();
+  // ---- the tokens ----
+  const int width = (int)min((int64_t)S, T - c0);
+  const int32_t* tokens = a.token_history + (g * T + c0) * W;
+  for (int h = 0; h < n; ++h) {
+    int32_t* out = a.out_token_ids + (g * n + h) * T + c0;
+    const int64_t end_h = (int64_t)s_len[h] - 2 - c0;
+    for (int t = tid; t < width; t += kTThreads) {
+      int32_t id = -1;
+      if (t <= end_h) id = tokens[(int64_t)t * W + beams[h * S + t]];
+      else if (t == end_h + 1 && s_len[h] > 0) id = s_token[h];
+      out[t] = id;
     }
   }
 }
 
 hipError_t launch_beam_finish(const mvsd_beam_finish_args& a, hipStream_t stream) {
-  hipLaunchKernelGGL(beam_finish_hyps_kernel, dim3((unsigned)a.num_groups), dim3(kThreads), 0,
-                     stream, a);
+  const int S = trace_chunk(a.beam_width, a.num_return, a.max_length);
+  const int chunks = (int)((a.max_length + S - 1) / S);
+  const int lds = trace_lds(a.beam_width, a.num_return, S);
+  const dim3 grid((unsigned)(a.num_groups * chunks)), block(kTThreads);
+  if (chunks == 1) {
+    hipLaunchKernelGGL((beam_trace_kernel<kTraceWhole>), grid, block, lds, stream, a, S, chunks,
+                       nullptr, nullptr);
+    return hipGetLastError();
+  }
+  uint8_t* maps = static_cast<uint8_t*>(a.workspace);
+  uint8_t* exits = maps + a.num_groups * chunks * a.beam_width;
+  hipLaunchKernelGGL((beam_trace_kernel<kTraceMaps>), grid, block, lds, stream, a, S, chunks, maps,
+                     exits);
+  hipLaunchKernelGGL((beam_trace_kernel<kTraceEmit>), grid, block, lds, stream, a, S, chunks, maps,
+                     exits);
   return hipGetLastError();
 }
 

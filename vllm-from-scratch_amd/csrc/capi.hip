@@ -1139,6 +1139,15 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
   return MVSD_OK;
 }
 
+int64_t mvsd_beam_finish_workspace_bytes(int64_t num_groups, int64_t beam_width,
+                                         int64_t max_length, int64_t num_return) {
+  if (num_groups < 0 || beam_width < 1 || beam_width > mvsd::kMaxBeams || max_length < 1 ||
+      num_return < 1 || num_return > beam_width || max_length > 0x7fffffff / mvsd::kMaxBeams ||
+      num_groups > 0x7fffffff / mvsd::kMaxBeams)
+    return 0;
+  return mvsd::beam_finish_workspace_bytes(num_groups, beam_width, max_length, num_return);
+}
+
 int mvsd_beam_finish(const mvsd_beam_finish_args* a, mvsd_stream_t stream) {
   if (!a || a->num_groups < 0 || a->beam_width < 1 || a->max_length < 1 || a->num_return < 1 ||
       a->num_return > a->beam_width)
@@ -1147,10 +1156,15 @@ int mvsd_beam_finish(const mvsd_beam_finish_args* a, mvsd_stream_t stream) {
       a->num_groups > 0x7fffffff / mvsd::kMaxBeams)
     return MVSD_E_RANGE;
   if (a->num_groups == 0) return MVSD_OK;
+  // one workgroup per group and chunk of at least 384 steps, 512 threads each: below 2^32 threads
+  if (a->num_groups * (a->max_length / 384 + 1) >= (1ll << 23)) return MVSD_E_RANGE;
   if (!a->scores || !a->lengths || !a->done || !a->finished_scores || !a->finished_beams ||
       !a->finished_token_ids || !a->finished_lengths || !a->token_history ||
       !a->parent_history || !a->out_token_ids || !a->out_lengths || !a->out_scores)
     return MVSD_E_INVALID;
+  const int64_t need = mvsd::beam_finish_workspace_bytes(a->num_groups, a->beam_width,
+                                                         a->max_length, a->num_return);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MVSD_E_WORKSPACE;
   return hip_status(mvsd::launch_beam_finish(*a, (hipStream_t)stream));
 }
 

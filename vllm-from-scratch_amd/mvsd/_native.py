@@ -136,6 +136,8 @@ class BeamFinishArgs(ctypes.Structure):
         ("out_token_ids", c_void_p),
         ("out_lengths", c_void_p),
         ("out_scores", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
     ]
 
 
@@ -235,6 +237,7 @@ SIGNATURES = {
     # the states: an array of mvsd_beam_state, eight int64 each
     "mvsd_beam_reorder": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_int64, c_int64, c_void_p]),
+    "mvsd_beam_finish_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "mvsd_beam_finish": (c_int, [ctypes.POINTER(BeamFinishArgs), c_void_p]),
     "mvsd_ngram_valid_sampled": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                          c_int64, c_int64, c_void_p, c_void_p, c_int64,

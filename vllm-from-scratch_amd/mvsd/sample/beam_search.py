@@ -297,13 +297,15 @@ def beam_search_finish(state: BeamState, num_return: int | None = None, *,
         out = BeamHypotheses(ids, two[0], two[1].view(torch.float32))
         if G == 0:
             return out
+        size = nat.lib().mvsd_beam_finish_workspace_bytes(G, W, T, n)
+        ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
         args = nat.BeamFinishArgs(
             G, W, T, n, float(length_penalty), state.scores.data_ptr(), state.lengths.data_ptr(),
             state.done.data_ptr(), state.finished_scores.data_ptr(),
             state.finished_beams.data_ptr(), state.finished_token_ids.data_ptr(),
             state.finished_lengths.data_ptr(), state.token_history.data_ptr(),
             state.parent_history.data_ptr(), ids.data_ptr(), two.data_ptr(),
-            two.data_ptr() + 4 * G * n)
+            two.data_ptr() + 4 * G * n, nat.ptr(ws), size)
         nat.check(nat.lib().mvsd_beam_finish(ctypes.byref(args), nat.stream_of(device)),
                   "mvsd_beam_finish")
     return out
