@@ -13,8 +13,8 @@
 //                       largest entry of every 16 lanes (a "top": 16 of them a chunk).
 //   beam_finish_kernel  one 512-thread workgroup per group:
 //     - lse_b in 64 bits from the chunks' sums;
-//     - theta, the C-th largest of the maxima of 512 disjoint unions of tops, as totals: at least C
-//       entries of the group reach it, so the candidates are among the entries that do, and these lie
+//     - theta, the C-th largest of the maxima of 512 disjoint unions of tops (64 for C <= 32), as
+//       totals: at least C entries of the group reach it, so the candidates are among the entries that do, and these lie
 //       under the tops that do (a few more than C);
 //     - per beam the logit that theta stands for (rounded down), so that tops and entries are compared
 //       as they are; the entries under the tops that reach it are gathered into LDS, their totals
@@ -37,6 +37,8 @@ constexpr int kFThreads = 512;
 constexpr int kFWaves = kFThreads / kWave;
 constexpr int kListCap = 2048;     // tops that reach theta
 constexpr int kCandCap = 1024;     // gathered entries
+constexpr int kHeld = 4;           // vectors of tops a thread keeps in registers
+constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 keys
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Columns per chunk: long ones, unless they leave compute units idle (fewer than 4 workgroups each)
@@ -132,26 +134,53 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
 
 // ------------------------------------------------------------------ finish -----------
 
+// Candidates in LDS, an array each.
+template <int N>
+struct Candidates {
+  double total[N];
+  float x[N];
+  int token[N], beam[N];
+};
+
 struct Candidate {
   double total;
   float x;
   int token, beam;
 };
 
-__device__ inline bool better(const Candidate& a, const Candidate& b) {
-  if (a.total != b.total) return a.total > b.total;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  if (a.x != b.x) return a.x > b.x;
-  return a.token < b.token;
+template <int N>
+__device__ inline Candidate get(const Candidates<N>& c, int i) {
+  return {c.total[i], c.x[i], c.token[i], c.beam[i]};
+}
+template <int N>
+__device__ inline void put(Candidates<N>& c, int i, const Candidate& o) {
+  c.total[i] = o.total;
+  c.x[i] = o.x;
+  c.token[i] = o.token;
+  c.beam[i] = o.beam;
+}
+
+// Whether candidate j of c comes before `mine` (equal totals are rare: the rest is read only then).
+template <int N>
+__device__ inline bool before(const Candidates<N>& c, int j, const Candidate& mine) {
+  const double t = c.total[j];
+  bool yes = t > mine.total;
+  if (t == mine.total) {
+    const int beam = c.beam[j], token = c.token[j];
+    const float x = c.x[j];
+    yes = beam != mine.beam ? beam < mine.beam : x != mine.x ? x > mine.x : token < mine.token;
+  }
+  return yes;
 }
 
 struct BeamSmem {
-  Candidate cand[kCandCap];
-  Candidate best[kMaxCandidates];  // the group's candidates in order
+  Candidates<kCandCap> cand;
+  Candidates<kMaxCandidates> best;  // the group's candidates in order
   int list[kListCap];
   __align__(16) float key[kFThreads];
+  __align__(16) float fold[kWave];
   double lse[kMaxBeams];
-  float score[kMaxBeams];
+  float score[kMaxBeams];  // -inf: proposes nothing
   float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
   int hist[256];
   int wave_cnt[kFWaves];
@@ -161,12 +190,6 @@ struct BeamSmem {
   uint32_t theta_key;
   float worst;
 };
-
-__device__ inline double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
-}
 
 // The C largest entries of one row, by (value desc, token asc), into cand[at ..]; returns how many.
 // Radix selection of the C-th largest key, eight bits at a time, then one pass for the entries
@@ -220,10 +243,7 @@ __device__ inline int row_largest(const typename Elem<DT>::storage* row, int V, 
     if (ordered_bits(x) > kth) {
       const int pos = atomicAdd(&sm.count, 1);
       if (pos < C) {
-        Candidate& o = sm.cand[at + pos];
-        o.x = x;
-        o.token = (int)i;
-        o.beam = beam;
+        put(sm.cand, at + pos, {0.0, x, (int)i, beam});
       }
     }
   }
@@ -245,10 +265,7 @@ __device__ inline int row_largest(const typename Elem<DT>::storage* row, int V, 
     }
     pos += __popcll(hit & ((1ull << lane) - 1ull));
     if (eq && pos < C) {
-      Candidate& o = sm.cand[at + pos];
-      o.x = x;
-      o.token = (int)i;
-      o.beam = beam;
+      put(sm.cand, at + pos, {0.0, x, (int)i, beam});
     }
     found = min(found + total, C);
     __syncthreads();
@@ -265,46 +282,94 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
   const int W = p.W, C = p.C, nch = p.nchunks;
   const int64_t first = (int64_t)g * W;
-  // ---- lse of every beam, one wave each ----
-  for (int w = wid; w < W; w += kFWaves) {
-    const float score = p.scores[first + w];
-    double lse = NAN;
+  // ---- the tops, four of one chunk at a time; the first ones stay in registers ----
+  const int per_row = nch * (kTops / 4), quads = W * per_row;
+  const float4* top4 = reinterpret_cast<const float4*>(p.tops + first * nch * kTops);
+  float4 held[kHeld];
+  int held_row[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int i = tid + k * kFThreads;
+    held_row[k] = i < quads ? i / per_row : -1;
+    held[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (i < quads) held[k] = top4[i];
+  }
+  // ---- lse of every beam: as many lanes each as there are, a power of two from 8 to 64 ----
+  const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
+  {
+    const int w = tid / lanes, l = tid & (lanes - 1);
+    const float score = w < W ? p.scores[first + w] : NAN;
+    float M = -INFINITY;
+    double s = 0.0;
     if (finite(score)) {
       const float2* st = p.stats + (first + w) * nch;
-      float m = -INFINITY;
-      for (int c = lane; c < nch; c += kWave) m = fmaxf(m, st[c].x);
-      const float M = wave_max(m);
-      double s = 0.0;
-      for (int c = lane; c < nch; c += kWave) {
+#pragma unroll 4
+      for (int c = l; c < nch; c += lanes) {
         const float2 v = st[c];
+        const float up = fmaxf(M, v.x);
         // a chunk of -inf alone adds its sum, 0 (NaN where it holds a NaN)
-        s += v.x == -INFINITY ? (double)v.y : (double)v.y * exp((double)v.x - (double)M);
+        if (up != -INFINITY) {
+          s = s * exp((double)M - (double)up) + (double)v.y * exp((double)v.x - (double)up);
+          M = up;
+        } else {
+          s += (double)v.y;
+        }
       }
-      s = wave_sum_f64(s);
-      lse = (double)M + log(s);
     }
-    if (lane == 0) {
-      const bool live = fabs(lse) < (double)INFINITY;
+    float all = M;
+    for (int off = lanes / 2; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor(all, off, kWave));
+    s = M == -INFINITY ? s : s * exp((double)M - (double)all);
+    for (int off = lanes / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    if (w < W && l == 0) {
+      const double lse = (double)all + log(s);
+      const bool live = finite(score) && fabs(lse) < (double)INFINITY;
       sm.lse[w] = live ? lse : 0.0;
       sm.score[w] = live ? score : -INFINITY;
     }
   }
-  if (tid == 0) sm.listed = sm.count = 0;
-  if (tid == 0) sm.theta_key = 0xffffffffu;
+  if (tid == 0) {
+    sm.listed = sm.count = 0;
+    sm.theta_key = 0xffffffffu;
+  }
   __syncthreads();
   // ---- theta ----
-  const int per_row = nch * kTops;
-  const int tops = W * per_row;
-  const float* top = p.tops + first * per_row;
+  // (a beam that proposes nothing may have no tops: whatever is there plus -inf is -inf or NaN)
+  auto total_of = [&](float x, int w) {
+    return (float)((double)sm.score[w] + ((double)x - sm.lse[w]));
+  };
   float own = -INFINITY;
-  for (int i = tid; i < tops; i += kFThreads) {
-    const int w = i / per_row;
-    if (sm.score[w] == -INFINITY) continue;
-    own = fmaxf(own, (float)((double)sm.score[w] + ((double)top[i] - sm.lse[w])));
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (held_row[k] >= 0) {
+      const float4 v = held[k];
+      own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), held_row[k]));
+    }
+  for (int i = tid + kHeld * kFThreads; i < quads; i += kFThreads) {
+    const float4 v = top4[i];
+    own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), i / per_row));
   }
   sm.key[tid] = own;
   __syncthreads();
-  {
+  // the C-th largest of the 512 threads' keys, or of 64 maxima of eight of them: fewer than C keys are
+  // above it, and it is the least such key
+  if (C <= kFoldC) {  // block-uniform
+    if (wid == 0) {
+#pragma unroll
+      for (int k = 1; k < kFWaves; ++k) own = fmaxf(own, sm.key[k * kWave + lane]);
+      sm.fold[lane] = own;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      int above = 0;
+      const float4* keys = reinterpret_cast<const float4*>(sm.fold);
+#pragma unroll
+      for (int j = 0; j < kWave / 4; ++j) {
+        const float4 o = keys[j];
+        above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+      }
+      if (above < C) atomicMin(&sm.theta_key, ordered_bits(own));
+    }
+  } else {
     int above = 0;
     const float4* keys = reinterpret_cast<const float4*>(sm.key);
 #pragma unroll 8
@@ -317,73 +382,92 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   __syncthreads();
   const float theta = key_float(sm.theta_key);
   // ---- the least logit of each beam that can reach theta, rounded down ----
-  for (int w = tid; w < W; w += kFThreads) {
+  if (tid < W) {
     float f = INFINITY;
-    if (sm.score[w] != -INFINITY) {
+    if (sm.score[tid] != -INFINITY) {
       f = -3.402823466e38f;  // -inf is no candidate
       if (theta != -INFINITY) {
         // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
         const double t = (double)theta - fabs((double)theta) * 0x1p-23;
-        f = fmaxf(f, __double2float_rd(t - (double)sm.score[w] + sm.lse[w]));
+        f = fmaxf(f, __double2float_rd(t - (double)sm.score[tid] + sm.lse[tid]));
       }
     }
-    sm.floor[w] = f;
+    sm.floor[tid] = f;
   }
   __syncthreads();
-  for (int i = tid; i < tops; i += kFThreads) {
-    const int w = i / per_row;
+  auto list = [&](const float4& v, int i, int w) {
     const float f = sm.floor[w];
-    if (f < INFINITY && top[i] >= f) {
-      const int pos = atomicAdd(&sm.listed, 1);
-      if (pos < kListCap) sm.list[pos] = i;
-    }
-  }
+    if (f == INFINITY) return;
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (e[k] >= f) {
+        const int pos = atomicAdd(&sm.listed, 1);
+        if (pos < kListCap) sm.list[pos] = i * 4 + k;
+      }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (held_row[k] >= 0) list(held[k], tid + k * kFThreads, held_row[k]);
+  for (int i = tid + kHeld * kFThreads; i < quads; i += kFThreads) list(top4[i], i, i / per_row);
   __syncthreads();
   const int listed = sm.listed;
   int found = 0;
   if (listed <= kListCap) {
-    // ---- the entries under the listed tops, 16 lanes each ----
-    for (int b = 0; b < listed; b += kFThreads / 16) {
-      const int li = b + tid / 16;
-      if (li >= listed) continue;
-      const int i = sm.list[li];
-      const int w = i / per_row, rest = i - w * per_row;
-      const int c = rest / kTops, lanes = rest - c * kTops;
-      const int64_t base = (int64_t)c * CH;
-      const int left = (int)min((int64_t)p.V - base, (int64_t)CH);
-      const S* row = beam_row<S>(p, first + w) + base;
-      const float f = sm.floor[w];
-      u32x4 q[NV];
-      const int col0 = (lanes * 16 + (tid & 15)) * VEC;
+    // ---- the entries under the listed tops, 16 lanes each, two tops at a time ----
+    constexpr int kTeams = kFThreads / 16;
+    for (int b = tid / 16; b < listed; b += 2 * kTeams) {
+      u32x4 q[2][NV];
+      int64_t base[2];
+      int row_of[2], col0[2], left[2];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) q[j] = load_vec_inside<DT>(row, col0 + j * kThreads * VEC, left);
+      for (int k = 0; k < 2; ++k) {
+        const int i = sm.list[min(b + k * kTeams, listed - 1)];
+        const int w = i / (nch * kTops), rest = i - w * (nch * kTops);
+        const int c = rest / kTops;
+        row_of[k] = w;
+        base[k] = (int64_t)c * CH;
+        left[k] = (int)min((int64_t)p.V - base[k], (int64_t)CH);
+        col0[k] = ((rest - c * kTops) * 16 + (tid & 15)) * VEC;
+        const S* row = beam_row<S>(p, first + w) + base[k];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j)
+          q[k][j] = load_vec_inside<DT>(row, col0[k] + j * kThreads * VEC, left[k]);
+      }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float x = vec_elem<DT>(q[j], e);
-          if (!(x >= f)) continue;
-          const int col = inside_col<DT>(col0 + j * kThreads * VEC, e, left);
-          if (col < 0) continue;
-          const int pos = atomicAdd(&sm.count, 1);
-          if (pos < kCandCap) {
-            Candidate& o = sm.cand[pos];
-            o.total = (double)sm.score[w] + ((double)x - sm.lse[w]);
-            o.x = x;
-            o.token = (int)(base + col);
-            o.beam = w;
+      for (int k = 0; k < 2; ++k) {
+        if (b + k * kTeams >= listed) continue;
+        const int w = row_of[k];
+        const float f = sm.floor[w];
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float x = vec_elem<DT>(q[k][j], e);
+            if (!(x >= f)) continue;
+            const int col = inside_col<DT>(col0[k] + j * kThreads * VEC, e, left[k]);
+            if (col < 0) continue;
+            const int pos = atomicAdd(&sm.count, 1);
+            if (pos < kCandCap)
+              put(sm.cand, pos,
+                  {(double)sm.score[w] + ((double)x - sm.lse[w]), x, (int)(base[k] + col), w});
           }
-        }
+      }
     }
     __syncthreads();
     found = sm.count;
   }
   if (listed <= kListCap && found <= kCandCap) {
-    for (int i = tid; i < found; i += kFThreads) {
-      const Candidate mine = sm.cand[i];
+    // ranked by counting, eight threads to a candidate
+    for (int i0 = 0; i0 < found; i0 += kFThreads / 8) {
+      const int i = i0 + tid / 8;
+      const Candidate mine = get(sm.cand, min(i, found - 1));
       int rank = 0;
-      for (int j = 0; j < found; ++j) rank += better(sm.cand[j], mine);
-      if (rank < C) sm.best[rank] = mine;
+      for (int j = tid & 7; j < found; j += 8) rank += before(sm.cand, j, mine);
+      rank += dpp_i32<kDppXor1>(rank);
+      rank += dpp_i32<kDppXor2>(rank);
+      rank += dpp_i32<kDppHalfMirror>(rank);
+      if (i < found && rank < C && (tid & 7) == 0) put(sm.best, rank, mine);
     }
     __syncthreads();
     return min(found, C);
@@ -399,16 +483,16 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     Candidate mine;
     const bool have = tid < found + got;
     if (have) {
-      mine = tid < found ? sm.best[tid] : sm.cand[tid - found];
+      mine = tid < found ? get(sm.best, tid) : get(sm.cand, tid - found);
       if (tid >= found) mine.total = (double)sm.score[w] + ((double)mine.x - sm.lse[w]);
     }
     __syncthreads();
-    if (have) sm.cand[tid] = mine;
+    if (have) put(sm.cand, tid, mine);
     __syncthreads();
     int rank = 0;
     if (have)
-      for (int j = 0; j < found + got; ++j) rank += better(sm.cand[j], mine);
-    if (have && rank < C) sm.best[rank] = mine;
+      for (int j = 0; j < found + got; ++j) rank += before(sm.cand, j, mine);
+    if (have && rank < C) put(sm.best, rank, mine);
     found = min(found + got, C);
   }
   __syncthreads();
@@ -424,9 +508,9 @@ __global__ __launch_bounds__(kFThreads) void beam_select_kernel(BeamScanParams p
   for (int i = threadIdx.x; i < p.C; i += kFThreads) {
     const int64_t at = (int64_t)g * p.C + i;
     const bool on = i < found;
-    o.token_ids[at] = on ? sm.best[i].token : -1;
-    o.parents[at] = on ? sm.best[i].beam : -1;
-    o.scores[at] = on ? (float)sm.best[i].total : -INFINITY;
+    o.token_ids[at] = on ? sm.best.token[i] : -1;
+    o.parents[at] = on ? sm.best.beam[i] : -1;
+    o.scores[at] = on ? (float)sm.best.total[i] : -INFINITY;
   }
 }
 
@@ -468,7 +552,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
     bool stop = false;
     if (tid < found)
       for (int64_t e = 0; e < a.num_stop_ids; ++e)
-        stop |= sm.best[tid].token == a.stop_token_ids[e];
+        stop |= sm.best.token[tid] == a.stop_token_ids[e];
     const uint64_t sb = __ballot(stop), ob = __ballot(tid < found && !stop);
     if (lane == 0) {
       sm.stop_mask[wid] = sb;
@@ -497,7 +581,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
     // the first candidate that goes on is the best running beam
     for (int k = kMaxCandidates / kWave - 1; k >= 0; --k)
       if (sm.on_mask[k])
-        next_best = (float)sm.best[k * kWave + __ffsll((long long)sm.on_mask[k]) - 1].total;
+        next_best = (float)sm.best.total[k * kWave + __ffsll((long long)sm.on_mask[k]) - 1];
   }
   const int64_t hist = ((int64_t)g * a.max_length + len) * W;
   auto put = [&](int w, float score, int token, int parent) {
@@ -510,17 +594,17 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   if (wid < kMaxCandidates / kWave && ((sm.on_mask[wid] >> lane) & 1)) {
     int place = __popcll(sm.on_mask[wid] & ((1ull << lane) - 1ull));
     for (int k = 0; k < wid; ++k) place += __popcll(sm.on_mask[k]);
-    if (place < W) put(place, (float)sm.best[tid].total, sm.best[tid].token, sm.best[tid].beam);
+    if (place < W) put(place, (float)sm.best.total[tid], sm.best.token[tid], sm.best.beam[tid]);
   }
   if (tid >= going && tid < W) put(tid, -INFINITY, -1, -1);
   // ---- finished hypotheses: entries [0, W) are the old ones, [W, 2 W) the candidates of rank < W ----
   if (tid >= W && tid < 2 * W) {
     const int r = tid - W;
     if (r < found && ((sm.stop_mask[r / kWave] >> (r % kWave)) & 1)) {
-      hyp = (float)((double)(float)sm.best[r].total / power);
+      hyp = (float)((double)(float)sm.best.total[r] / power);
       if (!(hyp > -INFINITY)) hyp = -INFINITY;
-      hyp_beam = sm.best[r].beam;
-      hyp_token = sm.best[r].token;
+      hyp_beam = sm.best.beam[r];
+      hyp_token = sm.best.token[r];
       hyp_len = new_len;
     }
   }
@@ -585,8 +669,8 @@ static hipError_t launch(BeamScanParams p, const BeamSelectOut* o, const mvsd_be
   const int64_t rows = (int64_t)p.G * p.W;
   const int chunk = beam_chunk(rows, p.V, p.C);
   p.nchunks = (int)(((int64_t)p.V + chunk - 1) / chunk);
-  p.stats = static_cast<float2*>(workspace);
-  p.tops = reinterpret_cast<float*>(p.stats + rows * p.nchunks);
+  p.tops = static_cast<float*>(workspace);
+  p.stats = reinterpret_cast<float2*>(p.tops + rows * p.nchunks * kTops);
   switch (dtype) {
     case MVSD_F32: launch_dt<MVSD_F32>(p, o, a, chunk, stream); break;
     case MVSD_BF16: launch_dt<MVSD_BF16>(p, o, a, chunk, stream); break;
