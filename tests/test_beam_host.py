@@ -7,6 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
+from mvsd import _hostops
 from mvsd import _native as nat
 from mvsd.sample import (BeamSearch, BeamState, beam_search_finish, beam_search_select,
                          beam_search_step, reorder_beams)
@@ -190,3 +191,51 @@ def test_search_arguments():
     assert torch.isneginf(search.state.scores[:, 1:]).all()
     with pytest.raises(RuntimeError):
         search.reorder(torch.zeros(8, 8))
+
+
+def test_tensor_table_takes_what_fits_and_names_the_first_that_does_not():
+    x, y = torch.zeros(3, 4), torch.zeros(5, dtype=torch.int32)
+    buf = (ctypes.c_int64 * 4)()
+    cpu = x.device
+
+    def table(tensors, dtypes=(torch.float32, torch.int32), shapes=((3, 4), (5,)), at=1,
+              device=cpu):
+        return _hostops.tensor_table(buf, at, tensors, dtypes, shapes, device)
+
+    assert table((x, y)) == -1
+    assert list(buf) == [0, x.data_ptr(), y.data_ptr(), 0]
+    assert table((x, y), dtypes=(torch.float32, torch.int64)) == 1
+    assert table((x, y), shapes=((4, 3), (5,))) == 0
+    assert table((x, y), shapes=((3, 4), (6,))) == 1
+    assert table((x, y), device=torch.device("cuda", 0)) == 0
+    assert table((x.t(), y), shapes=((4, 3), (5,))) == 0
+    assert table((x, None)) == 1 and table((3, y)) == 0
+    for bad in (dict(at=3), dict(at=-1), dict(dtypes=(torch.float32,)), dict(shapes=())):
+        with pytest.raises(ValueError):
+            table((x, y), **bad)
+    with pytest.raises(TypeError):
+        table([x, y])
+
+
+def test_state_table_lists_rows_pieces_and_entries():
+    x = torch.zeros(6, 3, 10, 4, dtype=torch.float16)
+    buf = (ctypes.c_int64 * 24)()
+    cpu = x.device
+
+    def table(states, outs=None, dim=2, device=cpu, least=6):
+        return _hostops.state_table(buf, states, states if outs is None else outs, dim, device, least)
+
+    assert table((x, x[:, :0], x[:, 1:2])) == 2  # the empty one has no entry
+    p = x.data_ptr()
+    assert list(buf)[:16] == [p, p, 240, 240, 6, 3, 10, 8, p + 80, p + 80, 240, 240, 6, 1, 10, 8]
+    assert table((x,), dim=3) == 1 and list(buf)[4:8] == [6, 30, 4, 2]
+    y = torch.zeros(12, 3, 10, 4, dtype=torch.float16)[::2]
+    assert table((x,), (y,)) == 1 and list(buf)[:4] == [p, y.data_ptr(), 240, 480]
+    for bad in (dict(states=(x,), least=7), dict(states=(x,), dim=4), dict(states=(x,), dim=0),
+                dict(states=(x.transpose(1, 2),)), dict(states=(x[..., ::2],)),
+                dict(states=(x,), outs=(x.float(),)), dict(states=(x,), outs=(x[:5],)),
+                dict(states=(x,), outs=(x, x)), dict(states=(None,)), dict(states=(x, 3)),
+                dict(states=(x,), device=torch.device("cuda", 0)),
+                dict(states=(x.new_zeros(1, 3, 10, 4).expand(6, 3, 10, 4),)),
+                dict(states=(x,) * 4)):
+        assert table(**bad) == -1, bad

@@ -22,10 +22,12 @@ and captured graphs share nothing.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass, fields
+import struct
+from dataclasses import dataclass
 
 import torch
 
+from .. import _hostops
 from .. import _native as nat
 
 PLACEHOLDER_TOKEN_ID = -1
@@ -97,9 +99,17 @@ class BeamHypotheses:
     scores: torch.Tensor     # fp32 [G, n], -inf: no such answer
 
 
-_STATE_FIELDS = tuple(f.name for f in fields(BeamState))
-_STATE_DTYPES = {"scores": torch.float32, "done": torch.bool, "finished_scores": torch.float32}
+# A state's tensors in the order of mvsd_beam_step_args and mvsd_beam_finish_args: seven that a step
+# replaces, then the histories.
+_FIELDS = ("scores", "lengths", "done", "finished_scores", "finished_beams", "finished_token_ids",
+           "finished_lengths")
 _HISTORIES = ("token_history", "parent_history")
+_I32, _F32 = torch.int32, torch.float32
+_DTYPES = (_F32, _I32, torch.bool, _F32, _I32, _I32, _I32)
+# the places of their addresses in the argument structures, in eight-byte words
+_STEP_HEAD, _STEP_TENSORS = struct.Struct("=10qdii"), 12
+_FINISH_HEAD, _FINISH_TENSORS = struct.Struct("=4qd"), 5
+_TAIL = struct.Struct("=2q")
 
 
 def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
@@ -114,20 +124,34 @@ def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
         raise ValueError(f"{name} is not contiguous")
 
 
-def _check_state(state: BeamState, name: str, device) -> tuple[int, int, int]:
-    """(G, W, max_length) of a state whose every tensor fits them."""
+def _addresses(args, at: int, names, tensors, dtypes, shapes, device) -> None:
+    """The tensors' addresses into a call's arguments; raises for one of another kind."""
+    bad = _hostops.tensor_table(args, at, tensors, dtypes, shapes, device)
+    if bad >= 0:
+        _check_array(tensors[bad], names[bad], dtypes[bad], shapes[bad], device)
+        raise ValueError(f"{names[bad]} is no tensor that can be passed on")
+
+
+def _fields(state: BeamState):
+    return (state.scores, state.lengths, state.done, state.finished_scores, state.finished_beams,
+            state.finished_token_ids, state.finished_lengths)
+
+
+def _extent(state: BeamState) -> tuple[int, int, int]:
     history = state.token_history
     if history.ndim != 3:
-        raise ValueError(f"{name}.token_history is not [G, max_length, W]")
+        raise ValueError("token_history is not [G, max_length, W]")
     G, T, W = history.shape
+    if not 1 <= W <= MAX_BEAMS:
+        raise ValueError(f"{W} beams: 1 to {MAX_BEAMS} are supported")
     if T < 1:
-        raise ValueError(f"{name} has max_length 0")
-    shapes = {"lengths": (G,), "done": (G,), "token_history": (G, T, W),
-              "parent_history": (G, T, W)}
-    for field in _STATE_FIELDS:
-        _check_array(getattr(state, field), f"{name}.{field}",
-                     _STATE_DTYPES.get(field, torch.int32), shapes.get(field, (G, W)), device)
-    return G, W, T
+        raise ValueError("the state has max_length 0")
+    return G, T, W
+
+
+def _elsewhere(device: torch.device) -> bool:
+    """Whether `device` is not the current one, to which launches and allocations go."""
+    return device.index is not None and device.index != torch.cuda.current_device()
 
 
 def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.device:
@@ -154,29 +178,11 @@ def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.devi
     return device
 
 
-def _workspace(G: int, W: int, V: int, C: int, device) -> torch.Tensor:
+def _workspace(G: int, W: int, V: int, C: int, device) -> tuple[torch.Tensor, int]:
     size = nat.lib().mvsd_beam_workspace_bytes(G, W, V, C)
     if size <= 0:
         raise ValueError(f"{G} groups of {W} beams over {V} tokens are more than one call takes")
-    return torch.empty(size, dtype=torch.uint8, device=device)
-
-
-class _on:
-    """Makes `device` the current one where it is not (launches go to the current device)."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.index is not None and self.index != self.before:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index is not None and self.index != self.before:
-            torch.cuda.set_device(self.before)
+    return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int, *,
@@ -195,23 +201,26 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
         raise ValueError("scores are [G, W]")
     G, W = scores.shape
     device = _check_rows(logits, G, W, target_rows)
-    _check_array(scores, "scores", torch.float32, scores.shape, device)
+    _check_array(scores, "scores", _F32, (G, W), device)
     C = int(num_candidates)
     if not 1 <= C <= MAX_CANDIDATES:
         raise ValueError(f"num_candidates={C}: 1 to {MAX_CANDIDATES} are supported")
-    with _on(device):
-        ids = torch.empty((3, G, C), dtype=torch.int32, device=device)
-        out = BeamCandidates(ids[0], ids[1], ids[2].view(torch.float32))
-        if G == 0:
-            return out
-        V = logits.shape[1]
-        ws = _workspace(G, W, V, C, device)
-        base = ids.data_ptr()
-        nat.check(nat.lib().mvsd_beam_select(
-            base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
-            nat.dtype_code(logits.dtype), logits.stride(0), logits.shape[0],
-            nat.ptr(target_rows), scores.data_ptr(), G, W, V, C, ws.data_ptr(), ws.numel(),
-            nat.stream_of(device)), "mvsd_beam_select")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return beam_search_select(logits, scores, C, target_rows=target_rows)
+    ids = torch.empty((3, G, C), dtype=_I32, device=device)
+    token_ids, parents, bits = ids.unbind(0)
+    out = BeamCandidates(token_ids, parents, bits.view(_F32))
+    if G == 0:
+        return out
+    rows, V = logits.shape
+    ws, size = _workspace(G, W, V, C, device)
+    base = ids.data_ptr()
+    nat.check(nat.lib().mvsd_beam_select(
+        base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
+        nat.dtype_code(logits.dtype), logits.stride(0), rows, nat.ptr(target_rows),
+        scores.data_ptr(), G, W, V, C, ws.data_ptr(), size, nat.stream_of(device)),
+        "mvsd_beam_select")
     return out
 
 
@@ -234,48 +243,59 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
     Other groups stay as they are (token_ids and parents -1).  The new state is written to ``out``
     (another :class:`BeamState` with the same histories), or to ``state`` itself.
     """
-    device = logits.device
-    nat.require_device_tensor(logits, "logits")
-    G, W, T = _check_state(state, "state", device)
-    _check_rows(logits, G, W, target_rows)
+    G, T, W = _extent(state)
+    device = _check_rows(logits, G, W, target_rows)
     if out is None:
         out = state
-    elif out is not state:
-        _check_state(out, "out", device)
-        for name in _HISTORIES:
-            if getattr(out, name).data_ptr() != getattr(state, name).data_ptr():
-                raise ValueError(f"out.{name} is another tensor than state.{name}")
-        if out.scores.shape != state.scores.shape:
-            raise ValueError("out has another shape than state")
+    token_history, parent_history = state.token_history, state.parent_history
+    if out is not state and (out.token_history is not token_history
+                             or out.parent_history is not parent_history):
+        if (out.token_history.data_ptr() != token_history.data_ptr()
+                or out.parent_history.data_ptr() != parent_history.data_ptr()
+                or out.token_history.shape != token_history.shape
+                or out.parent_history.shape != parent_history.shape):
+            raise ValueError("out has other histories than state")
     E = 0
     if stop_token_ids is not None:
         E = stop_token_ids.numel()
-        _check_array(stop_token_ids, "stop_token_ids", torch.int32, (E,), device)
+        _check_array(stop_token_ids, "stop_token_ids", _I32, (E,), device)
     C = W * (1 + E)
     if C > MAX_CANDIDATES:
         raise ValueError(f"{W} beams with {E} stop tokens: W * (1 + E) is over {MAX_CANDIDATES}")
-    with _on(device):
-        ids = torch.empty((2, G, W), dtype=torch.int32, device=device)
-        step = BeamStep(ids[0], ids[1], out)
-        if G == 0:
-            return step
-        V = logits.shape[1]
-        ws = _workspace(G, W, V, C, device)
-        base = ids.data_ptr()
-        args = nat.BeamStepArgs(
-            logits.data_ptr(), logits.stride(0), logits.shape[0], nat.ptr(target_rows), G, W, V,
-            T, nat.ptr(stop_token_ids), E, float(length_penalty), nat.dtype_code(logits.dtype),
-            int(bool(early_stopping)), state.scores.data_ptr(), state.lengths.data_ptr(),
-            state.done.data_ptr(), state.finished_scores.data_ptr(),
-            state.finished_beams.data_ptr(), state.finished_token_ids.data_ptr(),
-            state.finished_lengths.data_ptr(), out.scores.data_ptr(), out.lengths.data_ptr(),
-            out.done.data_ptr(), out.finished_scores.data_ptr(), out.finished_beams.data_ptr(),
-            out.finished_token_ids.data_ptr(), out.finished_lengths.data_ptr(),
-            state.token_history.data_ptr(), state.parent_history.data_ptr(), base,
-            base + 4 * G * W, ws.data_ptr(), ws.numel())
-        nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), nat.stream_of(device)),
-                  "mvsd_beam_step")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return beam_search_step(logits, state, stop_token_ids=stop_token_ids,
+                                    length_penalty=length_penalty, early_stopping=early_stopping,
+                                    target_rows=target_rows, out=out)
+    args = nat.BeamStepArgs()
+    a, b, c = (G, W), (G,), (G, T, W)
+    fields = (a, b, b, a, a, a, a)
+    old, new = _fields(state), _fields(out)
+    _addresses(args, _STEP_TENSORS, _STEP_NAMES, old + new + (token_history, parent_history),
+               _STEP_DTYPES, fields + fields + (c, c), device)
+    token_ids = torch.empty_like(state.finished_beams)
+    parents = torch.empty_like(state.finished_beams)
+    step = BeamStep(token_ids, parents, out)
+    if G == 0:
+        return step
+    rows, V = logits.shape
+    ws, size = _workspace(G, W, V, C, device)
+    _STEP_HEAD.pack_into(args, 0, logits.data_ptr(), logits.stride(0), rows,
+                         0 if target_rows is None else target_rows.data_ptr(), G, W, V, T,
+                         stop_token_ids.data_ptr() if E else 0, E, length_penalty,
+                         nat.dtype_code(logits.dtype), 1 if early_stopping else 0)
+    _TAIL.pack_into(args, 8 * (_STEP_TENSORS + 16), token_ids.data_ptr(), parents.data_ptr())
+    _TAIL.pack_into(args, 8 * (_STEP_TENSORS + 18), ws.data_ptr(), size)
+    nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), nat.stream_of(device)),
+              "mvsd_beam_step")
     return step
+
+
+_STEP_NAMES = tuple("state." + f for f in _FIELDS) + tuple("out." + f for f in _FIELDS) \
+    + tuple("state." + f for f in _HISTORIES)
+_STEP_DTYPES = _DTYPES + _DTYPES + (_I32, _I32)
+_FINISH_NAMES = tuple("state." + f for f in _FIELDS + _HISTORIES)
+_FINISH_DTYPES = _DTYPES + (_I32, _I32)
 
 
 def beam_search_finish(state: BeamState, num_return: int | None = None, *,
@@ -283,56 +303,56 @@ def beam_search_finish(state: BeamState, num_return: int | None = None, *,
     """The ``num_return`` (default W) best answers of every group: its finished hypotheses and, unless
     the group is done, its running beams (sum / length ** length_penalty); finished ones first where
     they are equal.  The sequences are read back from the histories; the state is left as it is."""
-    device = state.scores.device
     nat.require_device_tensor(state.scores, "state.scores")
-    G, W, T = _check_state(state, "state", device)
-    if not 1 <= W <= MAX_BEAMS:
-        raise ValueError(f"{W} beams: 1 to {MAX_BEAMS} are supported")
+    device = state.scores.device
+    G, T, W = _extent(state)
     n = W if num_return is None else int(num_return)
     if not 1 <= n <= W:
         raise ValueError(f"num_return={n}: 1 to {W} (the beams) are kept")
-    with _on(device):
-        ids = torch.empty((G, n, T), dtype=torch.int32, device=device)
-        two = torch.empty((2, G, n), dtype=torch.int32, device=device)
-        out = BeamHypotheses(ids, two[0], two[1].view(torch.float32))
-        if G == 0:
-            return out
-        size = nat.lib().mvsd_beam_finish_workspace_bytes(G, W, T, n)
-        ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-        args = nat.BeamFinishArgs(
-            G, W, T, n, float(length_penalty), state.scores.data_ptr(), state.lengths.data_ptr(),
-            state.done.data_ptr(), state.finished_scores.data_ptr(),
-            state.finished_beams.data_ptr(), state.finished_token_ids.data_ptr(),
-            state.finished_lengths.data_ptr(), state.token_history.data_ptr(),
-            state.parent_history.data_ptr(), ids.data_ptr(), two.data_ptr(),
-            two.data_ptr() + 4 * G * n, nat.ptr(ws), size)
-        nat.check(nat.lib().mvsd_beam_finish(ctypes.byref(args), nat.stream_of(device)),
-                  "mvsd_beam_finish")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return beam_search_finish(state, n, length_penalty=length_penalty)
+    args = nat.BeamFinishArgs()
+    a, b, c = (G, W), (G,), (G, T, W)
+    _addresses(args, _FINISH_TENSORS, _FINISH_NAMES,
+               _fields(state) + (state.token_history, state.parent_history), _FINISH_DTYPES,
+               (a, b, b, a, a, a, a, c, c), device)
+    ids = torch.empty((G, n, T), dtype=_I32, device=device)
+    lengths = torch.empty((G, n), dtype=_I32, device=device)
+    scores = torch.empty((G, n), dtype=_F32, device=device)
+    out = BeamHypotheses(ids, lengths, scores)
+    if G == 0:
+        return out
+    size = nat.lib().mvsd_beam_finish_workspace_bytes(G, W, T, n)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
+    _FINISH_HEAD.pack_into(args, 0, G, W, T, n, length_penalty)
+    _TAIL.pack_into(args, 8 * (_FINISH_TENSORS + 9), ids.data_ptr(), lengths.data_ptr())
+    _TAIL.pack_into(args, 8 * (_FINISH_TENSORS + 11), scores.data_ptr(),
+                    0 if ws is None else ws.data_ptr())
+    args.workspace_bytes = size
+    nat.check(nat.lib().mvsd_beam_finish(ctypes.byref(args), nat.stream_of(device)),
+              "mvsd_beam_finish")
     return out
 
 
-def _state_rows(x: torch.Tensor, name: str, length_dim: int, device) -> tuple:
-    """(row stride in bytes, rows, pieces, length, bytes of an entry) of a state tensor."""
-    if x.device != device:
-        nat.require_device_tensor(x, name)
-        raise ValueError(f"{name} is on {x.device}, parents on {device}")
-    shape = x.shape
-    if not 1 <= length_dim < len(shape):
-        raise ValueError(f"{name} has no dimension {length_dim} behind its rows")
-    stride, expect = x.stride(), 1
-    for d in range(len(shape) - 1, 0, -1):
-        if stride[d] != expect and shape[d] > 1 and expect:
-            raise ValueError(f"{name} is not contiguous within a row")
-        expect *= shape[d]
-    if shape[0] > 1 and stride[0] < expect:
-        raise ValueError(f"{name} has overlapping rows")
-    outer = inner = 1
-    for d in range(1, length_dim):
-        outer *= shape[d]
-    for d in range(length_dim + 1, len(shape)):
-        inner *= shape[d]
-    size = x.element_size()
-    return stride[0] * size, shape[0], outer, shape[length_dim], inner * size
+def _refuse_states(tensors, targets, length_dim: int, device, least_rows: int) -> None:
+    """Raises for the first of the tensors that is no state."""
+    for k, (x, to) in enumerate(zip(tensors, targets)):
+        for t, name in ((x, f"states[{k}]"), (to, f"out[{k}]")):
+            nat.require_device_tensor(t, name)
+            if t.device != device:
+                raise ValueError(f"{name} is on {t.device}, parents on {device}")
+            if not 1 <= length_dim < t.ndim:
+                raise ValueError(f"{name} has no dimension {length_dim} behind its rows")
+            if t.shape[0] < least_rows:
+                raise ValueError(f"{name} has {t.shape[0]} rows for {least_rows} beams")
+            if t.shape != x.shape or t.dtype != x.dtype:
+                raise ValueError(f"{name} has another shape or dtype than states[{k}]")
+            if t.numel() and not t[0].is_contiguous():
+                raise ValueError(f"{name} is not contiguous within a row")
+            if t.shape[0] > 1 and t.numel() and t.stride(0) < t[0].numel():
+                raise ValueError(f"{name} has overlapping rows")
+    raise ValueError("a state is no tensor that can be passed on")
 
 
 def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None = None,
@@ -368,32 +388,27 @@ def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None 
     if slots is not None:
         _check_array(slots, "slots", torch.int32, (G, W), device)
     single = isinstance(states, torch.Tensor)
-    tensors = [states] if single else list(states)
-    targets = tensors if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    tensors = (states,) if single else tuple(states)
+    targets = tensors if out is None else (out,) if isinstance(out, torch.Tensor) else tuple(out)
     if len(targets) != len(tensors):
         raise ValueError(f"{len(targets)} out tensors for {len(tensors)} states")
-    flat = []
-    for k, (x, to) in enumerate(zip(tensors, targets)):
-        stride, rows, outer, length, inner = _state_rows(x, f"states[{k}]", length_dim, device)
-        to_stride = stride
-        if to is not x:
-            if to.shape != x.shape or to.dtype != x.dtype:
-                raise ValueError(f"out[{k}] has another shape or dtype than states[{k}]")
-            to_stride = _state_rows(to, f"out[{k}]", length_dim, device)[0]
-        if slots is None and rows < G * W:
-            raise ValueError(f"states[{k}] has {rows} rows for {G} groups of {W} beams")
-        if rows and outer * length * inner:
-            flat += (x.data_ptr(), to.data_ptr(), stride, to_stride, rows, outer, length, inner)
-    n = len(flat) // 8
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return reorder_beams(states, parents, starts=starts, lengths=lengths,
+                                 length_dim=length_dim, slots=slots, out=out)
+    table = (ctypes.c_int64 * (8 * len(tensors)))()
+    n = _hostops.state_table(table, tensors, targets, length_dim, device,
+                             0 if slots is not None else G * W)
+    if n < 0:
+        _refuse_states(tensors, targets, length_dim, device, 0 if slots is not None else G * W)
     if n and G:
-        with _on(device):
-            status = nat.lib().mvsd_beam_reorder(
-                (ctypes.c_int64 * len(flat))(*flat), n, parents.data_ptr(), nat.ptr(starts),
-                nat.ptr(lengths), nat.ptr(slots), G, W, nat.stream_of(device))
+        status = nat.lib().mvsd_beam_reorder(
+            table, n, parents.data_ptr(), nat.ptr(starts), nat.ptr(lengths), nat.ptr(slots), G, W,
+            nat.stream_of(device))
         if status == -1:
             raise ValueError("the states (or out) share memory with each other")
         nat.check(status, "mvsd_beam_reorder")
-    return targets[0] if single else targets
+    return targets[0] if single else list(targets)
 
 
 class BeamSearch:
