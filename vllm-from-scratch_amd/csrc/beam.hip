@@ -35,11 +35,11 @@ namespace mvsd {
 constexpr int kTops = 16;          // of a chunk, 16 lanes each
 constexpr int kFThreads = 512;
 constexpr int kFWaves = kFThreads / kWave;
-constexpr int kListCap = 2048;     // tops that reach theta
+constexpr int kListCap = 1024;     // tops that reach theta
 constexpr int kCandCap = 1024;     // gathered entries
 constexpr int kHeld = 4;           // vectors of tops a thread keeps in registers
+constexpr int kStats = 2;          // chunks that a lane of a beam loads at a time
 constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 keys
-constexpr float kLog2e = 1.44269504088896340736f;
 
 // Columns per chunk: long ones, unless they leave compute units idle (fewer than 4 workgroups each)
 // or give a row fewer than two tops per candidate (a group may have one beam only), so that theta is
@@ -49,6 +49,12 @@ constexpr int kBeamLong = 8192, kBeamShort = 2048;
 static int beam_chunk(int64_t rows, int64_t V, int64_t C) {
   const int64_t chunks = (V + kBeamLong - 1) / kBeamLong;
   return rows * chunks < 1024 || chunks * kTops < 2 * C ? kBeamShort : kBeamLong;
+}
+
+// exp(d), d <= 0, as 2^(d log2(e)) with log2(e) in two parts, so that its rounding leaves no bias: the
+// mean error of a row's lse went from 3.8e-8 to below 1e-8.
+__device__ inline float exp_of(float d) {
+  return __builtin_amdgcn_exp2f(fmaf(d, 1.44269504f, d * 1.92596304e-8f));
 }
 
 __device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -105,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s += __builtin_amdgcn_exp2f((v[j][e] - wm) * kLog2e);
+      for (int e = 0; e < VEC; ++e) s += exp_of(v[j][e] - wm);
   } else {  // every entry is -inf or NaN
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -127,7 +133,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w)
       sum += s_m[w] == -INFINITY ? s_s[w]
-                                 : s_s[w] * __builtin_amdgcn_exp2f((s_m[w] - M) * kLog2e);
+                                 : s_s[w] * exp_of(s_m[w] - M);
     p.stats[slot] = make_float2(M, sum);
   }
 }
@@ -176,9 +182,11 @@ __device__ inline bool before(const Candidates<N>& c, int j, const Candidate& mi
 struct BeamSmem {
   Candidates<kCandCap> cand;
   Candidates<kMaxCandidates> best;  // the group's candidates in order
-  int list[kListCap];
+  int2 list[kListCap];  // beam, top of the beam's row
   __align__(16) float key[kFThreads];
-  __align__(16) float fold[kWave];
+  float fold[kFWaves];
+  int above_key[kWave];
+  int64_t row[kMaxBeams];  // the first element of each beam's row
   double lse[kMaxBeams];
   float score[kMaxBeams];  // -inf: proposes nothing
   float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
@@ -187,7 +195,6 @@ struct BeamSmem {
   uint64_t stop_mask[kMaxCandidates / kWave], on_mask[kMaxCandidates / kWave];
   float pool[2 * kMaxBeams];
   int listed, count, above, digit;
-  uint32_t theta_key;
   float worst;
 };
 
@@ -273,6 +280,43 @@ __device__ inline int row_largest(const typename Elem<DT>::storage* row, int V, 
   return found;
 }
 
+// Sums and maxima over `lanes` (a power of two from 8 to 64) neighbouring lanes, in each of them.
+template <int CTRL>
+__device__ inline double dpp_f64(double v) {
+  return __builtin_bit_cast(double, dpp_u64<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+__device__ inline double lanes_sum(double v, int lanes) {
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  if (lanes > 8) v += dpp_f64<kDppMirror>(v);
+  for (int off = 16; off < lanes; off *= 2) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+__device__ inline float lanes_max(float v, int lanes) {
+  v = fmaxf(v, dpp_f32<kDppXor1>(v));
+  v = fmaxf(v, dpp_f32<kDppXor2>(v));
+  v = fmaxf(v, dpp_f32<kDppHalfMirror>(v));
+  if (lanes > 8) v = fmaxf(v, dpp_f32<kDppMirror>(v));
+  for (int off = 16; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor(v, off, kWave));
+  return v;
+}
+
+// The 16-byte vector at column col of a row of V columns, and its columns, as load_vec_inside and
+// inside_col, for columns of every lane's own.
+template <int DT>
+__device__ inline u32x4 load_vec_at(const typename Elem<DT>::storage* row, int64_t col, int V) {
+  constexpr int VEC = Elem<DT>::kVec;
+  // uniform, so that a wave's loads stay in flight together (a branch of the lanes' own waits for each)
+  if (V >= VEC) return load_vec_any<DT>(row + min(col, (int64_t)(V - VEC)));
+  return load_vec_inside<DT>(row, (int)col, V);
+}
+template <int DT>
+__device__ inline int column_at(int64_t col, int e, int V) {
+  const int64_t i = min(col, (int64_t)max(V - Elem<DT>::kVec, 0)) + e;
+  return i >= col && i < V ? (int)i : -1;
+}
+
 // The group's candidates, in order, in sm.best; returns how many.
 template <int DT, int NV>
 __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem& sm) {
@@ -283,6 +327,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   const int W = p.W, C = p.C, nch = p.nchunks;
   const int64_t first = (int64_t)g * W;
   // ---- the tops, four of one chunk at a time; the first ones stay in registers ----
+  // (all of these loads are in flight together; a beam that was not scanned has whatever is there)
   const int per_row = nch * (kTops / 4), quads = W * per_row;
   const float4* top4 = reinterpret_cast<const float4*>(p.tops + first * nch * kTops);
   float4 held[kHeld];
@@ -294,32 +339,38 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     held[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     if (i < quads) held[k] = top4[i];
   }
+  if (tid < W) {
+    int64_t row = first + tid;
+    if (p.rows) row = min(max((int64_t)p.rows[first + tid], (int64_t)0), p.num_rows - 1);
+    sm.row[tid] = row * p.stride;
+  }
   // ---- lse of every beam: as many lanes each as there are, a power of two from 8 to 64 ----
-  const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
   {
+    const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
     const int w = tid / lanes, l = tid & (lanes - 1);
-    const float score = w < W ? p.scores[first + w] : NAN;
-    float M = -INFINITY;
-    double s = 0.0;
-    if (finite(score)) {
-      const float2* st = p.stats + (first + w) * nch;
-#pragma unroll 4
-      for (int c = l; c < nch; c += lanes) {
-        const float2 v = st[c];
-        const float up = fmaxf(M, v.x);
-        // a chunk of -inf alone adds its sum, 0 (NaN where it holds a NaN)
-        if (up != -INFINITY) {
-          s = s * exp((double)M - (double)up) + (double)v.y * exp((double)v.x - (double)up);
-          M = up;
-        } else {
-          s += (double)v.y;
-        }
-      }
+    float M = -INFINITY, score = NAN;
+    float2 v[kStats];
+    const float2* st = p.stats + (first + min(w, W - 1)) * nch;
+    if (w < W) score = p.scores[first + w];
+#pragma unroll
+    for (int k = 0; k < kStats; ++k) {
+      const int c = l + k * lanes;
+      v[k] = w < W && c < nch ? st[c] : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, v[k].x);
     }
-    float all = M;
-    for (int off = lanes / 2; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor(all, off, kWave));
-    s = M == -INFINITY ? s : s * exp((double)M - (double)all);
-    for (int off = lanes / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
+    if (w < W)
+      for (int c = l + kStats * lanes; c < nch; c += lanes) M = fmaxf(M, st[c].x);
+    const float all = lanes_max(M, lanes);
+    // a chunk of -inf alone adds its sum, 0 (NaN where it holds a NaN)
+    auto term = [&](float2 t) {
+      return t.x == -INFINITY ? (double)t.y : (double)t.y * exp((double)t.x - (double)all);
+    };
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < kStats; ++k) s += term(v[k]);
+    if (w < W)
+      for (int c = l + kStats * lanes; c < nch; c += lanes) s += term(st[c]);
+    s = lanes_sum(s, lanes);
     if (w < W && l == 0) {
       const double lse = (double)all + log(s);
       const bool live = finite(score) && fabs(lse) < (double)INFINITY;
@@ -327,13 +378,12 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
       sm.score[w] = live ? score : -INFINITY;
     }
   }
-  if (tid == 0) {
-    sm.listed = sm.count = 0;
-    sm.theta_key = 0xffffffffu;
-  }
+  if (tid < kWave) sm.above_key[tid] = 0;
+  if (tid == 0) sm.listed = sm.count = 0;
   __syncthreads();
-  // ---- theta ----
-  // (a beam that proposes nothing may have no tops: whatever is there plus -inf is -inf or NaN)
+  // ---- theta: the C-th largest of the 512 threads' keys, or of 64 maxima of eight of them: fewer
+  //      than C keys are above it, and it is the least such key ----
+  // (what is left of a beam that proposes nothing: whatever plus -inf, -inf or NaN)
   auto total_of = [&](float x, int w) {
     return (float)((double)sm.score[w] + ((double)x - sm.lse[w]));
   };
@@ -350,25 +400,18 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   }
   sm.key[tid] = own;
   __syncthreads();
-  // the C-th largest of the 512 threads' keys, or of 64 maxima of eight of them: fewer than C keys are
-  // above it, and it is the least such key
+  float theta;
   if (C <= kFoldC) {  // block-uniform
-    if (wid == 0) {
+    // every wave folds the keys, counts an eighth of the comparisons and reads the sums
 #pragma unroll
-      for (int k = 1; k < kFWaves; ++k) own = fmaxf(own, sm.key[k * kWave + lane]);
-      sm.fold[lane] = own;
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      int above = 0;
-      const float4* keys = reinterpret_cast<const float4*>(sm.fold);
+    for (int k = 1; k < kFWaves; ++k) own = fmaxf(own, sm.key[((wid + k) % kFWaves) * kWave + lane]);
+    int above = 0;
 #pragma unroll
-      for (int j = 0; j < kWave / 4; ++j) {
-        const float4 o = keys[j];
-        above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
-      }
-      if (above < C) atomicMin(&sm.theta_key, ordered_bits(own));
-    }
+    for (int j = 0; j < kWave / kFWaves; ++j)
+      above += readlane_f32(own, wid * (kWave / kFWaves) + j) > own;
+    atomicAdd(&sm.above_key[lane], above);
+    __syncthreads();
+    theta = -wave_max(sm.above_key[lane] < C ? -own : -INFINITY);
   } else {
     int above = 0;
     const float4* keys = reinterpret_cast<const float4*>(sm.key);
@@ -377,62 +420,66 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
       const float4 o = keys[j];
       above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
     }
-    if (above < C) atomicMin(&sm.theta_key, ordered_bits(own));
+    const float least = wave_max(above < C ? -own : -INFINITY);
+    if (lane == 0) sm.fold[wid] = least;
+    __syncthreads();
+    float all = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kFWaves; ++k) all = fmaxf(all, sm.fold[k]);
+    theta = -all;
   }
-  __syncthreads();
-  const float theta = key_float(sm.theta_key);
-  // ---- the least logit of each beam that can reach theta, rounded down ----
-  if (tid < W) {
-    float f = INFINITY;
-    if (sm.score[tid] != -INFINITY) {
-      f = -3.402823466e38f;  // -inf is no candidate
-      if (theta != -INFINITY) {
-        // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
-        const double t = (double)theta - fabs((double)theta) * 0x1p-23;
-        f = fmaxf(f, __double2float_rd(t - (double)sm.score[tid] + sm.lse[tid]));
-      }
+  // ---- the least logit of each beam that can reach theta, rounded down: lane w's of every wave ----
+  float floor_w = INFINITY;
+  if (lane < W && sm.score[lane] != -INFINITY) {
+    floor_w = -3.402823466e38f;  // -inf is no candidate
+    if (theta != -INFINITY) {
+      // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
+      const double t = (double)theta - fabs((double)theta) * 0x1p-23;
+      floor_w = fmaxf(floor_w, __double2float_rd(t - (double)sm.score[lane] + sm.lse[lane]));
     }
-    sm.floor[tid] = f;
   }
-  __syncthreads();
-  auto list = [&](const float4& v, int i, int w) {
-    const float f = sm.floor[w];
-    if (f == INFINITY) return;
+  if (tid < W) sm.floor[tid] = floor_w;
+  auto list = [&](const float4& v, int i, int w, float f) {
     const float e[4] = {v.x, v.y, v.z, v.w};
+    if (!(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= f) || f == INFINITY) return;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       if (e[k] >= f) {
         const int pos = atomicAdd(&sm.listed, 1);
-        if (pos < kListCap) sm.list[pos] = i * 4 + k;
+        if (pos < kListCap) sm.list[pos] = make_int2(w, (i - w * per_row) * 4 + k);
       }
   };
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (held_row[k] >= 0) list(held[k], tid + k * kFThreads, held_row[k]);
-  for (int i = tid + kHeld * kFThreads; i < quads; i += kFThreads) list(top4[i], i, i / per_row);
+  for (int k = 0; k < kHeld; ++k) {
+    const float f = __shfl(floor_w, max(held_row[k], 0), kWave);
+    if (held_row[k] >= 0) list(held[k], tid + k * kFThreads, held_row[k], f);
+  }
+  for (int i0 = kHeld * kFThreads; i0 < quads; i0 += kFThreads) {
+    const int i = i0 + tid, w = min(i, quads - 1) / per_row;
+    const float f = __shfl(floor_w, w, kWave);
+    if (i < quads) list(top4[i], i, w, f);
+  }
   __syncthreads();
   const int listed = sm.listed;
   int found = 0;
   if (listed <= kListCap) {
     // ---- the entries under the listed tops, 16 lanes each, two tops at a time ----
     constexpr int kTeams = kFThreads / 16;
+    const S* x0 = static_cast<const S*>(p.logits);
     for (int b = tid / 16; b < listed; b += 2 * kTeams) {
       u32x4 q[2][NV];
-      int64_t base[2];
-      int row_of[2], col0[2], left[2];
+      int64_t col0[2];
+      int row_of[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int i = sm.list[min(b + k * kTeams, listed - 1)];
-        const int w = i / (nch * kTops), rest = i - w * (nch * kTops);
-        const int c = rest / kTops;
+        const int2 i = sm.list[min(b + k * kTeams, listed - 1)];
+        const int w = i.x, c = i.y / kTops;
         row_of[k] = w;
-        base[k] = (int64_t)c * CH;
-        left[k] = (int)min((int64_t)p.V - base[k], (int64_t)CH);
-        col0[k] = ((rest - c * kTops) * 16 + (tid & 15)) * VEC;
-        const S* row = beam_row<S>(p, first + w) + base[k];
+        col0[k] = (int64_t)c * CH + ((i.y % kTops) * 16 + (tid & 15)) * VEC;
+        const S* row = x0 + sm.row[w];
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          q[k][j] = load_vec_inside<DT>(row, col0[k] + j * kThreads * VEC, left[k]);
+          q[k][j] = load_vec_at<DT>(row, col0[k] + j * kThreads * VEC, p.V);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
@@ -440,18 +487,23 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
         const int w = row_of[k];
         const float f = sm.floor[w];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+          float most = vec_elem<DT>(q[k][j], 0);
+#pragma unroll
+          for (int e = 1; e < VEC; ++e) most = fmaxf(most, vec_elem<DT>(q[k][j], e));
+          if (!(most >= f)) continue;
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             const float x = vec_elem<DT>(q[k][j], e);
             if (!(x >= f)) continue;
-            const int col = inside_col<DT>(col0[k] + j * kThreads * VEC, e, left[k]);
+            const int col = column_at<DT>(col0[k] + j * kThreads * VEC, e, p.V);
             if (col < 0) continue;
             const int pos = atomicAdd(&sm.count, 1);
             if (pos < kCandCap)
               put(sm.cand, pos,
-                  {(double)sm.score[w] + ((double)x - sm.lse[w]), x, (int)(base[k] + col), w});
+                  {(double)sm.score[w] + ((double)x - sm.lse[w]), x, col, w});
           }
+        }
       }
     }
     __syncthreads();
@@ -477,7 +529,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   for (int w = 0; w < W; ++w) {
     __syncthreads();
     if (sm.floor[w] == INFINITY) continue;
-    const int got = row_largest<DT>(beam_row<S>(p, first + w), p.V, C, w, sm, 0);
+    const int got = row_largest<DT>(static_cast<const S*>(p.logits) + sm.row[w], p.V, C, w, sm, 0);
     __syncthreads();
     // the best so far and the beam's own: at most 2 C = 512, one a thread
     Candidate mine;
