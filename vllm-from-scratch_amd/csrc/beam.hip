@@ -302,21 +302,6 @@ __device__ inline float lanes_max(float v, int lanes) {
   return v;
 }
 
-// The 16-byte vector at column col of a row of V columns, and its columns, as load_vec_inside and
-// inside_col, for columns of every lane's own.
-template <int DT>
-__device__ inline u32x4 load_vec_at(const typename Elem<DT>::storage* row, int64_t col, int V) {
-  constexpr int VEC = Elem<DT>::kVec;
-  // uniform, so that a wave's loads stay in flight together (a branch of the lanes' own waits for each)
-  if (V >= VEC) return load_vec_any<DT>(row + min(col, (int64_t)(V - VEC)));
-  return load_vec_inside<DT>(row, (int)col, V);
-}
-template <int DT>
-__device__ inline int column_at(int64_t col, int e, int V) {
-  const int64_t i = min(col, (int64_t)max(V - Elem<DT>::kVec, 0)) + e;
-  return i >= col && i < V ? (int)i : -1;
-}
-
 // The group's candidates, in order, in sm.best; returns how many.
 template <int DT, int NV>
 __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem& sm) {
@@ -326,36 +311,38 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
   const int W = p.W, C = p.C, nch = p.nchunks;
   const int64_t first = (int64_t)g * W;
-  // ---- the tops, four of one chunk at a time; the first ones stay in registers ----
-  // (all of these loads are in flight together; a beam that was not scanned has whatever is there)
+  // ---- what the scan left: every load is issued before the first is waited for, so indices are
+  //      clamped instead of branched on.  A beam that was not scanned has whatever is there. ----
+  // tops: four of one chunk at a time, the first ones stay in registers
   const int per_row = nch * (kTops / 4), quads = W * per_row;
   const float4* top4 = reinterpret_cast<const float4*>(p.tops + first * nch * kTops);
   float4 held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) held[k] = top4[min(tid + k * kFThreads, quads - 1)];
+  // log-sums: as many lanes per beam as there are, a power of two from 8 to 64
+  const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
+  const int lse_w = tid / lanes, l = tid & (lanes - 1);
+  const float2* st = p.stats + (first + min(lse_w, W - 1)) * nch;
+  float2 v[kStats];
+#pragma unroll
+  for (int k = 0; k < kStats; ++k) v[k] = st[min(l + k * lanes, nch - 1)];
+  const float score = p.scores[first + min(lse_w, W - 1)];
+  int64_t row = first + min(tid, W - 1);
+  if (p.rows) row = min(max((int64_t)p.rows[row], (int64_t)0), p.num_rows - 1);
+  if (tid < W) sm.row[tid] = row * p.stride;
   int held_row[kHeld];
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {
     const int i = tid + k * kFThreads;
     held_row[k] = i < quads ? i / per_row : -1;
-    held[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    if (i < quads) held[k] = top4[i];
   }
-  if (tid < W) {
-    int64_t row = first + tid;
-    if (p.rows) row = min(max((int64_t)p.rows[first + tid], (int64_t)0), p.num_rows - 1);
-    sm.row[tid] = row * p.stride;
-  }
-  // ---- lse of every beam: as many lanes each as there are, a power of two from 8 to 64 ----
+  // ---- lse of every beam ----
   {
-    const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
-    const int w = tid / lanes, l = tid & (lanes - 1);
-    float M = -INFINITY, score = NAN;
-    float2 v[kStats];
-    const float2* st = p.stats + (first + min(w, W - 1)) * nch;
-    if (w < W) score = p.scores[first + w];
+    const int w = lse_w;
+    float M = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kStats; ++k) {
-      const int c = l + k * lanes;
-      v[k] = w < W && c < nch ? st[c] : make_float2(-INFINITY, 0.f);
+      if (w >= W || l + k * lanes >= nch) v[k] = make_float2(-INFINITY, 0.f);
       M = fmaxf(M, v[k].x);
     }
     if (w < W)
@@ -463,45 +450,65 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   const int listed = sm.listed;
   int found = 0;
   if (listed <= kListCap) {
-    // ---- the entries under the listed tops, 16 lanes each, two tops at a time ----
-    constexpr int kTeams = kFThreads / 16;
     const S* x0 = static_cast<const S*>(p.logits);
-    for (int b = tid / 16; b < listed; b += 2 * kTeams) {
-      u32x4 q[2][NV];
-      int64_t col0[2];
-      int row_of[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int2 i = sm.list[min(b + k * kTeams, listed - 1)];
-        const int w = i.x, c = i.y / kTops;
-        row_of[k] = w;
-        col0[k] = (int64_t)c * CH + ((i.y % kTops) * 16 + (tid & 15)) * VEC;
-        const S* row = x0 + sm.row[w];
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          q[k][j] = load_vec_at<DT>(row, col0[k] + j * kThreads * VEC, p.V);
+    if (p.V < VEC) {  // uniform: rows shorter than a vector
+      for (int i = tid; i < W * p.V; i += kFThreads) {
+        const int w = i / p.V, col = i - w * p.V;
+        const float x = Elem<DT>::cvt(x0[sm.row[w] + col]);
+        if (x >= sm.floor[w]) {
+          const int pos = atomicAdd(&sm.count, 1);
+          if (pos < kCandCap) put(sm.cand, pos, {0.0, x, col, w});
+        }
       }
+    } else {
+      // ---- the entries under the listed tops, 16 lanes each, two tops at a time ----
+      constexpr int kTeams = kFThreads / 16;
+      for (int b = tid / 16; b < listed; b += 2 * kTeams) {
+        u32x4 q[2][NV];
+        int64_t col0[2];
+        int row_of[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (b + k * kTeams >= listed) continue;
-        const int w = row_of[k];
-        const float f = sm.floor[w];
+        for (int k = 0; k < 2; ++k) {
+          const int2 i = sm.list[min(b + k * kTeams, listed - 1)];
+          const int w = i.x, c = i.y / kTops;
+          row_of[k] = w;
+          col0[k] = (int64_t)c * CH + ((i.y % kTops) * 16 + (tid & 15)) * VEC;
+          const S* row = x0 + sm.row[w];
+          // as load_vec_inside: the vector is moved back where it would pass the row's end
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          float most = vec_elem<DT>(q[k][j], 0);
+          for (int j = 0; j < NV; ++j)
+            q[k][j] = load_vec_any<DT>(row + min(col0[k] + j * kThreads * VEC, (int64_t)p.V - VEC));
+        }
 #pragma unroll
-          for (int e = 1; e < VEC; ++e) most = fmaxf(most, vec_elem<DT>(q[k][j], e));
-          if (!(most >= f)) continue;
+        for (int k = 0; k < 2; ++k) {
+          if (b + k * kTeams >= listed) continue;
+          // the lane's entries that reach the floor, a bit each; one or two of the 16 lanes have any
+          const int w = row_of[k];
+          const float f = sm.floor[w];
+          const int64_t end = (int64_t)p.V - VEC;
+          uint32_t mask = 0;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float x = vec_elem<DT>(q[k][j], e);
-            if (!(x >= f)) continue;
-            const int col = column_at<DT>(col0[k] + j * kThreads * VEC, e, p.V);
-            if (col < 0) continue;
-            const int pos = atomicAdd(&sm.count, 1);
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              mask |= vec_elem<DT>(q[k][j], e) >= f ? 1u << (j * VEC + e) : 0u;
+          if (mask == 0) continue;
+          if (col0[k] + (NV - 1) * kThreads * VEC > end) {
+            // vectors that were moved back: not what is in front of their own columns
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+              const int64_t over = min(max(col0[k] + j * kThreads * VEC - end, (int64_t)0),
+                                       (int64_t)VEC);
+              mask &= ~(((1u << over) - 1u) << (j * VEC));
+            }
+          }
+          int pos = atomicAdd(&sm.count, __popc(mask));
+          const S* row = x0 + sm.row[w];
+          for (; mask != 0; mask &= mask - 1u, ++pos) {
+            const int bit = __ffs(mask) - 1;
+            const int64_t at = min(col0[k] + (bit / VEC) * kThreads * VEC, end) + bit % VEC;
             if (pos < kCandCap)
-              put(sm.cand, pos,
-                  {(double)sm.score[w] + ((double)x - sm.lse[w]), x, col, w});
+              put(sm.cand, pos, {0.0, Elem<DT>::cvt(row[at]), (int)at, w});
           }
         }
       }
@@ -510,12 +517,25 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     found = sm.count;
   }
   if (listed <= kListCap && found <= kCandCap) {
+    for (int i = tid; i < found; i += kFThreads)
+      sm.cand.total[i] = (double)sm.score[sm.cand.beam[i]] +
+                         ((double)sm.cand.x[i] - sm.lse[sm.cand.beam[i]]);
+    __syncthreads();
     // ranked by counting, eight threads to a candidate
     for (int i0 = 0; i0 < found; i0 += kFThreads / 8) {
       const int i = i0 + tid / 8;
       const Candidate mine = get(sm.cand, min(i, found - 1));
-      int rank = 0;
-      for (int j = tid & 7; j < found; j += 8) rank += before(sm.cand, j, mine);
+      int rank = 0, equal = 0;
+#pragma unroll 4
+      for (int j = tid & 7; j < found; j += 8) {
+        const double t = sm.cand.total[j];
+        rank += t > mine.total;
+        equal += t == mine.total;
+      }
+      if (equal > ((i & 7) == (tid & 7))) {  // others than itself
+        rank = 0;
+        for (int j = tid & 7; j < found; j += 8) rank += before(sm.cand, j, mine);
+      }
       rank += dpp_i32<kDppXor1>(rank);
       rank += dpp_i32<kDppXor2>(rank);
       rank += dpp_i32<kDppHalfMirror>(rank);
