@@ -630,6 +630,27 @@ def test_streams_and_graphs(device):
             assert torch.equal(a[2].token_ids, b[2].token_ids)
 
 
+def test_scratch_grows_and_is_kept_per_stream(device):
+    """Calls of growing and shrinking sizes on two streams at once."""
+    sizes = [(1, 4, 500), (8, 8, 30000), (2, 3, 9000), (64, 8, 50257), (1, 1, 40), (64, 8, 50257)]
+    cases = []
+    for k, (G, W, V) in enumerate(sizes):
+        gen = torch.Generator(device=device).manual_seed(k)
+        cases.append((torch.randn(G * W, V, device=device, generator=gen), make_scores(device, G, W, k)))
+    want = [beam_search_select(x, s, 8) for x, s in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for x, s in cases * 3:
+        for k, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[k].append(beam_search_select(x, s, 8))
+    torch.cuda.synchronize()
+    for mine in got:
+        for a, b in zip(mine, want * 3):
+            assert torch.equal(a.token_ids, b.token_ids) and torch.equal(a.scores, b.scores)
+
+
 def test_same_results_twice(device):
     G, W, V = 16, 8, 32000
     gen = torch.Generator(device=device).manual_seed(0)

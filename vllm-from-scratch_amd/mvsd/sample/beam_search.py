@@ -15,8 +15,8 @@ group's beams in the order g * W + w.
     answers = search.finish(n)                  # token ids, lengths and scores of the n best
 
 Nothing here synchronises the host.  Work is enqueued on the current stream of the logits' (or
-states') device; scratch comes from torch's allocator within the call, so calls on several streams
-and captured graphs share nothing.
+states') device.  Scratch is kept per stream; a captured call has its own, so calls on several
+streams and captured graphs share nothing.
 """
 
 from __future__ import annotations
@@ -109,7 +109,7 @@ _DTYPES = (_F32, _I32, torch.bool, _F32, _I32, _I32, _I32)
 # the places of their addresses in the argument structures, in eight-byte words
 _STEP_HEAD, _STEP_TENSORS = struct.Struct("=10qdii"), 12
 _FINISH_HEAD, _FINISH_TENSORS = struct.Struct("=4qd"), 5
-_TAIL = struct.Struct("=2q")
+_STEP_TAIL, _FINISH_TAIL = struct.Struct("=4q"), struct.Struct("=5q")
 
 
 def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
@@ -178,11 +178,29 @@ def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.devi
     return device
 
 
-def _workspace(G: int, W: int, V: int, C: int, device) -> tuple[torch.Tensor, int]:
+# Scratch of selections and steps, kept per (device, stream): calls on one stream follow each other.
+_SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, int, int]] = {}
+_SCRATCH_MOST = 1 << 24
+
+
+def _scratch(G: int, W: int, V: int, C: int, device: torch.device,
+             stream: int) -> tuple[torch.Tensor, int, int]:
+    """(workspace, its address, its size) of a call."""
     size = nat.lib().mvsd_beam_workspace_bytes(G, W, V, C)
+    kept = _SCRATCH.get((device.index, stream))
+    capturing = torch.cuda.is_current_stream_capturing()
+    if kept is not None and kept[2] >= size > 0 and not capturing:
+        return kept
     if size <= 0:
         raise ValueError(f"{G} groups of {W} beams over {V} tokens are more than one call takes")
-    return torch.empty(size, dtype=torch.uint8, device=device), size
+    keep = size <= _SCRATCH_MOST and not capturing
+    if keep and kept is not None:
+        size = min(max(size, 2 * kept[2]), _SCRATCH_MOST)
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    made = ws, ws.data_ptr(), size
+    if keep:  # a captured call can be replayed beside later ones on this stream: it has its own
+        _SCRATCH[device.index, stream] = made
+    return made
 
 
 def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int, *,
@@ -208,18 +226,19 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     if _elsewhere(device):
         with torch.cuda.device(device):
             return beam_search_select(logits, scores, C, target_rows=target_rows)
-    ids = torch.empty((3, G, C), dtype=_I32, device=device)
+    ids = torch.empty(3, G, C, dtype=_I32, device=device)
     token_ids, parents, bits = ids.unbind(0)
     out = BeamCandidates(token_ids, parents, bits.view(_F32))
     if G == 0:
         return out
     rows, V = logits.shape
-    ws, size = _workspace(G, W, V, C, device)
+    stream = nat.stream_of(device)
+    scratch = _scratch(G, W, V, C, device, stream)
     base = ids.data_ptr()
     nat.check(nat.lib().mvsd_beam_select(
         base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
         nat.dtype_code(logits.dtype), logits.stride(0), rows, nat.ptr(target_rows),
-        scores.data_ptr(), G, W, V, C, ws.data_ptr(), size, nat.stream_of(device)),
+        scores.data_ptr(), G, W, V, C, scratch[1], scratch[2], stream),
         "mvsd_beam_select")
     return out
 
@@ -279,15 +298,15 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
     if G == 0:
         return step
     rows, V = logits.shape
-    ws, size = _workspace(G, W, V, C, device)
+    stream = nat.stream_of(device)
+    scratch = _scratch(G, W, V, C, device, stream)
     _STEP_HEAD.pack_into(args, 0, logits.data_ptr(), logits.stride(0), rows,
                          0 if target_rows is None else target_rows.data_ptr(), G, W, V, T,
                          stop_token_ids.data_ptr() if E else 0, E, length_penalty,
                          nat.dtype_code(logits.dtype), 1 if early_stopping else 0)
-    _TAIL.pack_into(args, 8 * (_STEP_TENSORS + 16), token_ids.data_ptr(), parents.data_ptr())
-    _TAIL.pack_into(args, 8 * (_STEP_TENSORS + 18), ws.data_ptr(), size)
-    nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), nat.stream_of(device)),
-              "mvsd_beam_step")
+    _STEP_TAIL.pack_into(args, 8 * (_STEP_TENSORS + 16), token_ids.data_ptr(), parents.data_ptr(),
+                         scratch[1], scratch[2])
+    nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), stream), "mvsd_beam_step")
     return step
 
 
@@ -317,19 +336,17 @@ def beam_search_finish(state: BeamState, num_return: int | None = None, *,
     _addresses(args, _FINISH_TENSORS, _FINISH_NAMES,
                _fields(state) + (state.token_history, state.parent_history), _FINISH_DTYPES,
                (a, b, b, a, a, a, a, c, c), device)
-    ids = torch.empty((G, n, T), dtype=_I32, device=device)
-    lengths = torch.empty((G, n), dtype=_I32, device=device)
-    scores = torch.empty((G, n), dtype=_F32, device=device)
+    ids = torch.empty(G, n, T, dtype=_I32, device=device)
+    lengths = torch.empty(G, n, dtype=_I32, device=device)
+    scores = torch.empty(G, n, dtype=_F32, device=device)
     out = BeamHypotheses(ids, lengths, scores)
     if G == 0:
         return out
     size = nat.lib().mvsd_beam_finish_workspace_bytes(G, W, T, n)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
     _FINISH_HEAD.pack_into(args, 0, G, W, T, n, length_penalty)
-    _TAIL.pack_into(args, 8 * (_FINISH_TENSORS + 9), ids.data_ptr(), lengths.data_ptr())
-    _TAIL.pack_into(args, 8 * (_FINISH_TENSORS + 11), scores.data_ptr(),
-                    0 if ws is None else ws.data_ptr())
-    args.workspace_bytes = size
+    _FINISH_TAIL.pack_into(args, 8 * (_FINISH_TENSORS + 9), ids.data_ptr(), lengths.data_ptr(),
+                           scores.data_ptr(), 0 if ws is None else ws.data_ptr(), size)
     nat.check(nat.lib().mvsd_beam_finish(ctypes.byref(args), nat.stream_of(device)),
               "mvsd_beam_finish")
     return out
