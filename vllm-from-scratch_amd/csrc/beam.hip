@@ -619,7 +619,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   }
   const int found = group_candidates<DT, NV>(p, g, sm);
   const int new_len = len + 1;
-  const double power = pow((double)new_len, a.length_penalty);
+  const double power = len_power(new_len, a.length_penalty);
   if (wid < kMaxCandidates / kWave) {
     bool stop = false;
     if (tid < found)
