@@ -73,7 +73,20 @@ __device__ inline const S* beam_row(const BeamScanParams& p, int64_t r) {
   return static_cast<const S*>(p.logits) + row * p.stride;
 }
 
-template <int DT, int NV>
+// Rows of kStreamBytes together are read past the caches: what the model's last product left of them
+// does not fit the 256 MB that the memory side keeps, and nothing of a scan is read again but the few
+// entries of the finish.  bf16 rows, cached and past the caches: 78 MB 21.9 and
+// 22.0 us, 102 MB 26.4 and 26.7, 160 MB 35.7 and 34.2, 311 MB 61.8 and 56.4.
+constexpr int64_t kStreamBytes = 128ll << 20;
+
+template <int DT, bool STREAM>
+__device__ inline u32x4 load_scan(const typename Elem<DT>::storage* row, int col, int V) {
+  if (!STREAM || V < Elem<DT>::kVec) return load_vec_inside<DT>(row, col, V);
+  return __builtin_nontemporal_load(
+      reinterpret_cast<const Vec16<DT>*>(row + min(col, V - Elem<DT>::kVec)));
+}
+
+template <int DT, int NV, bool STREAM>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   using S = typename Elem<DT>::storage;
   constexpr int VEC = Elem<DT>::kVec;
@@ -88,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   row += base;
   u32x4 q[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) q[j] = load_vec_inside<DT>(row, (j * kThreads + tid) * VEC, left);
+  for (int j = 0; j < NV; ++j) q[j] = load_scan<DT, STREAM>(row, (j * kThreads + tid) * VEC, left);
   float v[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -193,6 +206,7 @@ struct BeamSmem {
   int hist[256];
   int wave_cnt[kFWaves];
   uint64_t stop_mask[kMaxCandidates / kWave], on_mask[kMaxCandidates / kWave];
+  int stop[kMaxCandidates];  // a step's stop tokens
   float pool[2 * kMaxBeams];
   int listed, count, above, digit;
   float worst;
@@ -597,21 +611,28 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
                                                                mvsd_beam_step_args a) {
   __shared__ BeamSmem sm;
   const int g = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wid = wave_id();
-  const int W = p.W, C = p.C;
-  const int64_t first = (int64_t)g * W;
+  const int W = p.W;
+  const int64_t first = (int64_t)g * W, at = first + min(tid, W - 1);
+  // the state, before anything is written (outputs may be inputs) and while the scan's results arrive
   const int len = p.lengths[g];
-  if (group_rests(p, g)) {  // block-uniform
+  const uint8_t was = a.done[g];
+  float hyp = a.finished_scores[at];
+  int hyp_beam = a.finished_beams[at], hyp_token = a.finished_token_ids[at];
+  int hyp_len = a.finished_lengths[at];
+  const float old_score = a.scores[at];
+  const int E = (int)a.num_stop_ids;
+  if (tid < E) sm.stop[tid] = a.stop_token_ids[tid];
+  if (was != 0 || len < 0 || len >= p.max_length) {  // the group rests (block-uniform)
     if (tid < W) {
       a.token_ids[first + tid] = -1;
       a.parents[first + tid] = -1;
-      a.out_scores[first + tid] = a.scores[first + tid];
-      a.out_finished_scores[first + tid] = a.finished_scores[first + tid];
-      a.out_finished_beams[first + tid] = a.finished_beams[first + tid];
-      a.out_finished_token_ids[first + tid] = a.finished_token_ids[first + tid];
-      a.out_finished_lengths[first + tid] = a.finished_lengths[first + tid];
+      a.out_scores[first + tid] = old_score;
+      a.out_finished_scores[first + tid] = hyp;
+      a.out_finished_beams[first + tid] = hyp_beam;
+      a.out_finished_token_ids[first + tid] = hyp_token;
+      a.out_finished_lengths[first + tid] = hyp_len;
     }
     if (tid == 0) {
-      const uint8_t was = a.done[g];
       a.out_lengths[g] = len;
       a.out_done[g] = was;
     }
@@ -622,26 +643,20 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   const double power = len_power(new_len, a.length_penalty);
   if (wid < kMaxCandidates / kWave) {
     bool stop = false;
-    if (tid < found)
-      for (int64_t e = 0; e < a.num_stop_ids; ++e)
-        stop |= sm.best.token[tid] == a.stop_token_ids[e];
+    if (tid < found) {
+      const int token = sm.best.token[tid];
+      for (int e = 0; e < E; ++e) stop |= token == sm.stop[e];
+    }
     const uint64_t sb = __ballot(stop), ob = __ballot(tid < found && !stop);
     if (lane == 0) {
       sm.stop_mask[wid] = sb;
       sm.on_mask[wid] = ob;
     }
   }
-  // the old hypotheses, and what they hold, before anything is written (outputs may be inputs)
-  float hyp = -INFINITY;
-  int hyp_beam = -1, hyp_token = -1, hyp_len = 0;
-  if (tid < W) {
-    hyp = a.finished_scores[first + tid];
-    if (!(hyp > -INFINITY)) hyp = -INFINITY;
-    else {
-      hyp_beam = a.finished_beams[first + tid];
-      hyp_token = a.finished_token_ids[first + tid];
-      hyp_len = a.finished_lengths[first + tid];
-    }
+  if (tid >= W || !(hyp > -INFINITY)) {
+    hyp = -INFINITY;
+    hyp_beam = hyp_token = -1;
+    hyp_len = 0;
   }
   __syncthreads();
   // ---- next beams ----
@@ -726,11 +741,14 @@ static void launch_dt(const BeamScanParams& p, const BeamSelectOut* o,
   constexpr int kShort = kBeamShort / (kThreads * Elem<DT>::kVec);
   const dim3 scan((unsigned)(p.G * p.W) * (unsigned)p.nchunks), groups(p.G);
   if (chunk == kBeamLong) {
-    hipLaunchKernelGGL((beam_scan_kernel<DT, kLong>), scan, dim3(kThreads), 0, stream, p);
+    if ((int64_t)p.G * p.W * p.V * (int64_t)sizeof(typename Elem<DT>::storage) >= kStreamBytes)
+      hipLaunchKernelGGL((beam_scan_kernel<DT, kLong, true>), scan, dim3(kThreads), 0, stream, p);
+    else
+      hipLaunchKernelGGL((beam_scan_kernel<DT, kLong, false>), scan, dim3(kThreads), 0, stream, p);
     if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *o);
     else hipLaunchKernelGGL((beam_step_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *a);
   } else {
-    hipLaunchKernelGGL((beam_scan_kernel<DT, kShort>), scan, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((beam_scan_kernel<DT, kShort, false>), scan, dim3(kThreads), 0, stream, p);
     if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *o);
     else hipLaunchKernelGGL((beam_step_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *a);
   }

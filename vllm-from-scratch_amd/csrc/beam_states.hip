@@ -147,7 +147,7 @@ constexpr int kSub = 16, kSpan = 8, kSpanSteps = kSub * kSpan;
 constexpr int kTraceLds = 50 * 1024;  // of W + n bytes a step; the maps and the padding add a fifth
 constexpr int kMapPiece = 4096;       // bytes of chunk maps held at a time
 constexpr int kAhead = 8;             // vectors of parents, and of tokens, that a thread holds
-constexpr int kTraceGroups = 512;     // workgroups that a launch is split into at least
+constexpr int kTraceGroups = 256;     // workgroups that a launch is split into at least
 enum { kTraceWhole, kTraceMaps, kTraceEmit };
 
 // Steps per chunk: the whole history where it fits LDS and is short, else 2048 steps or fewer.
@@ -510,8 +510,9 @@ hipError_t launch_beam_finish(const mvsd_beam_finish_args& a, hipStream_t stream
   const int S = trace_chunk(W, n, a.max_length);
   const int chunks = (int)((a.max_length + S - 1) / S);
   const int64_t wgs = a.num_groups * chunks;
-  // hypotheses shared out until there are kTraceGroups workgroups (64 groups of 8 hypotheses and 2048
-  // steps: SPLIT_FIGURES)
+  // hypotheses shared out until there are kTraceGroups workgroups, one per compute unit: 64 groups of 8
+  // beams and 2048 steps take 19.4 us unshared, 15.9 with 128, 14.2 with 256 and 19.4 with 512 (every
+  // workgroup reads the group's histories); 8 groups of 32 beams and 512 steps 16.7, 14.8, 13.7, 13.8
   const int64_t want = wgs < kTraceGroups ? (kTraceGroups + wgs - 1) / wgs : 1;
   const int per = want < n ? (int)((n + want - 1) / want) : 1;
   const int parts = (n + per - 1) / per;
