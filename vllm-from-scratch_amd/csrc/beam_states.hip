@@ -46,8 +46,9 @@ __device__ inline void move_rows(const char* src, char* dst, int64_t src_stride,
 #pragma unroll
     for (int w = 0; w < ROWS; ++w)
       if ((moves >> (b + w)) & 1)
-        *reinterpret_cast<U*>(dst + (int64_t)__builtin_amdgcn_readlane(to, b + w) * dst_stride +
-                              off) = v[w];
+        __builtin_nontemporal_store(
+            v[w], reinterpret_cast<U*>(
+                      dst + (int64_t)__builtin_amdgcn_readlane(to, b + w) * dst_stride + off));
   }
 }
 
