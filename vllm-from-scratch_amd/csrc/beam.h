@@ -50,7 +50,11 @@ struct BeamScanParams {
   int G, W, V, C;
   int max_length;  // step: T
   int nchunks;
-  float2* stats;  // [G * W, nchunks] chunk maximum and sum of exp(x - maximum)
+  struct alignas(16) Stat {
+    double sum;  // of exp(x - max)
+    float max;
+  };
+  Stat* stats;    // [G * W, nchunks] chunk maximum and sum
   float* tops;    // [G * W, nchunks, 16] the largest entry of 16 lanes each
 };
 

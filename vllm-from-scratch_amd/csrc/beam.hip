@@ -59,6 +59,28 @@ __device__ inline float exp_of(float d) {
 
 __device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// Sums and maxima over `lanes` (a power of two from 8 to 64) neighbouring lanes, in each of them.
+template <int CTRL>
+__device__ inline double dpp_f64(double v) {
+  return __builtin_bit_cast(double, dpp_u64<CTRL>(__builtin_bit_cast(uint64_t, v)));
+}
+__device__ inline double lanes_sum(double v, int lanes) {
+  v += dpp_f64<kDppXor1>(v);
+  v += dpp_f64<kDppXor2>(v);
+  v += dpp_f64<kDppHalfMirror>(v);
+  if (lanes > 8) v += dpp_f64<kDppMirror>(v);
+  for (int off = 16; off < lanes; off *= 2) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+__device__ inline float lanes_max(float v, int lanes) {
+  v = fmaxf(v, dpp_f32<kDppXor1>(v));
+  v = fmaxf(v, dpp_f32<kDppXor2>(v));
+  v = fmaxf(v, dpp_f32<kDppHalfMirror>(v));
+  if (lanes > 8) v = fmaxf(v, dpp_f32<kDppMirror>(v));
+  for (int off = 16; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor(v, off, kWave));
+  return v;
+}
+
 // Whether a step leaves the group as it is.
 __device__ inline bool group_rests(const BeamScanParams& p, int g) {
   if (!p.lengths) return false;
@@ -91,7 +113,8 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   using S = typename Elem<DT>::storage;
   constexpr int VEC = Elem<DT>::kVec;
   constexpr int CH = NV * kThreads * VEC;
-  __shared__ float s_m[kWaves], s_s[kWaves];
+  __shared__ float s_m[kWaves];
+  __shared__ double s_s[kWaves];
   const int r = blockIdx.x / p.nchunks, c = blockIdx.x - r * p.nchunks;
   if (!finite(p.scores[r]) || group_rests(p, r / p.W)) return;  // the finish does the same test
   const S* row = beam_row<S>(p, r);
@@ -131,24 +154,24 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += v[j][e] != v[j][e] ? NAN : 0.f;
   }
-  s = wave_sum(s);
+  const double sum64 = lanes_sum((double)s, kWave);
   const int64_t slot = (int64_t)r * p.nchunks + c;
   if ((tid & 15) == 0) p.tops[slot * kTops + tid / 16] = top;
   if (lane_id() == 0) {
     s_m[wave_id()] = wm;
-    s_s[wave_id()] = s;
+    s_s[wave_id()] = sum64;
   }
   __syncthreads();
-  if (tid == 0) {
-    float M = s_m[0], sum = 0.f;
+  if (wave_id() != 0) return;
+  // the waves' sums, each with its own maximum
+  float M = s_m[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w]);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      sum += s_m[w] == -INFINITY ? s_s[w]
-                                 : s_s[w] * exp_of(s_m[w] - M);
-    p.stats[slot] = make_float2(M, sum);
-  }
+  for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w]);
+  const int w = tid % kWaves;
+  double sum = s_m[w] == -INFINITY ? s_s[w] : s_s[w] * exp((double)s_m[w] - (double)M);
+  sum += dpp_f64<kDppXor1>(sum);
+  sum += dpp_f64<kDppXor2>(sum);
+  if (tid == 0) p.stats[slot] = {sum, M};
 }
 
 // ------------------------------------------------------------------ finish -----------
@@ -194,7 +217,7 @@ __device__ inline bool before(const Candidates<N>& c, int j, const Candidate& mi
 
 struct BeamSmem {
   Candidates<kCandCap> cand;
-  Candidates<kMaxCandidates> best;  // the group's candidates in order
+  Candidates<kMaxCandidates + 1> best;  // the group's candidates in order, and the next one
   int2 list[kListCap];  // beam, top of the beam's row
   __align__(16) float key[kFThreads];
   float fold[kFWaves];
@@ -202,6 +225,9 @@ struct BeamSmem {
   int64_t row[kMaxBeams];  // the first element of each beam's row
   double lse[kMaxBeams];
   float score[kMaxBeams];  // -inf: proposes nothing
+  float most[kMaxBeams];   // the row's largest entry
+  double red[kFWaves];
+  uint64_t near_ties;      // beams whose candidates' order depends on their lse's last digits
   float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
   int hist[256];
   int wave_cnt[kFWaves];
@@ -212,108 +238,200 @@ struct BeamSmem {
   float worst;
 };
 
-// The C largest entries of one row, by (value desc, token asc), into cand[at ..]; returns how many.
-// Radix selection of the C-th largest key, eight bits at a time, then one pass for the entries
-// above it and one, from the first column, for as many equal ones as are missing.
+// The C-th largest of the workgroup's keys (in sm.key, `own` the thread's): fewer than C keys are above
+// it, and it is the least such key.
+__device__ inline float block_theta(float own, int C, BeamSmem& sm) {
+  int above = 0;
+  const float4* keys = reinterpret_cast<const float4*>(sm.key);
+#pragma unroll 8
+  for (int j = 0; j < kFThreads / 4; ++j) {
+    const float4 o = keys[j];
+    above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+  }
+  const float least = wave_max(above < C ? -own : -INFINITY);
+  if (lane_id() == 0) sm.fold[wave_id()] = least;
+  __syncthreads();
+  float all = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kFWaves; ++k) all = fmaxf(all, sm.fold[k]);
+  return -all;
+}
+
+// Calls see(col, x) for a workgroup's share of the columns [from, to) of a row whose entries pass
+// test(x): four vectors of a thread in flight, a vector without such an entry is one comparison.
+template <int DT, typename Test, typename See>
+__device__ inline void sweep(const typename Elem<DT>::storage* row, int from, int to, Test&& test,
+                             See&& see) {
+  constexpr int VEC = Elem<DT>::kVec, kDeep = 4;
+  const int tid = threadIdx.x;
+  if (to - from < VEC) {
+    for (int i = from + tid; i < to; i += kFThreads) {
+      const float x = Elem<DT>::cvt(row[i]);
+      if (test(x)) see(i, x);
+    }
+    return;
+  }
+  for (int64_t b = from; b < to; b += kDeep * kFThreads * VEC) {
+    u32x4 q[kDeep];
+    int64_t col[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      col[k] = b + (int64_t)(k * kFThreads + tid) * VEC;
+      q[k] = load_vec_any<DT>(row + min(col[k], (int64_t)to - VEC));
+    }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int64_t at = min(col[k], (int64_t)to - VEC);  // moved back at the end
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) any |= test(vec_elem<DT>(q[k], e));
+      if (!any) continue;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (at + e >= col[k] && test(vec_elem<DT>(q[k], e))) see((int)(at + e), vec_elem<DT>(q[k], e));
+    }
+  }
+}
+
+// The C largest entries of beam w's row, by (value desc, token asc), into cand[at ..]; returns how
+// many.  Fewer than C unions of the row's tops are above the C-th largest union, theta.  Where fewer
+// than C entries are above theta (runs of one value: the case that comes here), they and the first
+// entries equal to theta are the answer: one sweep over the row, and one that ends early.  Otherwise a
+// radix selection of the C-th largest key, eight bits at a time, and those two sweeps again.
 template <int DT>
-__device__ inline int row_largest(const typename Elem<DT>::storage* row, int V, int C, int beam,
-                                  BeamSmem& sm, int at) {
+__device__ inline int row_largest(const BeamScanParams& p, int64_t beam_row, int beam, BeamSmem& sm,
+                                  int at) {
+  using S = typename Elem<DT>::storage;
   const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
   constexpr uint32_t kNinf = 0x007fffffu;  // ordered_bits(-inf): not a candidate
-  uint32_t prefix = 0, mask = 0;
-  int want = C;
-  bool all = false;  // fewer than C entries: take every one
-  for (int shift = 24; shift >= 0 && !all; shift -= 8) {
-    for (int i = tid; i < 256; i += kFThreads) sm.hist[i] = 0;
+  const S* row = static_cast<const S*>(p.logits) + sm.row[beam];
+  const int V = p.V, C = p.C;
+  float theta;
+  {
+    const float* tops = p.tops + beam_row * p.nchunks * kTops;
+    float own = -INFINITY;
+    for (int i = tid; i < p.nchunks * kTops; i += kFThreads) own = fmaxf(own, tops[i]);
+    sm.key[tid] = own;
+    if (tid == 0) sm.count = 0;
     __syncthreads();
-    for (int64_t i = tid; i < V; i += kFThreads) {
-      const uint32_t key = ordered_bits(Elem<DT>::cvt(row[i]));
-      const bool in = key > kNinf && (key & mask) == prefix;
-      const uint32_t digit = (key >> shift) & 255u;
-      const uint64_t live = __ballot(in);
-      if (live == 0) continue;
-      // one addition for the lanes that share the first one's digit, the rest one each
-      const int leader = __ffsll((long long)live) - 1;
-      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)digit, leader);
-      const uint64_t same = __ballot(in && digit == first);
-      if (lane == leader) atomicAdd(&sm.hist[first], __popcll(same));
-      if (in && digit != first) atomicAdd(&sm.hist[digit], 1);
-    }
+    theta = block_theta(own, C, sm);
+  }
+  auto keep = [&](int col, float x) {
+    const int pos = atomicAdd(&sm.count, 1);
+    if (pos < C) put(sm.cand, at + pos, {0.0, x, col, beam});
+  };
+  sweep<DT>(row, 0, V, [&](float x) { return x > theta; }, keep);
+  __syncthreads();
+  int found = sm.count;
+  if (found < C) {
+    if (theta == -INFINITY) return found;
+  } else {
+    theta = -INFINITY;  // to be found
+  }
+  if (theta == -INFINITY) {
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, d = 255;
-      while (d > 0 && above + sm.hist[d] < want) above += sm.hist[d--];
-      sm.digit = above + sm.hist[d] < want ? -1 : d;
-      sm.above = above;
-    }
-    __syncthreads();
-    if (sm.digit < 0) {
-      all = true;  // only in the first round: later ones count what the round before found
-    } else {
+    uint32_t prefix = 0, mask = 0;
+    int want = C;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += kFThreads) sm.hist[i] = 0;
+      __syncthreads();
+      sweep<DT>(
+          row, 0, V,
+          [&](float x) {
+            const uint32_t key = ordered_bits(x);
+            return key > kNinf && (key & mask) == prefix;
+          },
+          [&](int, float x) { atomicAdd(&sm.hist[(ordered_bits(x) >> shift) & 255u], 1); });
+      __syncthreads();
+      if (tid == 0) {
+        int above = 0, d = 255;  // at least C entries: every round finds its digit
+        while (d > 0 && above + sm.hist[d] < want) above += sm.hist[d--];
+        sm.digit = d;
+        sm.above = above;
+        sm.count = 0;
+      }
+      __syncthreads();
       want -= sm.above;
       prefix |= (uint32_t)sm.digit << shift;
       mask |= 255u << shift;
+      __syncthreads();
     }
+    theta = key_float(prefix);
+    sweep<DT>(row, 0, V, [&](float x) { return x > theta; }, keep);
     __syncthreads();
+    found = min(sm.count, C);
   }
-  const uint32_t kth = all ? kNinf : prefix;  // entries above it are taken, equal ones as wanted
-  if (tid == 0) sm.count = 0;
-  __syncthreads();
-  for (int64_t i = tid; i < V; i += kFThreads) {
-    const float x = Elem<DT>::cvt(row[i]);
-    if (ordered_bits(x) > kth) {
-      const int pos = atomicAdd(&sm.count, 1);
-      if (pos < C) {
-        put(sm.cand, at + pos, {0.0, x, (int)i, beam});
+  // as many entries equal to theta as are missing, from the first column
+  const int block = 8 * kFThreads * Elem<DT>::kVec;
+  for (int64_t b = 0; b < V && found < C; b += block) {
+    const int end = (int)min(b + block, (int64_t)V);
+    bool here = false;
+    sweep<DT>(row, (int)b, end, [&](float x) { return x == theta; }, [&](int, float) { here = true; });
+    if (!__syncthreads_or(here)) continue;
+    for (int64_t i0 = b; i0 < end && found < C; i0 += kFThreads) {
+      const int64_t i = i0 + tid;
+      const float x = i < end ? Elem<DT>::cvt(row[i]) : NAN;
+      const uint64_t hit = __ballot(x == theta);
+      if (lane == 0) sm.wave_cnt[wid] = __popcll(hit);
+      __syncthreads();
+      int pos = found, total = 0;
+      for (int w = 0; w < kFWaves; ++w) {
+        pos += w < wid ? sm.wave_cnt[w] : 0;
+        total += sm.wave_cnt[w];
       }
+      pos += __popcll(hit & ((1ull << lane) - 1ull));
+      if (x == theta && pos < C) put(sm.cand, at + pos, {0.0, x, (int)i, beam});
+      found = min(found + total, C);
+      __syncthreads();
     }
-  }
-  __syncthreads();
-  int found = min(sm.count, C);
-  __syncthreads();
-  if (all) return found;
-  for (int64_t b = 0; b < V && found < C; b += kFThreads) {
-    const int64_t i = b + tid;
-    const float x = i < V ? Elem<DT>::cvt(row[i]) : -INFINITY;
-    const bool eq = i < V && ordered_bits(x) == kth;
-    const uint64_t hit = __ballot(eq);
-    if (lane == 0) sm.wave_cnt[wid] = __popcll(hit);
-    __syncthreads();
-    int pos = found, total = 0;
-    for (int w = 0; w < kFWaves; ++w) {
-      pos += w < wid ? sm.wave_cnt[w] : 0;
-      total += sm.wave_cnt[w];
-    }
-    pos += __popcll(hit & ((1ull << lane) - 1ull));
-    if (eq && pos < C) {
-      put(sm.cand, at + pos, {0.0, x, (int)i, beam});
-    }
-    found = min(found + total, C);
-    __syncthreads();
   }
   return found;
 }
 
-// Sums and maxima over `lanes` (a power of two from 8 to 64) neighbouring lanes, in each of them.
-template <int CTRL>
-__device__ inline double dpp_f64(double v) {
-  return __builtin_bit_cast(double, dpp_u64<CTRL>(__builtin_bit_cast(uint64_t, v)));
+// The lse of a beam in 64 bits throughout, into sm.lse.
+template <int DT>
+__device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
+  using S = typename Elem<DT>::storage;
+  const int tid = threadIdx.x;
+  const S* row = static_cast<const S*>(p.logits) + sm.row[w];
+  const double most = (double)sm.most[w];
+  double s = 0.0;
+#pragma unroll 4
+  for (int64_t i = tid; i < p.V; i += kFThreads) s += exp((double)Elem<DT>::cvt(row[i]) - most);
+  s = lanes_sum(s, kWave);
+  if (lane_id() == 0) sm.red[wave_id()] = s;
+  __syncthreads();
+  if (tid == 0) {
+    double all = 0.0;
+    for (int k = 0; k < kFWaves; ++k) all += sm.red[k];
+    sm.lse[w] = most + log(all);
+  }
+  __syncthreads();
 }
-__device__ inline double lanes_sum(double v, int lanes) {
-  v += dpp_f64<kDppXor1>(v);
-  v += dpp_f64<kDppXor2>(v);
-  v += dpp_f64<kDppHalfMirror>(v);
-  if (lanes > 8) v += dpp_f64<kDppMirror>(v);
-  for (int off = 16; off < lanes; off *= 2) v += __shfl_xor(v, off, kWave);
-  return v;
-}
-__device__ inline float lanes_max(float v, int lanes) {
-  v = fmaxf(v, dpp_f32<kDppXor1>(v));
-  v = fmaxf(v, dpp_f32<kDppXor2>(v));
-  v = fmaxf(v, dpp_f32<kDppHalfMirror>(v));
-  if (lanes > 8) v = fmaxf(v, dpp_f32<kDppMirror>(v));
-  for (int off = 16; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor(v, off, kWave));
-  return v;
+
+// Of the first `have` candidates in sm.best: where two neighbours of different beams are closer than
+// kNear, the lse of both beams is formed again, in 64 bits throughout, and true returned: the totals
+// have to be formed and ranked again.  A row of 151936 entries takes about NEAR_US us; a group of 8
+// beams and 16 candidates has such a pair about once in ten thousand.
+constexpr double kNear = 0x1p-21;
+
+template <int DT>
+__device__ inline bool settle_near_ties(const BeamScanParams& p, int have, BeamSmem& sm) {
+  const int tid = threadIdx.x;
+  if (tid == 0) sm.near_ties = 0;
+  __syncthreads();
+  if (tid + 1 < have) {
+    const int a = sm.best.beam[tid], b = sm.best.beam[tid + 1];
+    const double t = sm.best.total[tid];
+    // (totals too large for the difference to show: masks of the type's lowest value)
+    if (a != b && fabs(t) < 0x1p20 && t - sm.best.total[tid + 1] < kNear)
+      atomicOr((unsigned long long*)&sm.near_ties, 1ull << a | 1ull << b);
+  }
+  __syncthreads();
+  const uint64_t beams = sm.near_ties;
+  for (uint64_t left = beams; left != 0; left &= left - 1)
+    exact_lse<DT>(p, __ffsll((long long)left) - 1, sm);
+  return beams != 0;
 }
 
 // The group's candidates, in order, in sm.best; returns how many.
@@ -336,8 +454,8 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   // log-sums: as many lanes per beam as there are, a power of two from 8 to 64
   const int lanes = max(8, min(kWave, 1 << (31 - __clz(kFThreads / W))));
   const int lse_w = tid / lanes, l = tid & (lanes - 1);
-  const float2* st = p.stats + (first + min(lse_w, W - 1)) * nch;
-  float2 v[kStats];
+  const BeamScanParams::Stat* st = p.stats + (first + min(lse_w, W - 1)) * nch;
+  BeamScanParams::Stat v[kStats];
 #pragma unroll
   for (int k = 0; k < kStats; ++k) v[k] = st[min(l + k * lanes, nch - 1)];
   const float score = p.scores[first + min(lse_w, W - 1)];
@@ -356,15 +474,15 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     float M = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kStats; ++k) {
-      if (w >= W || l + k * lanes >= nch) v[k] = make_float2(-INFINITY, 0.f);
-      M = fmaxf(M, v[k].x);
+      if (w >= W || l + k * lanes >= nch) v[k] = {0.0, -INFINITY};
+      M = fmaxf(M, v[k].max);
     }
     if (w < W)
-      for (int c = l + kStats * lanes; c < nch; c += lanes) M = fmaxf(M, st[c].x);
+      for (int c = l + kStats * lanes; c < nch; c += lanes) M = fmaxf(M, st[c].max);
     const float all = lanes_max(M, lanes);
     // a chunk of -inf alone adds its sum, 0 (NaN where it holds a NaN)
-    auto term = [&](float2 t) {
-      return t.x == -INFINITY ? (double)t.y : (double)t.y * exp((double)t.x - (double)all);
+    auto term = [&](const BeamScanParams::Stat& t) {
+      return t.max == -INFINITY ? t.sum : t.sum * exp((double)t.max - (double)all);
     };
     double s = 0.0;
 #pragma unroll
@@ -377,6 +495,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
       const bool live = finite(score) && fabs(lse) < (double)INFINITY;
       sm.lse[w] = live ? lse : 0.0;
       sm.score[w] = live ? score : -INFINITY;
+      sm.most[w] = all;
     }
   }
   if (tid < kWave) sm.above_key[tid] = 0;
@@ -414,20 +533,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     __syncthreads();
     theta = -wave_max(sm.above_key[lane] < C ? -own : -INFINITY);
   } else {
-    int above = 0;
-    const float4* keys = reinterpret_cast<const float4*>(sm.key);
-#pragma unroll 8
-    for (int j = 0; j < kFThreads / 4; ++j) {
-      const float4 o = keys[j];
-      above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
-    }
-    const float least = wave_max(above < C ? -own : -INFINITY);
-    if (lane == 0) sm.fold[wid] = least;
-    __syncthreads();
-    float all = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kFWaves; ++k) all = fmaxf(all, sm.fold[k]);
-    theta = -all;
+    theta = block_theta(own, C, sm);
   }
   // ---- the least logit of each beam that can reach theta, rounded down: lane w's of every wave ----
   float floor_w = INFINITY;
@@ -531,39 +637,45 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     found = sm.count;
   }
   if (listed <= kListCap && found <= kCandCap) {
-    for (int i = tid; i < found; i += kFThreads)
-      sm.cand.total[i] = (double)sm.score[sm.cand.beam[i]] +
-                         ((double)sm.cand.x[i] - sm.lse[sm.cand.beam[i]]);
-    __syncthreads();
-    // ranked by counting, eight threads to a candidate
-    for (int i0 = 0; i0 < found; i0 += kFThreads / 8) {
-      const int i = i0 + tid / 8;
-      const Candidate mine = get(sm.cand, min(i, found - 1));
-      int rank = 0, equal = 0;
-#pragma unroll 4
-      for (int j = tid & 7; j < found; j += 8) {
-        const double t = sm.cand.total[j];
-        rank += t > mine.total;
-        equal += t == mine.total;
+    int settled = 0;
+    do {
+      for (int i = tid; i < found; i += kFThreads)
+        sm.cand.total[i] = (double)sm.score[sm.cand.beam[i]] +
+                           ((double)sm.cand.x[i] - sm.lse[sm.cand.beam[i]]);
+      __syncthreads();
+      // ranked by counting, eight threads to a candidate
+      for (int i0 = 0; i0 < found; i0 += kFThreads / 8) {
+        const int i = i0 + tid / 8;
+        const Candidate mine = get(sm.cand, min(i, found - 1));
+        int rank = 0, equal = 0;
+  #pragma unroll 4
+        for (int j = tid & 7; j < found; j += 8) {
+          const double t = sm.cand.total[j];
+          rank += t > mine.total;
+          equal += t == mine.total;
+        }
+        if (equal > ((i & 7) == (tid & 7))) {  // others than itself
+          rank = 0;
+          for (int j = tid & 7; j < found; j += 8) rank += before(sm.cand, j, mine);
+        }
+        rank += dpp_i32<kDppXor1>(rank);
+        rank += dpp_i32<kDppXor2>(rank);
+        rank += dpp_i32<kDppHalfMirror>(rank);
+        if (i < found && rank <= C && (tid & 7) == 0) put(sm.best, rank, mine);
       }
-      if (equal > ((i & 7) == (tid & 7))) {  // others than itself
-        rank = 0;
-        for (int j = tid & 7; j < found; j += 8) rank += before(sm.cand, j, mine);
-      }
-      rank += dpp_i32<kDppXor1>(rank);
-      rank += dpp_i32<kDppXor2>(rank);
-      rank += dpp_i32<kDppHalfMirror>(rank);
-      if (i < found && rank < C && (tid & 7) == 0) put(sm.best, rank, mine);
-    }
-    __syncthreads();
+      __syncthreads();
+    } while (!settled++ && settle_near_ties<DT>(p, min(found, C + 1), sm));
     return min(found, C);
   }
-  // ---- too many: the beams one after the other ----
+  // ---- too many: the beams one after the other, by their lse in 64 bits where it can matter ----
+  if (W > 1 && (fabsf(theta) < 0x1p20f || theta == -INFINITY))
+    for (int w = 0; w < W; ++w)
+      if (sm.floor[w] < INFINITY) exact_lse<DT>(p, w, sm);
   found = 0;
   for (int w = 0; w < W; ++w) {
     __syncthreads();
     if (sm.floor[w] == INFINITY) continue;
-    const int got = row_largest<DT>(static_cast<const S*>(p.logits) + sm.row[w], p.V, C, w, sm, 0);
+    const int got = row_largest<DT>(p, first + w, w, sm, 0);
     __syncthreads();
     // the best so far and the beam's own: at most 2 C = 512, one a thread
     Candidate mine;
@@ -731,7 +843,7 @@ int64_t beam_workspace_bytes(int64_t G, int64_t W, int64_t V, int64_t C) {
   const int64_t chunk = beam_chunk(rows, V, C), nch = (V + chunk - 1) / chunk;
   // the scan's threads stay below 2^32
   if (rows * nch >= (1ll << 24)) return 0;
-  return rows * nch * (int64_t)(sizeof(float2) + kTops * sizeof(float));
+  return rows * nch * (int64_t)(sizeof(BeamScanParams::Stat) + kTops * sizeof(float));
 }
 
 template <int DT>
@@ -760,7 +872,7 @@ static hipError_t launch(BeamScanParams p, const BeamSelectOut* o, const mvsd_be
   const int chunk = beam_chunk(rows, p.V, p.C);
   p.nchunks = (int)(((int64_t)p.V + chunk - 1) / chunk);
   p.tops = static_cast<float*>(workspace);
-  p.stats = reinterpret_cast<float2*>(p.tops + rows * p.nchunks * kTops);
+  p.stats = reinterpret_cast<BeamScanParams::Stat*>(p.tops + rows * p.nchunks * kTops);
   switch (dtype) {
     case MVSD_F32: launch_dt<MVSD_F32>(p, o, a, chunk, stream); break;
     case MVSD_BF16: launch_dt<MVSD_BF16>(p, o, a, chunk, stream); break;
