@@ -166,6 +166,40 @@ def test_order_of_two_beams_is_that_of_the_64_bit_totals(device):
         assert got.parents[0].tolist() == [1, 0, 1, 0, 1, 0]
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V", [700, 9001, 50257])
+@pytest.mark.parametrize("heavier", [0, 1])
+def test_near_ties_follow_the_64_bit_totals(device, dtype, V, heavier):
+    """Two beams with the same logits in opposite orders, so that fp32 sums differ, and one of them
+    with a little more mass: its totals are lower by about 1e-8, far below what fp32 sums resolve and
+    far above what 64-bit ones do."""
+    G = 48
+    gen = torch.Generator(device=device).manual_seed(V)
+    x = (torch.randn(G, 2, V, device=device, generator=gen) * 2.5).to(DTYPES[dtype])
+    x[:, 0, V // 2] = x[:, 0, V - 1 - V // 2] = -math.inf  # the places that the flip maps there
+    x[:, 1] = x[:, 0].flip(-1)
+    lse = torch.logsumexp(x[:, heavier].double(), dim=-1)
+    x[:, heavier, V // 2] = (lse + math.log(1e-8)).to(x.dtype)
+    scores = torch.full((G, 2), -20.0, device=device)
+    got = check_select(x.reshape(2 * G, V), scores, 6)
+    assert (got.parents[:, 0] == 1 - heavier).all()
+    # at the last place: the better of the two is in, the other one is not
+    got = check_select(x.reshape(2 * G, V), scores, 1)
+    assert (got.parents[:, 0] == 1 - heavier).all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("C", [8, 40, 256])
+def test_rows_in_order(device, dtype, C):
+    """The largest entries side by side (more above the bound than the gather holds)."""
+    G, W, V = 2, 3, 60001
+    gen = torch.Generator(device=device).manual_seed(C)
+    x = (torch.randn(G * W, V, device=device, generator=gen) * 2.5).to(DTYPES[dtype])
+    x[:3] = x[:3].sort(dim=-1, descending=True).values
+    x[4] = x[4].sort(dim=-1).values
+    check_select(x, make_scores(device, G, W, 1), C)
+
+
 def test_huge_offsets(device):
     """Rows whose element offsets pass 2^31 (bf16, a row stride of 2^29)."""
     V, stride = 1500, 2 ** 29
@@ -423,6 +457,14 @@ def test_reorder_views(device):
     assert torch.equal(more[G * W:], tail)
 
 
+def test_reorder_takes_an_iterator(device):
+    parents = torch.tensor([[1, 0]], dtype=torch.int32, device=device)
+    states = [values(device, (2, 5), torch.int32, k) for k in range(3)]
+    want = [x.flip(0) for x in states]
+    got = reorder_beams(iter(states), parents)
+    assert all(torch.equal(x, w) for x, w in zip(got, want)) and len(got) == 3
+
+
 def test_reorder_many_tensors(device):
     """More states than one launch takes, of different shapes and types, empty ones among them."""
     G, W = 4, 3
@@ -678,7 +720,11 @@ def test_refusals(device):
                                          stop_token_ids=torch.zeros(64, **i32)),
                 lambda: beam_search_step(x, BeamState.new(2, 4, 8, device),
                                          out=BeamState.new(2, 4, 8, device)),
-                lambda: beam_search_step(x[:7], BeamState.new(2, 4, 8, device))):
+                lambda: beam_search_step(x[:7], BeamState.new(2, 4, 8, device)),
+                lambda: beam_search_step(x, BeamState.new(2, 4, 8, device),
+                                         length_penalty=math.nan),
+                lambda: beam_search_finish(BeamState.new(2, 4, 8, device),
+                                           length_penalty=math.inf)):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: beam_search_select(x.double(), s, 8),

@@ -23,10 +23,15 @@
 //       uniform row): the beams one after the other, each one's C largest by a radix selection.
 //   A step goes on in the same workgroup: stop tokens, finished hypotheses, histories.
 //
-// The sums of a chunk are fp32 (each of 32 or fewer terms of a lane, then a tree over the lanes), the
-// chunks are combined in fp64: lse is within about 1e-7 of the 64-bit value, and the totals are formed
-// and compared in 64 bits, so the order of two candidates of one beam is exact and that of candidates
-// of two beams is the 64-bit order unless they are closer than that.
+// Order: a lane's sum of up to 32 exponentials is fp32, everything after it fp64, which leaves an lse
+// with a deviation of 2e-8 (rows of 1000 columns) to 6e-9 (151936) from the 64-bit one.  Candidates of
+// one beam are ordered by their logits; where two neighbouring candidates of different beams are closer
+// than kNear, both beams' lse are formed again with 64-bit exponentials: the order is the 64-bit one.
+//
+// What bounds it (bf16 rows of 151936 columns, one MI355X): 1024 rows the scan, 48 us of 57 (6.45 TB/s);
+// four rows the chain of two launches, 3 and 6 us.  The finish is a chain too: the scan's results, 7
+// barriers, one gather.  One launch in which the last workgroup of a group finishes it was no faster
+// (four rows 9.7 us against 8.8, 256 rows 38 against 22: the agent-scope stores and counters).
 #include "beam.h"
 #include "mvsd_device.h"
 
@@ -52,7 +57,7 @@ static int beam_chunk(int64_t rows, int64_t V, int64_t C) {
 }
 
 // exp(d), d <= 0, as 2^(d log2(e)) with log2(e) in two parts, so that its rounding leaves no bias: the
-// mean error of a row's lse went from 3.8e-8 to below 1e-8.
+// mean error of a row's lse went from 4.0e-8 to 3e-9 and less.
 __device__ inline float exp_of(float d) {
   return __builtin_amdgcn_exp2f(fmaf(d, 1.44269504f, d * 1.92596304e-8f));
 }
@@ -217,7 +222,7 @@ __device__ inline bool before(const Candidates<N>& c, int j, const Candidate& mi
 
 struct BeamSmem {
   Candidates<kCandCap> cand;
-  Candidates<kMaxCandidates + 1> best;  // the group's candidates in order, and the next one
+  Candidates<kMaxCandidates> best;  // the group's candidates in order
   int2 list[kListCap];  // beam, top of the beam's row
   __align__(16) float key[kFThreads];
   float fold[kFWaves];
@@ -227,7 +232,7 @@ struct BeamSmem {
   float score[kMaxBeams];  // -inf: proposes nothing
   float most[kMaxBeams];   // the row's largest entry
   double red[kFWaves];
-  uint64_t near_ties;      // beams whose candidates' order depends on their lse's last digits
+  uint64_t near_ties, edge;  // beams whose candidates' order depends on their lse's last digits
   float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
   int hist[256];
   int wave_cnt[kFWaves];
@@ -409,16 +414,17 @@ __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
   __syncthreads();
 }
 
-// Of the first `have` candidates in sm.best: where two neighbours of different beams are closer than
-// kNear, the lse of both beams is formed again, in 64 bits throughout, and true returned: the totals
-// have to be formed and ranked again.  A row of 151936 entries takes about NEAR_US us; a group of 8
+// Of the `found` gathered candidates, the first C in sm.best: where two neighbours of different beams
+// are closer than kNear, or several beams have candidates so close to the last place, in it or behind
+// it, the lse of those beams is formed again, in 64 bits throughout, and true returned: the totals have
+// to be formed and ranked again.  A row of 151936 entries takes 33 us more; a group of 8
 // beams and 16 candidates has such a pair about once in ten thousand.
 constexpr double kNear = 0x1p-21;
 
 template <int DT>
-__device__ inline bool settle_near_ties(const BeamScanParams& p, int have, BeamSmem& sm) {
-  const int tid = threadIdx.x;
-  if (tid == 0) sm.near_ties = 0;
+__device__ inline bool settle_near_ties(const BeamScanParams& p, int found, BeamSmem& sm) {
+  const int tid = threadIdx.x, have = min(found, p.C);
+  if (tid == 0) sm.near_ties = sm.edge = 0;
   __syncthreads();
   if (tid + 1 < have) {
     const int a = sm.best.beam[tid], b = sm.best.beam[tid + 1];
@@ -427,8 +433,15 @@ __device__ inline bool settle_near_ties(const BeamScanParams& p, int have, BeamS
     if (a != b && fabs(t) < 0x1p20 && t - sm.best.total[tid + 1] < kNear)
       atomicOr((unsigned long long*)&sm.near_ties, 1ull << a | 1ull << b);
   }
+  if (found > have) {
+    const double last = sm.best.total[have - 1];
+    if (fabs(last) < 0x1p20)
+      for (int i = tid; i < found; i += kFThreads)
+        if (fabs(sm.cand.total[i] - last) < kNear)
+          atomicOr((unsigned long long*)&sm.edge, 1ull << sm.cand.beam[i]);
+  }
   __syncthreads();
-  const uint64_t beams = sm.near_ties;
+  const uint64_t beams = sm.near_ties | (__popcll(sm.edge) > 1 ? sm.edge : 0);
   for (uint64_t left = beams; left != 0; left &= left - 1)
     exact_lse<DT>(p, __ffsll((long long)left) - 1, sm);
   return beams != 0;
@@ -661,10 +674,10 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
         rank += dpp_i32<kDppXor1>(rank);
         rank += dpp_i32<kDppXor2>(rank);
         rank += dpp_i32<kDppHalfMirror>(rank);
-        if (i < found && rank <= C && (tid & 7) == 0) put(sm.best, rank, mine);
+        if (i < found && rank < C && (tid & 7) == 0) put(sm.best, rank, mine);
       }
       __syncthreads();
-    } while (!settled++ && settle_near_ties<DT>(p, min(found, C + 1), sm));
+    } while (!settled++ && settle_near_ties<DT>(p, found, sm));
     return min(found, C);
   }
   // ---- too many: the beams one after the other, by their lse in 64 bits where it can matter ----

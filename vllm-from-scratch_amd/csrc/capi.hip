@@ -1102,8 +1102,8 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
     const mvsd_beam_state& s = states[k];
     if (!s.src || !s.dst || s.num_rows < 1 || s.outer < 0 || s.length < 0 || s.inner < 0)
       return MVSD_E_INVALID;
-    // a row stays below 2^31 sixteen-byte units (sizes first, so that the products cannot overflow)
-    const int64_t most = 1ll << 35;
+    // a row stays below 2^31 eight-byte units (sizes first, so that the products cannot overflow)
+    const int64_t most = 1ll << 34;
     if (s.num_rows > 0x7fffffff || s.length > 0x7fffffff || s.inner > most || s.outer > most ||
         (s.inner > 0 && s.length > most / s.inner) ||
         (s.inner * s.length > 0 && s.outer > most / (s.inner * s.length)))

@@ -22,6 +22,7 @@ streams and captured graphs share nothing.
 from __future__ import annotations
 
 import ctypes
+import math
 import struct
 from dataclasses import dataclass
 
@@ -286,6 +287,8 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
             return beam_search_step(logits, state, stop_token_ids=stop_token_ids,
                                     length_penalty=length_penalty, early_stopping=early_stopping,
                                     target_rows=target_rows, out=out)
+    if not math.isfinite(length_penalty):
+        raise ValueError(f"length_penalty={length_penalty}")
     args = nat.BeamStepArgs()
     a, b, c = (G, W), (G,), (G, T, W)
     fields = (a, b, b, a, a, a, a)
@@ -331,6 +334,8 @@ def beam_search_finish(state: BeamState, num_return: int | None = None, *,
     if _elsewhere(device):
         with torch.cuda.device(device):
             return beam_search_finish(state, n, length_penalty=length_penalty)
+    if not math.isfinite(length_penalty):
+        raise ValueError(f"length_penalty={length_penalty}")
     args = nat.BeamFinishArgs()
     a, b, c = (G, W), (G,), (G, T, W)
     _addresses(args, _FINISH_TENSORS, _FINISH_NAMES,
@@ -409,19 +414,19 @@ def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None 
     targets = tensors if out is None else (out,) if isinstance(out, torch.Tensor) else tuple(out)
     if len(targets) != len(tensors):
         raise ValueError(f"{len(targets)} out tensors for {len(tensors)} states")
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return reorder_beams(states, parents, starts=starts, lengths=lengths,
-                                 length_dim=length_dim, slots=slots, out=out)
     table = (ctypes.c_int64 * (8 * len(tensors)))()
     n = _hostops.state_table(table, tensors, targets, length_dim, device,
                              0 if slots is not None else G * W)
     if n < 0:
         _refuse_states(tensors, targets, length_dim, device, 0 if slots is not None else G * W)
     if n and G:
-        status = nat.lib().mvsd_beam_reorder(
-            table, n, parents.data_ptr(), nat.ptr(starts), nat.ptr(lengths), nat.ptr(slots), G, W,
-            nat.stream_of(device))
+        call = (table, n, parents.data_ptr(), nat.ptr(starts), nat.ptr(lengths), nat.ptr(slots),
+                G, W, nat.stream_of(device))
+        if _elsewhere(device):
+            with torch.cuda.device(device):
+                status = nat.lib().mvsd_beam_reorder(*call)
+        else:
+            status = nat.lib().mvsd_beam_reorder(*call)
         if status == -1:
             raise ValueError("the states (or out) share memory with each other")
         nat.check(status, "mvsd_beam_reorder")
