@@ -49,13 +49,13 @@ struct BeamScanParams {
   const uint8_t* done;     // step: [G], else null
   int G, W, V, C;
   int max_length;  // step: T
-  int nchunks;
+  int nchunks, tops_per_chunk;
   struct alignas(16) Stat {
     double sum;  // of exp(x - max)
     float max;
   };
   Stat* stats;    // [G * W, nchunks] chunk maximum and sum
-  float* tops;    // [G * W, nchunks, 16] the largest entry of 16 lanes each
+  float* tops;    // [G * W, nchunks, tops_per_chunk] the largest entry of 16 or 2 lanes each
 };
 
 struct BeamSelectOut {

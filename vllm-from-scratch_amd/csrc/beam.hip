@@ -10,7 +10,7 @@
 //
 //   beam_scan_kernel    one 256-thread workgroup per (beam, chunk of columns) reads the chunk once,
 //                       into registers, and leaves its maximum, its sum of exp(x - maximum) and the
-//                       largest entry of every 16 lanes (a "top": 16 of them a chunk).
+//                       largest entry of every 16 or 2 lanes (a "top").
 //   beam_finish_kernel  one 512-thread workgroup per group:
 //     - lse_b in 64 bits from the chunks' sums;
 //     - theta, the C-th largest of the maxima of 512 disjoint unions of tops (64 for C <= 32), as
@@ -37,7 +37,6 @@
 
 namespace mvsd {
 
-constexpr int kTops = 16;          // of a chunk, 16 lanes each
 constexpr int kFThreads = 512;
 constexpr int kFWaves = kFThreads / kWave;
 constexpr int kListCap = 1024;     // tops that reach theta
@@ -46,14 +45,25 @@ constexpr int kHeld = 4;           // vectors of tops a thread keeps in register
 constexpr int kStats = 2;          // chunks that a lane of a beam loads at a time
 constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 keys
 
-// Columns per chunk: long ones, unless they leave compute units idle (fewer than 4 workgroups each)
-// or give a row fewer than two tops per candidate (a group may have one beam only), so that theta is
-// a poor bound or none.
+// How rows are split: columns per chunk, and the lanes that share a top (each holds NV vectors of the
+// chunk).  Long chunks, unless they leave compute units idle (fewer than 4 workgroups each) or give a
+// row fewer than two tops per candidate (a group may have one beam only), so that theta is a poor bound
+// or none.  Short rows can have too few even then: tops of two lanes (6 groups of 16 bf16 beams of 1088
+// columns, 64 candidates: 1170 us with tops of 16 lanes, where theta leaves more entries than LDS holds,
+// 20.5 us with tops of 2, single in the unions that give theta).
 constexpr int kBeamLong = 8192, kBeamShort = 2048;
+constexpr int kCoarse = 16, kFine = 2;
 
-static int beam_chunk(int64_t rows, int64_t V, int64_t C) {
-  const int64_t chunks = (V + kBeamLong - 1) / kBeamLong;
-  return rows * chunks < 1024 || chunks * kTops < 2 * C ? kBeamShort : kBeamLong;
+struct BeamSplit {
+  int chunk, lanes;
+  int64_t chunks;
+  int tops() const { return kThreads / lanes; }  // of a chunk
+};
+
+static BeamSplit beam_split(int64_t rows, int64_t V, int64_t C) {
+  const int64_t large = (V + kBeamLong - 1) / kBeamLong, small = (V + kBeamShort - 1) / kBeamShort;
+  if (rows * large >= 1024 && V / (kCoarse * 32) >= 2 * C) return {kBeamLong, kCoarse, large};
+  return {kBeamShort, V / (kCoarse * 8) >= 2 * C ? kCoarse : kFine, small};
 }
 
 // exp(d), d <= 0, as 2^(d log2(e)) with log2(e) in two parts, so that its rounding leaves no bias: the
@@ -113,8 +123,9 @@ __device__ inline u32x4 load_scan(const typename Elem<DT>::storage* row, int col
       reinterpret_cast<const Vec16<DT>*>(row + min(col, V - Elem<DT>::kVec)));
 }
 
-template <int DT, int NV, bool STREAM>
+template <int DT, int NV, int LANES, bool STREAM>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
+  constexpr int kTops = kThreads / LANES;
   using S = typename Elem<DT>::storage;
   constexpr int VEC = Elem<DT>::kVec;
   constexpr int CH = NV * kThreads * VEC;
@@ -144,9 +155,10 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) m = fmaxf(m, v[j][e]);
-  const float top = max16(m);
-  const float wm = fmaxf(fmaxf(readlane_f32(top, 0), readlane_f32(top, 16)),
-                         fmaxf(readlane_f32(top, 32), readlane_f32(top, 48)));
+  const float pair = fmaxf(m, dpp_f32<kDppXor1>(m)), top16 = max16(m);
+  const float top = LANES == kFine ? pair : top16;
+  const float wm = fmaxf(fmaxf(readlane_f32(top16, 0), readlane_f32(top16, 16)),
+                         fmaxf(readlane_f32(top16, 32), readlane_f32(top16, 48)));
   float s = 0.f;
   if (wm != -INFINITY) {  // +inf gives a NaN sum, as a NaN does
 #pragma unroll
@@ -161,7 +173,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   }
   const double sum64 = lanes_sum((double)s, kWave);
   const int64_t slot = (int64_t)r * p.nchunks + c;
-  if ((tid & 15) == 0) p.tops[slot * kTops + tid / 16] = top;
+  if (tid % LANES == 0) p.tops[slot * kTops + tid / LANES] = top;
   if (lane_id() == 0) {
     s_m[wave_id()] = wm;
     s_s[wave_id()] = sum64;
@@ -313,9 +325,10 @@ __device__ inline int row_largest(const BeamScanParams& p, int64_t beam_row, int
   const int V = p.V, C = p.C;
   float theta;
   {
-    const float* tops = p.tops + beam_row * p.nchunks * kTops;
+    const int row_tops = p.nchunks * p.tops_per_chunk;
+    const float* tops = p.tops + beam_row * row_tops;
     float own = -INFINITY;
-    for (int i = tid; i < p.nchunks * kTops; i += kFThreads) own = fmaxf(own, tops[i]);
+    for (int i = tid; i < row_tops; i += kFThreads) own = fmaxf(own, tops[i]);
     sm.key[tid] = own;
     if (tid == 0) sm.count = 0;
     __syncthreads();
@@ -448,11 +461,12 @@ __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, Beam
 }
 
 // The group's candidates, in order, in sm.best; returns how many.
-template <int DT, int NV>
+template <int DT, int NV, int LANES>
 __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem& sm) {
   using S = typename Elem<DT>::storage;
   constexpr int VEC = Elem<DT>::kVec;
   constexpr int CH = NV * kThreads * VEC;
+  constexpr int kTops = kThreads / LANES;
   const int tid = threadIdx.x, lane = lane_id(), wid = wave_id();
   const int W = p.W, C = p.C, nch = p.nchunks;
   const int64_t first = (int64_t)g * W;
@@ -520,33 +534,55 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   auto total_of = [&](float x, int w) {
     return (float)((double)sm.score[w] + ((double)x - sm.lse[w]));
   };
-  float own = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (held_row[k] >= 0) {
-      const float4 v = held[k];
-      own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), held_row[k]));
-    }
-  for (int i = tid + kHeld * kFThreads; i < quads; i += kFThreads) {
-    const float4 v = top4[i];
-    own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), i / per_row));
-  }
-  sm.key[tid] = own;
-  __syncthreads();
   float theta;
-  if (C <= kFoldC) {  // block-uniform
-    // every wave folds the keys, counts an eighth of the comparisons and reads the sums
-#pragma unroll
-    for (int k = 1; k < kFWaves; ++k) own = fmaxf(own, sm.key[((wid + k) % kFWaves) * kWave + lane]);
-    int above = 0;
-#pragma unroll
-    for (int j = 0; j < kWave / kFWaves; ++j)
-      above += readlane_f32(own, wid * (kWave / kFWaves) + j) > own;
-    atomicAdd(&sm.above_key[lane], above);
+  if (per_row < 2 * C) {  // block-uniform
+    // a row has few vectors of tops: unions of single tops, so that one beam alone gives C of them
+    uint32_t* bits = reinterpret_cast<uint32_t*>(sm.key);
+    bits[tid] = 0;
     __syncthreads();
-    theta = -wave_max(sm.above_key[lane] < C ? -own : -INFINITY);
-  } else {
+    for (int i = tid; i < quads; i += kFThreads) {
+      const float4 v = top4[i];
+      const float e[4] = {v.x, v.y, v.z, v.w};
+      const int w = i / per_row;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float t = total_of(e[k], w);
+        if (t > -INFINITY) atomicMax(&bits[(4 * i + k) % kFThreads], ordered_bits(t));
+      }
+    }
+    __syncthreads();
+    const float own = bits[tid] == 0 ? -INFINITY : key_float(bits[tid]);
+    sm.key[tid] = own;
+    __syncthreads();
     theta = block_theta(own, C, sm);
+  } else {
+    float own = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (held_row[k] >= 0) {
+        const float4 v = held[k];
+        own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), held_row[k]));
+      }
+    for (int i = tid + kHeld * kFThreads; i < quads; i += kFThreads) {
+      const float4 v = top4[i];
+      own = fmaxf(own, total_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), i / per_row));
+    }
+    sm.key[tid] = own;
+    __syncthreads();
+    if (C <= kFoldC) {  // block-uniform
+      // every wave folds the keys, counts an eighth of the comparisons and reads the sums
+#pragma unroll
+      for (int k = 1; k < kFWaves; ++k) own = fmaxf(own, sm.key[((wid + k) % kFWaves) * kWave + lane]);
+      int above = 0;
+#pragma unroll
+      for (int j = 0; j < kWave / kFWaves; ++j)
+        above += readlane_f32(own, wid * (kWave / kFWaves) + j) > own;
+      atomicAdd(&sm.above_key[lane], above);
+      __syncthreads();
+      theta = -wave_max(sm.above_key[lane] < C ? -own : -INFINITY);
+    } else {
+      theta = block_theta(own, C, sm);
+    }
   }
   // ---- the least logit of each beam that can reach theta, rounded down: lane w's of every wave ----
   float floor_w = INFINITY;
@@ -594,9 +630,9 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
         }
       }
     } else {
-      // ---- the entries under the listed tops, 16 lanes each, two tops at a time ----
-      constexpr int kTeams = kFThreads / 16;
-      for (int b = tid / 16; b < listed; b += 2 * kTeams) {
+      // ---- the entries under the listed tops, LANES lanes each, two tops at a time ----
+      constexpr int kTeams = kFThreads / LANES;
+      for (int b = tid / LANES; b < listed; b += 2 * kTeams) {
         u32x4 q[2][NV];
         int64_t col0[2];
         int row_of[2];
@@ -605,7 +641,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
           const int2 i = sm.list[min(b + k * kTeams, listed - 1)];
           const int w = i.x, c = i.y / kTops;
           row_of[k] = w;
-          col0[k] = (int64_t)c * CH + ((i.y % kTops) * 16 + (tid & 15)) * VEC;
+          col0[k] = (int64_t)c * CH + ((i.y % kTops) * LANES + tid % LANES) * VEC;
           const S* row = x0 + sm.row[w];
           // as load_vec_inside: the vector is moved back where it would pass the row's end
 #pragma unroll
@@ -615,7 +651,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (b + k * kTeams >= listed) continue;
-          // the lane's entries that reach the floor, a bit each; one or two of the 16 lanes have any
+          // the lane's entries that reach the floor, a bit each; one or two of a top's lanes have any
           const int w = row_of[k];
           const float f = sm.floor[w];
           const int64_t end = (int64_t)p.V - VEC;
@@ -710,12 +746,12 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   return found;
 }
 
-template <int DT, int NV>
+template <int DT, int NV, int LANES>
 __global__ __launch_bounds__(kFThreads) void beam_select_kernel(BeamScanParams p,
                                                                  BeamSelectOut o) {
   __shared__ BeamSmem sm;
   const int g = blockIdx.x;
-  const int found = group_candidates<DT, NV>(p, g, sm);
+  const int found = group_candidates<DT, NV, LANES>(p, g, sm);
   for (int i = threadIdx.x; i < p.C; i += kFThreads) {
     const int64_t at = (int64_t)g * p.C + i;
     const bool on = i < found;
@@ -731,7 +767,7 @@ __global__ __launch_bounds__(kFThreads) void beam_select_kernel(BeamScanParams p
 // that are no stop tokens are the next beams.  W (1 + E) candidates always hold W of the latter if
 // there are as many.  Finished hypotheses: the W best of the old and the new ones, the old first
 // where they are equal.
-template <int DT, int NV>
+template <int DT, int NV, int LANES>
 __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
                                                                mvsd_beam_step_args a) {
   __shared__ BeamSmem sm;
@@ -763,7 +799,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
     }
     return;
   }
-  const int found = group_candidates<DT, NV>(p, g, sm);
+  const int found = group_candidates<DT, NV, LANES>(p, g, sm);
   const int new_len = len + 1;
   const double power = len_power(new_len, a.length_penalty);
   if (wid < kMaxCandidates / kWave) {
@@ -852,44 +888,50 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
 
 int64_t beam_workspace_bytes(int64_t G, int64_t W, int64_t V, int64_t C) {
   if (G <= 0 || W <= 0 || V <= 0) return 0;
-  const int64_t rows = G * W;
-  const int64_t chunk = beam_chunk(rows, V, C), nch = (V + chunk - 1) / chunk;
-  // the scan's threads stay below 2^32
-  if (rows * nch >= (1ll << 24)) return 0;
-  return rows * nch * (int64_t)(sizeof(BeamScanParams::Stat) + kTops * sizeof(float));
+  const BeamSplit split = beam_split(G * W, V, C);
+  const int64_t slots = G * W * split.chunks;
+  if (slots >= (1ll << 24)) return 0;  // the scan's threads stay below 2^32
+  return slots * (int64_t)(sizeof(BeamScanParams::Stat) + split.tops() * sizeof(float));
+}
+
+template <int DT, int NV, int LANES, bool STREAM>
+static void launch_split(const BeamScanParams& p, const BeamSelectOut* o,
+                         const mvsd_beam_step_args* a, hipStream_t stream) {
+  hipLaunchKernelGGL((beam_scan_kernel<DT, NV, LANES, STREAM>),
+                     dim3((unsigned)(p.G * p.W) * (unsigned)p.nchunks), dim3(kThreads), 0, stream, p);
+  const dim3 groups(p.G), block(kFThreads);
+  if (o) hipLaunchKernelGGL((beam_select_kernel<DT, NV, LANES>), groups, block, 0, stream, p, *o);
+  else hipLaunchKernelGGL((beam_step_kernel<DT, NV, LANES>), groups, block, 0, stream, p, *a);
 }
 
 template <int DT>
 static void launch_dt(const BeamScanParams& p, const BeamSelectOut* o,
-                      const mvsd_beam_step_args* a, int chunk, hipStream_t stream) {
+                      const mvsd_beam_step_args* a, const BeamSplit& split, hipStream_t stream) {
   constexpr int kLong = kBeamLong / (kThreads * Elem<DT>::kVec);
   constexpr int kShort = kBeamShort / (kThreads * Elem<DT>::kVec);
-  const dim3 scan((unsigned)(p.G * p.W) * (unsigned)p.nchunks), groups(p.G);
-  if (chunk == kBeamLong) {
-    if ((int64_t)p.G * p.W * p.V * (int64_t)sizeof(typename Elem<DT>::storage) >= kStreamBytes)
-      hipLaunchKernelGGL((beam_scan_kernel<DT, kLong, true>), scan, dim3(kThreads), 0, stream, p);
-    else
-      hipLaunchKernelGGL((beam_scan_kernel<DT, kLong, false>), scan, dim3(kThreads), 0, stream, p);
-    if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *o);
-    else hipLaunchKernelGGL((beam_step_kernel<DT, kLong>), groups, dim3(kFThreads), 0, stream, p, *a);
-  } else {
-    hipLaunchKernelGGL((beam_scan_kernel<DT, kShort, false>), scan, dim3(kThreads), 0, stream, p);
-    if (o) hipLaunchKernelGGL((beam_select_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *o);
-    else hipLaunchKernelGGL((beam_step_kernel<DT, kShort>), groups, dim3(kFThreads), 0, stream, p, *a);
-  }
+  const int64_t bytes = (int64_t)p.G * p.W * p.V * (int64_t)sizeof(typename Elem<DT>::storage);
+  if (split.chunk == kBeamLong && bytes >= kStreamBytes)
+    launch_split<DT, kLong, kCoarse, true>(p, o, a, stream);
+  else if (split.chunk == kBeamLong)
+    launch_split<DT, kLong, kCoarse, false>(p, o, a, stream);
+  else if (split.lanes == kCoarse)
+    launch_split<DT, kShort, kCoarse, false>(p, o, a, stream);
+  else
+    launch_split<DT, kShort, kFine, false>(p, o, a, stream);
 }
 
 static hipError_t launch(BeamScanParams p, const BeamSelectOut* o, const mvsd_beam_step_args* a,
                          int dtype, void* workspace, hipStream_t stream) {
   const int64_t rows = (int64_t)p.G * p.W;
-  const int chunk = beam_chunk(rows, p.V, p.C);
-  p.nchunks = (int)(((int64_t)p.V + chunk - 1) / chunk);
+  const BeamSplit split = beam_split(rows, p.V, p.C);
+  p.nchunks = (int)split.chunks;
+  p.tops_per_chunk = split.tops();
   p.tops = static_cast<float*>(workspace);
-  p.stats = reinterpret_cast<BeamScanParams::Stat*>(p.tops + rows * p.nchunks * kTops);
+  p.stats = reinterpret_cast<BeamScanParams::Stat*>(p.tops + rows * split.chunks * split.tops());
   switch (dtype) {
-    case MVSD_F32: launch_dt<MVSD_F32>(p, o, a, chunk, stream); break;
-    case MVSD_BF16: launch_dt<MVSD_BF16>(p, o, a, chunk, stream); break;
-    case MVSD_F16: launch_dt<MVSD_F16>(p, o, a, chunk, stream); break;
+    case MVSD_F32: launch_dt<MVSD_F32>(p, o, a, split, stream); break;
+    case MVSD_BF16: launch_dt<MVSD_BF16>(p, o, a, split, stream); break;
+    case MVSD_F16: launch_dt<MVSD_F16>(p, o, a, split, stream); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
