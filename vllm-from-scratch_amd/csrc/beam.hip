@@ -50,7 +50,7 @@ constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 k
 // row fewer than two tops per candidate (a group may have one beam only), so that theta is a poor bound
 // or none.  Short rows can have too few even then: tops of two lanes (6 groups of 16 bf16 beams of 1088
 // columns, 64 candidates: 1170 us with tops of 16 lanes, where theta leaves more entries than LDS holds,
-// 20.5 us with tops of 2, single in the unions that give theta).
+// 36.7 us with tops of 2).
 constexpr int kBeamLong = 8192, kBeamShort = 2048;
 constexpr int kCoarse = 16, kFine = 2;
 
@@ -535,8 +535,9 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     return (float)((double)sm.score[w] + ((double)x - sm.lse[w]));
   };
   float theta;
-  if (per_row < 2 * C) {  // block-uniform
-    // a row has few vectors of tops: unions of single tops, so that one beam alone gives C of them
+  const int live = __popcll(__ballot(lane < W && sm.score[min(lane, W - 1)] != -INFINITY));
+  if (live * per_row < 2 * C) {  // block-uniform
+    // few vectors of tops (the first step's one beam, short rows): unions of single tops
     uint32_t* bits = reinterpret_cast<uint32_t*>(sm.key);
     bits[tid] = 0;
     __syncthreads();
