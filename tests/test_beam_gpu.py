@@ -481,6 +481,26 @@ def test_reorder_many_tensors(device):
             assert np.array_equal(as_bytes(x), w)
 
 
+def test_reorder_states_of_one_call_once(device):
+    """Empty states among many, through the C ABI: none is reordered twice."""
+    import ctypes
+
+    from mvsd import _native as nat
+
+    parents = torch.tensor([[1, 2, 0]], dtype=torch.int32, device=device)
+    states = [values(device, (3, 9), torch.uint8, k) for k in range(60)]
+    want = [x[[1, 2, 0]] for x in states]
+    flat = []
+    for k, x in enumerate(states):
+        flat += [x.data_ptr(), x.data_ptr(), 9, 9, 3, 1, 9, 1]
+        if k % 3 == 0:
+            flat += [x.data_ptr(), x.data_ptr(), 9, 9, 3, 1, 0, 1]  # no entries
+    assert nat.lib().mvsd_beam_reorder((ctypes.c_int64 * len(flat))(*flat), len(flat) // 8,
+                                       parents.data_ptr(), None, None, None, 1, 3,
+                                       nat.stream_of(device)) == 0
+    assert all(torch.equal(x, w) for x, w in zip(states, want))
+
+
 def test_reorder_many_groups(device):
     """More (group, state) pairs than one grid has rows."""
     G, W = 3000, 2

@@ -1124,10 +1124,9 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
   p.W = (int)beam_width;
   // blocks: one row of the grid per (group, state), at most 65535 rows
   const int64_t groups = 65535 / mvsd::kMaxBeamStates;
-  for (int64_t k = 0; k < num_states; k += mvsd::kMaxBeamStates) {
-    p.n = 0;
-    for (int64_t j = k; j < num_states && p.n < mvsd::kMaxBeamStates; ++j)
-      if (states[j].outer * states[j].length * states[j].inner > 0) p.state[p.n++] = states[j];
+  for (int64_t k = 0; k < num_states;) {
+    for (p.n = 0; k < num_states && p.n < mvsd::kMaxBeamStates; ++k)
+      if (states[k].outer * states[k].length * states[k].inner > 0) p.state[p.n++] = states[k];
     if (p.n == 0) continue;
     for (int64_t g = 0; g < num_groups; g += groups) {
       p.first_group = g;
