@@ -188,6 +188,21 @@ def test_near_ties_follow_the_64_bit_totals(device, dtype, V, heavier):
     assert (got.parents[:, 0] == 1 - heavier).all()
 
 
+@pytest.mark.parametrize("heavier", [0, 1])
+def test_near_ties_in_front_of_masked_tokens(device, heavier):
+    """Two tokens a beam allowed, the others at the type's lowest value: the last places are runs of
+    that value, the first ones near ties of the two beams (mass 1e-8 apart)."""
+    V = 30000
+    x = torch.full((2, V), torch.finfo(torch.float32).min, device=device)
+    x[:, 100], x[:, 20000] = 1.0, 0.25
+    lse = math.log(math.exp(1.0) + math.exp(0.25))
+    x[heavier, 7] = lse + math.log(1e-8)
+    scores = torch.tensor([[-20.0, -20.0]], device=device)
+    got = check_select(x, scores, 12)
+    assert got.parents[0, :2].tolist() == [1 - heavier, heavier]
+    assert got.token_ids[0, :4].tolist() == [100, 100, 20000, 20000]
+
+
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("C", [8, 40, 256])
 def test_rows_in_order(device, dtype, C):

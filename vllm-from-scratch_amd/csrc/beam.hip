@@ -717,33 +717,38 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     } while (!settled++ && settle_near_ties<DT>(p, found, sm));
     return min(found, C);
   }
-  // ---- too many: the beams one after the other, by their lse in 64 bits where it can matter ----
-  if (W > 1 && (fabsf(theta) < 0x1p20f || theta == -INFINITY))
+  // ---- too many: the beams one after the other, by their lse in 64 bits where it can matter for the
+  //      last place; once more where candidates in front of it are near ties ----
+  const bool exact = W > 1 && (fabsf(theta) < 0x1p20f || theta == -INFINITY);
+  if (exact)
     for (int w = 0; w < W; ++w)
       if (sm.floor[w] < INFINITY) exact_lse<DT>(p, w, sm);
-  found = 0;
-  for (int w = 0; w < W; ++w) {
-    __syncthreads();
-    if (sm.floor[w] == INFINITY) continue;
-    const int got = row_largest<DT>(p, first + w, w, sm, 0);
-    __syncthreads();
-    // the best so far and the beam's own: at most 2 C = 512, one a thread
-    Candidate mine;
-    const bool have = tid < found + got;
-    if (have) {
-      mine = tid < found ? get(sm.best, tid) : get(sm.cand, tid - found);
-      if (tid >= found) mine.total = (double)sm.score[w] + ((double)mine.x - sm.lse[w]);
+  int settled = 0;
+  do {
+    found = 0;
+    for (int w = 0; w < W; ++w) {
+      __syncthreads();
+      if (sm.floor[w] == INFINITY) continue;
+      const int got = row_largest<DT>(p, first + w, w, sm, 0);
+      __syncthreads();
+      // the best so far and the beam's own: at most 2 C = 512, one a thread
+      Candidate mine;
+      const bool have = tid < found + got;
+      if (have) {
+        mine = tid < found ? get(sm.best, tid) : get(sm.cand, tid - found);
+        if (tid >= found) mine.total = (double)sm.score[w] + ((double)mine.x - sm.lse[w]);
+      }
+      __syncthreads();
+      if (have) put(sm.cand, tid, mine);
+      __syncthreads();
+      int rank = 0;
+      if (have)
+        for (int j = 0; j < found + got; ++j) rank += before(sm.cand, j, mine);
+      if (have && rank < C) put(sm.best, rank, mine);
+      found = min(found + got, C);
     }
     __syncthreads();
-    if (have) put(sm.cand, tid, mine);
-    __syncthreads();
-    int rank = 0;
-    if (have)
-      for (int j = 0; j < found + got; ++j) rank += before(sm.cand, j, mine);
-    if (have && rank < C) put(sm.best, rank, mine);
-    found = min(found + got, C);
-  }
-  __syncthreads();
+  } while (!exact && !settled++ && settle_near_ties<DT>(p, found, sm));
   return found;
 }
 
