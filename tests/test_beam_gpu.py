@@ -189,6 +189,47 @@ def test_near_ties_follow_the_64_bit_totals(device, dtype, V, heavier):
 
 
 @pytest.mark.parametrize("heavier", [0, 1])
+def test_near_ties_of_totals_around_zero(device, heavier):
+    """Scores that bring the best totals to zero, where a bound in proportion to them is none."""
+    G, V = 64, 9001
+    gen = torch.Generator(device=device).manual_seed(heavier)
+    x = torch.randn(G, 2, V, device=device, generator=gen) * 2.5
+    x[:, 0, V // 2] = -math.inf
+    x[:, 1] = x[:, 0].flip(-1)
+    lse = torch.logsumexp(x[:, heavier].double(), dim=-1)
+    x[:, heavier, V // 2] = (lse + math.log(1e-8)).float()
+    scores = (lse - x[:, 0].amax(-1).double()).float()[:, None].expand(G, 2).contiguous()
+    for C in (1, 2, 3):
+        got = check_select(x.reshape(2 * G, V), scores, C)
+        assert (got.parents[:, 0] == 1 - heavier).all()
+
+
+@pytest.mark.parametrize("dtype,last", [("fp32", 7171), ("bf16", 6151)])
+@pytest.mark.parametrize("G", [2, 512])
+@pytest.mark.parametrize("heavier", [0, 1])
+def test_near_ties_of_rows_with_one_large_entry(device, dtype, last, G, heavier):
+    """An entry beside which each of the others vanishes in fp32 (5.6e-8 of it), but not their sum:
+    first or last in the order of columns.  (512 groups: rows long enough for the long chunks.)"""
+    V = 8192
+    x = torch.full((G, 2, V), -16.7, device=device, dtype=DTYPES[dtype])
+    x[:, 0, 0] = x[:, 1, last] = 0.0
+    x[:, :, 5000] = -math.inf
+    x[:, heavier, 5000] = math.log(1e-8)
+    got = check_select(x.reshape(2 * G, V), torch.full((G, 2), -20.0, device=device), 2)
+    assert (got.parents == torch.tensor([1 - heavier, heavier], device=device)).all()
+
+
+def test_equal_beams_in_front_of_large_masks(device):
+    """Masked tokens at -1e9: totals that 64 bits hold to 1e-7, of beams with the same mass."""
+    G, V = 48, 30000
+    gen = torch.Generator(device=device).manual_seed(2)
+    x = torch.full((G, 2, V), -1e9, device=device)
+    x[:, 0, 100:141] = torch.randn(G, 41, device=device, generator=gen)
+    x[:, 1] = x[:, 0].flip(-1)
+    check_select(x.reshape(2 * G, V), torch.full((G, 2), -20.0, device=device), 100)
+
+
+@pytest.mark.parametrize("heavier", [0, 1])
 def test_near_ties_in_front_of_masked_tokens(device, heavier):
     """Two tokens a beam allowed, the others at the type's lowest value: the last places are runs of
     that value, the first ones near ties of the two beams (mass 1e-8 apart)."""

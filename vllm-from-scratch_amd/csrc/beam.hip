@@ -23,8 +23,9 @@
 //       uniform row): the beams one after the other, each one's C largest by a radix selection.
 //   A step goes on in the same workgroup: stop tokens, finished hypotheses, histories.
 //
-// Order: a lane's sum of up to 32 exponentials is fp32, everything after it fp64, which leaves an lse
-// with a deviation of 2e-8 (rows of 1000 columns) to 6e-9 (151936) from the 64-bit one.  Candidates of
+// Order: a lane's sum of up to 32 exponentials is fp32, in pairs, everything after it fp64, which leaves
+// an lse with a deviation of 2e-8 (rows of 1000 columns) to 6e-9 (151936) from the 64-bit one, more
+// where one entry has most of the mass.  Candidates of
 // one beam are ordered by their logits; where two neighbouring candidates of different beams are closer
 // than kNear, both beams' lse are formed again with 64-bit exponentials: the order is the 64-bit one.
 //
@@ -70,6 +71,13 @@ static BeamSplit beam_split(int64_t rows, int64_t V, int64_t C) {
 // mean error of a row's lse went from 4.0e-8 to 3e-9 and less.
 __device__ inline float exp_of(float d) {
   return __builtin_amdgcn_exp2f(fmaf(d, 1.44269504f, d * 1.92596304e-8f));
+}
+
+// The sum of f(0) ... f(N - 1), N a power of two, in pairs: at most log2(N) roundings of each term.
+template <int N, typename F>
+__device__ inline float pair_sum(F&& f, int from = 0) {
+  if constexpr (N == 1) return f(from);
+  else return pair_sum<N / 2>(f, from) + pair_sum<N / 2>(f, from + N / 2);
 }
 
 __device__ inline bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -161,10 +169,7 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
                          fmaxf(readlane_f32(top16, 32), readlane_f32(top16, 48)));
   float s = 0.f;
   if (wm != -INFINITY) {  // +inf gives a NaN sum, as a NaN does
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s += exp_of(v[j][e] - wm);
+    s = pair_sum<NV * VEC>([&](int i) { return exp_of(v[i / VEC][i % VEC] - wm); });
   } else {  // every entry is -inf or NaN
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -427,13 +432,20 @@ __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
   __syncthreads();
 }
 
+// How close two totals of different beams have to be for the scan's lse not to decide.  An lse is off
+// by at most 1.3e-6: five roundings of a lane's sum (3.0e-7), each power's own (1.2e-7), and those of its
+// argument, the difference to the maximum (2^-21 where it is below 16) times log2(e) (0.7 2^-21 where the
+// product is), for rows that keep all their mass at one such distance.  Two differ by twice that at most.
+// Totals past 2^30 add their own rounding; past kFar it hides any lse's.
+constexpr double kNear = 0x1p-18, kFar = 0x1p44;
+
+__device__ inline double near_by(double total) { return kNear + fabs(total) * 0x1p-51; }
+
 // Of the `found` gathered candidates, the first C in sm.best: where two neighbours of different beams
 // are closer than kNear, or several beams have candidates so close to the last place, in it or behind
 // it, the lse of those beams is formed again, in 64 bits throughout, and true returned: the totals have
-// to be formed and ranked again.  A row of 151936 entries takes 33 us more; a group of 8
-// beams and 16 candidates has such a pair about once in ten thousand.
-constexpr double kNear = 0x1p-21;
-
+// to be formed and ranked again.  A row of 151936 entries takes 33 us more; a group of 8 beams and 16
+// candidates has such a pair about once in 1250.
 template <int DT>
 __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, BeamSmem& sm) {
   const int tid = threadIdx.x, have = min(found, p.C);
@@ -442,15 +454,14 @@ __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, Beam
   if (tid + 1 < have) {
     const int a = sm.best.beam[tid], b = sm.best.beam[tid + 1];
     const double t = sm.best.total[tid];
-    // (totals too large for the difference to show: masks of the type's lowest value)
-    if (a != b && fabs(t) < 0x1p20 && t - sm.best.total[tid + 1] < kNear)
+    if (a != b && fabs(t) < kFar && t - sm.best.total[tid + 1] < near_by(t))
       atomicOr((unsigned long long*)&sm.near_ties, 1ull << a | 1ull << b);
   }
   if (found > have) {
     const double last = sm.best.total[have - 1];
-    if (fabs(last) < 0x1p20)
+    if (fabs(last) < kFar)
       for (int i = tid; i < found; i += kFThreads)
-        if (fabs(sm.cand.total[i] - last) < kNear)
+        if (fabs(sm.cand.total[i] - last) < near_by(last))
           atomicOr((unsigned long long*)&sm.edge, 1ull << sm.cand.beam[i]);
   }
   __syncthreads();
@@ -591,7 +602,8 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     floor_w = -3.402823466e38f;  // -inf is no candidate
     if (theta != -INFINITY) {
       // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
-      const double t = (double)theta - fabs((double)theta) * 0x1p-23;
+      // (and the scan's lse for one near by)
+      const double t = (double)theta - fabs((double)theta) * 0x1p-23 - kNear;
       floor_w = fmaxf(floor_w, __double2float_rd(t - (double)sm.score[lane] + sm.lse[lane]));
     }
   }
@@ -719,7 +731,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
   }
   // ---- too many: the beams one after the other, by their lse in 64 bits where it can matter for the
   //      last place; once more where candidates in front of it are near ties ----
-  const bool exact = W > 1 && (fabsf(theta) < 0x1p20f || theta == -INFINITY);
+  const bool exact = W > 1 && (fabsf(theta) < (float)kFar || theta == -INFINITY);
   if (exact)
     for (int w = 0; w < W; ++w)
       if (sm.floor[w] < INFINITY) exact_lse<DT>(p, w, sm);
