@@ -265,6 +265,33 @@ def test_huge_offsets(device):
     check_select(x, make_scores(device, 2, 3, 5), 6)
 
 
+def test_threads_on_one_stream(device):
+    """Two threads enqueue on the same stream, selections and steps of different sizes."""
+    import threading
+
+    gen = torch.Generator(device=device).manual_seed(3)
+    work = []
+    for G, W, V in ((3, 4, 30011), (2, 8, 9001)):
+        x = torch.randn(G * W, V, device=device, generator=gen) * 2.5
+        scores = make_scores(device, G, W, V)
+        work.append((x, scores, beam_search_select(x, scores, 16)))
+    torch.cuda.synchronize(device)
+    wrong = []
+
+    def run(x, scores, want):
+        for _ in range(200):
+            got = beam_search_select(x, scores, 16)
+            if not torch.equal(got.token_ids, want.token_ids):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_empty_batch(device):
     got = beam_search_select(torch.zeros(0, 10, device=device), torch.zeros(0, 4, device=device), 8)
     assert got.token_ids.shape == (0, 8)

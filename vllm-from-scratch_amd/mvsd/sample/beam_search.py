@@ -24,6 +24,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -180,6 +181,8 @@ def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.devi
 
 
 # Scratch of selections and steps, kept per (device, stream): calls on one stream follow each other.
+# A call is two launches: _LOCK is held over both, so that two threads' do not mix on a stream.
+_LOCK = threading.Lock()
 _SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, int, int]] = {}
 _SCRATCH_MOST = 1 << 24
 
@@ -234,13 +237,14 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
         return out
     rows, V = logits.shape
     stream = nat.stream_of(device)
-    scratch = _scratch(G, W, V, C, device, stream)
     base = ids.data_ptr()
-    nat.check(nat.lib().mvsd_beam_select(
-        base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
-        nat.dtype_code(logits.dtype), logits.stride(0), rows, nat.ptr(target_rows),
-        scores.data_ptr(), G, W, V, C, scratch[1], scratch[2], stream),
-        "mvsd_beam_select")
+    with _LOCK:
+        scratch = _scratch(G, W, V, C, device, stream)
+        status = nat.lib().mvsd_beam_select(
+            base, base + 4 * G * C, base + 8 * G * C, logits.data_ptr(),
+            nat.dtype_code(logits.dtype), logits.stride(0), rows, nat.ptr(target_rows),
+            scores.data_ptr(), G, W, V, C, scratch[1], scratch[2], stream)
+    nat.check(status, "mvsd_beam_select")
     return out
 
 
@@ -302,14 +306,16 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
         return step
     rows, V = logits.shape
     stream = nat.stream_of(device)
-    scratch = _scratch(G, W, V, C, device, stream)
     _STEP_HEAD.pack_into(args, 0, logits.data_ptr(), logits.stride(0), rows,
                          0 if target_rows is None else target_rows.data_ptr(), G, W, V, T,
                          stop_token_ids.data_ptr() if E else 0, E, length_penalty,
                          nat.dtype_code(logits.dtype), 1 if early_stopping else 0)
-    _STEP_TAIL.pack_into(args, 8 * (_STEP_TENSORS + 16), token_ids.data_ptr(), parents.data_ptr(),
-                         scratch[1], scratch[2])
-    nat.check(nat.lib().mvsd_beam_step(ctypes.byref(args), stream), "mvsd_beam_step")
+    with _LOCK:
+        scratch = _scratch(G, W, V, C, device, stream)
+        _STEP_TAIL.pack_into(args, 8 * (_STEP_TENSORS + 16), token_ids.data_ptr(),
+                             parents.data_ptr(), scratch[1], scratch[2])
+        status = nat.lib().mvsd_beam_step(ctypes.byref(args), stream)
+    nat.check(status, "mvsd_beam_step")
     return step
 
 
