@@ -44,6 +44,7 @@ constexpr int kListCap = 1024;     // tops that reach theta
 constexpr int kCandCap = 1024;     // gathered entries
 constexpr int kHeld = 4;           // vectors of tops a thread keeps in registers
 constexpr int kStats = 2;          // chunks that a lane of a beam loads at a time
+constexpr int kPowerBits = 8, kPowers = 1 << kPowerBits;  // of a 64-bit exponential's table
 constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 keys
 
 // How rows are split: columns per chunk, and the lanes that share a top (each holds NV vectors of the
@@ -249,6 +250,7 @@ struct BeamSmem {
   float score[kMaxBeams];  // -inf: proposes nothing
   float most[kMaxBeams];   // the row's largest entry
   double red[kFWaves];
+  double power[kPowers];   // 2^(k / kPowers)
   uint64_t near_ties, edge;  // beams whose candidates' order depends on their lse's last digits
   float floor[kMaxBeams];  // the least logit that can be a candidate (+inf: none)
   int hist[256];
@@ -411,41 +413,74 @@ __device__ inline int row_largest(const BeamScanParams& p, int64_t beam_row, int
   return found;
 }
 
-// The lse of a beam in 64 bits throughout, into sm.lse.
+// The lse of a beam in 64 bits throughout, into sm.lse.  exp(d), d <= 0: with k = round(256 d / ln 2) and
+// r = d - k ln 2 / 256 it is 2^(k / 256) exp(r), the first from a table of 256 and k's upper bits in the
+// exponent, the second, |r| < 0.0014, its series up to r^4 (4e-17).  One compute unit's vector pipes
+// bound it.
 template <int DT>
 __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
   using S = typename Elem<DT>::storage;
-  const int tid = threadIdx.x;
+  constexpr double kStep = 0.69314718055994530942 / kPowers;
+  constexpr int kDeep = 8;
+  const int tid = threadIdx.x, V = p.V;
   const S* row = static_cast<const S*>(p.logits) + sm.row[w];
-  const double most = (double)sm.most[w];
+  const float most = sm.most[w], least = most - 600.f;
+  if (tid < kPowers) sm.power[tid] = exp2(tid / (double)kPowers);
+  __syncthreads();
   double s = 0.0;
-#pragma unroll 4
-  for (int64_t i = tid; i < p.V; i += kFThreads) s += exp((double)Elem<DT>::cvt(row[i]) - most);
+  auto add = [&](float x) {
+    x = fmaxf(x, least);  // -inf, masks: nothing beside the sum, which is at least 1
+    const double d = (double)x - (double)most;
+    const float n = rintf((x - most) * (float)(1.0 / kStep));
+    const double r = fma((double)n, -kStep, d);
+    double e = fma(r, 1.0 / 24, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    const int k = (int)n;
+    const uint64_t power = __builtin_bit_cast(uint64_t, sm.power[k & (kPowers - 1)]);
+    const uint32_t high = (uint32_t)(power >> 32) + ((uint32_t)(k & -kPowers) << (20 - kPowerBits));
+    s = fma(e, __builtin_bit_cast(double, (uint64_t)high << 32 | (uint32_t)power), s);
+  };
+  const int whole = V / (kDeep * kFThreads) * (kDeep * kFThreads);
+  for (int b = 0; b < whole; b += kDeep * kFThreads) {
+    S x[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) x[k] = row[b + k * kFThreads + tid];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) add(Elem<DT>::cvt(x[k]));
+  }
+  for (int i = whole + tid; i < V; i += kFThreads) add(Elem<DT>::cvt(row[i]));
   s = lanes_sum(s, kWave);
   if (lane_id() == 0) sm.red[wave_id()] = s;
   __syncthreads();
   if (tid == 0) {
     double all = 0.0;
     for (int k = 0; k < kFWaves; ++k) all += sm.red[k];
-    sm.lse[w] = most + log(all);
+    sm.lse[w] = (double)most + log(all);
   }
   __syncthreads();
 }
 
-// How close two totals of different beams have to be for the scan's lse not to decide.  An lse is off
-// by at most 1.3e-6: five roundings of a lane's sum (3.0e-7), each power's own (1.2e-7), and those of its
-// argument, the difference to the maximum (2^-21 where it is below 16) times log2(e) (0.7 2^-21 where the
-// product is), for rows that keep all their mass at one such distance.  Two differ by twice that at most.
-// Totals past 2^30 add their own rounding; past kFar it hides any lse's.
-constexpr double kNear = 0x1p-18, kFar = 0x1p44;
+// How close two totals of different beams have to be for the scan's lse not to decide: twice the most
+// that an lse can be off by, 9e-7 for 16-bit rows and 1.4e-6 for fp32 ones.  That is five roundings of a
+// lane's sum (3.0e-7), each power's own (1.2e-7), its argument's (ln 2 2^-21 below 16, twice that below
+// 32, where the entries have at most seven tenths of the mass: 4.6e-7) and for fp32 the difference to
+// the maximum (2^-21).  Totals past 2^30 add their own rounding; past kFar it hides any lse's.
+template <int DT>
+constexpr double kNear = DT == MVSD_F32 ? 0x1p-18 : 0x1p-19;
+constexpr double kFar = 0x1p44;
 
-__device__ inline double near_by(double total) { return kNear + fabs(total) * 0x1p-51; }
+template <int DT>
+__device__ inline double near_by(double total) {
+  return kNear<DT> + fabs(total) * 0x1p-51;
+}
 
 // Of the `found` gathered candidates, the first C in sm.best: where two neighbours of different beams
 // are closer than kNear, or several beams have candidates so close to the last place, in it or behind
 // it, the lse of those beams is formed again, in 64 bits throughout, and true returned: the totals have
-// to be formed and ranked again.  A row of 151936 entries takes 33 us more; a group of 8 beams and 16
-// candidates has such a pair about once in 1250.
+// to be formed and ranked again.  A row of 151936 entries takes 22 us more; a group of 8 beams and 16
+// candidates has such a pair about once in 2500 (16-bit rows).
 template <int DT>
 __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, BeamSmem& sm) {
   const int tid = threadIdx.x, have = min(found, p.C);
@@ -454,14 +489,14 @@ __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, Beam
   if (tid + 1 < have) {
     const int a = sm.best.beam[tid], b = sm.best.beam[tid + 1];
     const double t = sm.best.total[tid];
-    if (a != b && fabs(t) < kFar && t - sm.best.total[tid + 1] < near_by(t))
+    if (a != b && fabs(t) < kFar && t - sm.best.total[tid + 1] < near_by<DT>(t))
       atomicOr((unsigned long long*)&sm.near_ties, 1ull << a | 1ull << b);
   }
   if (found > have) {
     const double last = sm.best.total[have - 1];
     if (fabs(last) < kFar)
       for (int i = tid; i < found; i += kFThreads)
-        if (fabs(sm.cand.total[i] - last) < near_by(last))
+        if (fabs(sm.cand.total[i] - last) < near_by<DT>(last))
           atomicOr((unsigned long long*)&sm.edge, 1ull << sm.cand.beam[i]);
   }
   __syncthreads();
@@ -603,7 +638,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     if (theta != -INFINITY) {
       // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
       // (and the scan's lse for one near by)
-      const double t = (double)theta - fabs((double)theta) * 0x1p-23 - kNear;
+      const double t = (double)theta - fabs((double)theta) * 0x1p-23 - kNear<DT>;
       floor_w = fmaxf(floor_w, __double2float_rd(t - (double)sm.score[lane] + sm.lse[lane]));
     }
   }
