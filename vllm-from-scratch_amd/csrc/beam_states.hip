@@ -12,6 +12,12 @@ namespace mvsd {
 // In place, a thread owns a few bytes of all W rows of a group: it loads what each row needs into
 // registers, then stores, so no row is overwritten before it has been read, with no second buffer and
 // no order among threads.  Rows that keep their beam are neither read nor written.
+//
+// What bounds it: memory.  Each moved byte is read once (a parent of several beams once for each, the
+// others from the caches) and stored past the caches, since nothing here reads it again: 1355 MB of
+// eight caches move in 250 us with such stores and 271 with ordinary ones (5.4 TB/s read and written; a
+// large copy reaches 4.9), 72 MB of pages in 14.2 us and 17.6.  Sixteen bytes a thread of 8, 16 or 32
+// rows (the least that holds W) and eight of 64 stay in registers.
 
 typedef u32x4 u32x4_align1 __attribute__((aligned(1)));
 typedef u32x2 u32x2_align1 __attribute__((aligned(1)));
@@ -138,10 +144,13 @@ hipError_t launch_beam_reorder(const BeamStatesParams& p, bool in_place, hipStre
 //   4 and, for every span at once, through its sub-chunks;
 //   5 every sub-chunk is walked again from there, all at once, and leaves the beam of each step, by
 //     which the workgroup writes the sequences' tokens, on their way since the start.
+// What bounds it: the chain of LDS reads, 16 for each of the walks 1 and 5 and up to 8 for 2 to 4, and
+// before it the lengths and then the histories: 7.9 us for one group of 64 steps, 14 to 16 for 64 groups
+// of 8 beams and 2048 steps (10 MB).
 // Where there are few groups, several workgroups share a group's hypotheses; all of them compose.
 // Histories of one chunk take one launch.  Longer ones take two: the first leaves the hypotheses,
 // every chunk's map and, for a hypothesis that ends in the chunk, its beam below it; the second starts
-// from those.
+// from those (4 groups of 4 beams and 65536 steps: 7.0 and 11.4 us).
 
 constexpr int kTThreads = 512;
 constexpr int kSub = 16, kSpan = 8, kSpanSteps = kSub * kSpan;
