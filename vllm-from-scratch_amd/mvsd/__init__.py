@@ -12,6 +12,8 @@ Drop-in replacements for minivllm's verification path, module for module:
     mvsd.outputs                       <- minivllm/outputs.py (SamplerOutput, DraftTokenIds)
     mvsd.testing.spec_metadata         <- minivllm/testing/spec_metadata.py
 
+Beside them, without a counterpart there: beam search (mvsd.sample.beam_search).
+
 The arithmetic runs in hand-written HIP kernels for gfx950 (``csrc/``), reached through the C
 ABI of ``include/mvsd.h`` (libmvsd.so, loaded with ctypes by ``mvsd._native``).
 """
