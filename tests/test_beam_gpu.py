@@ -229,6 +229,15 @@ def test_equal_beams_in_front_of_large_masks(device):
     check_select(x.reshape(2 * G, V), torch.full((G, 2), -20.0, device=device), 100)
 
 
+@pytest.mark.parametrize("large", [1e10, -1e10, 1e30, -1e30])
+def test_near_ties_of_huge_logits(device, large):
+    """Logits so large that nothing but their maximum counts: two of it in one beam, three in the
+    others, of which two are equal."""
+    x = torch.full((3, 9001), -abs(large) * 4, device=device)
+    x[:, 5] = x[:, 8000] = x[1:, 40] = large
+    check_select(x, torch.full((1, 3), -20.0, device=device), 8)
+
+
 @pytest.mark.parametrize("heavier", [0, 1])
 def test_near_ties_in_front_of_masked_tokens(device, heavier):
     """Two tokens a beam allowed, the others at the type's lowest value: the last places are runs of

@@ -424,14 +424,14 @@ __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
   constexpr int kDeep = 8;
   const int tid = threadIdx.x, V = p.V;
   const S* row = static_cast<const S*>(p.logits) + sm.row[w];
-  const float most = sm.most[w], least = most - 600.f;
+  const float most = sm.most[w];
   if (tid < kPowers) sm.power[tid] = exp2(tid / (double)kPowers);
   __syncthreads();
   double s = 0.0;
   auto add = [&](float x) {
-    x = fmaxf(x, least);  // -inf, masks: nothing beside the sum, which is at least 1
-    const double d = (double)x - (double)most;
-    const float n = rintf((x - most) * (float)(1.0 / kStep));
+    // (-600 for masks and -inf: nothing beside the sum, which is at least 1)
+    const double d = fmax((double)x - (double)most, -600.0);
+    const float n = rintf(fmaxf(x - most, -600.f) * (float)(1.0 / kStep));
     const double r = fma((double)n, -kStep, d);
     double e = fma(r, 1.0 / 24, 1.0 / 6);
     e = fma(e, r, 0.5);

@@ -182,7 +182,7 @@ def _check_rows(logits: torch.Tensor, G: int, W: int, target_rows) -> torch.devi
 
 # Scratch of selections and steps, kept per (device, stream): calls on one stream follow each other.
 # A call is two launches: _LOCK is held over both, so that two threads' do not mix on a stream.
-_LOCK = threading.Lock()
+_LOCK = threading.RLock()
 _SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, int, int]] = {}
 _SCRATCH_MOST = 1 << 24
 
