@@ -463,24 +463,21 @@ __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
 }
 
 // How close two totals of different beams have to be for the scan's lse not to decide: twice the most
-// that an lse can be off by, 9e-7 for 16-bit rows and 1.4e-6 for fp32 ones.  That is five roundings of a
-// lane's sum (3.0e-7), each power's own (1.2e-7), its argument's (ln 2 2^-21 below 16, twice that below
-// 32, where the entries have at most seven tenths of the mass: 4.6e-7) and for fp32 the difference to
-// the maximum (2^-21).  Totals past 2^30 add their own rounding; past kFar it hides any lse's.
-template <int DT>
-constexpr double kNear = DT == MVSD_F32 ? 0x1p-18 : 0x1p-19;
-constexpr double kFar = 0x1p44;
+// that an lse is off by, 9.2e-7, for rows that keep nearly all their mass at one distance below the
+// maximum.  That is each power's own rounding (1.2e-7), its argument's (ln 2 2^-21 below 16, twice that
+// below 32, where the entries have at most seven tenths of the mass: 4.6e-7) and the difference to the
+// maximum (seven tenths of 2^-21; 16-bit rows: exact); the sums of entries that are alike are exact in
+// pairs, and five roundings of unlike ones cancel over the lanes.  (Rows drawn at random: 1e-8.)
+// Totals past 2^30 add their own rounding; past kFar it hides any lse's.
+constexpr double kNear = 0x1p-19, kFar = 0x1p44;
 
-template <int DT>
-__device__ inline double near_by(double total) {
-  return kNear<DT> + fabs(total) * 0x1p-51;
-}
+__device__ inline double near_by(double total) { return kNear + fabs(total) * 0x1p-51; }
 
 // Of the `found` gathered candidates, the first C in sm.best: where two neighbours of different beams
 // are closer than kNear, or several beams have candidates so close to the last place, in it or behind
 // it, the lse of those beams is formed again, in 64 bits throughout, and true returned: the totals have
 // to be formed and ranked again.  A row of 151936 entries takes 22 us more; a group of 8 beams and 16
-// candidates has such a pair about once in 2500 (16-bit rows).
+// candidates has such a pair about once in 2500.
 template <int DT>
 __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, BeamSmem& sm) {
   const int tid = threadIdx.x, have = min(found, p.C);
@@ -489,14 +486,14 @@ __device__ inline bool settle_near_ties(const BeamScanParams& p, int found, Beam
   if (tid + 1 < have) {
     const int a = sm.best.beam[tid], b = sm.best.beam[tid + 1];
     const double t = sm.best.total[tid];
-    if (a != b && fabs(t) < kFar && t - sm.best.total[tid + 1] < near_by<DT>(t))
+    if (a != b && fabs(t) < kFar && t - sm.best.total[tid + 1] < near_by(t))
       atomicOr((unsigned long long*)&sm.near_ties, 1ull << a | 1ull << b);
   }
   if (found > have) {
     const double last = sm.best.total[have - 1];
     if (fabs(last) < kFar)
       for (int i = tid; i < found; i += kFThreads)
-        if (fabs(sm.cand.total[i] - last) < near_by<DT>(last))
+        if (fabs(sm.cand.total[i] - last) < near_by(last))
           atomicOr((unsigned long long*)&sm.edge, 1ull << sm.cand.beam[i]);
   }
   __syncthreads();
@@ -638,7 +635,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     if (theta != -INFINITY) {
       // a rounded total at or above theta stands for one of at least theta - |theta| 2^-24
       // (and the scan's lse for one near by)
-      const double t = (double)theta - fabs((double)theta) * 0x1p-23 - kNear<DT>;
+      const double t = (double)theta - fabs((double)theta) * 0x1p-23 - kNear;
       floor_w = fmaxf(floor_w, __double2float_rd(t - (double)sm.score[lane] + sm.lse[lane]));
     }
   }
