@@ -678,7 +678,8 @@ int mvsd_beam_step(const mvsd_beam_step_args* args, mvsd_stream_t stream);
 /* or g * W + w; a row outside [0, num_rows) is neither read nor written.  A parent outside  */
 /* [0, W) is the beam itself.  dst == src in every state (with equal strides) reorders in    */
 /* place; else none of the dst may overlap a src, and rows that keep their beam are copied   */
-/* too.  Slots of one call are distinct.  Everything else is left as it was.                 */
+/* too.  Slots of one call are distinct.  At most 512 states, rows of at most 2^34 bytes.     */
+/* Everything else is left as it was.                                                        */
 /* ------------------------------------------------------------------------------------ */
 typedef struct mvsd_beam_state {
   const void* src;

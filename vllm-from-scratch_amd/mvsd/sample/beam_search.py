@@ -397,6 +397,9 @@ def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None 
     0..W-1 (the -1 of a resting group) keeps the beam's own row; a slot outside the pool is left
     alone.
 
+    At most 512 tensors a call, rows below 16 GiB, no memory in common except rows that interleave
+    with equal strides (keys and values of one tensor).
+
     Without ``out`` the states are reordered in place, in one pass and without a second buffer; with
     ``out`` (tensors of the same shapes that share no memory with the states) the rows are written
     there.  Returns the tensors written.  Nothing else is touched.
