@@ -847,3 +847,40 @@ def test_refusals(device):
             bad()
     with pytest.raises(NotImplementedError):
         beam_search_select(x, s.cpu(), 8)
+
+
+# ----------------------------------------------------------------- rows shorter than a vector
+
+
+def short_rows(device, dtype, V, G=4):
+    """Groups of four beams: +inf in the first one's row, a NaN in the second's, +inf throughout a row
+    whose beam has no finite score, and a fourth beam that goes on (in the last group not even that)."""
+    gen = torch.Generator(device=device).manual_seed(V)
+    x = torch.randn(G * 4, V, device=device, generator=gen).to(DTYPES[dtype])
+    x[0::4, V // 2] = math.inf
+    x[1::4, V - 1] = math.nan
+    x[2::4] = math.inf
+    x[-1] = math.inf
+    scores = make_scores(device, G, 4, V)
+    for g in range(G):
+        scores[g, 2] = (-math.inf, math.nan, math.inf, -math.inf)[g % 4]
+    return x, scores
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("V", [1, 2, 3, 4, 5, 7, 8, 9])
+def test_short_rows_of_beams_that_propose_nothing(device, dtype, V):
+    x, scores = short_rows(device, dtype, V)
+    for C in (1, V, 40, 256):
+        got = check_select(x, scores, C)
+        assert (got.parents[:-1, :min(C, V)] == 3).all() and (got.parents[-1] == -1).all()
+    state = random_state(device, 4, 4, 9, V)
+    state.scores = scores
+    # (not check_step, which compares the old state with itself: one of its scores is a NaN)
+    want = oracle.step(rows_of(x, 4), host(state), [0, 2])
+    got = beam_search_step(x, state, stop_token_ids=torch.tensor([0, 2], dtype=torch.int32,
+                                                                 device=device))
+    check_state(got.state, want)
+    assert np.array_equal(got.token_ids.cpu().numpy(), want["token_ids"])
+    assert np.array_equal(got.parents.cpu().numpy(), want["parents"])
+    assert bool(got.state.done[-1])

@@ -668,6 +668,7 @@ __device__ inline int group_candidates(const BeamScanParams& p, int g, BeamSmem&
     if (p.V < VEC) {  // uniform: rows shorter than a vector
       for (int i = tid; i < W * p.V; i += kFThreads) {
         const int w = i / p.V, col = i - w * p.V;
+        if (sm.floor[w] == INFINITY) continue;  // proposes nothing, whatever its row holds
         const float x = Elem<DT>::cvt(x0[sm.row[w] + col]);
         if (x >= sm.floor[w]) {
           const int pos = atomicAdd(&sm.count, 1);
