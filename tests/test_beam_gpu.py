@@ -884,3 +884,59 @@ def test_short_rows_of_beams_that_propose_nothing(device, dtype, V):
     assert np.array_equal(got.token_ids.cpu().numpy(), want["token_ids"])
     assert np.array_equal(got.parents.cpu().numpy(), want["parents"])
     assert bool(got.state.done[-1])
+
+
+# ----------------------------------------------------------------- how far scores may be off
+
+# Half the distance below which the order of two beams is settled in 64 bits: what the scan's log-sum may
+# be off by.  (The tolerance at the top counts a row's maximum for a wave's, and its errors one by one.)
+SCAN_ERROR = 2.0 ** -20
+
+
+def check_scores(x, C):
+    """Totals around zero, so that a score's own rounding hides nothing, of groups of one beam, where no
+    near tie has a log-sum formed again."""
+    lse = torch.logsumexp(x.double(), dim=-1)
+    scores = (lse - x.double().amax(-1)).float().view(-1, 1)
+    got = beam_search_select(x, scores, C)
+    ids, parents, want = oracle.select(rows_of(x, 1), scores.cpu().numpy(), C)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    assert np.array_equal(got.parents.cpu().numpy(), parents)
+    bar = SCAN_ERROR + 2.0 ** -24 * np.abs(want)
+    off = np.abs(got.scores.double().cpu().numpy() - want)
+    assert (off <= bar).all(), float((off - bar).max())
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("G,V", [(3, 700), (2, 9001), (2, 50257), (16, 151936), (8, 262144)])
+def test_scores_of_random_rows(device, dtype, G, V):
+    gen = torch.Generator(device=device).manual_seed(V)
+    x = torch.randn(G * 2, V, device=device, generator=gen)
+    for spread in (0.3, 2.5, 6.0):
+        check_scores((x * spread).to(DTYPES[dtype]), 3)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("G,V", [(2, 4096), (16, 151936), (16, 262144), (1, 1 << 20)])
+@pytest.mark.parametrize("every", [512, 2048, 1 << 30])
+def test_scores_of_rows_at_one_distance(device, dtype, G, V, every):
+    """Entries at one distance below the maximum, which there is once in the row, in every 2048 or in
+    every 512 columns: the scan's worst rows, at the distances where its exponentials round more coarsely."""
+    t = DTYPES[dtype]
+    for k, far in enumerate((0.7, 2.78, 4.02, 5.55, 6.3, 8.03, 9.9, 11.1, 13.0, 16.1)):
+        top = 0.3 + 0.0123 * k  # a value with all its bits set or not: differences round
+        x = torch.full((G * 2, V), top - far, device=device).to(t)
+        x[:, 7::every] = top
+        x[1::2, 11] = top - 0.01
+        check_scores(x, 2)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("far", [3.0, 6.5, 12.0, 20.0])
+def test_scores_of_peaked_rows(device, dtype, far):
+    """One entry above a row of others around `far` below it."""
+    gen = torch.Generator(device=device).manual_seed(int(far))
+    for G, V in ((3, 700), (16, 151936)):
+        x = torch.randn(G * 2, V, device=device, generator=gen) * 0.5 - far
+        x[:, V // 3] = 1.0
+        check_scores(x.to(DTYPES[dtype]), 2)

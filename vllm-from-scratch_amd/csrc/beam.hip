@@ -463,11 +463,14 @@ __device__ inline void exact_lse(const BeamScanParams& p, int w, BeamSmem& sm) {
 }
 
 // How close two totals of different beams have to be for the scan's lse not to decide: twice the most
-// that an lse is off by, 9.2e-7, for rows that keep nearly all their mass at one distance below the
-// maximum.  That is each power's own rounding (1.2e-7), its argument's (ln 2 2^-21 below 16, twice that
-// below 32, where the entries have at most seven tenths of the mass: 4.6e-7) and the difference to the
-// maximum (seven tenths of 2^-21; 16-bit rows: exact); the sums of entries that are alike are exact in
-// pairs, and five roundings of unlike ones cancel over the lanes.  (Rows drawn at random: 1e-8.)
+// that an lse is off by, 9.1e-7, whatever the row's type and length.  Every wave sums its 2048 columns (512
+// in short chunks) below their own maximum, and the waves' sums are joined in 64 bits, so the worst
+// relative error of a wave's sum is that of the row's.  An exponential at distance D below the maximum is
+// off by the power's own rounding (2^-23), its argument's (D < 5.54: ln 2 2^-22, < 11.1: ln 2 2^-21, and so
+// on) and, unless the values' exponents are near each other, the distance's (D < 8: 2^-22, < 16: 2^-21);
+// all of them together have at most 2047 e^-D / (1 + 2047 e^-D) of the sum.  The product is largest at
+// D = 5.55: 6.9e-7 of 0.89.  Five roundings of partial sums add 3.0e-7.  (The worst of waves searched for
+// it: 5.8e-7; rows drawn at random: 1e-8.)
 // Totals past 2^30 add their own rounding; past kFar it hides any lse's.
 constexpr double kNear = 0x1p-19, kFar = 0x1p44;
 
