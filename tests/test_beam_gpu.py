@@ -940,3 +940,30 @@ def test_scores_of_peaked_rows(device, dtype, far):
         x = torch.randn(G * 2, V, device=device, generator=gen) * 0.5 - far
         x[:, V // 3] = 1.0
         check_scores(x.to(DTYPES[dtype]), 2)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("G,V", [(3, 3), (5, 700), (4, 9001), (4, 151936), (64, 151936)])
+def test_scores_of_confident_rows(device, dtype, G, V):
+    """One entry has nearly all the mass: its log-probability, close to zero, is good to 2^-18 of itself
+    (the terms of the others, 44 or less below it, to 3.4e-6; their partial sums to 3.0e-7)."""
+    gen = torch.Generator(device=device).manual_seed(V)
+    noise = torch.randn(G, V, device=device, generator=gen)
+    for far in (7.0, 9.5, 12.0, 16.5, 20.0, 25.0, 31.0, 40.0):
+        for spread in (0.0, 0.7):
+            x = noise * spread - far
+            x[:, [V // 3 - 1, 0, V - 1][int(far) % 3]] = 0.37
+            if V > 8:
+                x[:, 5] = -math.inf
+                x[:, 6] = -3e4
+            x = x.to(DTYPES[dtype])
+            got = beam_search_select(x, torch.zeros(G, 1, device=device), 2)
+            ids, _, _ = oracle.select(rows_of(x, 1), np.zeros((G, 1)), 2)
+            assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+            rows = x.double()
+            top = rows.amax(-1, keepdim=True)
+            rest = torch.where(rows < top, (rows - top).exp(), 0.0).sum(-1)
+            want = -torch.log1p(rest)  # of the best token, of which there is one a row
+            off = (got.scores[:, 0].double() - want).abs()
+            # ... and up to 16 roundings of 64-bit sums between 1 and 2, 2^-53 each
+            assert (off <= want.abs() * (2.0 ** -18 + 2.0 ** -24) + 2.0 ** -49).all(), (far, spread)

@@ -132,6 +132,15 @@ __device__ inline u32x4 load_scan(const typename Elem<DT>::storage* row, int col
       reinterpret_cast<const Vec16<DT>*>(row + min(col, V - Elem<DT>::kVec)));
 }
 
+// A wave whose sum, its maximum's 1 included, is below kPeaked adds its exponentials again without that one
+// (no other is 1: the sum would be 2), which then comes in 64 bits.  In its lane's fp32 sum, what is below
+// 2^-24 beside it would be lost, and the log-probability of a confident model's best token is
+// -log(1 + rest) of such waves: with 151936 entries 20 below the best one it was 2e-4 of itself off, now at
+// most the 1.7e-6 of an exponential.  Above kPeaked the partial sums' 3.0e-7 are at most 1.4e-6 of
+// log(kPeaked).  (The branch costs nothing measurable where it is not taken; the largest entry left out
+// everywhere took 63 us instead of 58 for 128 groups of 8 bf16 rows of 151936.)
+constexpr double kPeaked = 1.25;
+
 template <int DT, int NV, int LANES, bool STREAM>
 __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
   constexpr int kTops = kThreads / LANES;
@@ -170,14 +179,25 @@ __global__ __launch_bounds__(kThreads) void beam_scan_kernel(BeamScanParams p) {
                          fmaxf(readlane_f32(top16, 32), readlane_f32(top16, 48)));
   float s = 0.f;
   if (wm != -INFINITY) {  // +inf gives a NaN sum, as a NaN does
-    s = pair_sum<NV * VEC>([&](int i) { return exp_of(v[i / VEC][i % VEC] - wm); });
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[j][e] = exp_of(v[j][e] - wm);
+    s = pair_sum<NV * VEC>([&](int i) { return v[i / VEC][i % VEC]; });
   } else {  // every entry is -inf or NaN
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) s += v[j][e] != v[j][e] ? NAN : 0.f;
   }
-  const double sum64 = lanes_sum((double)s, kWave);
+  double sum64 = lanes_sum((double)s, kWave);
+  if (wm != -INFINITY && sum64 < kPeaked) {  // wave-uniform; a NaN sum is not
+    s = pair_sum<NV * VEC>([&](int i) {
+      const float e = v[i / VEC][i % VEC];
+      return e == 1.f ? 0.f : e;
+    });
+    sum64 = 1.0 + lanes_sum((double)s, kWave);
+  }
   const int64_t slot = (int64_t)r * p.nchunks + c;
   if (tid % LANES == 0) p.tops[slot * kTops + tid / LANES] = top;
   if (lane_id() == 0) {
