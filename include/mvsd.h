@@ -705,8 +705,10 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
 /* first, the finished ones first where they are equal.  token_ids [G, num_return,           */
 /* max_length] (-1 behind a sequence), lengths and scores [G, num_return] (none: 0, -inf).   */
 /* The tokens of a hypothesis of L tokens are its last token at L - 1 and, from t = L - 2     */
-/* down, token_history[g, t, b] with b the beam at step t: the hypothesis' own, then          */
-/* parent_history[g, t, b] (outside [0, W): b itself).                                        */
+/* down, token_history[g, t, b] with b the beam at step t: the hypothesis' own (of a finished  */
+/* one finished_beams, outside [0, W): beam 0; of running beam w of L tokens                  */
+/* parent_history[g, L - 1, w]), then parent_history[g, t, b].  A parent outside [0, W) is    */
+/* the beam itself.                                                                           */
 /* workspace: mvsd_beam_finish_workspace_bytes() bytes (0: none needed), no initial contents  */
 /* needed; one per call in flight.                                                            */
 /* ------------------------------------------------------------------------------------ */

@@ -94,7 +94,9 @@ def finish(state: dict, count: int, length_penalty=1.0):
                 for j in range(W) if state["finished_scores"][g, j] > NINF]
         at = min(max(int(state["lengths"][g]), 0), T)
         if not state["done"][g] and at > 0:
-            pool += [(float(s) / float(at) ** length_penalty, state["parent_history"][g, at - 1, w],
+            parents = [int(p) if 0 <= p < W else w
+                       for w, p in enumerate(state["parent_history"][g, at - 1])]
+            pool += [(float(s) / float(at) ** length_penalty, parents[w],
                       state["token_history"][g, at - 1, w], at)
                      for w, s in enumerate(state["scores"][g]) if np.isfinite(s)]
         pool.sort(key=lambda h: -h[0])

@@ -967,3 +967,33 @@ def test_scores_of_confident_rows(device, dtype, G, V):
             off = (got.scores[:, 0].double() - want).abs()
             # ... and up to 16 roundings of 64-bit sums between 1 and 2, 2^-53 each
             assert (off <= want.abs() * (2.0 ** -18 + 2.0 ** -24) + 2.0 ** -49).all(), (far, spread)
+
+
+# ----------------------------------------------------------------- answers of odd states
+
+
+@pytest.mark.parametrize("T", [8, 5000])
+def test_a_running_beam_without_a_recorded_parent_is_its_own(device, T):
+    """The last recorded parent outside the group: the beam goes on from its own place."""
+    W, L = 5, T - 1
+    state = BeamState.new(1, W, T, device)
+    gen = torch.Generator(device=device).manual_seed(T)
+    state.token_history = torch.randint(0, 99, (1, T, W), device=device, generator=gen,
+                                        dtype=torch.int32)
+    state.parent_history = torch.arange(W, device=device, dtype=torch.int32).expand(1, T, W).clone()
+    state.parent_history[0, L - 1] = torch.tensor([-1, W, 4, 2 ** 31 - 1, -2 ** 31], device=device)
+    state.scores = -torch.arange(1, W + 1, device=device, dtype=torch.float32)[None] * L
+    state.lengths.fill_(L)
+    # a finished hypothesis of a beam outside the group counts as beam 0's
+    state.finished_scores[0, 0], state.finished_beams[0, 0] = -0.5, W
+    state.finished_token_ids[0, 0], state.finished_lengths[0, 0] = 7, L - 2
+    got = beam_search_finish(state)
+    assert got.lengths[0].tolist() == [L - 2] + [L] * 4
+    h = state.token_history[0]
+    assert torch.equal(got.token_ids[0, 0, :L - 3], h[:L - 3, 0]) and got.token_ids[0, 0, L - 3] == 7
+    for place, (w, own) in enumerate([(0, 0), (1, 1), (2, 4), (3, 3)], start=1):
+        assert torch.equal(got.token_ids[0, place, :L - 1], h[:L - 1, own])
+        assert got.token_ids[0, place, L - 1] == h[L - 1, w]
+    ids, lengths, scores = oracle.finish(host(state), W, 1.0)
+    assert np.array_equal(got.token_ids.cpu().numpy(), ids)
+    close(got.scores, scores)

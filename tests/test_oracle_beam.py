@@ -108,3 +108,14 @@ def test_reorder_reads_the_rows_before_the_call():
     want[0, :2], want[1, :2], want[2, :2] = x[1, :2], x[0, :2], x[1, :2]
     want[5] = x[3]
     assert (got == want).all()
+
+
+def test_a_running_beam_without_a_recorded_parent_is_its_own():
+    s = new_state(1, 3, 4)
+    s["token_history"] = np.arange(12).reshape(1, 4, 3)
+    s["parent_history"] = np.array([[[0, 1, 2], [0, 1, 2], [-1, 7, 0], [0, 0, 0]]])
+    s["scores"] = np.array([[-1.0, -2.0, -3.0]], np.float32)
+    s["lengths"][0] = 3
+    ids, lengths, _ = beam.finish(s, 3)
+    assert lengths.tolist() == [[3, 3, 3]]
+    assert ids[0, :, :3].tolist() == [[0, 3, 6], [1, 4, 7], [0, 3, 8]]

@@ -132,7 +132,8 @@ hipError_t launch_beam_reorder(const BeamStatesParams& p, bool in_place, hipStre
 // Of each group the n best of its finished hypotheses and, unless it is done, its running beams (a
 // running beam is its last token appended to its parent), the finished ones first where they are
 // equal; then each one's tokens, from the last step back: the token and the parent recorded in the
-// beam's place.  A parent outside [0, W) is the beam itself.
+// beam's place.  A parent outside [0, W) is the beam itself; a finished hypothesis' beam outside it, of
+// which there is no other record, counts as beam 0.
 //
 // With b_t the beam at step t, b_(t-1) = parent_t(b_t): a chain of T dependent reads.  The steps'
 // maps are composed instead.  A workgroup holds the parents of a chunk of steps in LDS, a byte each,
@@ -209,15 +210,15 @@ __device__ inline void best_hypotheses(const mvsd_beam_finish_args& a, int64_t g
     rank_old += (o > old || (o == old && j < lane)) + (r > old);
     rank_now += (o >= now) + (r > now || (r == now && j < lane));
   }
-  auto put = [&](int rank, float score, int b, int id, int l) {
+  auto put = [&](int rank, float score, int b, int own, int id, int l) {
     const bool any = score > -INFINITY;
-    sm.beam[rank] = any && b >= 0 && b < W ? b : 0;
+    sm.beam[rank] = !any ? 0 : b >= 0 && b < W ? b : own;
     sm.token[rank] = id;
     sm.len[rank] = any ? min(max(l, 0), T) : 0;
     sm.score[rank] = score;
   };
-  if (lane < W && rank_old < n) put(rank_old, old, old_beam, old_token, old_len);
-  if (lane < W && rank_now < n) put(rank_now, now, beam, token, len);
+  if (lane < W && rank_old < n) put(rank_old, old, old_beam, 0, old_token, old_len);
+  if (lane < W && rank_now < n) put(rank_now, now, beam, lane, token, len);
 }
 
 // Workgroup (group, chunk, part): hypotheses [part * per, part * per + per) of the group.  Sizes of
