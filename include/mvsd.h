@@ -622,7 +622,8 @@ int mvsd_beam_select(int32_t* token_ids, int32_t* parents, float* out_scores, co
 /* with the candidates of beam_select (W (1 + num_stop_ids) of them, at most 256) and        */
 /* L = length + 1:                                                                          */
 /*   - stop tokens among the W best candidates end a hypothesis of score                     */
-/*     fl32(fl32(total) / L^length_penalty); finished_* keep the W best old and new ones,    */
+/*     fl32(fl32(total) / L^length_penalty), or fp32's largest value where that is beyond it */
+/*     (as all such scores below); finished_* keep the W best old and new ones,              */
 /*     best first (the old first where they are equal; none: -inf, -1, -1, 0);               */
 /*   - the W best candidates that are no stop tokens are the next beams: out_scores,         */
 /*     token_ids, parents (none: -inf, -1, -1), also recorded at token_history and           */

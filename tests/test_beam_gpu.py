@@ -997,3 +997,38 @@ def test_a_running_beam_without_a_recorded_parent_is_its_own(device, T):
     ids, lengths, scores = oracle.finish(host(state), W, 1.0)
     assert np.array_equal(got.token_ids.cpu().numpy(), ids)
     close(got.scores, scores)
+
+
+@pytest.mark.parametrize("alpha", [-30.0, -400.0, -1e300])
+def test_scores_beyond_fp32_are_still_hypotheses(device, alpha):
+    """Penalties that take every score below fp32's lowest value: hypotheses are kept, in order."""
+    W, V, T, lowest = 3, 40, 30, -torch.finfo(torch.float32).max
+    x = torch.full((W, V), -4.0, device=device)
+    x[0, 5], x[1, 5], x[2, 8] = 3.0, 2.0, 4.0
+    state = BeamState.new(1, W, T, device)
+    state.scores = torch.tensor([[-8.0, -8.5, -8.6]], device=device)
+    state.lengths.fill_(19)
+    state.parent_history = torch.arange(W, device=device, dtype=torch.int32).expand(1, T, W).clone()
+    stop = torch.tensor([5], dtype=torch.int32, device=device)
+    step = beam_search_step(x, state, stop_token_ids=stop, length_penalty=alpha)
+    # the three best candidates: token 5 of beam 0, 8 of beam 2, 5 of beam 1
+    assert state.finished_scores[0].tolist() == [lowest, lowest, -math.inf]
+    assert state.finished_beams[0].tolist() == [0, 1, -1]
+    assert state.finished_lengths[0].tolist() == [20, 20, 0]
+    assert step.parents[0, 0] == 2 and step.token_ids[0, 0] == 8 and not state.done[0]
+    got = beam_search_finish(state, length_penalty=alpha)
+    assert got.scores[0].tolist() == [lowest] * 3 and got.lengths[0].tolist() == [20] * 3
+    assert got.token_ids[0, :, 19].tolist() == [5, 5, 8]
+
+
+@pytest.mark.parametrize("alpha", [400.0, 1e300])
+def test_scores_that_vanish_are_still_hypotheses(device, alpha):
+    W, V = 2, 40
+    x = torch.zeros(W, V, device=device)
+    state = BeamState.new(1, W, 30, device)
+    state.scores = torch.tensor([[0.0, 0.0]], device=device)
+    state.lengths.fill_(19)
+    stop = torch.tensor([0], dtype=torch.int32, device=device)
+    step = beam_search_step(x, state, stop_token_ids=stop, length_penalty=alpha)
+    assert state.finished_scores[0].tolist() == [0.0, -math.inf]
+    assert state.finished_token_ids[0].tolist() == [0, -1] and step.token_ids[0].tolist() == [1, 2]

@@ -13,7 +13,7 @@ constexpr int kMaxCandidates = 256;  // of a group
 constexpr int kMaxBeamStates = 24;   // state tensors of one launch (kernel arguments)
 
 #ifdef __HIPCC__
-// len^alpha, len >= 1, to about 2^-50: 2^(alpha log2(len)), the logarithm of the mantissa m in
+// len^alpha, len >= 1, inside 2^-1000 .. 2^1000, to about 2^-50: 2^(alpha log2(len)), the logarithm of the mantissa m in
 // [1/sqrt 2, sqrt 2) from the series of atanh((m - 1) / (m + 1)), the power of the fraction from that
 // of exp.  (The library's pow, exact to the last bit, took 3000 cycles of a group's 20000.)
 __device__ inline double len_power(int len, double alpha) {
@@ -30,12 +30,18 @@ __device__ inline double len_power(int len, double alpha) {
   for (int k = 19; k >= 1; k -= 2) ln = fma(ln, s2, 1.0 / k);
   ln *= 2.0 * s;
   const double y = alpha * ((double)e + ln * 1.4426950408889634074);
-  const double n = rint(fmin(fmax(y, -2000.0), 2000.0));
-  const double f = (y - n) * 0.69314718055994530942;
+  const double in = fmin(fmax(y, -1000.0), 1000.0), n = rint(in);
+  const double f = (in - n) * 0.69314718055994530942;
   double x = 1.0;
 #pragma unroll
   for (int k = 14; k >= 1; --k) x = fma(x, f * (1.0 / k), 1.0);
   return ldexp(x, (int)n);
+}
+
+// A hypothesis' score: fl32(total / power), and fp32's largest value beyond it, since -inf says that there
+// is no hypothesis (a negative alpha: 20 tokens to the 30th).
+__device__ inline float hypothesis_score(float total, double power) {
+  return fminf(fmaxf((float)((double)total / power), -3.402823466e38f), 3.402823466e38f);
 }
 #endif
 

@@ -923,8 +923,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   if (tid >= W && tid < 2 * W) {
     const int r = tid - W;
     if (r < found && ((sm.stop_mask[r / kWave] >> (r % kWave)) & 1)) {
-      hyp = (float)((double)(float)sm.best.total[r] / power);
-      if (!(hyp > -INFINITY)) hyp = -INFINITY;
+      hyp = hypothesis_score((float)sm.best.total[r], power);
       hyp_beam = sm.best.beam[r];
       hyp_token = sm.best.token[r];
       hyp_len = new_len;
@@ -951,7 +950,7 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   if (tid == 0) {
     const float worst = sm.worst;
     const bool full = worst > -INFINITY;
-    const float reach = (float)((double)next_best / power);
+    const float reach = hypothesis_score(next_best, power);
     const bool over = going == 0 || (full && (a.early_stopping || worst >= reach));
     a.out_lengths[g] = new_len;
     a.out_done[g] = over ? 1 : 0;

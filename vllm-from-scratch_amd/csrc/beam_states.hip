@@ -201,7 +201,7 @@ __device__ inline void best_hypotheses(const mvsd_beam_finish_args& a, int64_t g
   const int old_len = a.finished_lengths[at];
   const int beam = a.parent_history[last], token = a.token_history[last];
   const bool runs = a.done[g] == 0 && len > 0 && fabsf(running) < INFINITY;
-  float now = runs ? (float)((double)running / len_power(len, a.length_penalty)) : -INFINITY;
+  float now = runs ? hypothesis_score(running, len_power(len, a.length_penalty)) : -INFINITY;
   if (!(old > -INFINITY) || lane >= W) old = -INFINITY;
   if (!(now > -INFINITY) || lane >= W) now = -INFINITY;
   int rank_old = 0, rank_now = 0;

@@ -259,8 +259,8 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
     With the candidates of :func:`beam_search_select` and L = length + 1:
 
     * stop tokens (``stop_token_ids``, int32 on the device, W * (1 + their number) <= 256) among the
-      W best candidates end a hypothesis with score ``sum / L ** length_penalty``; each group keeps
-      its W best, an earlier one first where they are equal;
+      W best candidates end a hypothesis with score ``sum / L ** length_penalty`` (inside the range
+      of fp32); each group keeps its W best, an earlier one first where they are equal;
     * the W best candidates that are no stop tokens are the next beams, also recorded in the
       histories;
     * the group is done when no beam is left, or when W hypotheses are finished and, unless
