@@ -239,3 +239,12 @@ def test_state_table_lists_rows_pieces_and_entries():
                 dict(states=(x.new_zeros(1, 3, 10, 4).expand(6, 3, 10, 4),)),
                 dict(states=(x,) * 4)):
         assert table(**bad) == -1, bad
+
+
+@pytest.mark.parametrize("alpha", [float("nan"), float("inf"), -float("inf")])
+def test_length_penalties_are_finite(alpha):
+    assert nat.lib().mvsd_beam_step(ctypes.byref(step_args(length_penalty=alpha, workspace=None)),
+                                    None) == INVALID
+    assert nat.lib().mvsd_beam_finish(ctypes.byref(finish_args(length_penalty=alpha,
+                                                               max_length=9000, workspace=None)),
+                                      None) == INVALID

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <mutex>
 
 #include "beam.h"
@@ -1067,7 +1068,8 @@ int mvsd_beam_select(int32_t* token_ids, int32_t* parents, float* out_scores, co
 }
 
 int mvsd_beam_step(const mvsd_beam_step_args* a, mvsd_stream_t stream) {
-  if (!a || a->max_length < 1 || a->num_stop_ids < 0) return MVSD_E_INVALID;
+  if (!a || a->max_length < 1 || a->num_stop_ids < 0 || !std::isfinite(a->length_penalty))
+    return MVSD_E_INVALID;
   if (a->max_length > 0x7fffffff || a->num_stop_ids >= mvsd::kMaxCandidates) return MVSD_E_RANGE;
   mvsd::BeamScanParams p{};
   const int status = beam_scan_params(&p, a->logits, a->dtype, a->stride, a->num_rows,
@@ -1149,7 +1151,7 @@ int64_t mvsd_beam_finish_workspace_bytes(int64_t num_groups, int64_t beam_width,
 
 int mvsd_beam_finish(const mvsd_beam_finish_args* a, mvsd_stream_t stream) {
   if (!a || a->num_groups < 0 || a->beam_width < 1 || a->max_length < 1 || a->num_return < 1 ||
-      a->num_return > a->beam_width)
+      a->num_return > a->beam_width || !std::isfinite(a->length_penalty))
     return MVSD_E_INVALID;
   if (a->beam_width > mvsd::kMaxBeams || a->max_length > 0x7fffffff / mvsd::kMaxBeams ||
       a->num_groups > 0x7fffffff / mvsd::kMaxBeams)
