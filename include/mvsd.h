@@ -710,8 +710,8 @@ int mvsd_beam_reorder(const mvsd_beam_state* states, int64_t num_states, const i
 /* one finished_beams, outside [0, W): beam 0; of running beam w of L tokens                  */
 /* parent_history[g, L - 1, w]), then parent_history[g, t, b].  A parent outside [0, W) is    */
 /* the beam itself.                                                                           */
-/* workspace: mvsd_beam_finish_workspace_bytes() bytes (0: none needed), no initial contents  */
-/* needed; one per call in flight.  length_penalty is finite, as a step's.                    */
+/* workspace: mvsd_beam_finish_workspace_bytes() bytes (0: none needed), 4-byte aligned, no    */
+/* initial contents needed; one per call in flight.  length_penalty is finite, as a step's.    */
 /* ------------------------------------------------------------------------------------ */
 typedef struct mvsd_beam_finish_args {
   int64_t num_groups;

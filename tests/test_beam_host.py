@@ -248,3 +248,8 @@ def test_length_penalties_are_finite(alpha):
     assert nat.lib().mvsd_beam_finish(ctypes.byref(finish_args(length_penalty=alpha,
                                                                max_length=9000, workspace=None)),
                                       None) == INVALID
+
+
+def test_finish_workspace_alignment():
+    assert nat.lib().mvsd_beam_finish(ctypes.byref(finish_args(max_length=9000, workspace=P + 2)),
+                                      None) == WORKSPACE

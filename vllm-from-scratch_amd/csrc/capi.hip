@@ -1165,7 +1165,8 @@ int mvsd_beam_finish(const mvsd_beam_finish_args* a, mvsd_stream_t stream) {
     return MVSD_E_INVALID;
   const int64_t need = mvsd::beam_finish_workspace_bytes(a->num_groups, a->beam_width,
                                                          a->max_length, a->num_return);
-  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return MVSD_E_WORKSPACE;
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || ((uintptr_t)a->workspace & 3) != 0))
+    return MVSD_E_WORKSPACE;
   return hip_status(mvsd::launch_beam_finish(*a, (hipStream_t)stream));
 }
 
