@@ -631,7 +631,8 @@ int mvsd_beam_select(int32_t* token_ids, int32_t* parents, float* out_scores, co
 /*   - length becomes L; done becomes 1 when no beam is left, or W hypotheses are finished   */
 /*     and early_stopping != 0 or the worst of them is at least the best running             */
 /*     fl32(score / L^length_penalty).                                                       */
-/* Other groups stay as they are, their token_ids and parents are -1.  out_* may be the      */
+/* Other groups stay as they are, their token_ids and parents are -1 (done stays 0 in one    */
+/* that has reached max_length: its running beams are answers).  out_* may be the            */
 /* arrays they follow.  finished_beams: the beam the last token (finished_token_ids) was     */
 /* appended to; finished_lengths count that token.                                          */
 /* workspace: as beam_select with num_candidates = W (1 + num_stop_ids).                     */

@@ -253,3 +253,35 @@ def test_length_penalties_are_finite(alpha):
 def test_finish_workspace_alignment():
     assert nat.lib().mvsd_beam_finish(ctypes.byref(finish_args(max_length=9000, workspace=P + 2)),
                                       None) == WORKSPACE
+
+
+def test_the_example_ends_when_no_group_gets_done():
+    """The module's example, run on a search whose groups rest at max_length with their flags unset."""
+    import textwrap
+
+    from mvsd.sample import beam_search
+
+    lines = beam_search.__doc__.splitlines()
+    first = next(k for k, line in enumerate(lines) if line.startswith("    search ="))
+    last = next(k for k, line in enumerate(lines) if line.startswith("    answers ="))
+    calls = {"step": 0, "finish": 0}
+
+    class Search:
+        def __init__(self, *args, **kw):
+            self.state = BeamState.new(2, 3, 5, "cpu")
+
+        def step(self, logits):
+            calls["step"] += 1
+            assert calls["step"] <= 5, "a step after max_length"
+            return beam_search.BeamStep(torch.zeros(2, 3), torch.zeros(2, 3), self.state)
+
+        def reorder(self, states, **where):
+            return states
+
+        def finish(self, n):
+            calls["finish"] += 1
+
+    names = dict(BeamSearch=Search, G=2, W=3, max_length=5, device="cpu", eos=0, n=1, caches=[],
+                 prefill=lambda *a: None, decode=lambda *a: None, all_done=False)
+    exec(textwrap.dedent("\n".join(lines[first:last + 1])), names)
+    assert calls == {"step": 5, "finish": 1}

@@ -8,11 +8,14 @@ group's beams in the order g * W + w.
 
     search = BeamSearch(G, W, max_length, device, stop_token_ids=[eos])
     logits = prefill(...)                       # a row a beam (the first beam's counts)
-    while not all_done:
+    for _ in range(max_length):
         step = search.step(logits)              # step.token_ids, step.parents [G, W]
         search.reorder(caches, lengths=...)     # the beams' states follow their parents
         logits = decode(step.token_ids, caches)
     answers = search.finish(n)                  # token ids, lengths and scores of the n best
+
+``search.state.done`` tells which groups are done, for a loop that ends earlier (reading it waits for the
+device).  A group that reaches ``max_length`` rests with its flag unset: its running beams are answers.
 
 Nothing here synchronises the host.  Work is enqueued on the current stream of the logits' (or
 states') device.  Scratch is kept per stream; a captured call has its own, so calls on several
@@ -58,7 +61,7 @@ class BeamState:
 
     scores: torch.Tensor              # fp32 [G, W], -inf: no beam
     lengths: torch.Tensor             # int32 [G], steps taken = tokens of the running beams
-    done: torch.Tensor                # bool [G]
+    done: torch.Tensor                # bool [G]; not set by reaching max_length
     finished_scores: torch.Tensor     # fp32 [G, W], divided by length ** length_penalty
     finished_beams: torch.Tensor      # int32 [G, W]
     finished_token_ids: torch.Tensor  # int32 [G, W]
@@ -266,7 +269,8 @@ def beam_search_step(logits: torch.Tensor, state: BeamState, *,
     * the group is done when no beam is left, or when W hypotheses are finished and, unless
       ``early_stopping``, the worst of them is at least the best running sum / L ** length_penalty.
 
-    Other groups stay as they are (token_ids and parents -1).  The new state is written to ``out``
+    Other groups stay as they are (token_ids and parents -1), also one that reached ``max_length`` and is
+    not done: its running beams remain answers.  The new state is written to ``out``
     (another :class:`BeamState` with the same histories), or to ``state`` itself.
     """
     G, T, W = _extent(state)
