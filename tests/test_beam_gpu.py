@@ -1032,3 +1032,25 @@ def test_scores_that_vanish_are_still_hypotheses(device, alpha):
     step = beam_search_step(x, state, stop_token_ids=stop, length_penalty=alpha)
     assert state.finished_scores[0].tolist() == [0.0, -math.inf]
     assert state.finished_token_ids[0].tolist() == [0, -1] and step.token_ids[0].tolist() == [1, 2]
+
+
+# ----------------------------------------------------------------- reorder's reports
+
+
+def test_reorder_says_what_it_refuses(device):
+    parents = torch.tensor([[1, 0]], dtype=torch.int32, device=device)
+    x, y, to = (torch.zeros(2, 6, device=device) for _ in range(3))
+    with pytest.raises(ValueError, match="names some of the states"):
+        reorder_beams([x, y], parents, out=[x, to])
+    with pytest.raises(ValueError, match="names some of the states"):
+        reorder_beams([x, y], parents, out=[to, y])
+    with pytest.raises(ValueError, match="share memory"):
+        reorder_beams([x, y], parents, out=[to, to])
+    with pytest.raises(ValueError, match="share memory"):
+        reorder_beams([x, y], parents, out=[y, x])
+    base = torch.zeros(2, 12, device=device)
+    with pytest.raises(ValueError, match="another row stride"):
+        reorder_beams(base[:, :6], parents, out=base.view(4, 6)[:2])
+    with pytest.raises(RuntimeError):  # more than a call takes
+        reorder_beams([torch.zeros(2, 1, device=device) for _ in range(513)], parents)
+    assert not any(t.any() for t in (x, y, to, base))

@@ -389,6 +389,16 @@ def _refuse_states(tensors, targets, length_dim: int, device, least_rows: int) -
     raise ValueError("a state is no tensor that can be passed on")
 
 
+def _reorder_refusal(table, n: int) -> str:
+    """Why mvsd_beam_reorder refuses states that _hostops.state_table took."""
+    same = [table[8 * k] == table[8 * k + 1] for k in range(n)]
+    if any(same) and not all(same):
+        return "out names some of the states: all are reordered in place or none"
+    if any(s and table[8 * k + 2] != table[8 * k + 3] for k, s in enumerate(same)):
+        return "out has a state's memory with another row stride"
+    return "the states (or out) share memory with each other"
+
+
 def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None = None,
                   lengths: torch.Tensor | None = None, length_dim: int = 1,
                   slots: torch.Tensor | None = None, out=None):
@@ -443,7 +453,7 @@ def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None 
         else:
             status = nat.lib().mvsd_beam_reorder(*call)
         if status == -1:
-            raise ValueError("the states (or out) share memory with each other")
+            raise ValueError(_reorder_refusal(table, n))
         nat.check(status, "mvsd_beam_reorder")
     return targets[0] if single else list(targets)
 
