@@ -285,3 +285,23 @@ def test_the_example_ends_when_no_group_gets_done():
                  prefill=lambda *a: None, decode=lambda *a: None, all_done=False)
     exec(textwrap.dedent("\n".join(lines[first:last + 1])), names)
     assert calls == {"step": 5, "finish": 1}
+
+
+def test_the_package_is_imported_without_the_host_extension():
+    """As libmvsd.so, it is looked for when a call needs it."""
+    import sys
+
+    code = ("import sys\n"
+            "class Absent:\n"
+            "    def find_spec(self, name, path=None, target=None):\n"
+            "        if name == 'mvsd._hostops':\n"
+            "            raise ImportError(name)\n"
+            "sys.meta_path.insert(0, Absent())\n"
+            "import mvsd.sample\n"
+            "assert 'mvsd._hostops' not in sys.modules\n"
+            "import torch\n"
+            "state = mvsd.sample.BeamState.new(1, 2, 4, 'cpu')\n"
+            "print('imported')\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True,
+                          cwd=HEADER.parents[1] / "vllm-from-scratch_amd")
+    assert done.returncode == 0 and done.stdout == "imported\n", done.stderr[-500:]

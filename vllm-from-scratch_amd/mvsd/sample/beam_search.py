@@ -32,7 +32,6 @@ from dataclasses import dataclass
 
 import torch
 
-from .. import _hostops
 from .. import _native as nat
 
 PLACEHOLDER_TOKEN_ID = -1
@@ -117,6 +116,19 @@ _FINISH_HEAD, _FINISH_TENSORS = struct.Struct("=4qd"), 5
 _STEP_TAIL, _FINISH_TAIL = struct.Struct("=4q"), struct.Struct("=5q")
 
 
+_hostops = None
+
+
+def _host():
+    """The host extension, imported by the first call that needs it."""
+    global _hostops
+    if _hostops is None:
+        from .. import _hostops as module
+
+        _hostops = module
+    return _hostops
+
+
 def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
     if t.dtype != dtype:
         raise TypeError(f"{name} is {t.dtype}, {dtype} expected")
@@ -131,7 +143,7 @@ def _check_array(t: torch.Tensor, name: str, dtype, shape, device) -> None:
 
 def _addresses(args, at: int, names, tensors, dtypes, shapes, device) -> None:
     """The tensors' addresses into a call's arguments; raises for one of another kind."""
-    bad = _hostops.tensor_table(args, at, tensors, dtypes, shapes, device)
+    bad = _host().tensor_table(args, at, tensors, dtypes, shapes, device)
     if bad >= 0:
         _check_array(tensors[bad], names[bad], dtypes[bad], shapes[bad], device)
         raise ValueError(f"{names[bad]} is no tensor that can be passed on")
@@ -440,8 +452,8 @@ def reorder_beams(states, parents: torch.Tensor, *, starts: torch.Tensor | None 
     if len(targets) != len(tensors):
         raise ValueError(f"{len(targets)} out tensors for {len(tensors)} states")
     table = (ctypes.c_int64 * (8 * len(tensors)))()
-    n = _hostops.state_table(table, tensors, targets, length_dim, device,
-                             0 if slots is not None else G * W)
+    n = _host().state_table(table, tensors, targets, length_dim, device,
+                            0 if slots is not None else G * W)
     if n < 0:
         _refuse_states(tensors, targets, length_dim, device, 0 if slots is not None else G * W)
     if n and G:
