@@ -1054,3 +1054,85 @@ def test_reorder_says_what_it_refuses(device):
     with pytest.raises(RuntimeError):  # more than a call takes
         reorder_beams([torch.zeros(2, 1, device=device) for _ in range(513)], parents)
     assert not any(t.any() for t in (x, y, to, base))
+
+
+# ----------------------------------------------------------------- steps beside other calls
+
+
+def test_threads_of_steps_and_selections_on_one_stream(device):
+    """Steps and selections of different sizes from several threads: scratch is not mixed up."""
+    import threading
+
+    gen = torch.Generator(device=device).manual_seed(5)
+    stop = torch.tensor([3], dtype=torch.int32, device=device)
+    work = []
+    for k, (G, W, V) in enumerate(((3, 4, 30011), (2, 8, 9001), (5, 2, 50257))):
+        x = torch.randn(G * W, V, device=device, generator=gen) * 2.5
+        state = random_state(device, G, W, 6, k)
+        state.lengths.fill_(2)
+        out = clone(state)
+        out.token_history, out.parent_history = state.token_history, state.parent_history
+
+        def step(x=x, state=state, out=out):
+            got = beam_search_step(x, state, stop_token_ids=stop, out=out)
+            return got.token_ids, got.parents, out.scores, out.finished_scores
+
+        def select(x=x, scores=state.scores):
+            got = beam_search_select(x, scores, 16)
+            return got.token_ids, got.parents, got.scores
+
+        work += [(step, [t.clone() for t in step()]), (select, select())]
+    torch.cuda.synchronize(device)
+    wrong = []
+
+    def run(call, want):
+        for _ in range(100):
+            if not all(torch.equal(a, b) for a, b in zip(call(), want)):
+                wrong.append(call.__name__)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+# Exponents of length penalties: length ** alpha is formed to 2^-50, a quotient is rounded once.
+ALPHAS = [0.6, -0.5, 1.7, 2.0, -1.0, 0.001, 8.3]
+
+
+@pytest.mark.parametrize("alpha", ALPHAS)
+@pytest.mark.parametrize("T", [3, 1000, 70001])
+def test_scores_of_answers_at_any_exponent(device, alpha, T):
+    """Running beams of every length up to 1000, and of lengths around the powers of two up to T."""
+    lengths = list(range(1, min(T, 1000) + 1))
+    lengths += [n + d for n in 2 ** np.arange(10, 17) for d in (-1, 0, 1) if n + d <= T]
+    G = len(lengths)
+    if T > 1000:  # histories of T steps a group: a few groups at a time
+        lengths = lengths[-21:] + [T]
+        G = len(lengths)
+    state = BeamState.new(G, 2, T, device)
+    r = np.random.default_rng(T)
+    scores = -r.uniform(0.1, 300.0, (G, 2)).astype(np.float32)
+    state.scores = torch.tensor(scores, device=device)
+    state.lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
+    got = beam_search_finish(state, length_penalty=alpha)
+    want = scores.astype(np.float64) / np.array(lengths, np.float64)[:, None] ** alpha
+    want = -np.sort(-want, axis=1)
+    off = np.abs(got.scores.double().cpu().numpy() - want)
+    # one rounding to fp32, and 2^-50 of the power beside those of numpy's.  70001 ** 8.3 takes scores below
+    # 2^-126, where fp32 numbers are 2^-149 apart: a rounding is off by up to 2^-150 however small they are
+    assert (off <= np.abs(want) * (2.0 ** -24 + 2.0 ** -49) + 2.0 ** -150).all()
+    assert np.array_equal(got.lengths.cpu().numpy(), np.repeat(np.array(lengths)[:, None], 2, axis=1))
+
+
+@pytest.mark.parametrize("alpha", ALPHAS)
+def test_steps_at_any_exponent(device, alpha):
+    """Finished hypotheses' scores and the done flags that follow from them."""
+    G, W, V, T = 40, 3, 600, 60
+    gen = torch.Generator(device=device).manual_seed(1)
+    x = torch.randn(G * W, V, device=device, generator=gen) * 2.5
+    x[::2, 7] = 9.0
+    state = random_state(device, G, W, T, 4)
+    check_step(x, state, [7], alpha)
