@@ -1098,7 +1098,8 @@ def test_threads_of_steps_and_selections_on_one_stream(device):
     assert not wrong
 
 
-# Exponents of length penalties: length ** alpha is formed to 2^-50, a quotient is rounded once.
+# Exponents of length penalties: length ** alpha is formed to 2^-50 and, for an exponent y of two, |y| 2^-52
+# of itself (y's own rounding), a quotient is rounded once.
 ALPHAS = [0.6, -0.5, 1.7, 2.0, -1.0, 0.001, 8.3]
 
 
@@ -1121,9 +1122,10 @@ def test_scores_of_answers_at_any_exponent(device, alpha, T):
     want = scores.astype(np.float64) / np.array(lengths, np.float64)[:, None] ** alpha
     want = -np.sort(-want, axis=1)
     off = np.abs(got.scores.double().cpu().numpy() - want)
-    # one rounding to fp32, and 2^-50 of the power beside those of numpy's.  70001 ** 8.3 takes scores below
-    # 2^-126, where fp32 numbers are 2^-149 apart: a rounding is off by up to 2^-150 however small they are
-    assert (off <= np.abs(want) * (2.0 ** -24 + 2.0 ** -49) + 2.0 ** -150).all()
+    # one rounding to fp32, and the power's beside those of numpy's.  70001 ** 8.3 takes scores below 2^-126,
+    # where fp32 numbers are 2^-149 apart: a rounding is off by up to 2^-150 however small they are
+    power = 2.0 ** -49 + 2.0 ** -52 * np.abs(alpha * np.log2(np.array(lengths, np.float64)))[:, None]
+    assert (off <= np.abs(want) * (2.0 ** -24 + power) + 2.0 ** -150).all()
     assert np.array_equal(got.lengths.cpu().numpy(), np.repeat(np.array(lengths)[:, None], 2, axis=1))
 
 

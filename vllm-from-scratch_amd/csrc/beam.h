@@ -13,9 +13,10 @@ constexpr int kMaxCandidates = 256;  // of a group
 constexpr int kMaxBeamStates = 24;   // state tensors of one launch (kernel arguments)
 
 #ifdef __HIPCC__
-// len^alpha, len >= 1, inside 2^-1000 .. 2^1000, to about 2^-50: 2^(alpha log2(len)), the logarithm of the mantissa m in
-// [1/sqrt 2, sqrt 2) from the series of atanh((m - 1) / (m + 1)), the power of the fraction from that
-// of exp.  (The library's pow, exact to the last bit, took 3000 cycles of a group's 20000.)
+// len^alpha, len >= 1, inside 2^-1000 .. 2^1000: 2^y, y = alpha log2(len), to about (1 + |y| / 4) 2^-50; the
+// logarithm of the mantissa m in [1/sqrt 2, sqrt 2) from the series of atanh((m - 1) / (m + 1)), the power
+// of the fraction from that of exp.  (The library's pow, exact to the last bit, took 3000 cycles of a
+// group's 20000.)
 __device__ inline double len_power(int len, double alpha) {
   if (alpha == 1.0) return (double)len;
   int e = 32 - __clz(len);  // len = m 2^e

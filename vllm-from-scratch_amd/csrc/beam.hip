@@ -11,11 +11,11 @@
 //   beam_scan_kernel    one 256-thread workgroup per (beam, chunk of columns) reads the chunk once,
 //                       into registers, and leaves its maximum, its sum of exp(x - maximum) and the
 //                       largest entry of every 16 or 2 lanes (a "top").
-//   beam_finish_kernel  one 512-thread workgroup per group:
+//   beam_select_kernel, beam_step_kernel: the finish, one 512-thread workgroup per group:
 //     - lse_b in 64 bits from the chunks' sums;
 //     - theta, the C-th largest of the maxima of 512 disjoint unions of tops (64 for C <= 32), as
-//       totals: at least C entries of the group reach it, so the candidates are among the entries that do, and these lie
-//       under the tops that do (a few more than C);
+//       totals: at least C entries of the group reach it, so the candidates are among the entries
+//       that do, and these lie under the tops that do (a few more than C);
 //     - per beam the logit that theta stands for (rounded down), so that tops and entries are compared
 //       as they are; the entries under the tops that reach it are gathered into LDS, their totals
 //       formed in 64 bits, and ranked by counting;
@@ -24,15 +24,18 @@
 //   A step goes on in the same workgroup: stop tokens, finished hypotheses, histories.
 //
 // Order: a lane's sum of up to 32 exponentials is fp32, in pairs, everything after it fp64, which leaves
-// an lse with a deviation of 2e-8 (rows of 1000 columns) to 6e-9 (151936) from the 64-bit one, more
-// where one entry has most of the mass.  Candidates of
+// an lse with a deviation of 2e-8 (rows of 1000 columns) to 6e-9 (151936) from the 64-bit one, at most
+// 9.1e-7 for any row (at kNear) and 2^-18 of a log-probability close to zero (at kPeaked).  Candidates of
 // one beam are ordered by their logits; where two neighbouring candidates of different beams are closer
 // than kNear, both beams' lse are formed again with 64-bit exponentials: the order is the 64-bit one.
 //
 // What bounds it (bf16 rows of 151936 columns, one MI355X): 1024 rows the scan, 48 us of 57 (6.45 TB/s);
-// four rows the chain of two launches, 3 and 6 us.  The finish is a chain too: the scan's results, 7
-// barriers, one gather.  One launch in which the last workgroup of a group finishes it was no faster
-// (four rows 9.7 us against 8.8, 256 rows 38 against 22: the agent-scope stores and counters).
+// four rows the chain of two launches, 3 and 6 us.  Scans of 20 to 30 MB are one round of workgroups, whose
+// reads and arithmetic follow each other: of 10.5 us for 512 fp16 rows of 32000 columns an empty kernel
+// takes 2.8, the reads 4.0 more and the arithmetic 3.7 (0.7 of it the exponentials).  The finish is a chain
+// too: the scan's results, 7 barriers, one gather.  One launch in which the last workgroup of a group
+// finishes it was no faster (four rows 9.7 us against 8.8, 256 rows 38 against 22: the agent-scope stores
+// and counters).
 #include "beam.h"
 #include "mvsd_device.h"
 
@@ -50,9 +53,9 @@ constexpr int kFoldC = 32;         // the largest C whose theta is read off 64 k
 // How rows are split: columns per chunk, and the lanes that share a top (each holds NV vectors of the
 // chunk).  Long chunks, unless they leave compute units idle (fewer than 4 workgroups each) or give a
 // row fewer than two tops per candidate (a group may have one beam only), so that theta is a poor bound
-// or none.  Short rows can have too few even then: tops of two lanes (6 groups of 16 bf16 beams of 1088
-// columns, 64 candidates: 1170 us with tops of 16 lanes, where theta leaves more entries than LDS holds,
-// 36.7 us with tops of 2).
+// or none.  Short rows can have too few even then: tops of two lanes (6 groups of 16 bf16 beams, 64
+// candidates: rows of 1088 columns 114 us with tops of 16 lanes and 23.6 with tops of 2; of 4096 columns
+// 1285, where theta leaves more entries than LDS holds, and 19.0; 8 candidates of 1088 10.5 and 9.8).
 constexpr int kBeamLong = 8192, kBeamShort = 2048;
 constexpr int kCoarse = 16, kFine = 2;
 

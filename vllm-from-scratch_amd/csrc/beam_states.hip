@@ -17,7 +17,11 @@ namespace mvsd {
 // others from the caches) and stored past the caches, since nothing here reads it again: 1355 MB of
 // eight caches move in 250 us with such stores and 271 with ordinary ones (5.4 TB/s read and written; a
 // large copy reaches 4.9), 72 MB of pages in 14.2 us and 17.6.  Sixteen bytes a thread of 8, 16 or 32
-// rows (the least that holds W) and eight of 64 stay in registers.
+// rows (the least that holds W) and eight of 64 stay in registers.  64 rows of eight caches, 4.2 MB a
+// row, half of the beams copied onto the others, TB/s: W = 8 5.8, 16 5.6, 24 5.0, 32 5.0, 48 4.0, 64 3.7
+// (a copy of 1 GiB there 5.1); with vectors of eight bytes for 16 and 32 rows 5.0 and 4.5, of sixteen for
+// 64 (past the registers) 3.8 with 48 and 64 beams.  Into `out`, eight rows at a time, the others read
+// again: W = 4 5.6, 8 5.4, 16 4.7, 32 4.5, 64 4.1.
 
 typedef u32x4 u32x4_align1 __attribute__((aligned(1)));
 typedef u32x2 u32x2_align1 __attribute__((aligned(1)));
@@ -37,7 +41,7 @@ struct AnyAlign<uint8_t> {
   using type = uint8_t;
 };
 
-template <int ROWS, typename T, bool IN_PLACE>
+template <int ROWS, typename T>
 __device__ inline void move_rows(const char* src, char* dst, int64_t src_stride,
                                  int64_t dst_stride, int64_t off, uint64_t moves, int from, int to,
                                  int W) {
@@ -93,13 +97,12 @@ __global__ __launch_bounds__(kThreads) void beam_reorder_kernel(BeamStatesParams
     const uint32_t i = (uint32_t)(u - o * units);
     const int64_t at = o * piece + start * s.inner;
     if (i < whole)
-      move_rows<ROWS, T, IN_PLACE>((const char*)s.src, (char*)s.dst, s.src_stride, s.dst_stride,
-                                   at + (int64_t)i * (int64_t)sizeof(T), moves, from, to, W);
+      move_rows<ROWS, T>((const char*)s.src, (char*)s.dst, s.src_stride, s.dst_stride,
+                         at + (int64_t)i * (int64_t)sizeof(T), moves, from, to, W);
     else
-      move_rows<ROWS, uint8_t, IN_PLACE>((const char*)s.src, (char*)s.dst, s.src_stride,
-                                         s.dst_stride,
-                                         at + (int64_t)whole * (int64_t)sizeof(T) + (i - whole),
-                                         moves, from, to, W);
+      move_rows<ROWS, uint8_t>((const char*)s.src, (char*)s.dst, s.src_stride, s.dst_stride,
+                               at + (int64_t)whole * (int64_t)sizeof(T) + (i - whole), moves, from,
+                               to, W);
   }
 }
 
@@ -145,9 +148,11 @@ hipError_t launch_beam_reorder(const BeamStatesParams& p, bool in_place, hipStre
 //   4 and, for every span at once, through its sub-chunks;
 //   5 every sub-chunk is walked again from there, all at once, and leaves the beam of each step, by
 //     which the workgroup writes the sequences' tokens, on their way since the start.
-// What bounds it: the chain of LDS reads, 16 for each of the walks 1 and 5 and up to 8 for 2 to 4, and
-// before it the lengths and then the histories: 7.9 us for one group of 64 steps, 14 to 16 for 64 groups
-// of 8 beams and 2048 steps (10 MB).
+// What bounds it: latencies in a row.  Of a workgroup's 23400 cycles (27400 the slowest) of 64 groups of 8
+// beams and 2048 steps, 10 MB in 15.6 us, the lengths, histories and hypotheses take 6400, the walks 3300,
+// 1800, 1500, 1800 and 2700 (16 dependent LDS reads each in 1 and 5, up to 8 in the others) and the tokens'
+// way out 6000; an empty launch is 2.8 us.  One group of 64 steps takes 7.9 us, 16500 cycles: 4600, 8700
+// and 3000.
 // Where there are few groups, several workgroups share a group's hypotheses; all of them compose.
 // Histories of one chunk take one launch.  Longer ones take two: the first leaves the hypotheses,
 // every chunk's map and, for a hypothesis that ends in the chunk, its beam below it; the second starts

@@ -230,11 +230,11 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     bf16 or fp16, any row stride): row g * W + w, or ``target_rows [G, W]`` (int32) into a larger
     tensor (indices outside it read its nearest row).  Candidate (beam, token) has the score
     ``scores[beam] + log_softmax(row)[token]``; the order, that of the 64-bit scores, is score
-    descending, beam ascending, logit descending, token ascending.  The scores returned are formed in
-    64 bits from log-softmax values that are off by at most 2^-20, and by 2^-18 of themselves (fp32
-    exponentials), and rounded to fp32.  A beam whose
-    score is not finite, or whose row is -inf throughout or holds a NaN or +inf, proposes nothing;
-    tokens at -inf are no candidates.
+    descending, beam ascending, logit descending, token ascending (scores that differ in the last digits
+    of 64-bit sums, as of a row and its permutation, may come either way).  The scores returned are
+    formed in 64 bits from log-softmax values that are off by at most 2^-20, and by 2^-18 of themselves
+    (fp32 exponentials), and rounded to fp32.  A beam whose score is not finite, or whose row is -inf
+    throughout or holds a NaN or +inf, proposes nothing; tokens at -inf are no candidates.
     """
     if scores.ndim != 2:
         raise ValueError("scores are [G, W]")
