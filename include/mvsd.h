@@ -601,7 +601,8 @@ int mvsd_topk_scores(int32_t* ids, float* scores, int32_t* ranks, const float* l
 /* its permutation, may come either way).  out_scores: formed in 64 bits from a row's        */
 /* log-sum and rounded to fp32.  The log-sum's exponentials and their first sums are fp32,   */
 /* so that a log-probability in them is off by at most 2^-20, and by 2^-18 of itself (and by */
-/* what 64 bits resolve beside scores and logits).  Row of beam (g, b): logits +             */
+/* what 64 bits resolve beside scores and logits); a total below fp32's range has its lowest */
+/* value.  Row of beam (g, b): logits +                                                      */
 /* target_rows[g * W + b] * stride (clamped to [0, num_rows)), or g * W + b without         */
 /* target_rows; dtype MVSD_F32 / MVSD_BF16 / MVSD_F16, any alignment.  A beam whose score or */
 /* whose row's log-sum is not finite (no beam, a row of -inf, a NaN or +inf) proposes        */

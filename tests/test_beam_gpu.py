@@ -1138,3 +1138,22 @@ def test_steps_at_any_exponent(device, alpha):
     x[::2, 7] = 9.0
     state = random_state(device, G, W, T, 4)
     check_step(x, state, [7], alpha)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_totals_below_fp32_are_still_candidates(device, dtype):
+    """Tokens whose log-probability is below fp32's range: beams with the lowest score, not none."""
+    W, V, T, lowest = 2, 40, 4, -torch.finfo(torch.float32).max
+    x = torch.full((W, V), -3e38, device=device).to(DTYPES[dtype])
+    x[:, 3] = 3e38
+    got = beam_search_select(x, torch.tensor([[0.0, -1.0]], device=device), 4)
+    assert got.token_ids[0].tolist() == [3, 3, 0, 1] and got.parents[0].tolist() == [0, 1, 0, 0]
+    assert got.scores[0].tolist() == [0.0, -1.0, lowest, lowest]
+    state = BeamState.new(1, W, T, device)
+    step = beam_search_step(x, state)
+    assert step.token_ids[0].tolist() == [3, 0] and state.scores[0].tolist() == [0.0, lowest]
+    step = beam_search_step(x, state, stop_token_ids=torch.tensor([3], dtype=torch.int32,
+                                                                  device=device))
+    # the stop token ends both beams, and what goes on is below fp32 again
+    assert state.finished_scores[0].tolist() == [0.0, lowest / 2] and bool(state.done[0])
+    assert step.parents[0].tolist() == [0, 0] and state.scores[0].tolist() == [lowest, lowest]

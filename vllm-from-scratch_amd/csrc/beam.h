@@ -39,6 +39,12 @@ __device__ inline double len_power(int len, double alpha) {
   return ldexp(x, (int)n);
 }
 
+// A candidate's score: fl32(total), and fp32's lowest value below it, since -inf says that there is no beam
+// (two tokens masked by the type's lowest value in one sequence).
+__device__ inline float candidate_score(double total) {
+  return fmaxf((float)total, -3.402823466e38f);
+}
+
 // A hypothesis' score: fl32(total / power), and fp32's largest value beyond it, since -inf says that there
 // is no hypothesis (a negative alpha: 20 tokens to the 30th).
 __device__ inline float hypothesis_score(float total, double power) {

@@ -834,7 +834,7 @@ __global__ __launch_bounds__(kFThreads) void beam_select_kernel(BeamScanParams p
     const bool on = i < found;
     o.token_ids[at] = on ? sm.best.token[i] : -1;
     o.parents[at] = on ? sm.best.beam[i] : -1;
-    o.scores[at] = on ? (float)sm.best.total[i] : -INFINITY;
+    o.scores[at] = on ? candidate_score(sm.best.total[i]) : -INFINITY;
   }
 }
 
@@ -906,7 +906,8 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
     // the first candidate that goes on is the best running beam
     for (int k = kMaxCandidates / kWave - 1; k >= 0; --k)
       if (sm.on_mask[k])
-        next_best = (float)sm.best.total[k * kWave + __ffsll((long long)sm.on_mask[k]) - 1];
+        next_best =
+            candidate_score(sm.best.total[k * kWave + __ffsll((long long)sm.on_mask[k]) - 1]);
   }
   const int64_t hist = ((int64_t)g * a.max_length + len) * W;
   auto put = [&](int w, float score, int token, int parent) {
@@ -919,14 +920,15 @@ __global__ __launch_bounds__(kFThreads) void beam_step_kernel(BeamScanParams p,
   if (wid < kMaxCandidates / kWave && ((sm.on_mask[wid] >> lane) & 1)) {
     int place = __popcll(sm.on_mask[wid] & ((1ull << lane) - 1ull));
     for (int k = 0; k < wid; ++k) place += __popcll(sm.on_mask[k]);
-    if (place < W) put(place, (float)sm.best.total[tid], sm.best.token[tid], sm.best.beam[tid]);
+    if (place < W)
+      put(place, candidate_score(sm.best.total[tid]), sm.best.token[tid], sm.best.beam[tid]);
   }
   if (tid >= going && tid < W) put(tid, -INFINITY, -1, -1);
   // ---- finished hypotheses: entries [0, W) are the old ones, [W, 2 W) the candidates of rank < W ----
   if (tid >= W && tid < 2 * W) {
     const int r = tid - W;
     if (r < found && ((sm.stop_mask[r / kWave] >> (r % kWave)) & 1)) {
-      hyp = hypothesis_score((float)sm.best.total[r], power);
+      hyp = hypothesis_score(candidate_score(sm.best.total[r]), power);
       hyp_beam = sm.best.beam[r];
       hyp_token = sm.best.token[r];
       hyp_len = new_len;

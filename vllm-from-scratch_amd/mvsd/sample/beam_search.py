@@ -233,7 +233,7 @@ def beam_search_select(logits: torch.Tensor, scores: torch.Tensor, num_candidate
     descending, beam ascending, logit descending, token ascending (scores that differ in the last digits
     of 64-bit sums, as of a row and its permutation, may come either way).  The scores returned are
     formed in 64 bits from log-softmax values that are off by at most 2^-20, and by 2^-18 of themselves
-    (fp32 exponentials), and rounded to fp32.  A beam whose score is not finite, or whose row is -inf
+    (fp32 exponentials), and rounded to fp32 (not past its lowest value).  A beam whose score is not finite, or whose row is -inf
     throughout or holds a NaN or +inf, proposes nothing; tokens at -inf are no candidates.
     """
     if scores.ndim != 2:
