@@ -497,7 +497,8 @@ def _own(s):
         out["grad"], = torch.autograd.grad(got.loss, x)
         return out
     got = ops.preference_loss(x, s["tokens"], s["ref"], cu_num_tokens=s["cu"], beta=BETA,
-                              loss_type=s["how"], label_smoothing=s["smooth"],
+                              loss_type=s["how"],
+                              label_smoothing=s["smooth"] if s["how"] == "sigmoid" else 0.0,
                               average=s["average"], temperature=s["T"])
     return {"loss": got.loss.detach(), "logprobs": got.logprobs,
             "grad": torch.autograd.grad(got.loss, x)[0]}
