@@ -743,6 +743,102 @@ int64_t mvsd_beam_finish_workspace_bytes(int64_t num_groups, int64_t beam_width,
                                          int64_t max_length, int64_t num_return);
 int mvsd_beam_finish(const mvsd_beam_finish_args* args, mvsd_stream_t stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* row_loss — training losses on rows of logits.  Row n of num_rows starts at               */
+/* logits + (n / inner_rows) * outer_stride + (n % inner_rows) * stride (elements; dtype     */
+/* MVSD_F32 / MVSD_BF16 / MVSD_F16, any alignment; inner_rows = num_rows for a matrix).      */
+/* p = softmax(row / temperature), lp = log p[token].  kind:                                 */
+/*   MVSD_LOSS_LOGPROBS    logprobs [N] = lp, entropy [N] (may be NULL) = -sum p log p;       */
+/*   MVSD_LOSS_DISTILL     num_teacher (K, at most 512) entries a row, token_ids and          */
+/*     teacher_logprobs [N, K]; an id below 0 is no entry, an id that stands there already    */
+/*     neither.  With tail the outcomes are the entries, q = exp(teacher_logprobs), and the    */
+/*     rest of the vocabulary, q = max(1 - their sum, 2^-24) (no outcome where the entries are */
+/*     the vocabulary); p of the rest is its tokens' sum.  Without tail q is                  */
+/*     softmax(teacher_logprobs / temperature) over the entries.  divergence:                 */
+/*     MVSD_KL_FORWARD sum q (log q - log p), MVSD_KL_REVERSE sum p (log p - log q),          */
+/*     MVSD_JS the mean of both against (p + q) / 2; the last two need tail;                  */
+/*   MVSD_LOSS_POLICY      r = exp(lp - old_logprobs) (NULL: 1, with lp's gradient),           */
+/*     l = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1)           */
+/*     - entropy_coef H, d = ref_logprobs - lp (NULL: no such term); a ratio at a border of    */
+/*     the clip has the unclipped gradient.  logprobs [N], entropy and kl [N] (may be NULL);   */
+/*   MVSD_LOSS_PREFERENCE  2 num_pairs sequences, the chosen then the rejected ones: rows      */
+/*     [cu_num_tokens[s - 1], cu_num_tokens[s]) (cut to the rows there are), or num_rows /     */
+/*     (2 num_pairs) rows each without cu_num_tokens.  S = sum of lp (average: over their      */
+/*     number), m = (S - ref)_chosen - (S - ref)_rejected (ref_logprobs [2 num_pairs] or       */
+/*     NULL), h = beta m - margin; MVSD_PREF_SIGMOID -(1 - label_smoothing) log sigmoid(h)      */
+/*     - label_smoothing log sigmoid(-h), MVSD_PREF_HINGE max(0, 1 - h), MVSD_PREF_SQUARED     */
+/*     (m - margin - 1 / (2 beta))^2.  logprobs [2 num_pairs] = S.                             */
+/* token_ids (int32 or int64 by ids_dtype): a row with an id below 0 (distillation: without    */
+/* an entry) or of weight 0 is left out: its logits are not read, its values and its gradient  */
+/* are 0 (a pair of weight 0 adds nothing).  An id of vocab_size or more, a NaN, a +inf or nothing but -inf in a row: NaN.       */
+/* weights: fp32 [N] (preference: [num_pairs]) or NULL (1).  reduction: MVSD_REDUCE_SUM        */
+/* loss[0] = sum w l, MVSD_REDUCE_MEAN over sum w of the rows that are not left out (0: 0),    */
+/* MVSD_REDUCE_NONE loss[n] = w l.                                                            */
+/* saved: mvsd_loss_saved_bytes() bytes for mvsd_loss_gradient, or NULL.                       */
+/* workspace: mvsd_loss_workspace_bytes() bytes, no initial contents needed, one per call in    */
+/* flight.  Both are 16-byte aligned; a size of 0 or below: arguments that no call takes.      */
+/* ------------------------------------------------------------------------------------ */
+enum { MVSD_LOSS_LOGPROBS = 0, MVSD_LOSS_DISTILL = 1, MVSD_LOSS_POLICY = 2, MVSD_LOSS_PREFERENCE = 3 };
+enum { MVSD_REDUCE_SUM = 0, MVSD_REDUCE_MEAN = 1, MVSD_REDUCE_NONE = 2 };
+enum { MVSD_KL_FORWARD = 0, MVSD_KL_REVERSE = 1, MVSD_JS = 2 };
+enum { MVSD_PREF_SIGMOID = 0, MVSD_PREF_HINGE = 1, MVSD_PREF_SQUARED = 2 };
+
+typedef struct mvsd_loss_args {
+  int32_t kind;
+  int32_t dtype;
+  int32_t ids_dtype;
+  int32_t reduction;
+  int32_t divergence;
+  int32_t tail;
+  int32_t loss_type;
+  int32_t average;
+  const void* logits;
+  int64_t stride;
+  int64_t outer_stride;
+  int64_t inner_rows;
+  int64_t num_rows;
+  int64_t vocab_size;
+  double temperature;
+  const void* token_ids;
+  int64_t num_teacher;
+  const float* teacher_logprobs;
+  const float* weights;
+  const float* old_logprobs;
+  const float* ref_logprobs;
+  const float* advantages;
+  double clip_low;
+  double clip_high;
+  double kl_coef;
+  double entropy_coef;
+  const int32_t* cu_num_tokens;
+  int64_t num_pairs;
+  double beta;
+  double margin;
+  double label_smoothing;
+  float* loss;
+  float* logprobs;
+  float* entropy;
+  float* kl;
+  void* saved;
+  void* grad;
+  void* workspace;
+  int64_t workspace_bytes;
+} mvsd_loss_args;
+
+int64_t mvsd_loss_saved_bytes(const mvsd_loss_args* args);
+int64_t mvsd_loss_workspace_bytes(const mvsd_loss_args* args);
+int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* loss_gradient — the gradient of the logits from the saved of mvsd_row_loss (same args), */
+/* grad [N, V] contiguous in the logits' dtype, every row written.  upstream[n * up_stride]  */
+/* is the gradient of loss (LOGPROBS: of logprobs; PREFERENCE: index the pair;               */
+/* up_stride 0: one value), upstream_entropy that of LOGPROBS' entropy; NULL: 0.              */
+/* ------------------------------------------------------------------------------------ */
+int mvsd_loss_gradient(const mvsd_loss_args* args, const float* upstream, int64_t up_stride,
+                       const float* upstream_entropy, int64_t up_entropy_stride,
+                       mvsd_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

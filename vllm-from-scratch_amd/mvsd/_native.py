@@ -141,6 +141,52 @@ class BeamFinishArgs(ctypes.Structure):
     ]
 
 
+class LossArgs(ctypes.Structure):
+    """Mirror of ``mvsd_loss_args``."""
+
+    _fields_ = [
+        ("kind", c_int32),
+        ("dtype", c_int32),
+        ("ids_dtype", c_int32),
+        ("reduction", c_int32),
+        ("divergence", c_int32),
+        ("tail", c_int32),
+        ("loss_type", c_int32),
+        ("average", c_int32),
+        ("logits", c_void_p),
+        ("stride", c_int64),
+        ("outer_stride", c_int64),
+        ("inner_rows", c_int64),
+        ("num_rows", c_int64),
+        ("vocab_size", c_int64),
+        ("temperature", c_double),
+        ("token_ids", c_void_p),
+        ("num_teacher", c_int64),
+        ("teacher_logprobs", c_void_p),
+        ("weights", c_void_p),
+        ("old_logprobs", c_void_p),
+        ("ref_logprobs", c_void_p),
+        ("advantages", c_void_p),
+        ("clip_low", c_double),
+        ("clip_high", c_double),
+        ("kl_coef", c_double),
+        ("entropy_coef", c_double),
+        ("cu_num_tokens", c_void_p),
+        ("num_pairs", c_int64),
+        ("beta", c_double),
+        ("margin", c_double),
+        ("label_smoothing", c_double),
+        ("loss", c_void_p),
+        ("logprobs", c_void_p),
+        ("entropy", c_void_p),
+        ("kl", c_void_p),
+        ("saved", c_void_p),
+        ("grad", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/mvsd.h declares
 SIGNATURES = {
     "mvsd_version": (c_int, []),
@@ -239,6 +285,11 @@ SIGNATURES = {
                                   c_int64, c_int64, c_void_p]),
     "mvsd_beam_finish_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "mvsd_beam_finish": (c_int, [ctypes.POINTER(BeamFinishArgs), c_void_p]),
+    "mvsd_loss_saved_bytes": (c_int64, [ctypes.POINTER(LossArgs)]),
+    "mvsd_loss_workspace_bytes": (c_int64, [ctypes.POINTER(LossArgs)]),
+    "mvsd_row_loss": (c_int, [ctypes.POINTER(LossArgs), c_void_p]),
+    "mvsd_loss_gradient": (c_int, [ctypes.POINTER(LossArgs), c_void_p, c_int64, c_void_p, c_int64,
+                                   c_void_p]),
     "mvsd_ngram_valid_sampled": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                          c_int64, c_int64, c_void_p, c_void_p, c_int64,
                                          c_void_p, c_int64, c_int64, c_void_p]),

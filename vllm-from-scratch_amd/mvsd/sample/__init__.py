@@ -3,6 +3,8 @@
 from .beam_search import (BeamCandidates, BeamHypotheses, BeamSearch, BeamState, BeamStep,
                           beam_search_finish, beam_search_select, beam_search_step,
                           reorder_beams)
+from .losses import (PolicyLoss, PreferenceLoss, distillation_loss, policy_loss, preference_loss,
+                     token_logprobs)
 from .metadata import SAMPLING_EPS, SamplingMetadata
 from .ops.topk_topp_sampler import apply_top_k_top_p
 from .rejection_sampler import (MAX_SPEC_LEN, PLACEHOLDER_TOKEN_ID, RejectionSampler,
@@ -17,4 +19,5 @@ __all__ = ["SamplingMetadata", "SAMPLING_EPS", "apply_top_k_top_p", "RejectionSa
            "sampling_masks", "PLACEHOLDER_TOKEN_ID", "MAX_SPEC_LEN", "Sampler",
            "TopKTopPSampler", "generate_sampler_noise", "random_sample", "BeamSearch", "BeamState",
            "BeamStep", "BeamCandidates", "BeamHypotheses", "beam_search_select",
-           "beam_search_step", "beam_search_finish", "reorder_beams"]
+           "beam_search_step", "beam_search_finish", "reorder_beams", "token_logprobs",
+           "distillation_loss", "policy_loss", "preference_loss", "PolicyLoss", "PreferenceLoss"]
