@@ -823,10 +823,15 @@ typedef struct mvsd_loss_args {
   void* grad;
   void* workspace;
   int64_t workspace_bytes;
+  int64_t unit_gradient;
 } mvsd_loss_args;
 
 int64_t mvsd_loss_saved_bytes(const mvsd_loss_args* args);
 int64_t mvsd_loss_workspace_bytes(const mvsd_loss_args* args);
+/* 1 where mvsd_row_loss reads a row once for its loss and its gradient: it then writes grad    */
+/* (if that is not NULL) for an upstream of 1, which mvsd_loss_gradient with unit_gradient       */
+/* leaves as it is if that is what the upstream holds.                                          */
+int mvsd_loss_one_pass(const mvsd_loss_args* args);
 int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
 
 /* ------------------------------------------------------------------------------------ */
@@ -834,6 +839,7 @@ int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
 /* grad [N, V] contiguous in the logits' dtype, every row written.  upstream[n * up_stride]  */
 /* is the gradient of loss (LOGPROBS: of logprobs; PREFERENCE: index the pair;               */
 /* up_stride 0: one value), upstream_entropy that of LOGPROBS' entropy; NULL: 0.              */
+/* unit_gradient (with one upstream): grad holds the gradient for 1 already.                  */
 /* ------------------------------------------------------------------------------------ */
 int mvsd_loss_gradient(const mvsd_loss_args* args, const float* upstream, int64_t up_stride,
                        const float* upstream_entropy, int64_t up_entropy_stride,

@@ -34,11 +34,13 @@ struct LossParams {
   int norm_parts;
   float* row_loss;    // [N] (preference: [pairs]), weighted
   float* row_lp;      // preference: [N]
+  float2* teach;      // distillation: [N] what the teacher's kernel gives of a row, its weight (0: left out)
   LossRecord* records;    // [N] or null
   float* over;            // distillation: [N, K] gradients of the given tokens for unit upstream
-  int32_t* over_ids;      // [N, K], -1: nothing
+  int32_t* over_ids;      // [N, K] the entries that count, -1: none
 };
 
+bool loss_one_pass(const mvsd_loss_args& a);
 int64_t loss_workspace_bytes(const mvsd_loss_args& a);
 int64_t loss_saved_bytes(const mvsd_loss_args& a);
 hipError_t launch_loss(const mvsd_loss_args& a, hipStream_t stream);

@@ -16,6 +16,7 @@
 #include <float.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "losses.h"
 #include "mvsd_device.h"
@@ -115,20 +116,18 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
   const int part = blockIdx.x - (int)(row * p.nch);
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
   int token = -1;
-  if (row_weight(p.a, row) == 0.f) return;
   if constexpr (LIST) {
+    if (p.teach[row].y == 0.f) return;
     for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
     __syncthreads();
-    int any = 0;
     for (int k = threadIdx.x; k < p.K; k += kLossThreads) {
-      const int id = token_at(p.a, row * p.K + k, p.V);
-      any |= id >= 0;
+      const int id = p.over_ids[row * p.K + k];
       if (id >= begin && id < end) atomicOr(&bits[(id - begin) >> 5], 1u << ((id - begin) & 31));
     }
-    if (!__syncthreads_or(any)) return;
+    __syncthreads();
   } else {
     token = token_at(p.a, row, p.V);
-    if (token < 0) return;
+    if (token < 0 || row_weight(p.a, row) == 0.f) return;
   }
   const auto* x = logits_row<DT>(p.a, row);
   Stat st = {-INFINITY, 0.f, 0.f};
@@ -177,30 +176,21 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
 
 // ------------------------------------------------------------------ the mean's divisor ----------
 
-// Partial sums of the weights of the rows that are not left out: a wave a row where it has a list.
-template <bool LIST>
+// Partial sums of the weights of the rows that are not left out.
 __global__ __launch_bounds__(kLossThreads) void loss_norm_kernel(LossParams p) {
   __shared__ float scratch[kWaves];
   const int64_t each = (p.a.num_rows + gridDim.x - 1) / gridDim.x;
   const int64_t first = blockIdx.x * each, last = min(p.a.num_rows, first + each);
   float sum[1] = {0.f};
-  if constexpr (LIST) {
-    for (int64_t row = first + wave_id(); row < last; row += kWaves) {
-      bool any = false;
-      for (int k = lane_id(); k < p.K; k += kWave) any |= token_at(p.a, row * p.K + k, p.V) >= 0;
-      if (__any(any) && lane_id() == 0) sum[0] += row_weight(p.a, row);
-    }
-  } else {
-    for (int64_t row = first + threadIdx.x; row < last; row += kLossThreads)
-      if (token_at(p.a, row, p.V) >= 0) sum[0] += row_weight(p.a, row);
-  }
+  for (int64_t row = first + threadIdx.x; row < last; row += kLossThreads)
+    if (token_at(p.a, row, p.V) >= 0) sum[0] += row_weight(p.a, row);
   block_sum<1>(sum, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = sum[0];
 }
 
 // What a row's weight is multiplied by, in every thread of a wave.
 __device__ inline float mean_factor(const LossParams& p) {
-  if (p.a.reduction != MVSD_REDUCE_MEAN || p.norm_parts == 0) return 1.f;
+  if (p.a.reduction != MVSD_REDUCE_MEAN) return 1.f;
   float sum = 0.f;
   for (int i = lane_id(); i < p.norm_parts; i += kWave) sum += p.norm[i];
   sum = wave_sum(sum);
@@ -244,10 +234,19 @@ struct PolicyRow {
   float loss, c, kl;
 };
 
-__device__ inline PolicyRow policy_row(const mvsd_loss_args& a, int64_t row, float lp, float H) {
+// What a policy's row is given besides its logits.
+struct PolicyIn {
+  float A, old, ref;
+};
+__device__ inline PolicyIn policy_in(const mvsd_loss_args& a, int64_t row) {
+  return {a.advantages[row], a.old_logprobs ? a.old_logprobs[row] : 0.f,
+          a.ref_logprobs ? a.ref_logprobs[row] : 0.f};
+}
+
+__device__ inline PolicyRow policy_row(const mvsd_loss_args& a, const PolicyIn& in, float lp, float H) {
   PolicyRow o;
-  const float A = a.advantages[row];
-  const float r = a.old_logprobs ? expf(lp - a.old_logprobs[row]) : lp == lp ? 1.f : lp;
+  const float A = in.A;
+  const float r = a.old_logprobs ? expf(lp - in.old) : lp == lp ? 1.f : lp;
   const float free = r * A;
   const float bound = fminf(fmaxf(r, (float)(1.0 - a.clip_low)), (float)(1.0 + a.clip_high)) * A;
   const bool clipped = free > bound;
@@ -255,7 +254,7 @@ __device__ inline PolicyRow policy_row(const mvsd_loss_args& a, int64_t row, flo
   o.c = clipped ? 0.f : -free;
   o.kl = 0.f;
   if (a.ref_logprobs) {
-    const float d = a.ref_logprobs[row] - lp, e1 = expm1f(d);
+    const float d = in.ref - lp, e1 = expm1f(d);
     // e^d - d - 1: its series where the difference of the two would be rounding
     o.kl = fabsf(d) < 0.25f
                ? d * d * (0.5f + d * (1.f / 6 + d * (1.f / 24 + d * (1.f / 120 + d * (1.f / 720 + d * (1.f / 5040 + d * (1.f / 40320)))))))
@@ -296,7 +295,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_token_rows_kernel(LossParam
     r.rec.c = 1.f;
     r.rec.cH = 1.f;
     if (a.kind == MVSD_LOSS_POLICY) {
-      o = policy_row(a, row, r.lp, r.H);
+      o = policy_row(a, policy_in(a, row), r.lp, r.H);
       r.rec.c = o.c * w * mean;
       r.rec.cH = -(float)a.entropy_coef * w * mean;
     } else if (a.kind == MVSD_LOSS_PREFERENCE) {
@@ -394,103 +393,137 @@ __global__ __launch_bounds__(kLossThreads) void loss_pairs_kernel(LossParams p) 
 
 // ------------------------------------------------------------------ distillation ----------------
 
-template <int T>
-struct DistillScratch {
-  int ids[kMaxTeacher];
-  float red[4 * (T / kWave)];
-  double sum[T / kWave];
-};
-
 __device__ inline double wave_sum_f64(double v) {
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
   return v;
 }
 
-// One row's loss by a workgroup of T threads, from the statistics of its rest.  Writes the gradients of the
-// given tokens (over, over_ids: -1 where an entry does not count) and returns the loss; *k is the record's.
-// `weight` is the row's, after the mean.
-template <int DT, int T>
-__device__ inline float distill_row(const LossParams& p, int64_t row, Stat st, float weight,
-                                    DistillScratch<T>& sm, float* over, int32_t* over_ids, float* k_out) {
-  constexpr int NW = T / kWave, E = (kMaxTeacher + T - 1) / T;
+// The teacher's side, a wave a row: which entries count (over_ids, -1: not), the mass of the rest (0 where
+// the rest is no outcome) or, without a tail, the log of the entries' sum, the row's weight (0: left out),
+// and the partial sums of the weights.
+__global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p) {
+  constexpr int E = kMaxTeacher / kWave;
+  __shared__ __attribute__((aligned(16))) int s_ids[kWaves][kMaxTeacher];
+  __shared__ float scratch[kWaves];
   const mvsd_loss_args& a = p.a;
-  const int tid = threadIdx.x, K = p.K;
-  const auto* xrow = logits_row<DT>(a, row);
-  int id[E];
+  const int64_t each = (a.num_rows + gridDim.x - 1) / gridDim.x;
+  const int64_t first = blockIdx.x * each, last = min(a.num_rows, first + each);
+  const int K = p.K, lane = lane_id();
+  int* ids = s_ids[wave_id()];
+  float weights[1] = {0.f};
+  for (int64_t row = first + wave_id(); row < last; row += kWaves) {
+    int id[E];
+    float v[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int k = i * kWave + lane;
+      id[i] = k < K ? token_at(a, row * K + k, p.V) : -1;
+      v[i] = k < K ? a.teacher_logprobs[row * K + k] : -INFINITY;
+      ids[k] = id[i];  // a wave's own places: its reads below follow
+    }
+    __builtin_amdgcn_wave_barrier();
+    bool before[E] = {};
+    for (int j = 0; j < K; j += 4) {
+      const int4 other = *reinterpret_cast<const int4*>(ids + j);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (i * kWave >= K) break;
+        const int k = i * kWave + lane;
+        before[i] |= (other.x == id[i] && j < k) | (other.y == id[i] && j + 1 < k) |
+                     (other.z == id[i] && j + 2 < k) | (other.w == id[i] && j + 3 < k);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    int count = 0;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (i * kWave >= K) break;
+      const int k = i * kWave + lane;
+      if (id[i] >= 0 && before[i]) id[i] = -1;
+      if (id[i] < 0) v[i] = -INFINITY;
+      count += __popcll(__ballot(id[i] >= 0));
+      top = fmaxf(top, v[i]);
+      if (k < K) p.over_ids[row * K + k] = id[i];
+    }
+    float value;
+    if (a.tail) {
+      double mass = 0.0;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i * kWave < K) mass += exp((double)v[i]);
+      mass = wave_sum_f64(mass);
+      value = count >= p.V ? 0.f : mass != mass ? NAN : (float)fmax(1.0 - mass, 0x1p-24);
+    } else {
+      top = base_of(wave_max(top));
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i * kWave < K) sum += expf((v[i] - top) * p.inv_t);
+      value = top * p.inv_t + logf(wave_sum(sum));
+    }
+    const float w = count == 0 ? 0.f : row_weight(a, row);
+    if (lane == 0) p.teach[row] = make_float2(value, w);
+    weights[0] += w;
+  }
+  if (lane != 0) weights[0] = 0.f;
+  block_sum<1>(weights, scratch);
+  if (threadIdx.x == 0) p.norm[blockIdx.x] = weights[0];
+}
+
+// A row's entries, entry i * T + thread in each thread.
+template <int E>
+struct Entries {
+  int id[E];  // -1: it does not count
   float x[E], v[E];
+};
+
+template <int T, int E>
+__device__ inline void load_entries(const LossParams& p, int64_t row, Entries<E>& in) {
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const int k = i * T + tid;
-    id[i] = k < K ? token_at(a, row * K + k, p.V) : -1;
-    x[i] = id[i] < 0 ? -INFINITY : id[i] < p.V ? Elem<DT>::cvt(xrow[id[i]]) : NAN;
+    const int k = i * T + (int)threadIdx.x;
+    in.id[i] = -1;
+    in.v[i] = 0.f;
+    if (k < p.K) {
+      in.id[i] = p.over_ids[row * p.K + k];
+      in.v[i] = p.a.teacher_logprobs[row * p.K + k];
+    }
+  }
+}
+template <int DT, int E>
+__device__ inline void load_entry_logits(const LossParams& p, int64_t row, Entries<E>& in) {
+  const auto* x = logits_row<DT>(p.a, row);
+#pragma unroll
+  for (int i = 0; i < E; ++i) in.x[i] = in.id[i] >= 0 && in.id[i] < p.V ? Elem<DT>::cvt(x[in.id[i]]) : NAN;
+}
+
+// One row's loss by a workgroup of T threads, from the statistics of its rest, its entries and what the
+// teacher's kernel gave of it.  Gives the gradients of the given tokens (over, at id, -1: none) and returns
+// the loss; *k is the record's.  `weight` is the row's, after the mean; red holds 2 T / 64 floats.
+template <int T, int E>
+__device__ inline float distill_row(const LossParams& p, Stat st, float teacher, float weight, float* red,
+                                    Entries<E>& in, float (&over)[E], float* k_out) {
+  constexpr int NW = T / kWave;
+  const mvsd_loss_args& a = p.a;
+  int (&id)[E] = in.id;
+  float (&x)[E] = in.x;
+  float top[1] = {st.m};
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (id[i] < 0) x[i] = -INFINITY;
     if (x[i] == INFINITY) x[i] = NAN;
-    v[i] = id[i] < 0 ? -INFINITY : a.teacher_logprobs[row * K + k];
-    if (k < K) sm.ids[k] = id[i];
-  }
-  __syncthreads();
-  // an id that stands before does not count
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int k = i * T + tid;
-    if (i * T >= K) break;
-    bool twice = false;
-    const int last = min(K, (i + 1) * T);
-    for (int j = 0; j < last; ++j) twice |= j < k && sm.ids[j] == id[i];
-    if (twice) id[i] = -1, x[i] = v[i] = -INFINITY;
-  }
-  // the row's maximum, the teacher's, and the number of entries
-  float top[2] = {st.m, -INFINITY}, count[1] = {0.f};
-  double mass = 0.0;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
     top[0] = fmaxf(top[0], x[i]);
-    top[1] = fmaxf(top[1], v[i]);
-    count[0] += id[i] >= 0 ? 1.f : 0.f;
-    if (id[i] >= 0 && a.tail) mass += exp((double)v[i]);
   }
-  block_max<2, NW>(top, sm.red);
-  block_sum<1, NW>(count, sm.red);
+  block_max<1, NW>(top, red);
   const float base = base_of(top[0]), rest_base = base_of(st.m);
-  float q[E], log_q[E], rest_q = 0.f;
-  bool tail = false;
-  if (a.tail) {
-    mass = wave_sum_f64(mass);
-    if (lane_id() == 0) sm.sum[wave_id()] = mass;
-    __syncthreads();
-    mass = 0.0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) mass += sm.sum[w];
-    tail = (int)count[0] < p.V;
-    rest_q = tail ? (float)fmax(1.0 - mass, 0x1p-24) : 0.f;
-    if (mass != mass) rest_q = NAN;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      log_q[i] = v[i];
-      q[i] = expf(v[i]);
-    }
-  } else {
-    float sum[1] = {0.f};
-    const float vb = base_of(top[1]);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      log_q[i] = (v[i] - vb) * p.inv_t;
-      q[i] = expf(log_q[i]);
-      sum[0] += q[i];
-    }
-    block_sum<1, NW>(sum, sm.red);
-    const float lg = logf(sum[0]), inv = 1.f / sum[0];
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      log_q[i] -= lg;
-      q[i] *= inv;
-    }
-  }
+  const bool tail = a.tail && teacher != 0.f;
   // the student's normaliser
   float z[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < E; ++i) z[0] += expf((x[i] - base) * p.inv_t);
-  block_sum<1, NW>(z, sm.red);
+  block_sum<1, NW>(z, red);
   const float rest_d = st.m == -INFINITY ? 0.f : (rest_base - base) * p.inv_t;
   const float log_z = logf(z[0] + st.s * expf(rest_d));
   const float rest_lp = rest_d + logf(st.s) - log_z, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
@@ -511,49 +544,56 @@ __device__ inline float distill_row(const LossParams& p, int64_t row, Stat st, f
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const float lp = (x[i] - base) * p.inv_t - log_z;
+    const float log_q = a.tail ? in.v[i] : in.v[i] * p.inv_t - teacher;
     float term = 0.f;
     pr[i] = expf(lp);
     pd[i] = 0.f;
-    if (id[i] >= 0) outcome(q[i], log_q[i], pr[i], lp, term, pd[i]);
+    if (id[i] >= 0) outcome(expf(log_q), log_q, pr[i], lp, term, pd[i]);
     both[0] += term;
     both[1] += pd[i];
   }
-  block_sum<2, NW>(both, sm.red);
+  block_sum<2, NW>(both, red);
   float rest_pd = 0.f;
   if (tail) {
     float term;
-    outcome(rest_q, logf(rest_q), rest_p, rest_lp, term, rest_pd);
+    outcome(teacher, logf(teacher), rest_p, rest_lp, term, rest_pd);
     both[0] += term;
     both[1] += rest_pd;
   }
   const float f = weight * p.inv_t;
   *k_out = st.s == 0.f ? 0.f : -f * (rest_pd - rest_p * both[1]) / st.s;
-  if (over) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int k = i * T + tid;
-      if (k < K) {
-        over[k] = f * (pd[i] - pr[i] * both[1]);
-        over_ids[k] = id[i] < p.V ? id[i] : -1;
-      }
-    }
+  for (int i = 0; i < E; ++i) {
+    over[i] = f * (pd[i] - pr[i] * both[1]);
+    if (id[i] >= p.V) id[i] = -1;
   }
   return both[0] * weight;
+}
+
+template <int T, int E>
+__device__ inline void save_over(const LossParams& p, int64_t row, const Entries<E>& in, const float (&over)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int k = i * T + (int)threadIdx.x;
+    if (k < p.K) {
+      p.over[row * p.K + k] = over[i];
+    }
+  }
 }
 
 // A workgroup a row.
 template <int DT>
 __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossParams p) {
-  __shared__ DistillScratch<kLossThreads> sm;
+  constexpr int E = kMaxTeacher / kLossThreads;
+  __shared__ float red[2 * kWaves];
   const int64_t row = blockIdx.x;
-  const mvsd_loss_args& a = p.a;
-  const float w = row_weight(a, row) * mean_factor(p);
-  bool any = false;
-  for (int k = threadIdx.x; k < p.K; k += kLossThreads) any |= token_at(a, row * p.K + k, p.V) >= 0;
-  const bool out = !__syncthreads_or(any) || row_weight(a, row) == 0.f;
+  const float2 teacher = p.teach[row];
   float loss = 0.f;
   LossRecord rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
-  if (!out) {
+  if (teacher.y != 0.f) {
+    Entries<E> in;
+    load_entries<kLossThreads>(p, row, in);
+    load_entry_logits<DT>(p, row, in);
     Stat st = {-INFINITY, 0.f, 0.f};
     for (int i = lane_id(); i < p.nch; i += kWave) {
       const float4 v = p.parts[row * p.nch + i];
@@ -562,8 +602,9 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
     st = wave_join(st, p.c1);
     rec.M = base_of(st.m);
     rec.c = 1.f;
-    loss = distill_row<DT, kLossThreads>(p, row, st, w, sm, p.records ? p.over + row * p.K : nullptr,
-                                         p.over_ids + row * p.K, &rec.k);
+    float over[E];
+    loss = distill_row<kLossThreads, E>(p, st, teacher.x, teacher.y * mean_factor(p), red, in, over, &rec.k);
+    if (p.records) save_over<kLossThreads, E>(p, row, in, over);
   }
   if (threadIdx.x == 0) {
     p.row_loss[row] = loss;
@@ -583,6 +624,23 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(float* loss, const float
 }
 
 // ------------------------------------------------------------------ the gradient ----------------
+
+// The gradient at the rest, e (a + b log2 e), and at the given token, for the factors g and gH.  Both
+// gradient kernels go through these, so that they give the same bits.
+struct RestGradient {
+  float a, b;
+};
+__device__ inline RestGradient rest_gradient(const LossRecord& r, float g, float gH) {
+  return {-r.k * fmaf(gH, r.h, g), -r.k * gH * kLn2};
+}
+__device__ inline float token_gradient(const LossRecord& r, float g, float gH) {
+  return fmaf(gH, r.o2, g * r.o1);
+}
+template <bool ENT>
+__device__ inline float rest_value(float x, float M, float c1, RestGradient k) {
+  const float y = (x - M) * c1, w = __builtin_amdgcn_exp2f(y);
+  return w * (ENT ? fmaf(k.b, fmaxf(y, kLeast), k.a) : k.a);
+}
 
 template <int DT>
 __device__ inline u32x4 pack_vec(const float (&g)[Elem<DT>::kVec]) {
@@ -628,6 +686,7 @@ template <int DT, bool LIST, bool ENT>
 __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams p, const float* up, int64_t us,
                                                                      const float* up_h, int64_t uhs) {
   constexpr int VEC = Elem<DT>::kVec;
+  if (p.a.unit_gradient && up[0] == 1.f) return;  // it is there already
   const int64_t row = blockIdx.x / p.nch;
   const int part = blockIdx.x - (int)(row * p.nch);
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
@@ -643,16 +702,15 @@ __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams 
     return;
   }
   const auto* x = logits_row<DT>(p.a, row);
-  const float ka = -rec.k * (g + gH * rec.h), kb = -rec.k * gH * kLn2;
+  const RestGradient rest = rest_gradient(rec, g, gH);
   const int token = LIST ? -1 : token_at(p.a, row, p.V);
-  const float at_token = g * rec.o1 + gH * rec.o2;
+  const float at_token = token_gradient(rec, g, gH);
   for (int col = begin + (int)threadIdx.x * VEC; col < end; col += kLossThreads * VEC) {
     float v[VEC];
     load_filled<DT>(x, col, end, v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const float y = (v[e] - rec.M) * p.c1, w = __builtin_amdgcn_exp2f(y);
-      v[e] = w * (ENT ? fmaf(kb, fmaxf(y, kLeast), ka) : ka);
+      v[e] = rest_value<ENT>(v[e], rec.M, p.c1, rest);
     }
     if (!LIST && token >= col && token < col + VEC) {
 #pragma unroll
@@ -666,6 +724,338 @@ __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams 
       const int id = p.over_ids[row * p.K + k];
       if (id >= begin && id < end) out[id] = to_storage<DT>(g * p.over[row * p.K + k]);
     }
+  }
+}
+
+// ------------------------------------------------------------------ values and gradient in one pass ---
+
+constexpr int kHeld = 18;  // full vectors of a row in each thread's registers (72 of 128), beside the last columns'
+
+// The elements of `marks` become -inf.
+template <int DT>
+__device__ inline void mask_vec(u32x4& r, unsigned marks) {
+  if constexpr (DT == MVSD_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = marks >> e & 1 ? 0xff800000u : r[e];
+  } else {
+    constexpr uint32_t ninf = DT == MVSD_BF16 ? 0xff80u : 0xfc00u;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      r[w] = marks >> (2 * w) & 1 ? (r[w] & 0xffff0000u) | ninf : r[w];
+      r[w] = marks >> (2 * w + 1) & 1 ? (r[w] & 0x0000ffffu) | ninf << 16 : r[w];
+    }
+  }
+}
+
+// Adds a vector, or two, to a thread's statistics.
+template <int DT, bool ENT, int N>
+__device__ inline void add_vecs(Stat& st, const u32x4 (&r)[N], float c1) {
+  constexpr int VEC = Elem<DT>::kVec;
+  float m = st.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m = fmaxf(m, vec_elem<DT>(r[i], e));
+  const float base = base_of(m);
+  const float d = fmaxf((st.m - base) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
+  if constexpr (ENT) st.t = fmaf(st.s, d, st.t) * f;
+  st.s *= f;
+  st.m = m;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float y = (vec_elem<DT>(r[i], e) - base) * c1, w = __builtin_amdgcn_exp2f(y);
+      st.s += w;
+      if constexpr (ENT) st.t = fmaf(w, fmaxf(y, kLeast), st.t);
+    }
+}
+
+// Both sums against a new maximum.
+__device__ inline void rebase(Stat& st, float m, float c1) {
+  const float d = fmaxf((st.m - base_of(m)) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
+  st.t = fmaf(st.s, d, st.t) * f;
+  st.s *= f;
+  st.m = m;
+}
+
+__device__ inline float sum16(float v) {
+  v += dpp_f32<kDppXor1>(v);
+  v += dpp_f32<kDppXor2>(v);
+  v += dpp_f32<kDppHalfMirror>(v);
+  return v + dpp_f32<kDppMirror>(v);
+}
+
+// Rows by a workgroup of T threads, one after the other, every row in its registers: read once, written once.
+// A turn of the loop writes the gradient of one row and, vector by vector, loads the next one in its place
+// and adds it to its statistics a few vectors later, so that memory is busy except in the reductions and
+// the row's own loss between two turns.  Columns behind kHeld vectors a thread are read again.
+template <int DT, int T, bool LIST, bool ENT>
+__global__ __launch_bounds__(T, 4) void loss_rows_kernel(LossParams p) {
+  using S = typename Elem<DT>::storage;
+  constexpr int VEC = Elem<DT>::kVec, NW = T / kWave, E = LIST ? (kMaxTeacher + T - 1) / T : 1, kDelay = 8;
+  extern __shared__ uint32_t bits[];
+  __shared__ float4 s_part[2][NW];
+  __shared__ float red[2 * NW];
+  const mvsd_loss_args& a = p.a;
+  const int tid = threadIdx.x, V = p.V, K = p.K, N = (int)a.num_rows, step = gridDim.x;
+  constexpr int kSpan = T * VEC;  // columns of one vector a thread
+  const int nv = min(kHeld, V / kSpan), behind = nv * kSpan;  // full vectors, the columns in them
+  const bool longer = V - behind > kSpan;
+  const unsigned own = tid * VEC;  // the thread's place in a span
+  // the thread's last columns, moved back where they would pass the row's end by `shift`
+  const int last_col = behind + (int)own, last_at = min(last_col, max(V - VEC, 0)), shift = last_col - last_at;
+  const bool last_here = !longer && shift < VEC;
+  const float mean = mean_factor(p), c1 = p.c1;
+  const bool want = a.grad != nullptr;
+
+  if constexpr (LIST) {
+    for (int i = tid; i < (V + 31) / 32; i += T) bits[i] = 0;
+    __syncthreads();
+  }
+
+  // the row whose logits are loaded in this turn, and the one whose gradient is written
+  int row = blockIdx.x, cur = -1, parity = 0;
+  int token = -1, cur_token = -1;
+  const uint8_t* marks_of = reinterpret_cast<const uint8_t*>(bits) + (own >> 3);
+  float w = 0.f;
+  Entries<E> in = {}, after = {};
+  int pend_id[E];
+  float pend[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) pend_id[i] = -1;
+  if constexpr (LIST) {
+    if (row < N) load_entries<T>(p, row, after);
+  }
+  enum { kNothing, kZeros, kGradient };
+  int store = kNothing;
+  float cur_M = 0.f, at_token = 0.f;
+  RestGradient rest = {0.f, 0.f};
+  const S* cur_x = nullptr;
+  u32x4 r[kHeld] = {}, last = {};
+
+  for (;;) {
+    bool load = false;
+    float xt = NAN, teacher = 0.f;
+    PolicyIn given = {0.f, 0.f, 0.f};
+    const S* x = nullptr;
+    if (row < N) {
+      x = logits_row<DT>(a, row);
+      if constexpr (LIST) {
+        in = after;
+        const float2 t = p.teach[row];
+        teacher = t.x;
+        w = t.y;
+        load = w != 0.f;
+        if (load) {
+          load_entry_logits<DT>(p, row, in);
+#pragma unroll
+          for (int i = 0; i < E; ++i)
+            if (in.id[i] >= 0 && in.id[i] < V) atomicOr(&bits[in.id[i] >> 5], 1u << (in.id[i] & 31));
+        }
+        if (row + step < N) load_entries<T>(p, row + step, after);
+        __syncthreads();
+      } else {
+        token = token_at(a, row, V);
+        w = row_weight(a, row);
+        load = token >= 0 && w != 0.f;
+        if (load) {
+          xt = token < V ? Elem<DT>::cvt(x[token]) : NAN;
+          given = policy_in(a, row);
+        }
+      }
+    }
+
+    S* out = want && cur >= 0 ? static_cast<S*>(a.grad) + (int64_t)cur * V : nullptr;
+    Stat st = {-INFINITY, 0.f, 0.f};
+    // the span and thread that hold the given token
+    const int spot = token / VEC, cur_spot = cur_token / VEC;
+    const int span = token < 0 ? -1 : spot / T, cur_span = store != kGradient || cur_token < 0 ? -1 : cur_spot / T;
+    const bool holds = tid == spot % T, cur_holds = tid == cur_spot % T;
+    // vector i of the row that was loaded: its given tokens become -inf
+    auto clean = [&](u32x4& v, int i) {
+      if constexpr (LIST) {
+        const unsigned marks = marks_of[i * (kSpan / 8)] >> (own & 7) & ((1u << VEC) - 1);
+        if (marks) mask_vec<DT>(v, marks);
+      } else if (i == span) {
+        if (holds) mask_vec<DT>(v, 1u << token % VEC);
+      }
+    };
+    auto gradient = [&](const u32x4& v, int i, float (&g)[VEC]) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[e] = rest_value<ENT>(vec_elem<DT>(v, e), cur_M, c1, rest);
+      if (!LIST && i == cur_span) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] = cur_holds && cur_token % VEC == e ? at_token : g[e];
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld + kDelay; ++i) {
+      if (i < kHeld && i < nv) {
+        if (store != kNothing) {
+          float g[VEC] = {};
+          if (store == kGradient) gradient(r[i], i, g);
+          *reinterpret_cast<Vec16<DT>*>(out + i * kSpan + own) = pack_vec<DT>(g);
+        }
+        if (load) r[i] = load_vec_any<DT>(x + i * kSpan + own);
+      }
+      if (i >= kDelay + 1 && (i - kDelay) % 2 == 1) {
+        const int j = i - kDelay - 1;
+        if (load && j < nv) {
+          clean(r[j], j);
+          if (j + 1 < nv) {
+            clean(r[j + 1], j + 1);
+            add_vecs<DT, ENT, 2>(st, {r[j], r[j + 1]}, c1);
+          } else {
+            add_vecs<DT, ENT, 1>(st, {r[j]}, c1);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // vectors in their order: more of them at once do not fit the registers
+    }
+    if (last_here) {
+      if (store != kNothing) {
+        float g[VEC] = {};
+        if (store == kGradient) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            g[e] = rest_value<ENT>(vec_elem<DT>(last, e), cur_M, c1, rest);
+            if (!LIST) g[e] = cur_token == last_at + e ? at_token : g[e];
+          }
+        }
+        if (shift == 0) {
+          *reinterpret_cast<Vec16<DT>*>(out + last_at) = pack_vec<DT>(g);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e >= shift) out[last_at + e] = to_storage<DT>(g[e]);
+        }
+      }
+      if (load) {
+        last = load_vec_any<DT>(x + last_at);
+        if constexpr (LIST)
+          mask_vec<DT>(last, marks_at(bits, last_col, VEC) << shift);
+        else if (token >= last_at && token < last_at + VEC)
+          mask_vec<DT>(last, 1u << (token - last_at));
+        mask_vec<DT>(last, (1u << shift) - 1);  // what the thread before holds
+        add_vecs<DT, ENT, 1>(st, {last}, c1);
+      }
+    }
+    if (longer) {
+      if (store != kNothing)
+        for (int col = last_col; col < V; col += kSpan) {
+          float g[VEC] = {};
+          if (store == kGradient) {
+            load_filled<DT>(cur_x, col, V, g);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              g[e] = rest_value<ENT>(g[e], cur_M, c1, rest);
+              if (!LIST) g[e] = cur_token == col + e ? at_token : g[e];
+            }
+          }
+          store_filled<DT>(out, col, V, g);
+        }
+      if (load)
+        for (int col = last_col; col < V; col += kSpan) {
+          u32x4 v[1];
+          if (col + VEC <= V) {
+            v[0] = load_vec_any<DT>(x + col);
+          } else {
+            S tail[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) tail[e] = col + e < V ? x[col + e] : Elem<DT>::ninf();
+            v[0] = *reinterpret_cast<const u32x4_align2*>(tail);
+          }
+          if constexpr (LIST) {
+            const unsigned marks = marks_at(bits, col, VEC);
+            if (marks) mask_vec<DT>(v[0], marks);
+          } else {
+            if (token >= col && token < col + VEC) mask_vec<DT>(v[0], 1u << (token - col));
+          }
+          add_vecs<DT, ENT, 1>(st, v, c1);
+        }
+    }
+
+    if (load) {
+      rebase(st, wave_max(st.m), c1);
+      st.s = wave_sum(st.s);
+      if constexpr (ENT) st.t = wave_sum(st.t);
+      if (lane_id() == 0) s_part[parity][wave_id()] = make_float4(st.m, st.s, st.t, 0.f);
+    }
+    __syncthreads();
+    if constexpr (LIST) {
+      // behind every store of the row: its given tokens' own values
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (pend_id[i] >= 0 && out) out[pend_id[i]] = to_storage<DT>(pend[i]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        pend_id[i] = -1;
+        if (row < N && in.id[i] >= 0 && in.id[i] < V) bits[in.id[i] >> 5] = 0;
+      }
+    }
+    if (row >= N) break;
+    if (load) {
+      const int part = lane_id() % 16;
+      const float4 v = part < NW ? s_part[parity][part] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      st = {v.x, v.y, v.z};
+      rebase(st, readlane_f32(max16(st.m), 0), c1);
+      st.s = readlane_f32(sum16(st.s), 0);  // one lane's: a sum's last bit may be another in each
+      if constexpr (ENT) st.t = readlane_f32(sum16(st.t), 0);
+      parity ^= 1;
+    }
+
+    // the row's loss
+    LossRecord rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
+    float loss = 0.f;
+    store = want ? kZeros : kNothing;
+    if constexpr (LIST) {
+      if (load) {
+        rec.M = base_of(st.m);
+        rec.c = 1.f;
+        float over[E];
+        loss = distill_row<T, E>(p, st, teacher, w * mean, red, in, over, &rec.k);
+        if (p.records) save_over<T, E>(p, row, in, over);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          pend_id[i] = want ? in.id[i] : -1;
+          pend[i] = over[i];
+        }
+      }
+      __syncthreads();  // the marks are gone, the next row's may be set
+    } else {
+      TokenRow o = {0.f, 0.f, rec};
+      PolicyRow q = {0.f, 0.f, 0.f};
+      if (load) {
+        o = token_row(p, st, xt);
+        q = policy_row(a, given, o.lp, o.H);
+        rec = o.rec;
+        rec.c = q.c * w * mean;
+        rec.cH = -(float)a.entropy_coef * w * mean;
+        rec.pair = 0;
+        loss = q.loss * w * mean;
+      }
+      if (tid == 0) {
+        a.logprobs[row] = o.lp;
+        if (a.entropy) a.entropy[row] = o.H;
+        if (a.kl) a.kl[row] = q.kl;
+      }
+    }
+    if (tid == 0) {
+      p.row_loss[row] = loss;
+      if (p.records) p.records[row] = rec;
+    }
+    if (want && load) {
+      const float gH = ENT ? rec.cH : 0.f;
+      if (!(rec.c == 0.f && gH == 0.f)) store = kGradient;
+      cur_M = rec.M;
+      rest = rest_gradient(rec, rec.c, gH);
+      at_token = token_gradient(rec, rec.c, gH);
+    }
+    cur = row;
+    cur_x = x;
+    cur_token = token;
+    row += step;
   }
 }
 
@@ -686,6 +1076,24 @@ int chunk_of(int64_t rows, int V, int dtype) {
   return (int)std::min(std::max(each, (int64_t)1) * step, kMaxChunk);
 }
 
+int num_cus() {
+  static std::atomic<int> cus[64];
+  int device = 0, n = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) return 256;
+  if ((n = cus[device].load(std::memory_order_relaxed)) > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1) n = 256;
+  cus[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Threads of a workgroup of loss_rows_kernel: the fewest whose registers hold a row of V columns.
+int row_threads(int64_t V, int dtype) {
+  const int64_t each = (dtype == MVSD_F32 ? 4 : 8) * (kHeld + 1);
+  return V <= 256 * each ? 256 : V <= 512 * each ? 512 : 1024;
+}
+
+constexpr int64_t kMaxMarked = 1 << 18;  // columns whose marks are 32 KiB
+
 LossParams make_params(const mvsd_loss_args& a) {
   LossParams p = {};
   p.a = a;
@@ -705,16 +1113,31 @@ LossParams make_params(const mvsd_loss_args& a) {
   p.row_loss = a.reduction == MVSD_REDUCE_NONE && a.loss ? a.loss : reinterpret_cast<float*>(w);
   w += up16(std::max(N, a.num_pairs) * 4);
   p.row_lp = reinterpret_cast<float*>(w);
+  p.teach = reinterpret_cast<float2*>(w);  // of a distillation, which has no row_lp
+  w += up16(N * 8);
+  p.over_ids = reinterpret_cast<int32_t*>(w);
   if (a.saved) {
     p.records = static_cast<LossRecord*>(a.saved);
     p.over = reinterpret_cast<float*>(p.records + N);
     p.over_ids = reinterpret_cast<int32_t*>(p.over + N * p.K);
   }
-  const bool weighs = a.kind == MVSD_LOSS_DISTILL || a.kind == MVSD_LOSS_POLICY;
-  p.norm_parts = weighs && a.reduction == MVSD_REDUCE_MEAN
-                     ? (int)std::min(N / 64 + 1, (int64_t)kNormParts)
-                     : 0;
+  // the distillation's kernel has a wave a row where there are few
+  if (a.kind == MVSD_LOSS_DISTILL)
+    p.norm_parts = (int)std::min((N + kWaves - 1) / kWaves, (int64_t)kNormParts);
+  else if (a.kind == MVSD_LOSS_POLICY && a.reduction == MVSD_REDUCE_MEAN)
+    p.norm_parts = (int)std::min(N / 64 + 1, (int64_t)kNormParts);
   return p;
+}
+
+template <int DT, int T>
+void launch_rows(const LossParams& p, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min(p.a.num_rows, (int64_t)num_cus() * (1024 / T))), block(T);
+  if (has_list(p.a))
+    hipLaunchKernelGGL((loss_rows_kernel<DT, T, true, false>), grid, block, (unsigned)((p.V + 31) / 32 * 4), stream, p);
+  else if (p.entropy)
+    hipLaunchKernelGGL((loss_rows_kernel<DT, T, false, true>), grid, block, 0, stream, p);
+  else
+    hipLaunchKernelGGL((loss_rows_kernel<DT, T, false, false>), grid, block, 0, stream, p);
 }
 
 template <int DT>
@@ -723,9 +1146,17 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)(a.num_rows * p.nch)), block(kLossThreads);
   if (p.norm_parts) {
     if (has_list(a))
-      hipLaunchKernelGGL(loss_norm_kernel<true>, dim3(p.norm_parts), block, 0, stream, p);
+      hipLaunchKernelGGL(loss_teacher_kernel, dim3(p.norm_parts), block, 0, stream, p);
     else
-      hipLaunchKernelGGL(loss_norm_kernel<false>, dim3(p.norm_parts), block, 0, stream, p);
+      hipLaunchKernelGGL(loss_norm_kernel, dim3(p.norm_parts), block, 0, stream, p);
+  }
+  if (loss_one_pass(a)) {
+    switch (row_threads(p.V, DT)) {
+      case 256: launch_rows<DT, 256>(p, stream); break;
+      case 512: launch_rows<DT, 512>(p, stream); break;
+      default: launch_rows<DT, 1024>(p, stream); break;
+    }
+    return hipGetLastError();
   }
   if (has_list(a)) {
     const unsigned lds = (unsigned)((p.chunk + 31) / 32 * 4);
@@ -757,11 +1188,18 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
 
 }  // namespace
 
+bool loss_one_pass(const mvsd_loss_args& a) {
+  if ((a.kind != MVSD_LOSS_DISTILL && a.kind != MVSD_LOSS_POLICY) || a.reduction == MVSD_REDUCE_NONE) return false;
+  if (a.vocab_size < 8 || (has_list(a) && a.vocab_size > kMaxMarked)) return false;
+  return a.num_rows >= 128 * (1024 / row_threads(a.vocab_size, a.dtype));
+}
+
 int64_t loss_workspace_bytes(const mvsd_loss_args& a) {
   const int64_t chunk = chunk_of(a.num_rows, (int)a.vocab_size, a.dtype);
   const int64_t nch = (a.vocab_size + chunk - 1) / chunk;
   return a.num_rows * nch * (int64_t)sizeof(float4) + kNormParts * 4 +
-         up16(std::max(a.num_rows, a.num_pairs) * 4) + up16(a.num_rows * 4);
+         up16(std::max(a.num_rows, a.num_pairs) * 4) + up16(a.num_rows * 8) +
+         (has_list(a) ? a.num_rows * a.num_teacher * 4 : 0);
 }
 
 int64_t loss_saved_bytes(const mvsd_loss_args& a) {
@@ -863,6 +1301,11 @@ int64_t mvsd_loss_saved_bytes(const mvsd_loss_args* args) {
 int64_t mvsd_loss_workspace_bytes(const mvsd_loss_args* args) {
   const int status = check_sizes(args);
   return status != MVSD_OK ? status : mvsd::loss_workspace_bytes(*args);
+}
+
+int mvsd_loss_one_pass(const mvsd_loss_args* args) {
+  const int status = check_sizes(args);
+  return status != MVSD_OK ? status : mvsd::loss_one_pass(*args) ? 1 : 0;
 }
 
 int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream) {

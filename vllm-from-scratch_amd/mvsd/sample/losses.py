@@ -118,7 +118,7 @@ def _weights(t: torch.Tensor | None, shape, device) -> torch.Tensor | None:
 class _Call:
     """One call: its arguments and the tensors they point to."""
 
-    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "device")
+    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "grad", "device")
 
     def __init__(self, kind: int, logits: torch.Tensor, temperature: float, reduction: int):
         nat.require_device_tensor(logits, "logits")
@@ -130,7 +130,7 @@ class _Call:
         if not 1e-6 <= temperature <= 1e6:
             raise ValueError(f"temperature={temperature}")
         self.kind, self.logits, self.device = kind, logits, logits.device
-        self.keep, self.outputs, self.saved = [], (), None
+        self.keep, self.outputs, self.saved, self.grad = [], (), None, None
         a = self.args = nat.LossArgs()
         a.kind, a.reduction, a.temperature = kind, reduction, temperature
         self._rows(logits)
@@ -175,6 +175,9 @@ class _Call:
             self.saved = torch.empty(handle.mvsd_loss_saved_bytes(ctypes.byref(a)),
                                      dtype=torch.uint8, device=self.device)
             a.saved = self.saved.data_ptr() or None
+            if handle.mvsd_loss_one_pass(ctypes.byref(a)):
+                self.grad = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.device)
+                a.grad = self.grad.data_ptr()
         nat.check(handle.mvsd_row_loss(ctypes.byref(a), nat.stream_of(self.device)), "mvsd_row_loss")
         self.keep = []
 
@@ -183,7 +186,11 @@ class _Call:
         a = self.args
         self._rows(logits)
         a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr() or None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        # that of an upstream of 1, which is there already, goes out once: a kept graph's next is made anew
+        grad, self.grad = self.grad, None
+        a.unit_gradient = 0 if grad is None else 1
+        if grad is None:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if grad.numel() == 0:
             return grad
         a.grad = grad.data_ptr()
