@@ -10,7 +10,7 @@ namespace mvsd {
 
 constexpr int kMaxTeacher = 512;            // teacher entries of a row: two a thread of a finishing workgroup
 constexpr int kRecord = 8;                  // floats of a row that its gradient needs
-constexpr int kNormParts = 256;             // partial sums of the rows' weights
+constexpr int kNormParts = 1024;            // partial sums of the rows' weights
 
 // A row's record for the gradient of unit upstream: with e_j = 2^((x_j - M) c1) of the tokens that are
 // none of the row's given ones ("the rest", M their maximum), g the upstream times c and gH the entropy's
@@ -28,10 +28,13 @@ struct LossParams {
   int V;
   int K;        // given tokens of a row
   int chunk, nch;   // columns of a workgroup, workgroups of a row
+  int active;       // threads that hold a row
+  void* aside;      // a span of them for each workgroup
   bool entropy;
   float4* parts;      // [N, nch] maximum, sum, sum of e log2 e
   float* norm;        // [kNormParts] partial sums of weights (mean)
   int norm_parts;
+  int* tickets;       // rows that loss_rows_kernel's workgroups have taken behind their first
   float* row_loss;    // [N] (preference: [pairs]), weighted
   float* row_lp;      // preference: [N]
   float2* teach;      // distillation: [N] what the teacher's kernel gives of a row, its weight (0: left out)

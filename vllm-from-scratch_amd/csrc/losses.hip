@@ -102,7 +102,7 @@ __device__ inline void load_filled(const typename Elem<DT>::storage* row, int co
 }
 
 // Marks of the given tokens among a chunk's columns, a bit each.
-__device__ inline unsigned marks_at(const uint32_t* bits, int col, int n) {  // n divides 32, col is its multiple
+__device__ inline unsigned marks_at(const uint32_t* bits, unsigned col, int n) {  // n divides 32, col is its multiple
   return (bits[col >> 5] >> (col & 31)) & ((1u << n) - 1u);
 }
 
@@ -186,6 +186,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_norm_kernel(LossParams p) {
     if (token_at(p.a, row, p.V) >= 0) sum[0] += row_weight(p.a, row);
   block_sum<1>(sum, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = sum[0];
+  if (threadIdx.x == 0 && blockIdx.x == 0) *p.tickets = 0;
 }
 
 // What a row's weight is multiplied by, in every thread of a wave.
@@ -470,17 +471,18 @@ __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p
   if (lane != 0) weights[0] = 0.f;
   block_sum<1>(weights, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = weights[0];
+  if (threadIdx.x == 0 && blockIdx.x == 0) *p.tickets = 0;
 }
 
-// A row's entries, entry i * T + thread in each thread.
+// A row's entries, entry i * T + thread in each of T threads.
 template <int E>
 struct Entries {
   int id[E];  // -1: it does not count
   float x[E], v[E];
 };
 
-template <int T, int E>
-__device__ inline void load_entries(const LossParams& p, int64_t row, Entries<E>& in) {
+template <int E>
+__device__ inline void load_entries(const LossParams& p, int64_t row, int T, Entries<E>& in) {
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int k = i * T + (int)threadIdx.x;
@@ -499,31 +501,61 @@ __device__ inline void load_entry_logits(const LossParams& p, int64_t row, Entri
   for (int i = 0; i < E; ++i) in.x[i] = in.id[i] >= 0 && in.id[i] < p.V ? Elem<DT>::cvt(x[in.id[i]]) : NAN;
 }
 
-// One row's loss by a workgroup of T threads, from the statistics of its rest, its entries and what the
+__device__ inline float sum16(float v) {
+  v += dpp_f32<kDppXor1>(v);
+  v += dpp_f32<kDppXor2>(v);
+  v += dpp_f32<kDppHalfMirror>(v);
+  return v + dpp_f32<kDppMirror>(v);
+}
+
+// Sums (or maxima) over the NW waves of a workgroup, in one order; two barriers.
+template <int N>
+__device__ inline void waves_sum(float (&v)[N], float* red, int NW) {
+#pragma unroll
+  for (int g = 0; g < N; ++g) v[g] = wave_sum(v[g]);
+  if (lane_id() == 0) {
+#pragma unroll
+    for (int g = 0; g < N; ++g) red[g * NW + wave_id()] = v[g];
+  }
+  __syncthreads();
+  const int part = lane_id() % 16;
+#pragma unroll
+  for (int g = 0; g < N; ++g) v[g] = readlane_f32(sum16(part < NW ? red[g * NW + part] : 0.f), 0);
+  __syncthreads();
+}
+__device__ inline float waves_max(float v, float* red, int NW) {
+  v = wave_max(v);
+  if (lane_id() == 0) red[wave_id()] = v;
+  __syncthreads();
+  const int part = lane_id() % 16;
+  v = readlane_f32(max16(part < NW ? red[part] : -INFINITY), 0);
+  __syncthreads();
+  return v;
+}
+
+// One row's loss by a workgroup of NW waves, from the statistics of its rest, its entries and what the
 // teacher's kernel gave of it.  Gives the gradients of the given tokens (over, at id, -1: none) and returns
-// the loss; *k is the record's.  `weight` is the row's, after the mean; red holds 2 T / 64 floats.
-template <int T, int E>
-__device__ inline float distill_row(const LossParams& p, Stat st, float teacher, float weight, float* red,
+// the loss; *k is the record's.  `weight` is the row's, after the mean; red holds 2 NW floats.
+template <int E>
+__device__ inline float distill_row(const LossParams& p, Stat st, float teacher, float weight, float* red, int NW,
                                     Entries<E>& in, float (&over)[E], float* k_out) {
-  constexpr int NW = T / kWave;
   const mvsd_loss_args& a = p.a;
   int (&id)[E] = in.id;
   float (&x)[E] = in.x;
-  float top[1] = {st.m};
+  float top = st.m;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     if (id[i] < 0) x[i] = -INFINITY;
     if (x[i] == INFINITY) x[i] = NAN;
-    top[0] = fmaxf(top[0], x[i]);
+    top = fmaxf(top, x[i]);
   }
-  block_max<1, NW>(top, red);
-  const float base = base_of(top[0]), rest_base = base_of(st.m);
+  const float base = base_of(waves_max(top, red, NW)), rest_base = base_of(st.m);
   const bool tail = a.tail && teacher != 0.f;
   // the student's normaliser
   float z[1] = {0.f};
 #pragma unroll
   for (int i = 0; i < E; ++i) z[0] += expf((x[i] - base) * p.inv_t);
-  block_sum<1, NW>(z, red);
+  waves_sum<1>(z, red, NW);
   const float rest_d = st.m == -INFINITY ? 0.f : (rest_base - base) * p.inv_t;
   const float log_z = logf(z[0] + st.s * expf(rest_d));
   const float rest_lp = rest_d + logf(st.s) - log_z, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
@@ -552,7 +584,7 @@ __device__ inline float distill_row(const LossParams& p, Stat st, float teacher,
     both[0] += term;
     both[1] += pd[i];
   }
-  block_sum<2, NW>(both, red);
+  waves_sum<2>(both, red, NW);
   float rest_pd = 0.f;
   if (tail) {
     float term;
@@ -570,14 +602,12 @@ __device__ inline float distill_row(const LossParams& p, Stat st, float teacher,
   return both[0] * weight;
 }
 
-template <int T, int E>
-__device__ inline void save_over(const LossParams& p, int64_t row, const Entries<E>& in, const float (&over)[E]) {
+template <int E>
+__device__ inline void save_over(const LossParams& p, int64_t row, int T, const float (&over)[E]) {
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int k = i * T + (int)threadIdx.x;
-    if (k < p.K) {
-      p.over[row * p.K + k] = over[i];
-    }
+    if (k < p.K) p.over[row * p.K + k] = over[i];
   }
 }
 
@@ -592,7 +622,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
   LossRecord rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
   if (teacher.y != 0.f) {
     Entries<E> in;
-    load_entries<kLossThreads>(p, row, in);
+    load_entries<E>(p, row, kLossThreads, in);
     load_entry_logits<DT>(p, row, in);
     Stat st = {-INFINITY, 0.f, 0.f};
     for (int i = lane_id(); i < p.nch; i += kWave) {
@@ -603,8 +633,8 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
     rec.M = base_of(st.m);
     rec.c = 1.f;
     float over[E];
-    loss = distill_row<kLossThreads, E>(p, st, teacher.x, teacher.y * mean_factor(p), red, in, over, &rec.k);
-    if (p.records) save_over<kLossThreads, E>(p, row, in, over);
+    loss = distill_row<E>(p, st, teacher.x, teacher.y * mean_factor(p), red, kWaves, in, over, &rec.k);
+    if (p.records) save_over<E>(p, row, kLossThreads, over);
   }
   if (threadIdx.x == 0) {
     p.row_loss[row] = loss;
@@ -681,14 +711,13 @@ __device__ inline void store_filled(typename Elem<DT>::storage* row, int col, in
   }
 }
 
-// One workgroup a chunk of a row, from its record.
+// A chunk of a row by a workgroup, from the row's record.
 template <int DT, bool LIST, bool ENT>
-__global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams p, const float* up, int64_t us,
-                                                                     const float* up_h, int64_t uhs) {
+__device__ inline void gradient_chunk(const LossParams& p, const float* up, int64_t us, const float* up_h,
+                                      int64_t uhs, int64_t chunk) {
   constexpr int VEC = Elem<DT>::kVec;
-  if (p.a.unit_gradient && up[0] == 1.f) return;  // it is there already
-  const int64_t row = blockIdx.x / p.nch;
-  const int part = blockIdx.x - (int)(row * p.nch);
+  const int64_t row = chunk / p.nch;
+  const int part = chunk - row * p.nch;
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
   const LossRecord rec = p.records[row];
   const int64_t n = p.a.kind == MVSD_LOSS_PREFERENCE ? rec.pair : row;
@@ -727,9 +756,18 @@ __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams 
   }
 }
 
+template <int DT, bool LIST, bool ENT>
+__global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams p, const float* up, int64_t us,
+                                                                     const float* up_h, int64_t uhs) {
+  if (p.a.unit_gradient && up[0] == 1.f) return;  // it is there already
+  for (int64_t chunk = blockIdx.x; chunk < p.a.num_rows * p.nch; chunk += gridDim.x)
+    gradient_chunk<DT, LIST, ENT>(p, up, us, up_h, uhs, chunk);
+}
+
 // ------------------------------------------------------------------ values and gradient in one pass ---
 
-constexpr int kHeld = 18;  // full vectors of a row in each thread's registers (72 of 128), beside the last columns'
+constexpr int kMostHeld = 18;  // vectors of a row in each thread's registers (72 of 128)
+constexpr int kRowThreads = 1024;
 
 // The elements of `marks` become -inf.
 template <int DT>
@@ -747,28 +785,52 @@ __device__ inline void mask_vec(u32x4& r, unsigned marks) {
   }
 }
 
-// Adds a vector, or two, to a thread's statistics.
-template <int DT, bool ENT, int N>
-__device__ inline void add_vecs(Stat& st, const u32x4 (&r)[N], float c1) {
-  constexpr int VEC = Elem<DT>::kVec;
+// vec_elem, by instructions of its own: the compiler would keep what the statistics converted until the
+// gradient converts it again, and a row would take twice the registers.
+template <int DT>
+__device__ inline float vec_elem_again(const u32x4& r, int j) {
+  if constexpr (DT == MVSD_F32) {
+    return __uint_as_float(r[j]);
+  } else {
+    float v;
+    const uint32_t w = r[j / 2];
+    if (DT == MVSD_BF16 && j % 2 == 0)
+      asm("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(w));
+    else if (DT == MVSD_BF16)
+      asm("v_and_b32 %0, 0xffff0000, %1" : "=v"(v) : "v"(w));
+    else if (j % 2 == 0)
+      asm("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(w));
+    else
+      asm("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v) : "v"(w));
+    return v;
+  }
+}
+
+// Adds values to a thread's statistics.
+template <bool ENT, int N>
+__device__ inline void add_values(Stat& st, const float (&v)[N], float c1) {
   float m = st.m;
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) m = fmaxf(m, vec_elem<DT>(r[i], e));
+  for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
   const float base = base_of(m);
   const float d = fmaxf((st.m - base) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
   if constexpr (ENT) st.t = fmaf(st.s, d, st.t) * f;
   st.s *= f;
   st.m = m;
 #pragma unroll
-  for (int i = 0; i < N; ++i)
+  for (int e = 0; e < N; ++e) {
+    const float y = (v[e] - base) * c1, w = __builtin_amdgcn_exp2f(y);
+    st.s += w;
+    if constexpr (ENT) st.t = fmaf(w, fmaxf(y, kLeast), st.t);
+  }
+}
+template <int DT, bool ENT, int N>
+__device__ inline void add_vecs(Stat& st, const u32x4 (&r)[N], float c1) {
+  constexpr int VEC = Elem<DT>::kVec;
+  float v[N * VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float y = (vec_elem<DT>(r[i], e) - base) * c1, w = __builtin_amdgcn_exp2f(y);
-      st.s += w;
-      if constexpr (ENT) st.t = fmaf(w, fmaxf(y, kLeast), st.t);
-    }
+  for (int i = 0; i < N * VEC; ++i) v[i] = vec_elem<DT>(r[i / VEC], i % VEC);
+  add_values<ENT, N * VEC>(st, v, c1);
 }
 
 // Both sums against a new maximum.
@@ -779,262 +841,244 @@ __device__ inline void rebase(Stat& st, float m, float c1) {
   st.m = m;
 }
 
-__device__ inline float sum16(float v) {
-  v += dpp_f32<kDppXor1>(v);
-  v += dpp_f32<kDppXor2>(v);
-  v += dpp_f32<kDppHalfMirror>(v);
-  return v + dpp_f32<kDppMirror>(v);
-}
-
-// Rows by a workgroup of T threads, one after the other, every row in its registers: read once, written once.
-// A turn of the loop writes the gradient of one row and, vector by vector, loads the next one in its place
-// and adds it to its statistics a few vectors later, so that memory is busy except in the reductions and
-// the row's own loss between two turns.  Columns behind kHeld vectors a thread are read again.
-template <int DT, int T, bool LIST, bool ENT>
-__global__ __launch_bounds__(T, 4) void loss_rows_kernel(LossParams p) {
+// Rows by a workgroup, one after the other (by tickets: some are left out), every row in its registers: read once, written once.  A turn of the
+// loop writes the gradient of one row and, vector by vector, loads the next one in its place and adds it to
+// its statistics kDelay vectors later, so that memory is busy except in the reductions and the row's own loss
+// between two turns.  `active` threads hold NV vectors each, those of one i side by side (a span, a multiple
+// of 32 columns); the columns behind the spans (few, or what the registers do not hold) are read again.
+// A turn's loads and stores are unconditional, with a first turn that only loads and a last one that only
+// stores (a conditional load makes the compiler wait for all of them at once); rows that are left out are
+// passed by, their gradient written on the way.
+template <int DT, int NV, bool LIST, bool ENT, bool WANT>
+__global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p) {
   using S = typename Elem<DT>::storage;
-  constexpr int VEC = Elem<DT>::kVec, NW = T / kWave, E = LIST ? (kMaxTeacher + T - 1) / T : 1, kDelay = 8;
+  constexpr int VEC = Elem<DT>::kVec, E = 1, kDelay = NV > 8 ? 8 : NV - NV % 2;
   extern __shared__ uint32_t bits[];
-  __shared__ float4 s_part[2][NW];
-  __shared__ float red[2 * NW];
+  __shared__ float4 s_part[2][kRowThreads / kWave];
+  __shared__ float red[2 * kRowThreads / kWave];
+  __shared__ int s_ticket;
   const mvsd_loss_args& a = p.a;
-  const int tid = threadIdx.x, V = p.V, K = p.K, N = (int)a.num_rows, step = gridDim.x;
-  constexpr int kSpan = T * VEC;  // columns of one vector a thread
-  const int nv = min(kHeld, V / kSpan), behind = nv * kSpan;  // full vectors, the columns in them
-  const bool longer = V - behind > kSpan;
-  const unsigned own = tid * VEC;  // the thread's place in a span
-  // the thread's last columns, moved back where they would pass the row's end by `shift`
-  const int last_col = behind + (int)own, last_at = min(last_col, max(V - VEC, 0)), shift = last_col - last_at;
-  const bool last_here = !longer && shift < VEC;
+  const int tid = threadIdx.x, V = p.V, N = (int)a.num_rows, T = blockDim.x, NW = T / kWave;
+  const int span = p.active * VEC, behind = NV * span;
+  // threads behind the active ones do what the last of those does, and count for nothing
+  const unsigned own = min(tid, p.active - 1) * VEC;
+  const int tail_col = behind + tid * VEC;
   const float mean = mean_factor(p), c1 = p.c1;
-  const bool want = a.grad != nullptr;
-
   if constexpr (LIST) {
     for (int i = tid; i < (V + 31) / 32; i += T) bits[i] = 0;
     __syncthreads();
   }
 
-  // the row whose logits are loaded in this turn, and the one whose gradient is written
-  int row = blockIdx.x, cur = -1, parity = 0;
-  int token = -1, cur_token = -1;
-  const uint8_t* marks_of = reinterpret_cast<const uint8_t*>(bits) + (own >> 3);
-  float w = 0.f;
-  Entries<E> in = {}, after = {};
-  int pend_id[E];
-  float pend[E];
+  // What a row is given beside its logits, and what its gradient is formed from.
+  int row = blockIdx.x, ticket = 0, token = -1, parity = 0;
+  float w = 0.f, teacher = 0.f, xt = NAN;
+  PolicyIn given = {0.f, 0.f, 0.f};
+  Entries<E> in = {};
+  const S* x = nullptr;
+  int cur = -1, cur_token = -1, pend_id[E];
+  float pend[E], cur_M = 0.f, at_token = 0.f;
+  RestGradient rest = {0.f, 0.f};
+  bool zeros = true;  // the gradient is 0
+  const S* cur_x = nullptr;
 #pragma unroll
   for (int i = 0; i < E; ++i) pend_id[i] = -1;
-  if constexpr (LIST) {
-    if (row < N) load_entries<T>(p, row, after);
-  }
-  enum { kNothing, kZeros, kGradient };
-  int store = kNothing;
-  float cur_M = 0.f, at_token = 0.f;
-  RestGradient rest = {0.f, 0.f};
-  const S* cur_x = nullptr;
-  u32x4 r[kHeld] = {}, last = {};
-
-  for (;;) {
-    bool load = false;
-    float xt = NAN, teacher = 0.f;
-    PolicyIn given = {0.f, 0.f, 0.f};
-    const S* x = nullptr;
-    if (row < N) {
-      x = logits_row<DT>(a, row);
+  // of the row after it, loaded while this one's loss is formed
+  Entries<E> after = {};
+  float2 teach = {0.f, 0.f};
+  int next_token = -1;
+  float next_w = 0.f;
+  auto announce = [&](int n) {
+    if (n >= N) return;
+    if constexpr (LIST) {
+      load_entries<E>(p, n, T, after);
+      teach = p.teach[n];
+    } else {
+      next_token = token_at(a, n, V);
+      next_w = row_weight(a, n);
+    }
+  };
+  // The next row that is not left out becomes `row`; false: there is none.
+  auto advance = [&]() {
+    for (; row < N; announce(row)) {
       if constexpr (LIST) {
         in = after;
-        const float2 t = p.teach[row];
-        teacher = t.x;
-        w = t.y;
-        load = w != 0.f;
-        if (load) {
-          load_entry_logits<DT>(p, row, in);
-#pragma unroll
-          for (int i = 0; i < E; ++i)
-            if (in.id[i] >= 0 && in.id[i] < V) atomicOr(&bits[in.id[i] >> 5], 1u << (in.id[i] & 31));
-        }
-        if (row + step < N) load_entries<T>(p, row + step, after);
-        __syncthreads();
+        teacher = teach.x;
+        w = teach.y;
       } else {
-        token = token_at(a, row, V);
-        w = row_weight(a, row);
-        load = token >= 0 && w != 0.f;
-        if (load) {
-          xt = token < V ? Elem<DT>::cvt(x[token]) : NAN;
-          given = policy_in(a, row);
+        token = next_token;
+        w = next_w;
+      }
+      if (w != 0.f && (LIST || token >= 0)) break;
+      if (tid == 0) {
+        p.row_loss[row] = 0.f;
+        if (p.records) p.records[row] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
+        if constexpr (!LIST) {
+          a.logprobs[row] = 0.f;
+          if (a.entropy) a.entropy[row] = 0.f;
+          if (a.kl) a.kl[row] = 0.f;
         }
       }
+      if (WANT) {
+        const float zero[VEC] = {};
+        S* out = static_cast<S*>(a.grad) + (int64_t)row * V;
+        for (int col = tid * VEC; col < V; col += T * VEC) store_filled<DT>(out, col, V, zero);
+      }
+      if (tid == 0) s_ticket = atomicAdd(p.tickets, 1);
+      __syncthreads();
+      row = gridDim.x + s_ticket;
+      __syncthreads();
     }
+    if (row >= N) return false;
+    if (tid == 0) ticket = atomicAdd(p.tickets, 1);  // the next row's, which finish() gives to all
+    x = logits_row<DT>(a, row);
+    if constexpr (LIST) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (in.id[i] >= 0 && in.id[i] < V) atomicOr(&bits[in.id[i] >> 5], 1u << (in.id[i] & 31));
+      load_entry_logits<DT>(p, row, in);
+      __syncthreads();
+    } else {
+      xt = token < V ? Elem<DT>::cvt(x[token]) : NAN;
+      given = policy_in(a, row);
+    }
+    return true;
+  };
 
-    S* out = want && cur >= 0 ? static_cast<S*>(a.grad) + (int64_t)cur * V : nullptr;
-    Stat st = {-INFINITY, 0.f, 0.f};
-    // the span and thread that hold the given token
-    const int spot = token / VEC, cur_spot = cur_token / VEC;
-    const int span = token < 0 ? -1 : spot / T, cur_span = store != kGradient || cur_token < 0 ? -1 : cur_spot / T;
-    const bool holds = tid == spot % T, cur_holds = tid == cur_spot % T;
-    // vector i of the row that was loaded: its given tokens become -inf
-    auto clean = [&](u32x4& v, int i) {
+  Stat st;
+  u32x4 r[NV] = {};
+  bool more = true;
+  // A turn's loads and stores are unconditional: a conditional one makes the compiler wait for all of them at
+  // once.  The first turn stores to a place of the workgroup's own, the last loads one span again and again.
+  S* const aside = static_cast<S*>(p.aside) + (int64_t)blockIdx.x * span;
+  auto turn = [&]() {
+    st = {-INFINITY, 0.f, 0.f};
+    const bool stores = cur >= 0;
+    S* out = WANT && stores ? static_cast<S*>(a.grad) + (int64_t)cur * V : aside;
+    const unsigned to_step = stores ? span : 0, from_step = more ? span : 0;
+    // the span and thread that hold a given token
+    const int spot = token >= 0 && token < behind ? token / VEC : -1;
+    const int at_span = spot < 0 ? -1 : spot / p.active;
+    const bool holds = (int)own == (spot - at_span * p.active) * VEC;
+    const int cur_spot = !zeros && cur_token >= 0 && cur_token < behind ? cur_token / VEC : -1;
+    const int cur_span = cur_spot < 0 ? -1 : cur_spot / p.active;
+    const bool cur_holds = (int)own == (cur_spot - cur_span * p.active) * VEC;
+    // uniform offsets, kept so: the compiler would keep each thread's for every vector
+    unsigned from = 0, to = 0;
+    const uint32_t* marks_from = bits + (own >> 5);
+    auto clean = [&](u32x4& v, int i) {  // the given tokens become -inf
       if constexpr (LIST) {
-        const unsigned marks = marks_of[i * (kSpan / 8)] >> (own & 7) & ((1u << VEC) - 1);
+        const unsigned marks = *marks_from >> (own & 31) & ((1u << VEC) - 1);
+        marks_from += span / 32;
+        asm("" : "+v"(marks_from));
         if (marks) mask_vec<DT>(v, marks);
-      } else if (i == span) {
+      } else if (i == at_span) {
         if (holds) mask_vec<DT>(v, 1u << token % VEC);
       }
     };
-    auto gradient = [&](const u32x4& v, int i, float (&g)[VEC]) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) g[e] = rest_value<ENT>(vec_elem<DT>(v, e), cur_M, c1, rest);
-      if (!LIST && i == cur_span) {
+    for (int i = 0; i < NV + kDelay; ++i) {
+      if (i < NV) {
+        if constexpr (WANT) {
+          u32x4 v = {0u, 0u, 0u, 0u};
+          if (!zeros) {
+            float g[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = cur_holds && cur_token % VEC == e ? at_token : g[e];
-      }
-    };
+            for (int e = 0; e < VEC; ++e) g[e] = rest_value<ENT>(vec_elem_again<DT>(r[i], e), cur_M, c1, rest);
+            if (!LIST && i == cur_span) {
 #pragma unroll
-    for (int i = 0; i < kHeld + kDelay; ++i) {
-      if (i < kHeld && i < nv) {
-        if (store != kNothing) {
-          float g[VEC] = {};
-          if (store == kGradient) gradient(r[i], i, g);
-          *reinterpret_cast<Vec16<DT>*>(out + i * kSpan + own) = pack_vec<DT>(g);
-        }
-        if (load) r[i] = load_vec_any<DT>(x + i * kSpan + own);
-      }
-      if (i >= kDelay + 1 && (i - kDelay) % 2 == 1) {
-        const int j = i - kDelay - 1;
-        if (load && j < nv) {
-          clean(r[j], j);
-          if (j + 1 < nv) {
-            clean(r[j + 1], j + 1);
-            add_vecs<DT, ENT, 2>(st, {r[j], r[j + 1]}, c1);
-          } else {
-            add_vecs<DT, ENT, 1>(st, {r[j]}, c1);
+              for (int e = 0; e < VEC; ++e) g[e] = cur_holds && cur_token % VEC == e ? at_token : g[e];
+            }
+            v = pack_vec<DT>(g);
           }
+          asm("" : "+s"(to));
+          *reinterpret_cast<Vec16<DT>*>(out + to + own) = v;
+          to += to_step;
+        }
+        asm("" : "+s"(from));
+        r[i] = load_vec_any<DT>(x + from + own);
+        from += from_step;
+      }
+      const int j = i - kDelay;  // pairs, and a last one alone
+      if (more && (j == NV - 1 || (j >= 0 && j % 2 == 1))) {
+        if (j % 2 == 1) {
+          clean(r[j - 1], j - 1);
+          clean(r[j], j);
+          add_vecs<DT, ENT, 2>(st, {r[j - 1], r[j]}, c1);
+        } else {
+          clean(r[j], j);
+          add_vecs<DT, ENT, 1>(st, {r[j]}, c1);
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // vectors in their order: more of them at once do not fit the registers
     }
-    if (last_here) {
-      if (store != kNothing) {
-        float g[VEC] = {};
-        if (store == kGradient) {
+    if (tid >= p.active) st = {-INFINITY, 0.f, 0.f};
+    for (int col = tail_col; col < V; col += T * VEC) {
+      float v[VEC];
+      if (WANT && stores) {
+        load_filled<DT>(cur_x, col, V, v);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            g[e] = rest_value<ENT>(vec_elem<DT>(last, e), cur_M, c1, rest);
-            if (!LIST) g[e] = cur_token == last_at + e ? at_token : g[e];
-          }
+        for (int e = 0; e < VEC; ++e) {
+          const float g = rest_value<ENT>(v[e], cur_M, c1, rest);
+          v[e] = zeros ? 0.f : !LIST && cur_token == col + e ? at_token : g;
         }
-        if (shift == 0) {
-          *reinterpret_cast<Vec16<DT>*>(out + last_at) = pack_vec<DT>(g);
-        } else {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (e >= shift) out[last_at + e] = to_storage<DT>(g[e]);
-        }
+        store_filled<DT>(out, col, V, v);
       }
-      if (load) {
-        last = load_vec_any<DT>(x + last_at);
-        if constexpr (LIST)
-          mask_vec<DT>(last, marks_at(bits, last_col, VEC) << shift);
-        else if (token >= last_at && token < last_at + VEC)
-          mask_vec<DT>(last, 1u << (token - last_at));
-        mask_vec<DT>(last, (1u << shift) - 1);  // what the thread before holds
-        add_vecs<DT, ENT, 1>(st, {last}, c1);
+      if (more) {
+        load_filled<DT>(x, col, V, v);
+        const unsigned marks = LIST ? marks_at(bits, col, VEC) : 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (LIST ? marks >> e & 1 : token == col + e) ? -INFINITY : v[e];
+        add_values<ENT, VEC>(st, v, c1);
       }
     }
-    if (longer) {
-      if (store != kNothing)
-        for (int col = last_col; col < V; col += kSpan) {
-          float g[VEC] = {};
-          if (store == kGradient) {
-            load_filled<DT>(cur_x, col, V, g);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              g[e] = rest_value<ENT>(g[e], cur_M, c1, rest);
-              if (!LIST) g[e] = cur_token == col + e ? at_token : g[e];
-            }
-          }
-          store_filled<DT>(out, col, V, g);
-        }
-      if (load)
-        for (int col = last_col; col < V; col += kSpan) {
-          u32x4 v[1];
-          if (col + VEC <= V) {
-            v[0] = load_vec_any<DT>(x + col);
-          } else {
-            S tail[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) tail[e] = col + e < V ? x[col + e] : Elem<DT>::ninf();
-            v[0] = *reinterpret_cast<const u32x4_align2*>(tail);
-          }
-          if constexpr (LIST) {
-            const unsigned marks = marks_at(bits, col, VEC);
-            if (marks) mask_vec<DT>(v[0], marks);
-          } else {
-            if (token >= col && token < col + VEC) mask_vec<DT>(v[0], 1u << (token - col));
-          }
-          add_vecs<DT, ENT, 1>(st, v, c1);
-        }
-    }
-
-    if (load) {
-      rebase(st, wave_max(st.m), c1);
-      st.s = wave_sum(st.s);
-      if constexpr (ENT) st.t = wave_sum(st.t);
-      if (lane_id() == 0) s_part[parity][wave_id()] = make_float4(st.m, st.s, st.t, 0.f);
-    }
-    __syncthreads();
-    if constexpr (LIST) {
-      // behind every store of the row: its given tokens' own values
+  };
+  // Behind every store of a row: its given tokens' own values.
+  auto give = [&]() {
+    if constexpr (LIST && WANT) {
+      S* out = static_cast<S*>(a.grad) + (int64_t)cur * V;
 #pragma unroll
       for (int i = 0; i < E; ++i)
-        if (pend_id[i] >= 0 && out) out[pend_id[i]] = to_storage<DT>(pend[i]);
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        pend_id[i] = -1;
-        if (row < N && in.id[i] >= 0 && in.id[i] < V) bits[in.id[i] >> 5] = 0;
-      }
+        if (pend_id[i] >= 0) out[pend_id[i]] = to_storage<DT>(pend[i]);
     }
-    if (row >= N) break;
-    if (load) {
-      const int part = lane_id() % 16;
-      const float4 v = part < NW ? s_part[parity][part] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      st = {v.x, v.y, v.z};
-      rebase(st, readlane_f32(max16(st.m), 0), c1);
-      st.s = readlane_f32(sum16(st.s), 0);  // one lane's: a sum's last bit may be another in each
-      if constexpr (ENT) st.t = readlane_f32(sum16(st.t), 0);
-      parity ^= 1;
-    }
-
-    // the row's loss
+  };
+  // The loss of `row`, which becomes `cur`.
+  auto finish = [&]() {
+    rebase(st, wave_max(st.m), c1);
+    st.s = wave_sum(st.s);
+    if constexpr (ENT) st.t = wave_sum(st.t);
+    if (lane_id() == 0) s_part[parity][wave_id()] = make_float4(st.m, st.s, st.t, 0.f);
+    if (tid == 0) s_ticket = ticket;
+    __syncthreads();
+    const int next = gridDim.x + s_ticket;
+    announce(next);
+    give();
+    const int part = lane_id() % 16;
+    const float4 v = part < NW ? s_part[parity][part] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    st = {v.x, v.y, v.z};
+    rebase(st, readlane_f32(max16(st.m), 0), c1);
+    st.s = readlane_f32(sum16(st.s), 0);  // one lane's: a sum's last bit may be another in each
+    if constexpr (ENT) st.t = readlane_f32(sum16(st.t), 0);
+    parity ^= 1;
     LossRecord rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
-    float loss = 0.f;
-    store = want ? kZeros : kNothing;
+    float loss;
     if constexpr (LIST) {
-      if (load) {
-        rec.M = base_of(st.m);
-        rec.c = 1.f;
-        float over[E];
-        loss = distill_row<T, E>(p, st, teacher, w * mean, red, in, over, &rec.k);
-        if (p.records) save_over<T, E>(p, row, in, over);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          pend_id[i] = want ? in.id[i] : -1;
-          pend[i] = over[i];
-        }
-      }
-      __syncthreads();  // the marks are gone, the next row's may be set
+      for (int i = 0; i < E; ++i)  // distill_row's barriers are between this and the next row's marks
+        if (in.id[i] >= 0 && in.id[i] < V) bits[in.id[i] >> 5] = 0;
+      rec.M = base_of(st.m);
+      rec.c = 1.f;
+      loss = distill_row<E>(p, st, teacher, w * mean, red, NW, in, pend, &rec.k);
+      if (p.records) save_over<E>(p, row, T, pend);
+#pragma unroll
+      for (int i = 0; i < E; ++i) pend_id[i] = in.id[i];
     } else {
-      TokenRow o = {0.f, 0.f, rec};
-      PolicyRow q = {0.f, 0.f, 0.f};
-      if (load) {
-        o = token_row(p, st, xt);
-        q = policy_row(a, given, o.lp, o.H);
-        rec = o.rec;
-        rec.c = q.c * w * mean;
-        rec.cH = -(float)a.entropy_coef * w * mean;
-        rec.pair = 0;
-        loss = q.loss * w * mean;
-      }
+      const TokenRow o = token_row(p, st, xt);
+      const PolicyRow q = policy_row(a, given, o.lp, o.H);
+      rec = o.rec;
+      rec.c = q.c * w * mean;
+      rec.cH = -(float)a.entropy_coef * w * mean;
+      rec.pair = 0;
+      loss = q.loss * w * mean;
       if (tid == 0) {
         a.logprobs[row] = o.lp;
         if (a.entropy) a.entropy[row] = o.H;
@@ -1045,18 +1089,28 @@ __global__ __launch_bounds__(T, 4) void loss_rows_kernel(LossParams p) {
       p.row_loss[row] = loss;
       if (p.records) p.records[row] = rec;
     }
-    if (want && load) {
-      const float gH = ENT ? rec.cH : 0.f;
-      if (!(rec.c == 0.f && gH == 0.f)) store = kGradient;
-      cur_M = rec.M;
-      rest = rest_gradient(rec, rec.c, gH);
-      at_token = token_gradient(rec, rec.c, gH);
-    }
+    const float gH = ENT ? rec.cH : 0.f;
+    zeros = rec.c == 0.f && gH == 0.f;
+    cur_M = rec.M;
+    rest = rest_gradient(rec, rec.c, gH);
+    at_token = token_gradient(rec, rec.c, gH);
     cur = row;
     cur_x = x;
     cur_token = token;
-    row += step;
+    row = next;
+  };
+
+  announce(row);
+  if (!advance()) return;
+  for (;;) {
+    turn();
+    if (!more) break;
+    finish();
+    more = advance();
+    if (!WANT && !more) return;
   }
+  __syncthreads();
+  give();
 }
 
 // ------------------------------------------------------------------ host ------------------------
@@ -1086,10 +1140,38 @@ int num_cus() {
   return n;
 }
 
-// Threads of a workgroup of loss_rows_kernel: the fewest whose registers hold a row of V columns.
-int row_threads(int64_t V, int dtype) {
-  const int64_t each = (dtype == MVSD_F32 ? 4 : 8) * (kHeld + 1);
-  return V <= 256 * each ? 256 : V <= 512 * each ? 512 : 1024;
+// How loss_rows_kernel holds a row of V columns: NV vectors in each of `active` threads.
+struct RowPlan {
+  int held, active, threads;
+};
+RowPlan row_plan(const mvsd_loss_args& a) {
+  const int64_t vectors = a.vocab_size / (a.dtype == MVSD_F32 ? 4 : 8);
+  RowPlan best = {0, 0, 0};
+  int most = 0;
+  for (int held : {18, 16, 13, 10, 6, 3}) {
+    if (held < kMostHeld && vectors / held > kRowThreads) break;  // columns would be read again
+    RowPlan r;
+    r.held = held;
+    r.active = (int)std::min(vectors / held, (int64_t)kRowThreads) / 8 * 8;
+    r.threads = (r.active + kWave - 1) / kWave * kWave;
+    if (has_list(a)) r.threads = std::max(r.threads, (int)(a.num_teacher + kWave - 1) / kWave * kWave);  // an entry each
+    // the active threads of a CU, whose registers hold 1024
+    const int busy = r.active == 0 ? 0 : kRowThreads / r.threads * r.active;
+    if (busy > most) best = r, most = busy;
+  }
+  return best;
+}
+
+// Its workgroups: as many as run at once.
+int64_t row_groups(const mvsd_loss_args& a, const RowPlan& plan) {
+  return std::min(a.num_rows, (int64_t)num_cus() * (kRowThreads / plan.threads));
+}
+
+// What its first turns store.
+int64_t aside_bytes(const mvsd_loss_args& a) {
+  if (!loss_one_pass(a)) return 0;
+  const RowPlan plan = row_plan(a);
+  return row_groups(a, plan) * plan.active * 16;
 }
 
 constexpr int64_t kMaxMarked = 1 << 18;  // columns whose marks are 32 KiB
@@ -1106,10 +1188,14 @@ LossParams make_params(const mvsd_loss_args& a) {
   p.entropy = (a.kind == MVSD_LOSS_LOGPROBS || a.kind == MVSD_LOSS_POLICY) && (a.entropy || a.entropy_coef != 0.0);
   const int64_t N = a.num_rows;
   char* w = static_cast<char*>(a.workspace);
+  p.aside = w;
+  w += aside_bytes(a);
   p.parts = reinterpret_cast<float4*>(w);
   w += N * p.nch * sizeof(float4);
   p.norm = reinterpret_cast<float*>(w);
   w += kNormParts * sizeof(float);
+  p.tickets = reinterpret_cast<int*>(w);
+  w += 16;
   p.row_loss = a.reduction == MVSD_REDUCE_NONE && a.loss ? a.loss : reinterpret_cast<float*>(w);
   w += up16(std::max(N, a.num_pairs) * 4);
   p.row_lp = reinterpret_cast<float*>(w);
@@ -1124,20 +1210,29 @@ LossParams make_params(const mvsd_loss_args& a) {
   // the distillation's kernel has a wave a row where there are few
   if (a.kind == MVSD_LOSS_DISTILL)
     p.norm_parts = (int)std::min((N + kWaves - 1) / kWaves, (int64_t)kNormParts);
-  else if (a.kind == MVSD_LOSS_POLICY && a.reduction == MVSD_REDUCE_MEAN)
+  else if (a.kind == MVSD_LOSS_POLICY && (a.reduction == MVSD_REDUCE_MEAN || loss_one_pass(a)))
     p.norm_parts = (int)std::min(N / 64 + 1, (int64_t)kNormParts);
   return p;
 }
 
-template <int DT, int T>
-void launch_rows(const LossParams& p, hipStream_t stream) {
-  const dim3 grid((unsigned)std::min(p.a.num_rows, (int64_t)num_cus() * (1024 / T))), block(T);
+template <int DT, int NV, bool WANT>
+void launch_rows_of(const LossParams& p, const RowPlan& plan, hipStream_t stream) {
+  const dim3 grid((unsigned)row_groups(p.a, plan));
+  const dim3 block(plan.threads);
   if (has_list(p.a))
-    hipLaunchKernelGGL((loss_rows_kernel<DT, T, true, false>), grid, block, (unsigned)((p.V + 31) / 32 * 4), stream, p);
+    hipLaunchKernelGGL((loss_rows_kernel<DT, NV, true, false, WANT>), grid, block, (unsigned)((p.V + 31) / 32 * 4), stream, p);
   else if (p.entropy)
-    hipLaunchKernelGGL((loss_rows_kernel<DT, T, false, true>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((loss_rows_kernel<DT, NV, false, true, WANT>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((loss_rows_kernel<DT, T, false, false>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((loss_rows_kernel<DT, NV, false, false, WANT>), grid, block, 0, stream, p);
+}
+
+template <int DT, int NV>
+void launch_rows(const LossParams& p, const RowPlan& plan, hipStream_t stream) {
+  if (p.a.grad)
+    launch_rows_of<DT, NV, true>(p, plan, stream);
+  else
+    launch_rows_of<DT, NV, false>(p, plan, stream);
 }
 
 template <int DT>
@@ -1151,10 +1246,16 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
       hipLaunchKernelGGL(loss_norm_kernel, dim3(p.norm_parts), block, 0, stream, p);
   }
   if (loss_one_pass(a)) {
-    switch (row_threads(p.V, DT)) {
-      case 256: launch_rows<DT, 256>(p, stream); break;
-      case 512: launch_rows<DT, 512>(p, stream); break;
-      default: launch_rows<DT, 1024>(p, stream); break;
+    const RowPlan plan = row_plan(a);
+    LossParams q = p;
+    q.active = plan.active;
+    switch (plan.held) {
+      case 3: launch_rows<DT, 3>(q, plan, stream); break;
+      case 6: launch_rows<DT, 6>(q, plan, stream); break;
+      case 10: launch_rows<DT, 10>(q, plan, stream); break;
+      case 13: launch_rows<DT, 13>(q, plan, stream); break;
+      case 16: launch_rows<DT, 16>(q, plan, stream); break;
+      default: launch_rows<DT, kMostHeld>(q, plan, stream); break;
     }
     return hipGetLastError();
   }
@@ -1176,7 +1277,9 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
 template <int DT>
 hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, const float* up_h, int64_t uhs,
                               hipStream_t stream) {
-  const dim3 grid((unsigned)(p.a.num_rows * p.nch)), block(kLossThreads);
+  // mostly the gradient is there where a value of 1 is expected: few workgroups look for it
+  const int64_t chunks = p.a.num_rows * p.nch;
+  const dim3 grid((unsigned)(p.a.unit_gradient ? std::min(chunks, (int64_t)num_cus() * 4) : chunks)), block(kLossThreads);
   if (has_list(p.a))
     hipLaunchKernelGGL((loss_gradient_kernel<DT, true, false>), grid, block, 0, stream, p, up, us, up_h, uhs);
   else if (p.entropy)
@@ -1190,14 +1293,14 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
 
 bool loss_one_pass(const mvsd_loss_args& a) {
   if ((a.kind != MVSD_LOSS_DISTILL && a.kind != MVSD_LOSS_POLICY) || a.reduction == MVSD_REDUCE_NONE) return false;
-  if (a.vocab_size < 8 || (has_list(a) && a.vocab_size > kMaxMarked)) return false;
-  return a.num_rows >= 128 * (1024 / row_threads(a.vocab_size, a.dtype));
+  if (a.vocab_size < 256 || (has_list(a) && a.vocab_size > kMaxMarked)) return false;
+  return a.num_rows >= 128 * (kRowThreads / row_plan(a).threads);
 }
 
 int64_t loss_workspace_bytes(const mvsd_loss_args& a) {
   const int64_t chunk = chunk_of(a.num_rows, (int)a.vocab_size, a.dtype);
   const int64_t nch = (a.vocab_size + chunk - 1) / chunk;
-  return a.num_rows * nch * (int64_t)sizeof(float4) + kNormParts * 4 +
+  return aside_bytes(a) + a.num_rows * nch * (int64_t)sizeof(float4) + kNormParts * 4 + 16 +
          up16(std::max(a.num_rows, a.num_pairs) * 4) + up16(a.num_rows * 8) +
          (has_list(a) ? a.num_rows * a.num_teacher * 4 : 0);
 }
