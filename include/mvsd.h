@@ -824,6 +824,8 @@ typedef struct mvsd_loss_args {
   void* workspace;
   int64_t workspace_bytes;
   int64_t unit_gradient;
+  int64_t saved_bytes; /* given by mvsd_loss_plan, as the next */
+  int64_t one_pass;
 } mvsd_loss_args;
 
 int64_t mvsd_loss_saved_bytes(const mvsd_loss_args* args);
@@ -832,6 +834,8 @@ int64_t mvsd_loss_workspace_bytes(const mvsd_loss_args* args);
 /* (if that is not NULL) for an upstream of 1, which mvsd_loss_gradient with unit_gradient       */
 /* leaves as it is if that is what the upstream holds.                                          */
 int mvsd_loss_one_pass(const mvsd_loss_args* args);
+/* All three at once, into args' workspace_bytes, saved_bytes and one_pass. */
+int mvsd_loss_plan(mvsd_loss_args* args);
 int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
 
 /* ------------------------------------------------------------------------------------ */

@@ -106,72 +106,76 @@ __device__ inline unsigned marks_at(const uint32_t* bits, unsigned col, int n) {
   return (bits[col >> 5] >> (col & 31)) & ((1u << n) - 1u);
 }
 
-// One workgroup a chunk of a row: statistics of its rest.
-template <int DT, bool LIST, bool ENT>
-__global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) {
-  constexpr int VEC = Elem<DT>::kVec, U = 4;
-  extern __shared__ uint32_t bits[];
-  __shared__ Stat s_stat[kWaves];
-  const int64_t row = blockIdx.x / p.nch;
-  const int part = blockIdx.x - (int)(row * p.nch);
-  const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
-  int token = -1;
-  if constexpr (LIST) {
-    if (p.teach[row].y == 0.f) return;
-    for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
-    __syncthreads();
-    for (int k = threadIdx.x; k < p.K; k += kLossThreads) {
-      const int id = p.over_ids[row * p.K + k];
-      if (id >= begin && id < end) atomicOr(&bits[(id - begin) >> 5], 1u << ((id - begin) & 31));
-    }
-    __syncthreads();
+// The elements of `marks` become -inf.
+template <int DT>
+__device__ inline void mask_vec(u32x4& r, unsigned marks) {
+  if constexpr (DT == MVSD_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = marks >> e & 1 ? 0xff800000u : r[e];
   } else {
-    token = token_at(p.a, row, p.V);
-    if (token < 0 || row_weight(p.a, row) == 0.f) return;
-  }
-  const auto* x = logits_row<DT>(p.a, row);
-  Stat st = {-INFINITY, 0.f, 0.f};
-  for (int col = begin + (int)threadIdx.x * VEC; col < end; col += kLossThreads * VEC * U) {
-    float v[U][VEC];
-    float m = st.m;
+    constexpr uint32_t ninf = DT == MVSD_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_filled<DT>(x, col + u * kLossThreads * VEC, end, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = col + u * kLossThreads * VEC;
-      if constexpr (LIST) {
-        const unsigned marks = at < end ? marks_at(bits, at - begin, VEC) : 0;
-        if (marks)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) v[u][e] = marks >> e & 1 ? -INFINITY : v[u][e];
-      } else if (token >= at && token < at + VEC) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[u][e] = token == at + e ? -INFINITY : v[u][e];
-      }
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) m = fmaxf(m, v[u][e]);
+    for (int w = 0; w < 4; ++w) {
+      r[w] = marks >> (2 * w) & 1 ? (r[w] & 0xffff0000u) | ninf : r[w];
+      r[w] = marks >> (2 * w + 1) & 1 ? (r[w] & 0x0000ffffu) | ninf << 16 : r[w];
     }
-    const float base = base_of(m);
-    const float d = fmaxf((st.m - base) * p.c1, kLeast), f = __builtin_amdgcn_exp2f(d);
-    if constexpr (ENT) st.t = (st.t + st.s * d) * f;
-    st.s *= f;
-    st.m = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float y = (v[u][e] - base) * p.c1, w = __builtin_amdgcn_exp2f(y);
-        st.s += w;
-        if constexpr (ENT) st.t += w * fmaxf(y, kLeast);
-      }
   }
-  st = wave_join(st, p.c1);
-  if (lane_id() == 0) s_stat[wave_id()] = st;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    st = join(join(s_stat[0], s_stat[1], p.c1), join(s_stat[2], s_stat[3], p.c1), p.c1);
-    p.parts[blockIdx.x] = make_float4(st.m, st.s, st.t, 0.f);
+}
+
+// vec_elem, by instructions of its own: the compiler would keep what the statistics converted until the
+// gradient converts it again, and a row would take twice the registers.
+template <int DT>
+__device__ inline float vec_elem_again(const u32x4& r, int j) {
+  if constexpr (DT == MVSD_F32) {
+    return __uint_as_float(r[j]);
+  } else {
+    float v;
+    const uint32_t w = r[j / 2];
+    if (DT == MVSD_BF16 && j % 2 == 0)
+      asm("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(w));
+    else if (DT == MVSD_BF16)
+      asm("v_and_b32 %0, 0xffff0000, %1" : "=v"(v) : "v"(w));
+    else if (j % 2 == 0)
+      asm("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(w));
+    else
+      asm("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v) : "v"(w));
+    return v;
   }
+}
+
+// Adds values to a thread's statistics.
+template <bool ENT, int N>
+__device__ inline void add_values(Stat& st, const float (&v)[N], float c1) {
+  float m = st.m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
+  const float base = base_of(m);
+  const float d = fmaxf((st.m - base) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
+  if constexpr (ENT) st.t = fmaf(st.s, d, st.t) * f;
+  st.s *= f;
+  st.m = m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float y = (v[e] - base) * c1, w = __builtin_amdgcn_exp2f(y);
+    st.s += w;
+    if constexpr (ENT) st.t = fmaf(w, fmaxf(y, kLeast), st.t);
+  }
+}
+template <int DT, bool ENT, int N>
+__device__ inline void add_vecs(Stat& st, const u32x4 (&r)[N], float c1) {
+  constexpr int VEC = Elem<DT>::kVec;
+  float v[N * VEC];
+#pragma unroll
+  for (int i = 0; i < N * VEC; ++i) v[i] = vec_elem<DT>(r[i / VEC], i % VEC);
+  add_values<ENT, N * VEC>(st, v, c1);
+}
+
+// Both sums against a new maximum.
+__device__ inline void rebase(Stat& st, float m, float c1) {
+  const float d = fmaxf((st.m - base_of(m)) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
+  st.t = fmaf(st.s, d, st.t) * f;
+  st.s *= f;
+  st.m = m;
 }
 
 // ------------------------------------------------------------------ the mean's divisor ----------
@@ -269,36 +273,26 @@ __device__ inline PolicyRow policy_row(const mvsd_loss_args& a, const PolicyIn& 
   return o;
 }
 
-// A wave a row: the chunks' statistics together, then the row's loss.
+// The row's values and its record, by a wave, from the statistics of its rest; `out`: it is left out.
 template <int DT>
-__global__ __launch_bounds__(kLossThreads) void loss_token_rows_kernel(LossParams p) {
-  const int64_t row = (int64_t)blockIdx.x * kWaves + wave_id();
-  if (row >= p.a.num_rows) return;
+__device__ inline void finish_token_row(const LossParams& p, int64_t row, int token, bool out, Stat st) {
   const mvsd_loss_args& a = p.a;
-  const float mean = mean_factor(p);
-  const int token = token_at(a, row, p.V);
-  const float w = row_weight(a, row);
-  const bool out = token < 0 || w == 0.f;
   TokenRow r;
   PolicyRow o = {0.f, 0.f, 0.f};
+  float w = 0.f;
   r.lp = r.H = 0.f;
   r.rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
   if (!out) {
     const float x = token < p.V ? Elem<DT>::cvt(logits_row<DT>(a, row)[token]) : NAN;
-    Stat st = {-INFINITY, 0.f, 0.f};
-    for (int i = lane_id(); i < p.nch; i += kWave) {
-      const float4 v = p.parts[row * p.nch + i];
-      st = join(st, {v.x, v.y, v.z}, p.c1);
-    }
-    st = wave_join(st, p.c1);
     r = token_row(p, st, x);
     r.rec.pair = 0;
     r.rec.c = 1.f;
     r.rec.cH = 1.f;
     if (a.kind == MVSD_LOSS_POLICY) {
       o = policy_row(a, policy_in(a, row), r.lp, r.H);
-      r.rec.c = o.c * w * mean;
-      r.rec.cH = -(float)a.entropy_coef * w * mean;
+      w = row_weight(a, row) * mean_factor(p);
+      r.rec.c = o.c * w;
+      r.rec.cH = -(float)a.entropy_coef * w;
     } else if (a.kind == MVSD_LOSS_PREFERENCE) {
       r.rec.c = r.rec.cH = 0.f;  // its sequence's, once that is known
     }
@@ -311,10 +305,114 @@ __global__ __launch_bounds__(kLossThreads) void loss_token_rows_kernel(LossParam
     if (a.entropy) a.entropy[row] = r.H;
   }
   if (a.kind == MVSD_LOSS_POLICY) {
-    p.row_loss[row] = out ? 0.f : o.loss * w * mean;
+    p.row_loss[row] = out ? 0.f : o.loss * w;
     if (a.kl) a.kl[row] = o.kl;
   }
   if (p.records) p.records[row] = r.rec;
+}
+
+// A wave a row: the chunks' statistics together, then the row's loss.
+template <int DT>
+__global__ __launch_bounds__(kLossThreads) void loss_token_rows_kernel(LossParams p) {
+  const int64_t row = (int64_t)blockIdx.x * kWaves + wave_id();
+  if (row >= p.a.num_rows) return;
+  const int token = token_at(p.a, row, p.V);
+  const bool out = token < 0 || row_weight(p.a, row) == 0.f;
+  Stat st = {-INFINITY, 0.f, 0.f};
+  if (!out) {
+    for (int i = lane_id(); i < p.nch; i += kWave) {
+      const float4 v = p.parts[row * p.nch + i];
+      st = join(st, {v.x, v.y, v.z}, p.c1);
+    }
+    st = wave_join(st, p.c1);
+  }
+  finish_token_row<DT>(p, row, token, out, st);
+}
+
+// One workgroup a chunk of a row: statistics of its rest.  Blocks of kBlock vectors a thread, the next one's
+// loads in flight while one is added.  A row of one chunk (of token rows) is finished on the spot.
+template <int DT, bool LIST, bool ENT>
+__global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) {
+  constexpr int VEC = Elem<DT>::kVec, kBlock = 4, kStep = kLossThreads * VEC;
+  extern __shared__ uint32_t bits[];
+  __shared__ Stat s_stat[kWaves];
+  const int64_t row = blockIdx.x / p.nch;
+  const int part = blockIdx.x - (int)(row * p.nch);
+  const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
+  const bool whole = !LIST && p.nch == 1;
+  int token = -1;
+  if constexpr (LIST) {
+    if (p.teach[row].y == 0.f) return;
+    for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < p.K; k += kLossThreads) {
+      const int id = p.over_ids[row * p.K + k];
+      if (id >= begin && id < end) atomicOr(&bits[(id - begin) >> 5], 1u << ((id - begin) & 31));
+    }
+    __syncthreads();
+  } else {
+    token = token_at(p.a, row, p.V);
+    if (token < 0 || row_weight(p.a, row) == 0.f) {
+      if (whole && wave_id() == 0) finish_token_row<DT>(p, row, token, true, {-INFINITY, 0.f, 0.f});
+      return;
+    }
+  }
+  const auto* x = logits_row<DT>(p.a, row);
+  Stat st = {-INFINITY, 0.f, 0.f};
+  const int mine = begin + (int)threadIdx.x * VEC;
+  const int blocks = (end - begin) / (kStep * kBlock);
+  auto load = [&](u32x4 (&v)[kBlock], int block) {
+#pragma unroll
+    for (int u = 0; u < kBlock; ++u) v[u] = load_vec_any<DT>(x + mine + (block * kBlock + u) * kStep);
+  };
+  auto add = [&](u32x4 (&v)[kBlock], int block) {
+#pragma unroll
+    for (int u = 0; u < kBlock; ++u) {
+      const int col = mine + (block * kBlock + u) * kStep;
+      if constexpr (LIST) {
+        const unsigned marks = marks_at(bits, col - begin, VEC);
+        if (marks) mask_vec<DT>(v[u], marks);
+      } else if (token >= col && token < col + VEC) {
+        mask_vec<DT>(v[u], 1u << (token - col));
+      }
+    }
+    add_vecs<DT, ENT, kBlock>(st, v, p.c1);
+  };
+  if (blocks > 0) {
+    u32x4 a[kBlock], b[kBlock];
+    load(a, 0);
+    int k = 0;
+    for (; k + 2 < blocks; k += 2) {
+      load(b, k + 1);
+      add(a, k);
+      load(a, k + 2);
+      add(b, k + 1);
+    }
+    if (k + 1 < blocks) {
+      load(b, k + 1);
+      add(a, k);
+      add(b, k + 1);
+    } else {
+      add(a, k);
+    }
+  }
+  for (int col = mine + blocks * kBlock * kStep; col < end; col += kStep) {
+    float v[VEC];
+    load_filled<DT>(x, col, end, v);
+    const unsigned marks = LIST ? marks_at(bits, col - begin, VEC) : 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (LIST ? marks >> e & 1 : token == col + e) ? -INFINITY : v[e];
+    add_values<ENT, VEC>(st, v, p.c1);
+  }
+  st = wave_join(st, p.c1);
+  if (lane_id() == 0) s_stat[wave_id()] = st;
+  __syncthreads();
+  if (wave_id() != 0) return;
+  st = join(join(s_stat[0], s_stat[1], p.c1), join(s_stat[2], s_stat[3], p.c1), p.c1);
+  if (whole)
+    finish_token_row<DT>(p, row, token, false, st);
+  else if (lane_id() == 0)
+    p.parts[blockIdx.x] = make_float4(st.m, st.s, st.t, 0.f);
 }
 
 // A workgroup a pair: the sums over its two sequences, its loss, its rows' factors.
@@ -698,12 +796,16 @@ __device__ inline typename Elem<DT>::storage to_storage(float g) {
   else return __builtin_bit_cast(uint16_t, (__bf16)g);
 }
 
-template <int DT>
+// PAST: past the caches.
+template <int DT, bool PAST = false>
 __device__ inline void store_filled(typename Elem<DT>::storage* row, int col, int end,
                                     const float (&g)[Elem<DT>::kVec]) {
   constexpr int VEC = Elem<DT>::kVec;
   if (col + VEC <= end) {
-    *reinterpret_cast<Vec16<DT>*>(row + col) = pack_vec<DT>(g);
+    if constexpr (PAST)
+      __builtin_nontemporal_store(pack_vec<DT>(g), reinterpret_cast<Vec16<DT>*>(row + col));
+    else
+      *reinterpret_cast<Vec16<DT>*>(row + col) = pack_vec<DT>(g);
   } else {
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
@@ -712,12 +814,12 @@ __device__ inline void store_filled(typename Elem<DT>::storage* row, int col, in
 }
 
 // A chunk of a row by a workgroup, from the row's record.
-template <int DT, bool LIST, bool ENT>
+template <int DT, bool LIST, bool ENT, bool PAST>
 __device__ inline void gradient_chunk(const LossParams& p, const float* up, int64_t us, const float* up_h,
                                       int64_t uhs, int64_t chunk) {
   constexpr int VEC = Elem<DT>::kVec;
-  const int64_t row = chunk / p.nch;
-  const int part = chunk - row * p.nch;
+  const int64_t at = chunk / p.nch, row = p.a.num_rows - 1 - at;
+  const int part = chunk - at * p.nch;
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
   const LossRecord rec = p.records[row];
   const int64_t n = p.a.kind == MVSD_LOSS_PREFERENCE ? rec.pair : row;
@@ -727,7 +829,7 @@ __device__ inline void gradient_chunk(const LossParams& p, const float* up, int6
   if (g == 0.f && gH == 0.f) {
     const float zero[VEC] = {};
     for (int col = begin + (int)threadIdx.x * VEC; col < end; col += kLossThreads * VEC)
-      store_filled<DT>(out, col, end, zero);
+      store_filled<DT, PAST>(out, col, end, zero);
     return;
   }
   const auto* x = logits_row<DT>(p.a, row);
@@ -745,7 +847,7 @@ __device__ inline void gradient_chunk(const LossParams& p, const float* up, int6
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[e] = token == col + e ? at_token : v[e];
     }
-    store_filled<DT>(out, col, end, v);
+    store_filled<DT, PAST>(out, col, end, v);
   }
   if constexpr (LIST) {
     __syncthreads();
@@ -756,90 +858,20 @@ __device__ inline void gradient_chunk(const LossParams& p, const float* up, int6
   }
 }
 
-template <int DT, bool LIST, bool ENT>
+// The last rows first: the statistics were read in the rows' order, so that the last of them are still in
+// the caches, where a gradient that is larger than those (PAST) leaves them by being stored past them.
+template <int DT, bool LIST, bool ENT, bool PAST>
 __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams p, const float* up, int64_t us,
                                                                      const float* up_h, int64_t uhs) {
   if (p.a.unit_gradient && up[0] == 1.f) return;  // it is there already
   for (int64_t chunk = blockIdx.x; chunk < p.a.num_rows * p.nch; chunk += gridDim.x)
-    gradient_chunk<DT, LIST, ENT>(p, up, us, up_h, uhs, chunk);
+    gradient_chunk<DT, LIST, ENT, PAST>(p, up, us, up_h, uhs, chunk);
 }
 
 // ------------------------------------------------------------------ values and gradient in one pass ---
 
 constexpr int kMostHeld = 18;  // vectors of a row in each thread's registers (72 of 128)
 constexpr int kRowThreads = 1024;
-
-// The elements of `marks` become -inf.
-template <int DT>
-__device__ inline void mask_vec(u32x4& r, unsigned marks) {
-  if constexpr (DT == MVSD_F32) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = marks >> e & 1 ? 0xff800000u : r[e];
-  } else {
-    constexpr uint32_t ninf = DT == MVSD_BF16 ? 0xff80u : 0xfc00u;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      r[w] = marks >> (2 * w) & 1 ? (r[w] & 0xffff0000u) | ninf : r[w];
-      r[w] = marks >> (2 * w + 1) & 1 ? (r[w] & 0x0000ffffu) | ninf << 16 : r[w];
-    }
-  }
-}
-
-// vec_elem, by instructions of its own: the compiler would keep what the statistics converted until the
-// gradient converts it again, and a row would take twice the registers.
-template <int DT>
-__device__ inline float vec_elem_again(const u32x4& r, int j) {
-  if constexpr (DT == MVSD_F32) {
-    return __uint_as_float(r[j]);
-  } else {
-    float v;
-    const uint32_t w = r[j / 2];
-    if (DT == MVSD_BF16 && j % 2 == 0)
-      asm("v_lshlrev_b32 %0, 16, %1" : "=v"(v) : "v"(w));
-    else if (DT == MVSD_BF16)
-      asm("v_and_b32 %0, 0xffff0000, %1" : "=v"(v) : "v"(w));
-    else if (j % 2 == 0)
-      asm("v_cvt_f32_f16 %0, %1" : "=v"(v) : "v"(w));
-    else
-      asm("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v) : "v"(w));
-    return v;
-  }
-}
-
-// Adds values to a thread's statistics.
-template <bool ENT, int N>
-__device__ inline void add_values(Stat& st, const float (&v)[N], float c1) {
-  float m = st.m;
-#pragma unroll
-  for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
-  const float base = base_of(m);
-  const float d = fmaxf((st.m - base) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
-  if constexpr (ENT) st.t = fmaf(st.s, d, st.t) * f;
-  st.s *= f;
-  st.m = m;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float y = (v[e] - base) * c1, w = __builtin_amdgcn_exp2f(y);
-    st.s += w;
-    if constexpr (ENT) st.t = fmaf(w, fmaxf(y, kLeast), st.t);
-  }
-}
-template <int DT, bool ENT, int N>
-__device__ inline void add_vecs(Stat& st, const u32x4 (&r)[N], float c1) {
-  constexpr int VEC = Elem<DT>::kVec;
-  float v[N * VEC];
-#pragma unroll
-  for (int i = 0; i < N * VEC; ++i) v[i] = vec_elem<DT>(r[i / VEC], i % VEC);
-  add_values<ENT, N * VEC>(st, v, c1);
-}
-
-// Both sums against a new maximum.
-__device__ inline void rebase(Stat& st, float m, float c1) {
-  const float d = fmaxf((st.m - base_of(m)) * c1, kLeast), f = __builtin_amdgcn_exp2f(d);
-  st.t = fmaf(st.s, d, st.t) * f;
-  st.s *= f;
-  st.m = m;
-}
 
 // Rows by a workgroup, one after the other (by tickets: some are left out), every row in its registers: read once, written once.  A turn of the
 // loop writes the gradient of one row and, vector by vector, loads the next one in its place and adds it to
@@ -1176,6 +1208,8 @@ int64_t aside_bytes(const mvsd_loss_args& a) {
 
 constexpr int64_t kMaxMarked = 1 << 18;  // columns whose marks are 32 KiB
 
+constexpr int64_t kCacheBytes = 256ll << 20;  // of the last level
+
 LossParams make_params(const mvsd_loss_args& a) {
   LossParams p = {};
   p.a = a;
@@ -1268,7 +1302,8 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
       hipLaunchKernelGGL((loss_stats_kernel<DT, false, true>), grid, block, 0, stream, p);
     else
       hipLaunchKernelGGL((loss_stats_kernel<DT, false, false>), grid, block, 0, stream, p);
-    hipLaunchKernelGGL(loss_token_rows_kernel<DT>, dim3((unsigned)((a.num_rows + kWaves - 1) / kWaves)), block, 0,
+    if (p.nch > 1)
+      hipLaunchKernelGGL(loss_token_rows_kernel<DT>, dim3((unsigned)((a.num_rows + kWaves - 1) / kWaves)), block, 0,
                        stream, p);
   }
   return hipGetLastError();
@@ -1280,12 +1315,14 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
   // mostly the gradient is there where a value of 1 is expected: few workgroups look for it
   const int64_t chunks = p.a.num_rows * p.nch;
   const dim3 grid((unsigned)(p.a.unit_gradient ? std::min(chunks, (int64_t)num_cus() * 4) : chunks)), block(kLossThreads);
+  const bool past = p.a.num_rows * p.V * (DT == MVSD_F32 ? 4 : 2) > kCacheBytes;
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, up, us, up_h, uhs); };
   if (has_list(p.a))
-    hipLaunchKernelGGL((loss_gradient_kernel<DT, true, false>), grid, block, 0, stream, p, up, us, up_h, uhs);
+    past ? launch(loss_gradient_kernel<DT, true, false, true>) : launch(loss_gradient_kernel<DT, true, false, false>);
   else if (p.entropy)
-    hipLaunchKernelGGL((loss_gradient_kernel<DT, false, true>), grid, block, 0, stream, p, up, us, up_h, uhs);
+    past ? launch(loss_gradient_kernel<DT, false, true, true>) : launch(loss_gradient_kernel<DT, false, true, false>);
   else
-    hipLaunchKernelGGL((loss_gradient_kernel<DT, false, false>), grid, block, 0, stream, p, up, us, up_h, uhs);
+    past ? launch(loss_gradient_kernel<DT, false, false, true>) : launch(loss_gradient_kernel<DT, false, false, false>);
   return hipGetLastError();
 }
 
@@ -1409,6 +1446,15 @@ int64_t mvsd_loss_workspace_bytes(const mvsd_loss_args* args) {
 int mvsd_loss_one_pass(const mvsd_loss_args* args) {
   const int status = check_sizes(args);
   return status != MVSD_OK ? status : mvsd::loss_one_pass(*args) ? 1 : 0;
+}
+
+int mvsd_loss_plan(mvsd_loss_args* args) {
+  const int status = check_sizes(args);
+  if (status != MVSD_OK) return status;
+  args->workspace_bytes = mvsd::loss_workspace_bytes(*args);
+  args->saved_bytes = mvsd::loss_saved_bytes(*args);
+  args->one_pass = mvsd::loss_one_pass(*args) ? 1 : 0;
+  return MVSD_OK;
 }
 
 int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream) {

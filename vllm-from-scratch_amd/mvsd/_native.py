@@ -185,6 +185,8 @@ class LossArgs(ctypes.Structure):
         ("workspace", c_void_p),
         ("workspace_bytes", c_int64),
         ("unit_gradient", c_int64),
+        ("saved_bytes", c_int64),
+        ("one_pass", c_int64),
     ]
 
 
@@ -289,6 +291,7 @@ SIGNATURES = {
     "mvsd_loss_saved_bytes": (c_int64, [ctypes.POINTER(LossArgs)]),
     "mvsd_loss_workspace_bytes": (c_int64, [ctypes.POINTER(LossArgs)]),
     "mvsd_loss_one_pass": (c_int, [ctypes.POINTER(LossArgs)]),
+    "mvsd_loss_plan": (c_int, [ctypes.POINTER(LossArgs)]),
     "mvsd_row_loss": (c_int, [ctypes.POINTER(LossArgs), c_void_p]),
     "mvsd_loss_gradient": (c_int, [ctypes.POINTER(LossArgs), c_void_p, c_int64, c_void_p, c_int64,
                                    c_void_p]),

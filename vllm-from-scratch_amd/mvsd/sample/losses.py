@@ -86,18 +86,18 @@ def _check_device(t: torch.Tensor, name: str, device: torch.device) -> None:
 
 
 def _check_ids(ids: torch.Tensor, name: str, shape, device) -> torch.Tensor:
+    if ids.dtype in _ID_DTYPES and ids.shape == shape and ids.device == device:
+        return ids if ids.is_contiguous() else ids.contiguous()
     _check_device(ids, name, device)
     if ids.dtype not in _ID_DTYPES:
         raise TypeError(f"{name} is {ids.dtype}, int32 or int64 expected")
-    if ids.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(ids.shape)}, {tuple(shape)} expected")
-    return ids.contiguous()
+    raise ValueError(f"{name} has shape {tuple(ids.shape)}, {tuple(shape)} expected")
 
 
-def _values(t: torch.Tensor | None, name: str, shape, device) -> torch.Tensor | None:
+def _values(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
     """An fp32 value for every place of `shape`."""
-    if t is None:
-        return None
+    if t.dtype is torch.float32 and t.shape == shape and t.device == device and t.is_contiguous():
+        return t
     _check_device(t, name, device)
     if t.dtype != torch.float32:
         raise TypeError(f"{name} is {t.dtype}, torch.float32 expected")
@@ -107,12 +107,6 @@ def _values(t: torch.Tensor | None, name: str, shape, device) -> torch.Tensor | 
         except RuntimeError:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, {tuple(shape)} expected") from None
     return t.detach().contiguous()
-
-
-def _weights(t: torch.Tensor | None, shape, device) -> torch.Tensor | None:
-    if t is not None and t.dtype == torch.bool:
-        t = t.to(torch.float32)
-    return _values(t, "weights", shape, device)
 
 
 class _Call:
@@ -130,35 +124,39 @@ class _Call:
         if not 1e-6 <= temperature <= 1e6:
             raise ValueError(f"temperature={temperature}")
         self.kind, self.logits, self.device = kind, logits, logits.device
-        self.keep, self.outputs, self.saved, self.grad = [], (), None, None
+        self.keep, self.saved, self.grad = [], None, None
         a = self.args = nat.LossArgs()
         a.kind, a.reduction, a.temperature = kind, reduction, temperature
         self._rows(logits)
 
     def _rows(self, logits: torch.Tensor) -> None:
-        a = self.args
-        if logits.stride(-1) != 1 and logits.shape[-1] > 1:
+        a, shape, strides = self.args, logits.shape, logits.stride()
+        if strides[-1] != 1 and shape[-1] > 1:
             raise ValueError("logits need rows with unit stride")
         a.dtype = nat.dtype_code(logits.dtype)
-        a.logits, a.vocab_size = logits.data_ptr(), logits.shape[-1]
-        a.stride = logits.stride(-2)
-        if logits.ndim == 3:
-            a.num_rows = logits.shape[0] * logits.shape[1]
-            a.inner_rows, a.outer_stride = max(logits.shape[1], 1), logits.stride(0)
+        a.logits, a.vocab_size, a.stride = logits.data_ptr(), shape[-1], strides[-2]
+        if len(shape) == 3:
+            a.num_rows = shape[0] * shape[1]
+            a.inner_rows, a.outer_stride = max(shape[1], 1), strides[0]
         else:
-            a.num_rows = logits.shape[0]
-            a.inner_rows, a.outer_stride = max(a.num_rows, 1), 0
+            a.num_rows = shape[0]
+            a.inner_rows, a.outer_stride = max(shape[0], 1), 0
 
     def take_ids(self, ids: torch.Tensor) -> None:
         self.ids = ids
         self.args.token_ids, self.args.ids_dtype = ids.data_ptr(), nat.dtype_code(ids.dtype)
 
-    def take(self, name: str, t: torch.Tensor | None) -> None:
+    def take(self, name: str, t: torch.Tensor | None, shape) -> None:
         if t is not None:
+            t = _values(t, name, shape, self.device)
             self.keep.append(t)
             setattr(self.args, name, t.data_ptr())
 
-    def empty(self, name: str, *shape) -> torch.Tensor:
+    def take_weights(self, t: torch.Tensor | None, shape) -> None:
+        if t is not None:
+            self.take("weights", t.to(torch.float32) if t.dtype is torch.bool else t, shape)
+
+    def empty(self, name: str, shape) -> torch.Tensor:
         out = torch.empty(shape, dtype=torch.float32, device=self.device)
         setattr(self.args, name, out.data_ptr())
         return out
@@ -166,20 +164,22 @@ class _Call:
     def run(self, train: bool) -> None:
         """Enqueue the values, and what the gradient needs of them."""
         a, handle = self.args, nat.lib()
-        size = handle.mvsd_loss_workspace_bytes(ctypes.byref(a))
-        if size < 0:
+        ref = ctypes.byref(a)
+        if handle.mvsd_loss_plan(ref) != 0:
             raise ValueError(f"logits {tuple(self.logits.shape)} are more than one call takes")
-        workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+        device = self.device
         if train:
-            self.saved = torch.empty(handle.mvsd_loss_saved_bytes(ctypes.byref(a)),
-                                     dtype=torch.uint8, device=self.device)
+            self.saved = torch.empty(a.saved_bytes, dtype=torch.uint8, device=device)
             a.saved = self.saved.data_ptr() or None
-            if handle.mvsd_loss_one_pass(ctypes.byref(a)):
-                self.grad = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.device)
+            if a.one_pass:
+                self.grad = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=device)
                 a.grad = self.grad.data_ptr()
-        nat.check(handle.mvsd_row_loss(ctypes.byref(a), nat.stream_of(self.device)), "mvsd_row_loss")
-        self.keep = []
+        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
+        a.workspace = workspace.data_ptr()
+        status = handle.mvsd_row_loss(ref, nat.stream_of(device))
+        if status != 0:
+            nat.check(status, "mvsd_row_loss")
+        self.keep = None
 
     def gradient(self, logits, ids, saved, upstream, upstream_entropy) -> torch.Tensor:
         """The logits' gradient for the outputs' (a tensor may lie elsewhere than when it was saved)."""
@@ -196,13 +196,29 @@ class _Call:
         a.grad = grad.data_ptr()
         ups = []
         for g in (upstream, upstream_entropy):
-            if g is not None:
+            if g is None:
+                ups += (None, 0)
+                continue
+            if g.dtype is not torch.float32 or not g.is_contiguous():
                 g = g.to(torch.float32).contiguous()
-            ups += [g, 0 if g is None or g.ndim == 0 else 1]
-        nat.check(nat.lib().mvsd_loss_gradient(
-            ctypes.byref(a), nat.ptr(ups[0]), ups[1], nat.ptr(ups[2]), ups[3],
-            nat.stream_of(logits.device)), "mvsd_loss_gradient")
+                self.keep = g
+            ups += (g.data_ptr(), 1 if g.ndim else 0)
+        status = nat.lib().mvsd_loss_gradient(ctypes.byref(a), *ups, nat.stream_of(logits.device))
+        if status != 0:
+            nat.check(status, "mvsd_loss_gradient")
         return grad
+
+
+def _backward(ctx, upstream, *others):
+    logits, ids, saved = ctx.saved_tensors
+    call = ctx.call
+    entropy = others[0] if call.kind == _LOGPROBS and others else None
+    if upstream is None and entropy is None:
+        return None, None
+    if logits.device.index == torch.cuda.current_device():
+        return call.gradient(logits, ids, saved, upstream, entropy), None
+    with torch.cuda.device(logits.device):
+        return call.gradient(logits, ids, saved, upstream, entropy), None
 
 
 class _RowLoss(torch.autograd.Function):
@@ -210,7 +226,7 @@ class _RowLoss(torch.autograd.Function):
     def forward(ctx, logits, call):
         call.run(True)
         ctx.set_materialize_grads(False)
-        if call.kind != _LOGPROBS:
+        if call.kind != _LOGPROBS and len(call.outputs) > 1:
             ctx.mark_non_differentiable(*call.outputs[1:])
         ctx.save_for_backward(logits, call.ids, call.saved)
         outputs, call.outputs, call.logits, call.ids, call.saved = call.outputs, (), None, None, None
@@ -218,19 +234,18 @@ class _RowLoss(torch.autograd.Function):
         return outputs
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, upstream, *others):
-        logits, ids, saved = ctx.saved_tensors
-        entropy = others[0] if ctx.call.kind == _LOGPROBS and others else None
-        if upstream is None and entropy is None:
-            return None, None
-        with torch.cuda.device(logits.device):
-            return ctx.call.gradient(logits, ids, saved, upstream, entropy), None
+    def backward(ctx, *upstream):
+        if torch.is_grad_enabled():  # a graph of the gradient is asked for, which there is not
+            return _refusing_backward(ctx, *upstream)
+        return _backward(ctx, *upstream)
+
+
+_refusing_backward = torch.autograd.function.once_differentiable(_backward)
 
 
 def _finish(call: _Call):
     """The call's outputs, part of the graph where the logits want a gradient."""
-    if torch.is_grad_enabled() and call.logits.requires_grad:
+    if call.logits.requires_grad and torch.is_grad_enabled():
         return _RowLoss.apply(call.logits, call)
     call.run(False)
     return call.outputs
@@ -255,9 +270,9 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, temperature
     call = _Call(_LOGPROBS, logits, temperature, 0)
     lead = logits.shape[:-1]
     call.take_ids(_check_ids(token_ids, "token_ids", lead, call.device))
-    call.outputs = (call.empty("logprobs", *lead),)
+    call.outputs = (call.empty("logprobs", lead),)
     if return_entropy:
-        call.outputs += (call.empty("entropy", *lead),)
+        call.outputs += (call.empty("entropy", lead),)
     out = _finish(call)
     return out if return_entropy else out[0]
 
@@ -298,10 +313,9 @@ def distillation_loss(logits: torch.Tensor, teacher_token_ids: torch.Tensor,
     if not 1 <= K <= MAX_TEACHER_TOKENS:
         raise ValueError(f"{K} teacher tokens: 1 to {MAX_TEACHER_TOKENS} are supported")
     call.take_ids(_check_ids(teacher_token_ids, "teacher_token_ids", lead + (K,), call.device))
-    call.take("teacher_logprobs",
-              _values(teacher_logprobs, "teacher_logprobs", lead + (K,), call.device))
-    call.take("weights", _weights(weights, lead, call.device))
-    call.outputs = (call.empty("loss", *(lead if reduction == "none" else ())),)
+    call.take("teacher_logprobs", teacher_logprobs, lead + (K,))
+    call.take_weights(weights, lead)
+    call.outputs = (call.empty("loss", lead if reduction == "none" else ()),)
     return _finish(call)[0]
 
 
@@ -335,16 +349,16 @@ def policy_loss(logits: torch.Tensor, token_ids: torch.Tensor, old_logprobs: tor
     call.take_ids(_check_ids(token_ids, "token_ids", lead, call.device))
     if advantages is None:
         raise ValueError("advantages are needed")
-    call.take("advantages", _values(advantages, "advantages", lead, call.device))
-    call.take("old_logprobs", _values(old_logprobs, "old_logprobs", lead, call.device))
-    call.take("ref_logprobs", _values(ref_logprobs, "ref_logprobs", lead, call.device))
-    call.take("weights", _weights(weights, lead, call.device))
-    outputs = [call.empty("loss", *(lead if reduction == "none" else ())),
-               call.empty("logprobs", *lead)]
+    call.take("advantages", advantages, lead)
+    call.take("old_logprobs", old_logprobs, lead)
+    call.take("ref_logprobs", ref_logprobs, lead)
+    call.take_weights(weights, lead)
+    outputs = [call.empty("loss", lead if reduction == "none" else ()),
+               call.empty("logprobs", lead)]
     if a.entropy_coef != 0:
-        outputs.append(call.empty("entropy", *lead))
+        outputs.append(call.empty("entropy", lead))
     if ref_logprobs is not None:
-        outputs.append(call.empty("kl", *lead))
+        outputs.append(call.empty("kl", lead))
     call.outputs = tuple(outputs)
     with_entropy = a.entropy_coef != 0
     loss, logprobs, *rest = _finish(call)
@@ -394,15 +408,16 @@ def preference_loss(logits: torch.Tensor, token_ids: torch.Tensor,
         if cu_num_tokens.dtype != torch.int32 or cu_num_tokens.ndim != 1:
             raise TypeError("cu_num_tokens is int32 [2B]")
         sequences = cu_num_tokens.shape[0]
-        call.take("cu_num_tokens", cu_num_tokens.contiguous())
+        call.keep.append(cu_num_tokens.contiguous())
+        a.cu_num_tokens = call.keep[0].data_ptr()
     else:
         sequences = lead[0]
     if sequences % 2:
         raise ValueError(f"{sequences} sequences are no pairs")
     B = a.num_pairs = sequences // 2
     call.take_ids(_check_ids(token_ids, "token_ids", lead, call.device))
-    call.take("ref_logprobs", _values(ref_logprobs, "ref_logprobs", torch.Size((2 * B,)), call.device))
-    call.take("weights", _weights(weights, torch.Size((B,)), call.device))
-    call.outputs = (call.empty("loss", *((B,) if reduction == "none" else ())),
-                    call.empty("logprobs", 2 * B))
+    call.take("ref_logprobs", ref_logprobs, (2 * B,))
+    call.take_weights(weights, (B,))
+    call.outputs = (call.empty("loss", (B,) if reduction == "none" else ()),
+                    call.empty("logprobs", (2 * B,)))
     return PreferenceLoss(*_finish(call))
