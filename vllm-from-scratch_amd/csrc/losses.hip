@@ -40,11 +40,13 @@ __device__ inline const typename Elem<DT>::storage* logits_row(const mvsd_loss_a
          (row - outer * a.inner_rows) * a.stride;
 }
 
-// A token id, V for every one of V or more, -1 for every one below 0.
-__device__ inline int clean_id(int64_t id, int V) { return id < 0 ? -1 : id >= V ? V : (int)id; }
+// Token id i, V for every one of V or more, -1 for every one below 0.  Its two halves are loaded (one word
+// twice of an int32), so that several ids' loads need no branch between them.
 __device__ inline int token_at(const mvsd_loss_args& a, int64_t i, int V) {
-  return clean_id(a.ids_dtype == MVSD_I64 ? static_cast<const int64_t*>(a.token_ids)[i]
-                                          : (int64_t) static_cast<const int32_t*>(a.token_ids)[i], V);
+  const int words = a.ids_dtype == MVSD_I64 ? 2 : 1;
+  const int32_t* id = static_cast<const int32_t*>(a.token_ids) + i * words;
+  const int low = id[0], high = id[words - 1];
+  return high < 0 ? -1 : (words == 2 && high > 0) || (uint32_t)low >= (uint32_t)V ? V : low;
 }
 
 // A row's weight before the mean's division (a preference's weights are its pairs').
@@ -501,9 +503,9 @@ __device__ inline double wave_sum_f64(double v) {
 // The teacher's side, a wave a row: which entries count (over_ids, -1: not), the mass of the rest (0 where
 // the rest is no outcome) or, without a tail, the log of the entries' sum, the row's weight (0: left out),
 // and the partial sums of the weights.
+template <int E>  // entries a lane
 __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p) {
-  constexpr int E = kMaxTeacher / kWave;
-  __shared__ __attribute__((aligned(16))) int s_ids[kWaves][kMaxTeacher];
+  __shared__ __attribute__((aligned(16))) int s_ids[kWaves][E * kWave];
   __shared__ float scratch[kWaves];
   const mvsd_loss_args& a = p.a;
   const int64_t each = (a.num_rows + gridDim.x - 1) / gridDim.x;
@@ -516,10 +518,14 @@ __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p
     float v[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int k = i * kWave + lane;
-      id[i] = k < K ? token_at(a, row * K + k, p.V) : -1;
-      v[i] = k < K ? a.teacher_logprobs[row * K + k] : -INFINITY;
-      ids[k] = id[i];  // a wave's own places: its reads below follow
+      const int k = min(i * kWave + lane, K - 1);
+      id[i] = token_at(a, row * K + k, p.V);
+      v[i] = a.teacher_logprobs[row * K + k];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (i * kWave + lane >= K) id[i] = -1;
+      ids[i * kWave + lane] = id[i];  // a wave's own places: its reads below follow
     }
     __builtin_amdgcn_wave_barrier();
     bool before[E] = {};
@@ -1275,7 +1281,10 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)(a.num_rows * p.nch)), block(kLossThreads);
   if (p.norm_parts) {
     if (has_list(a))
-      hipLaunchKernelGGL(loss_teacher_kernel, dim3(p.norm_parts), block, 0, stream, p);
+      hipLaunchKernelGGL(p.K <= kWave       ? loss_teacher_kernel<1>
+                         : p.K <= 2 * kWave ? loss_teacher_kernel<2>
+                                            : loss_teacher_kernel<kMaxTeacher / kWave>,
+                         dim3(p.norm_parts), block, 0, stream, p);
     else
       hipLaunchKernelGGL(loss_norm_kernel, dim3(p.norm_parts), block, 0, stream, p);
   }
