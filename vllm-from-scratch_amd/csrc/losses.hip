@@ -637,33 +637,64 @@ __device__ inline float waves_max(float v, float* red, int NW) {
   return v;
 }
 
-// One row's loss by a workgroup of NW waves, from the statistics of its rest, its entries and what the
-// teacher's kernel gave of it.  Gives the gradients of the given tokens (over, at id, -1: none) and returns
-// the loss; *k is the record's.  `weight` is the row's, after the mean; red holds 2 NW floats.
+// What a row's entries give without the rest of the row, over a workgroup: their maximum, and sums of
+// e_k = exp((x_k - top) / T) and of what the divergence needs.
+struct EntrySums {
+  float top, z, s1, s2;
+};
+
 template <int E>
-__device__ inline float distill_row(const LossParams& p, Stat st, float teacher, float weight, float* red, int NW,
-                                    Entries<E>& in, float (&over)[E], float* k_out) {
+__device__ inline void teacher_of(const LossParams& p, const Entries<E>& in, int i, float teacher, float& q,
+                                  float& log_q) {
+  log_q = p.a.tail ? in.v[i] : in.v[i] * p.inv_t - teacher;
+  q = expf(log_q);
+}
+
+// red holds 3 NW floats.
+template <int E>
+__device__ inline EntrySums sum_entries(const LossParams& p, float teacher, float* red, int NW, Entries<E>& in) {
   const mvsd_loss_args& a = p.a;
-  int (&id)[E] = in.id;
-  float (&x)[E] = in.x;
-  float top = st.m;
+  float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    if (id[i] < 0) x[i] = -INFINITY;
-    if (x[i] == INFINITY) x[i] = NAN;
-    top = fmaxf(top, x[i]);
+    if (in.id[i] < 0) in.x[i] = -INFINITY;
+    if (in.x[i] == INFINITY) in.x[i] = NAN;
+    top = fmaxf(top, in.x[i]);
   }
-  const float base = base_of(waves_max(top, red, NW)), rest_base = base_of(st.m);
-  const bool tail = a.tail && teacher != 0.f;
-  // the student's normaliser
-  float z[1] = {0.f};
+  top = base_of(waves_max(top, red, NW));
+  float v[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < E; ++i) z[0] += expf((x[i] - base) * p.inv_t);
-  waves_sum<1>(z, red, NW);
-  const float rest_d = st.m == -INFINITY ? 0.f : (rest_base - base) * p.inv_t;
-  const float log_z = logf(z[0] + st.s * expf(rest_d));
-  const float rest_lp = rest_d + logf(st.s) - log_z, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
-  // the divergence's terms, and p dL/dp of every outcome
+  for (int i = 0; i < E; ++i) {
+    const float d = (in.x[i] - top) * p.inv_t, e = expf(d);
+    float q, log_q;
+    teacher_of(p, in, i, teacher, q, log_q);
+    if (in.id[i] < 0) continue;
+    v[0] += e;
+    if (a.divergence == MVSD_KL_FORWARD) {
+      v[1] += q == 0.f ? 0.f : q * (log_q - d);
+      v[2] += q;
+    } else {
+      v[1] += e == 0.f ? 0.f : e * (d - log_q);
+    }
+  }
+  waves_sum<3>(v, red, NW);
+  return {top, v[0], v[1], v[2]};
+}
+
+// One row's loss by a workgroup of NW waves, from the statistics of its rest, its entries and what the
+// teacher's kernel gave of it.  Gives the gradients of the given tokens (over, at id, -1: none) and returns
+// the loss; *k is the record's.  `weight` is the row's, after the mean.  With d_k = (x_k - top) / T and lz the
+// log of the row's sum against top, the entries' part of sum q (log q - log p) is s1 + lz s2, that of
+// sum p (log p - log q) is (s1 - lz z) / e^lz; only a Jensen-Shannon divergence needs sums behind lz.
+template <int E>
+__device__ inline float distill_row(const LossParams& p, Stat st, const EntrySums& k, float teacher, float weight,
+                                    float* red, int NW, Entries<E>& in, float (&over)[E], float* k_out) {
+  const mvsd_loss_args& a = p.a;
+  const bool tail = a.tail && teacher != 0.f;
+  const float rest_d = st.m == -INFINITY ? 0.f : (st.m - k.top) * p.inv_t, far = fmaxf(rest_d, 0.f);
+  const float lz = far + logf(k.z * expf(-far) + st.s * expf(rest_d - far));
+  const float rest_lp = rest_d + logf(st.s) - lz, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
+  // the divergence's term, and p dL/dp, of an outcome
   auto outcome = [&](float q, float log_q, float pr, float lp, float& term, float& pd) {
     if (a.divergence == MVSD_KL_FORWARD) {
       term = q == 0.f ? 0.f : q * (log_q - lp);
@@ -676,19 +707,26 @@ __device__ inline float distill_row(const LossParams& p, Stat st, float teacher,
       term = pd + (q == 0.f ? 0.f : 0.5f * q * (log_q - lm));
     }
   };
-  float both[2] = {0.f, 0.f}, pr[E], pd[E];
+  float both[2] = {0.f, 0.f}, pr[E], pd[E];  // the sums of terms, and of p dL/dp
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const float lp = (x[i] - base) * p.inv_t - log_z;
-    const float log_q = a.tail ? in.v[i] : in.v[i] * p.inv_t - teacher;
-    float term = 0.f;
+    const float lp = (in.x[i] - k.top) * p.inv_t - lz;
+    float q, log_q, term = 0.f;
+    teacher_of(p, in, i, teacher, q, log_q);
     pr[i] = expf(lp);
     pd[i] = 0.f;
-    if (id[i] >= 0) outcome(expf(log_q), log_q, pr[i], lp, term, pd[i]);
+    if (in.id[i] >= 0) outcome(q, log_q, pr[i], lp, term, pd[i]);
     both[0] += term;
     both[1] += pd[i];
   }
-  waves_sum<2>(both, red, NW);
+  if (a.divergence == MVSD_KL_FORWARD) {
+    both[0] = k.s1 + lz * k.s2;
+    both[1] = -k.s2;
+  } else if (a.divergence == MVSD_KL_REVERSE) {
+    both[0] = both[1] = (k.s1 - lz * k.z) * expf(-lz);
+  } else {
+    waves_sum<2>(both, red, NW);
+  }
   float rest_pd = 0.f;
   if (tail) {
     float term;
@@ -701,7 +739,7 @@ __device__ inline float distill_row(const LossParams& p, Stat st, float teacher,
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     over[i] = f * (pd[i] - pr[i] * both[1]);
-    if (id[i] >= p.V) id[i] = -1;
+    if (in.id[i] >= p.V) in.id[i] = -1;
   }
   return both[0] * weight;
 }
@@ -719,7 +757,7 @@ __device__ inline void save_over(const LossParams& p, int64_t row, int T, const 
 template <int DT>
 __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossParams p) {
   constexpr int E = kMaxTeacher / kLossThreads;
-  __shared__ float red[2 * kWaves];
+  __shared__ float red[3 * kWaves];
   const int64_t row = blockIdx.x;
   const float2 teacher = p.teach[row];
   float loss = 0.f;
@@ -737,7 +775,8 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
     rec.M = base_of(st.m);
     rec.c = 1.f;
     float over[E];
-    loss = distill_row<E>(p, st, teacher.x, teacher.y * mean_factor(p), red, kWaves, in, over, &rec.k);
+    const EntrySums sums = sum_entries<E>(p, teacher.x, red, kWaves, in);
+    loss = distill_row<E>(p, st, sums, teacher.x, teacher.y * mean_factor(p), red, kWaves, in, over, &rec.k);
     if (p.records) save_over<E>(p, row, kLossThreads, over);
   }
   if (threadIdx.x == 0) {
@@ -879,6 +918,9 @@ __global__ __launch_bounds__(kLossThreads) void loss_gradient_kernel(LossParams 
 constexpr int kMostHeld = 18;  // vectors of a row in each thread's registers (72 of 128)
 constexpr int kRowThreads = 1024;
 
+// A value that all lanes have, in a scalar register.
+__device__ inline float scalar(float v) { return readlane_f32(v, 0); }
+
 // Rows by a workgroup, one after the other (by tickets: some are left out), every row in its registers: read once, written once.  A turn of the
 // loop writes the gradient of one row and, vector by vector, loads the next one in its place and adds it to
 // its statistics kDelay vectors later, so that memory is busy except in the reductions and the row's own loss
@@ -893,7 +935,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   constexpr int VEC = Elem<DT>::kVec, E = 1, kDelay = NV > 8 ? 8 : NV - NV % 2;
   extern __shared__ uint32_t bits[];
   __shared__ float4 s_part[2][kRowThreads / kWave];
-  __shared__ float red[2 * kRowThreads / kWave];
+  __shared__ float red[3 * kRowThreads / kWave];
   __shared__ int s_ticket;
   const mvsd_loss_args& a = p.a;
   const int tid = threadIdx.x, V = p.V, N = (int)a.num_rows, T = blockDim.x, NW = T / kWave;
@@ -901,9 +943,11 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   // threads behind the active ones do what the last of those does, and count for nothing
   const unsigned own = min(tid, p.active - 1) * VEC;
   const int tail_col = behind + tid * VEC;
-  const float mean = mean_factor(p), c1 = p.c1;
+  const float mean = scalar(mean_factor(p)), c1 = p.c1;
+  const int words = (V + 31) / 32;
+  uint32_t* marked = bits;  // the marks of this turn's row: two sets in turn, the other one is cleared
   if constexpr (LIST) {
-    for (int i = tid; i < (V + 31) / 32; i += T) bits[i] = 0;
+    for (int i = tid; i < 2 * words; i += T) bits[i] = 0;
     __syncthreads();
   }
 
@@ -912,6 +956,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   float w = 0.f, teacher = 0.f, xt = NAN;
   PolicyIn given = {0.f, 0.f, 0.f};
   Entries<E> in = {};
+  EntrySums sums = {0.f, 0.f, 0.f, 0.f};
   const S* x = nullptr;
   int cur = -1, cur_token = -1, pend_id[E];
   float pend[E], cur_M = 0.f, at_token = 0.f;
@@ -940,11 +985,11 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     for (; row < N; announce(row)) {
       if constexpr (LIST) {
         in = after;
-        teacher = teach.x;
-        w = teach.y;
+        teacher = scalar(teach.x);
+        w = scalar(teach.y);
       } else {
-        token = next_token;
-        w = next_w;
+        token = __builtin_amdgcn_readfirstlane(next_token);
+        w = scalar(next_w);
       }
       if (w != 0.f && (LIST || token >= 0)) break;
       if (tid == 0) {
@@ -963,19 +1008,13 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
       }
       if (tid == 0) s_ticket = atomicAdd(p.tickets, 1);
       __syncthreads();
-      row = gridDim.x + s_ticket;
+      row = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket);
       __syncthreads();
     }
     if (row >= N) return false;
     if (tid == 0) ticket = atomicAdd(p.tickets, 1);  // the next row's, which finish() gives to all
     x = logits_row<DT>(a, row);
-    if constexpr (LIST) {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (in.id[i] >= 0 && in.id[i] < V) atomicOr(&bits[in.id[i] >> 5], 1u << (in.id[i] & 31));
-      load_entry_logits<DT>(p, row, in);
-      __syncthreads();
-    } else {
+    if constexpr (!LIST) {
       xt = token < V ? Elem<DT>::cvt(x[token]) : NAN;
       given = policy_in(a, row);
     }
@@ -1002,7 +1041,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     const bool cur_holds = (int)own == (cur_spot - cur_span * p.active) * VEC;
     // uniform offsets, kept so: the compiler would keep each thread's for every vector
     unsigned from = 0, to = 0;
-    const uint32_t* marks_from = bits + (own >> 5);
+    const uint32_t* marks_from = marked + (own >> 5);
     auto clean = [&](u32x4& v, int i) {  // the given tokens become -inf
       if constexpr (LIST) {
         const unsigned marks = *marks_from >> (own & 31) & ((1u << VEC) - 1);
@@ -1013,8 +1052,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
         if (holds) mask_vec<DT>(v, 1u << token % VEC);
       }
     };
-#pragma unroll
-    for (int i = 0; i < NV + kDelay; ++i) {
+    auto vector = [&](int i) {
       if (i < NV) {
         if constexpr (WANT) {
           u32x4 v = {0u, 0u, 0u, 0u};
@@ -1048,7 +1086,24 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // vectors in their order: more of them at once do not fit the registers
+    };
+#pragma unroll
+    for (int i = 0; i < kDelay; ++i) vector(i);
+    if (LIST && more) {  // while the first vectors come: the marks
+#pragma unroll
+      for (int n = 0; n < E; ++n)
+        if (in.id[n] >= 0 && in.id[n] < V) atomicOr(&marked[in.id[n] >> 5], 1u << (in.id[n] & 31));
+      load_entry_logits<DT>(p, row, in);
+      __syncthreads();
     }
+#pragma unroll
+    for (int i = kDelay; i < NV; ++i) vector(i);
+    if (LIST && more) {  // while the last ones come
+      sums = sum_entries<E>(p, teacher, red, NW, in);
+      sums = {scalar(sums.top), scalar(sums.z), scalar(sums.s1), scalar(sums.s2)};
+    }
+#pragma unroll
+    for (int i = NV; i < NV + kDelay; ++i) vector(i);
     if (tid >= p.active) st = {-INFINITY, 0.f, 0.f};
     for (int col = tail_col; col < V; col += T * VEC) {
       float v[VEC];
@@ -1063,7 +1118,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
       }
       if (more) {
         load_filled<DT>(x, col, V, v);
-        const unsigned marks = LIST ? marks_at(bits, col, VEC) : 0;
+        const unsigned marks = LIST ? marks_at(marked, col, VEC) : 0;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = (LIST ? marks >> e & 1 : token == col + e) ? -INFINITY : v[e];
         add_values<ENT, VEC>(st, v, c1);
@@ -1087,7 +1142,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     if (lane_id() == 0) s_part[parity][wave_id()] = make_float4(st.m, st.s, st.t, 0.f);
     if (tid == 0) s_ticket = ticket;
     __syncthreads();
-    const int next = gridDim.x + s_ticket;
+    const int next = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket);  // one of all, in a scalar register
     announce(next);
     give();
     const int part = lane_id() % 16;
@@ -1101,11 +1156,12 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     float loss;
     if constexpr (LIST) {
 #pragma unroll
-      for (int i = 0; i < E; ++i)  // distill_row's barriers are between this and the next row's marks
-        if (in.id[i] >= 0 && in.id[i] < V) bits[in.id[i] >> 5] = 0;
+      for (int i = 0; i < E; ++i)
+        if (in.id[i] >= 0 && in.id[i] < V) marked[in.id[i] >> 5] = 0;
+      marked = marked == bits ? bits + words : bits;
       rec.M = base_of(st.m);
       rec.c = 1.f;
-      loss = distill_row<E>(p, st, teacher, w * mean, red, NW, in, pend, &rec.k);
+      loss = distill_row<E>(p, st, sums, teacher, w * mean, red, NW, in, pend, &rec.k);
       if (p.records) save_over<E>(p, row, T, pend);
 #pragma unroll
       for (int i = 0; i < E; ++i) pend_id[i] = in.id[i];
@@ -1129,9 +1185,10 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     }
     const float gH = ENT ? rec.cH : 0.f;
     zeros = rec.c == 0.f && gH == 0.f;
-    cur_M = rec.M;
+    cur_M = scalar(rec.M);
     rest = rest_gradient(rec, rec.c, gH);
-    at_token = token_gradient(rec, rec.c, gH);
+    rest = {scalar(rest.a), scalar(rest.b)};
+    at_token = scalar(token_gradient(rec, rec.c, gH));
     cur = row;
     cur_x = x;
     cur_token = token;
@@ -1212,7 +1269,7 @@ int64_t aside_bytes(const mvsd_loss_args& a) {
   return row_groups(a, plan) * plan.active * 16;
 }
 
-constexpr int64_t kMaxMarked = 1 << 18;  // columns whose marks are 32 KiB
+constexpr int64_t kMaxMarked = 3 << 16;  // columns whose two sets of marks are 48 KiB
 
 constexpr int64_t kCacheBytes = 256ll << 20;  // of the last level
 
@@ -1260,7 +1317,7 @@ void launch_rows_of(const LossParams& p, const RowPlan& plan, hipStream_t stream
   const dim3 grid((unsigned)row_groups(p.a, plan));
   const dim3 block(plan.threads);
   if (has_list(p.a))
-    hipLaunchKernelGGL((loss_rows_kernel<DT, NV, true, false, WANT>), grid, block, (unsigned)((p.V + 31) / 32 * 4), stream, p);
+    hipLaunchKernelGGL((loss_rows_kernel<DT, NV, true, false, WANT>), grid, block, (unsigned)((p.V + 31) / 32 * 8), stream, p);
   else if (p.entropy)
     hipLaunchKernelGGL((loss_rows_kernel<DT, NV, false, true, WANT>), grid, block, 0, stream, p);
   else
