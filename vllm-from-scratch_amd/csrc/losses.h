@@ -34,7 +34,7 @@ struct LossParams {
   float4* parts;      // [N, nch] maximum, sum, sum of e log2 e
   float* norm;        // [kNormParts] partial sums of weights (mean)
   int norm_parts;
-  int* tickets;       // rows that loss_rows_kernel's workgroups have taken behind their first
+  int* counters;      // [2], see losses.hip
   float* row_loss;    // [N] (preference: [pairs]), weighted
   float* row_lp;      // preference: [N]
   float2* teach;      // distillation: [N] what the teacher's kernel gives of a row, its weight (0: left out)

@@ -180,6 +180,43 @@ __device__ inline void rebase(Stat& st, float m, float c1) {
   st.m = m;
 }
 
+// ------------------------------------------------------------------ the loss of all rows --------
+
+// counters[0]: rows that loss_rows_kernel's workgroups have taken behind their first; [1]: workgroups whose rows
+// have their losses.  An earlier launch of the call clears them.
+__device__ inline void clear_counters(const LossParams& p) {
+  if (threadIdx.x < 2) p.counters[threadIdx.x] = 0;
+}
+
+// loss[0] = the sum of n row losses, by a workgroup, in one order.
+__device__ inline void sum_losses(const LossParams& p, int64_t n) {
+  __shared__ float s_sum[16];
+  float sum = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) sum += p.row_loss[i];
+  sum = wave_sum(sum);
+  if (lane_id() == 0) s_sum[wave_id()] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0.f;
+    for (int w = 0; w < (int)blockDim.x / kWave; ++w) sum += s_sum[w];
+    p.a.loss[0] = sum;
+  }
+}
+
+// The same by the last of a launch's workgroups, each of which comes here once, behind its rows' losses.
+__device__ inline void sum_by_the_last(const LossParams& p, int64_t n) {
+  if (p.a.reduction == MVSD_REDUCE_NONE) return;
+  __shared__ int s_last;
+  __syncthreads();  // all of the workgroup's losses are stored
+  if (threadIdx.x == 0) s_last = atomic_add_acq_rel(p.counters + 1, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (s_last) sum_losses(p, n);
+}
+
+// Behind loss_rows_kernel, whose workgroups would write their gradients back from L2 before they count
+// themselves (12 us of 260, 30 of 125, against 6 for this launch); and for calls without rows.
+__global__ __launch_bounds__(1024) void loss_sum_kernel(LossParams p, int64_t n) { sum_losses(p, n); }
+
 // ------------------------------------------------------------------ the mean's divisor ----------
 
 // Partial sums of the weights of the rows that are not left out.
@@ -192,7 +229,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_norm_kernel(LossParams p) {
     if (token_at(p.a, row, p.V) >= 0) sum[0] += row_weight(p.a, row);
   block_sum<1>(sum, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = sum[0];
-  if (threadIdx.x == 0 && blockIdx.x == 0) *p.tickets = 0;
+  if (blockIdx.x == 0) clear_counters(p);
 }
 
 // What a row's weight is multiplied by, in every thread of a wave.
@@ -317,18 +354,20 @@ __device__ inline void finish_token_row(const LossParams& p, int64_t row, int to
 template <int DT>
 __global__ __launch_bounds__(kLossThreads) void loss_token_rows_kernel(LossParams p) {
   const int64_t row = (int64_t)blockIdx.x * kWaves + wave_id();
-  if (row >= p.a.num_rows) return;
-  const int token = token_at(p.a, row, p.V);
-  const bool out = token < 0 || row_weight(p.a, row) == 0.f;
-  Stat st = {-INFINITY, 0.f, 0.f};
-  if (!out) {
-    for (int i = lane_id(); i < p.nch; i += kWave) {
-      const float4 v = p.parts[row * p.nch + i];
-      st = join(st, {v.x, v.y, v.z}, p.c1);
+  if (row < p.a.num_rows) {
+    const int token = token_at(p.a, row, p.V);
+    const bool out = token < 0 || row_weight(p.a, row) == 0.f;
+    Stat st = {-INFINITY, 0.f, 0.f};
+    if (!out) {
+      for (int i = lane_id(); i < p.nch; i += kWave) {
+        const float4 v = p.parts[row * p.nch + i];
+        st = join(st, {v.x, v.y, v.z}, p.c1);
+      }
+      st = wave_join(st, p.c1);
     }
-    st = wave_join(st, p.c1);
+    finish_token_row<DT>(p, row, token, out, st);
   }
-  finish_token_row<DT>(p, row, token, out, st);
+  if (p.a.kind == MVSD_LOSS_POLICY) sum_by_the_last(p, p.a.num_rows);
 }
 
 // One workgroup a chunk of a row: statistics of its rest.  Blocks of kBlock vectors a thread, the next one's
@@ -343,6 +382,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
   const bool whole = !LIST && p.nch == 1;
   int token = -1;
+  if (!LIST && p.a.kind == MVSD_LOSS_PREFERENCE && blockIdx.x == 0) clear_counters(p);  // its pairs' kernel counts
   if constexpr (LIST) {
     if (p.teach[row].y == 0.f) return;
     for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
@@ -356,6 +396,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
     token = token_at(p.a, row, p.V);
     if (token < 0 || row_weight(p.a, row) == 0.f) {
       if (whole && wave_id() == 0) finish_token_row<DT>(p, row, token, true, {-INFINITY, 0.f, 0.f});
+      if (whole && p.a.kind == MVSD_LOSS_POLICY) sum_by_the_last(p, p.a.num_rows);
       return;
     }
   }
@@ -409,12 +450,14 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
   st = wave_join(st, p.c1);
   if (lane_id() == 0) s_stat[wave_id()] = st;
   __syncthreads();
-  if (wave_id() != 0) return;
-  st = join(join(s_stat[0], s_stat[1], p.c1), join(s_stat[2], s_stat[3], p.c1), p.c1);
-  if (whole)
-    finish_token_row<DT>(p, row, token, false, st);
-  else if (lane_id() == 0)
-    p.parts[blockIdx.x] = make_float4(st.m, st.s, st.t, 0.f);
+  if (wave_id() == 0) {
+    st = join(join(s_stat[0], s_stat[1], p.c1), join(s_stat[2], s_stat[3], p.c1), p.c1);
+    if (whole)
+      finish_token_row<DT>(p, row, token, false, st);
+    else if (lane_id() == 0)
+      p.parts[blockIdx.x] = make_float4(st.m, st.s, st.t, 0.f);
+  }
+  if (whole && p.a.kind == MVSD_LOSS_POLICY) sum_by_the_last(p, p.a.num_rows);
 }
 
 // A workgroup a pair: the sums over its two sequences, its loss, its rows' factors.
@@ -481,6 +524,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_pairs_kernel(LossParams p) 
     a.logprobs[pair] = S[0];
     a.logprobs[pair + B] = S[1];
   }
+  if (a.num_rows > 0) sum_by_the_last(p, B);
   if (!p.records || out) return;
 #pragma unroll
   for (int side = 0; side < 2; ++side)
@@ -575,7 +619,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p
   if (lane != 0) weights[0] = 0.f;
   block_sum<1>(weights, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = weights[0];
-  if (threadIdx.x == 0 && blockIdx.x == 0) *p.tickets = 0;
+  if (blockIdx.x == 0) clear_counters(p);
 }
 
 // A row's entries, entry i * T + thread in each of T threads.
@@ -783,17 +827,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
     p.row_loss[row] = loss;
     if (p.records) p.records[row] = rec;
   }
-}
-
-// ------------------------------------------------------------------ sums ------------------------
-
-// loss[0] = sum of n values, in one order.
-__global__ __launch_bounds__(1024) void loss_sum_kernel(float* loss, const float* v, int64_t n) {
-  __shared__ float scratch[16];
-  float sum[1] = {0.f};
-  for (int64_t i = threadIdx.x; i < n; i += 1024) sum[0] += v[i];
-  block_sum<1, 16>(sum, scratch);
-  if (threadIdx.x == 0) loss[0] = sum[0];
+  sum_by_the_last(p, p.a.num_rows);
 }
 
 // ------------------------------------------------------------------ the gradient ----------------
@@ -1006,13 +1040,13 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
         S* out = static_cast<S*>(a.grad) + (int64_t)row * V;
         for (int col = tid * VEC; col < V; col += T * VEC) store_filled<DT>(out, col, V, zero);
       }
-      if (tid == 0) s_ticket = atomicAdd(p.tickets, 1);
+      if (tid == 0) s_ticket = atomicAdd(p.counters, 1);
       __syncthreads();
       row = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket);
       __syncthreads();
     }
     if (row >= N) return false;
-    if (tid == 0) ticket = atomicAdd(p.tickets, 1);  // the next row's, which finish() gives to all
+    if (tid == 0) ticket = atomicAdd(p.counters, 1);  // the next row's, which finish() gives to all
     x = logits_row<DT>(a, row);
     if constexpr (!LIST) {
       xt = token < V ? Elem<DT>::cvt(x[token]) : NAN;
@@ -1196,16 +1230,17 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   };
 
   announce(row);
-  if (!advance()) return;
-  for (;;) {
-    turn();
-    if (!more) break;
-    finish();
-    more = advance();
-    if (!WANT && !more) return;
+  if (advance()) {
+    for (;;) {
+      turn();
+      if (!more) break;
+      finish();
+      more = advance();
+      if (!WANT && !more) break;
+    }
+    __syncthreads();
+    give();
   }
-  __syncthreads();
-  give();
 }
 
 // ------------------------------------------------------------------ host ------------------------
@@ -1291,7 +1326,7 @@ LossParams make_params(const mvsd_loss_args& a) {
   w += N * p.nch * sizeof(float4);
   p.norm = reinterpret_cast<float*>(w);
   w += kNormParts * sizeof(float);
-  p.tickets = reinterpret_cast<int*>(w);
+  p.counters = reinterpret_cast<int*>(w);
   w += 16;
   p.row_loss = a.reduction == MVSD_REDUCE_NONE && a.loss ? a.loss : reinterpret_cast<float*>(w);
   w += up16(std::max(N, a.num_pairs) * 4);
@@ -1307,7 +1342,7 @@ LossParams make_params(const mvsd_loss_args& a) {
   // the distillation's kernel has a wave a row where there are few
   if (a.kind == MVSD_LOSS_DISTILL)
     p.norm_parts = (int)std::min((N + kWaves - 1) / kWaves, (int64_t)kNormParts);
-  else if (a.kind == MVSD_LOSS_POLICY && (a.reduction == MVSD_REDUCE_MEAN || loss_one_pass(a)))
+  else if (a.kind == MVSD_LOSS_POLICY && a.reduction != MVSD_REDUCE_NONE)
     p.norm_parts = (int)std::min(N / 64 + 1, (int64_t)kNormParts);
   return p;
 }
@@ -1380,7 +1415,7 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
                               hipStream_t stream) {
   // mostly the gradient is there where a value of 1 is expected: few workgroups look for it
   const int64_t chunks = p.a.num_rows * p.nch;
-  const dim3 grid((unsigned)(p.a.unit_gradient ? std::min(chunks, (int64_t)num_cus() * 4) : chunks)), block(kLossThreads);
+  const dim3 grid((unsigned)(p.a.unit_gradient ? std::min(chunks, (int64_t)num_cus()) : chunks)), block(kLossThreads);
   const bool past = p.a.num_rows * p.V * (DT == MVSD_F32 ? 4 : 2) > kCacheBytes;
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, up, us, up_h, uhs); };
   if (has_list(p.a))
@@ -1423,13 +1458,12 @@ hipError_t launch_loss(const mvsd_loss_args& a, hipStream_t stream) {
     }
     if (err != hipSuccess) return err;
   }
-  int64_t losses = a.num_rows;
-  if (a.kind == MVSD_LOSS_PREFERENCE) {
-    losses = a.num_pairs;
-    if (losses > 0) hipLaunchKernelGGL(loss_pairs_kernel, dim3((unsigned)losses), dim3(kLossThreads), 0, stream, p);
-  }
-  if (a.kind != MVSD_LOSS_LOGPROBS && a.reduction != MVSD_REDUCE_NONE)
-    hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, stream, a.loss, p.row_loss, losses);
+  if (a.kind == MVSD_LOSS_PREFERENCE && a.num_pairs > 0)
+    hipLaunchKernelGGL(loss_pairs_kernel, dim3((unsigned)a.num_pairs), dim3(kLossThreads), 0, stream, p);
+  const int64_t losses = a.kind == MVSD_LOSS_PREFERENCE ? a.num_pairs : a.num_rows;
+  if (a.kind != MVSD_LOSS_LOGPROBS && a.reduction != MVSD_REDUCE_NONE &&
+      (losses == 0 || a.num_rows == 0 || loss_one_pass(a)))
+    hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, stream, p, losses);
   return hipGetLastError();
 }
 
