@@ -1432,7 +1432,10 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
 bool loss_one_pass(const mvsd_loss_args& a) {
   if ((a.kind != MVSD_LOSS_DISTILL && a.kind != MVSD_LOSS_POLICY) || a.reduction == MVSD_REDUCE_NONE) return false;
   if (a.vocab_size < 256 || (has_list(a) && a.vocab_size > kMaxMarked)) return false;
-  return a.num_rows >= 128 * (kRowThreads / row_plan(a).threads);
+  // Where rows are few, workgroups that share a row are faster (bf16, kernels' us, one pass against split:
+  // policy loss, V = 151936: 96 rows 35.5 / 31.6, 160 rows 37.8 / 39.3; V = 32000: 96 rows 21.7 / 19.2, 256 rows
+  // 25.5 / 25.8; distillation, V = 151936: 96 rows 44.1 / 42.3, 160 rows 47.1 / 54.4; V = 32000: 48 rows 25.7 / 25.7)
+  return a.num_rows >= (has_list(a) ? 80 : 128);
 }
 
 int64_t loss_workspace_bytes(const mvsd_loss_args& a) {
