@@ -59,7 +59,7 @@ BOTH = [
     (DISTILL, {"teacher_logprobs": None}, INVALID), (DISTILL, {"divergence": 3}, INVALID),
     (DISTILL, {"divergence": 1, "tail": 0}, INVALID), (DISTILL, {"divergence": 2, "tail": 0}, INVALID),
     (PREFERENCE, {"loss_type": 3}, INVALID), (PREFERENCE, {"num_pairs": -1}, INVALID),
-    (PREFERENCE, {"num_pairs": 2 ** 40}, RANGE),
+    (PREFERENCE, {"num_pairs": 2 ** 40}, RANGE), (PREFERENCE, {"num_pairs": 2 ** 23 + 1}, RANGE),
     (PREFERENCE, {"cu_num_tokens": None, "num_pairs": 3}, INVALID),
     (PREFERENCE, {"loss_type": 2, "beta": 0.0}, INVALID),
 ]

@@ -970,7 +970,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   extern __shared__ uint32_t bits[];
   __shared__ float4 s_part[2][kRowThreads / kWave];
   __shared__ float red[3 * kRowThreads / kWave];
-  __shared__ int s_ticket;
+  __shared__ int s_ticket[2], s_next;  // two of what is read behind a turn's one barrier: a wave may be a turn ahead
   const mvsd_loss_args& a = p.a;
   const int tid = threadIdx.x, V = p.V, N = (int)a.num_rows, T = blockDim.x, NW = T / kWave;
   const int span = p.active * VEC, behind = NV * span;
@@ -1040,9 +1040,9 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
         S* out = static_cast<S*>(a.grad) + (int64_t)row * V;
         for (int col = tid * VEC; col < V; col += T * VEC) store_filled<DT>(out, col, V, zero);
       }
-      if (tid == 0) s_ticket = atomicAdd(p.counters, 1);
+      if (tid == 0) s_next = atomicAdd(p.counters, 1);
       __syncthreads();
-      row = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket);
+      row = gridDim.x + __builtin_amdgcn_readfirstlane(s_next);
       __syncthreads();
     }
     if (row >= N) return false;
@@ -1174,9 +1174,9 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
     st.s = wave_sum(st.s);
     if constexpr (ENT) st.t = wave_sum(st.t);
     if (lane_id() == 0) s_part[parity][wave_id()] = make_float4(st.m, st.s, st.t, 0.f);
-    if (tid == 0) s_ticket = ticket;
+    if (tid == 0) s_ticket[parity] = ticket;
     __syncthreads();
-    const int next = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket);  // one of all, in a scalar register
+    const int next = gridDim.x + __builtin_amdgcn_readfirstlane(s_ticket[parity]);  // one of all, in a scalar register
     announce(next);
     give();
     const int part = lane_id() % 16;
@@ -1501,7 +1501,7 @@ int check_sizes(const mvsd_loss_args* a) {
   }
   if (a->kind == MVSD_LOSS_PREFERENCE) {
     if (a->num_pairs < 0) return MVSD_E_INVALID;
-    if (a->num_pairs > 0x3fffffff) return MVSD_E_RANGE;
+    if (a->num_pairs > 1 << 23) return MVSD_E_RANGE;
   }
   return MVSD_OK;
 }

@@ -194,14 +194,14 @@ class _Call:
         if grad.numel() == 0:
             return grad
         a.grad = grad.data_ptr()
-        ups = []
+        ups, kept = [], []
         for g in (upstream, upstream_entropy):
             if g is None:
                 ups += (None, 0)
                 continue
             if g.dtype is not torch.float32 or not g.is_contiguous():
                 g = g.to(torch.float32).contiguous()
-                self.keep = g
+                kept.append(g)
             ups += (g.data_ptr(), 1 if g.ndim else 0)
         status = nat.lib().mvsd_loss_gradient(ctypes.byref(a), *ups, nat.stream_of(logits.device))
         if status != 0:
