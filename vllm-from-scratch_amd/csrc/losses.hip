@@ -966,7 +966,7 @@ __device__ inline float scalar(float v) { return readlane_f32(v, 0); }
 template <int DT, int NV, bool LIST, bool ENT, bool WANT>
 __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p) {
   using S = typename Elem<DT>::storage;
-  constexpr int VEC = Elem<DT>::kVec, E = 1, kDelay = NV > 8 ? 8 : NV - NV % 2;
+  constexpr int VEC = Elem<DT>::kVec, E = 1, kDelay = NV > 4 ? 4 : 2;
   extern __shared__ uint32_t bits[];
   __shared__ float4 s_part[2][kRowThreads / kWave];
   __shared__ float red[3 * kRowThreads / kWave];
