@@ -31,6 +31,7 @@ struct LossParams {
   int active;       // threads that hold a row
   void* aside;      // a span of them for each workgroup
   bool entropy;
+  bool whole;       // the statistics' kernel finishes token rows, of one chunk each
   float4* parts;      // [N, nch] maximum, sum, sum of e log2 e
   float* norm;        // [kNormParts] partial sums of weights (mean)
   int norm_parts;

@@ -236,6 +236,10 @@ __global__ __launch_bounds__(kLossThreads) void loss_norm_kernel(LossParams p) {
 __device__ inline float mean_factor(const LossParams& p) {
   if (p.a.reduction != MVSD_REDUCE_MEAN) return 1.f;
   float sum = 0.f;
+  if (p.norm_parts == 0) {  // a policy's few rows, added by whom it concerns
+    for (int64_t row = lane_id(); row < p.a.num_rows; row += kWave)
+      sum += token_at(p.a, row, p.V) >= 0 ? row_weight(p.a, row) : 0.f;
+  }
   for (int i = lane_id(); i < p.norm_parts; i += kWave) sum += p.norm[i];
   sum = wave_sum(sum);
   return sum == 0.f ? 0.f : 1.f / sum;
@@ -380,9 +384,9 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
   const int64_t row = blockIdx.x / p.nch;
   const int part = blockIdx.x - (int)(row * p.nch);
   const int begin = part * p.chunk, end = min(p.V, begin + p.chunk);
-  const bool whole = !LIST && p.nch == 1;
+  const bool whole = !LIST && p.whole;
   int token = -1;
-  if (!LIST && p.a.kind == MVSD_LOSS_PREFERENCE && blockIdx.x == 0) clear_counters(p);  // its pairs' kernel counts
+  if (!LIST && p.norm_parts == 0 && blockIdx.x == 0) clear_counters(p);  // a later kernel counts
   if constexpr (LIST) {
     if (p.teach[row].y == 0.f) return;
     for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
@@ -1306,6 +1310,7 @@ int64_t aside_bytes(const mvsd_loss_args& a) {
 
 constexpr int64_t kMaxMarked = 3 << 16;  // columns whose two sets of marks are 48 KiB
 
+constexpr int64_t kFewRows = 512;  // whose weights every wave adds by itself (a launch less)
 constexpr int64_t kCacheBytes = 256ll << 20;  // of the last level
 
 LossParams make_params(const mvsd_loss_args& a) {
@@ -1342,8 +1347,10 @@ LossParams make_params(const mvsd_loss_args& a) {
   // the distillation's kernel has a wave a row where there are few
   if (a.kind == MVSD_LOSS_DISTILL)
     p.norm_parts = (int)std::min((N + kWaves - 1) / kWaves, (int64_t)kNormParts);
-  else if (a.kind == MVSD_LOSS_POLICY && a.reduction != MVSD_REDUCE_NONE)
+  else if (a.kind == MVSD_LOSS_POLICY && a.reduction != MVSD_REDUCE_NONE && (N > kFewRows || loss_one_pass(a)))
     p.norm_parts = (int)std::min(N / 64 + 1, (int64_t)kNormParts);
+  // a workgroup that counts itself needs counters that an earlier launch cleared
+  p.whole = p.nch == 1 && (a.kind != MVSD_LOSS_POLICY || a.reduction == MVSD_REDUCE_NONE || p.norm_parts > 0);
   return p;
 }
 
@@ -1403,7 +1410,7 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
       hipLaunchKernelGGL((loss_stats_kernel<DT, false, true>), grid, block, 0, stream, p);
     else
       hipLaunchKernelGGL((loss_stats_kernel<DT, false, false>), grid, block, 0, stream, p);
-    if (p.nch > 1)
+    if (!p.whole)
       hipLaunchKernelGGL(loss_token_rows_kernel<DT>, dim3((unsigned)((a.num_rows + kWaves - 1) / kWaves)), block, 0,
                        stream, p);
   }

@@ -38,9 +38,10 @@ import torch
 from .. import _native as nat
 
 MAX_TEACHER_TOKENS = 512
+_SMALL_SCRATCH = 1 << 18
 
-_ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_ID_DTYPES = (torch.int32, torch.int64)
+_ROW_CODES = {t: nat.dtype_code(t) for t in (torch.float32, torch.bfloat16, torch.float16)}
+_ID_CODES = {t: nat.dtype_code(t) for t in (torch.int32, torch.int64)}
 _LOGPROBS, _DISTILL, _POLICY, _PREFERENCE = range(4)
 _REDUCTIONS = {"sum": 0, "mean": 1, "none": 2}
 _DIVERGENCES = {"forward": 0, "reverse": 1, "js": 2}
@@ -86,10 +87,10 @@ def _check_device(t: torch.Tensor, name: str, device: torch.device) -> None:
 
 
 def _check_ids(ids: torch.Tensor, name: str, shape, device) -> torch.Tensor:
-    if ids.dtype in _ID_DTYPES and ids.shape == shape and ids.device == device:
+    if ids.dtype in _ID_CODES and ids.shape == shape and ids.device == device:
         return ids if ids.is_contiguous() else ids.contiguous()
     _check_device(ids, name, device)
-    if ids.dtype not in _ID_DTYPES:
+    if ids.dtype not in _ID_CODES:
         raise TypeError(f"{name} is {ids.dtype}, int32 or int64 expected")
     raise ValueError(f"{name} has shape {tuple(ids.shape)}, {tuple(shape)} expected")
 
@@ -112,11 +113,13 @@ def _values(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
 class _Call:
     """One call: its arguments and the tensors they point to."""
 
-    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "grad", "device")
+    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "grad", "device",
+                 "layout")
 
     def __init__(self, kind: int, logits: torch.Tensor, temperature: float, reduction: int):
-        nat.require_device_tensor(logits, "logits")
-        if logits.ndim not in (2, 3) or logits.dtype not in _ROW_DTYPES:
+        if not logits.is_cuda:
+            nat.require_device_tensor(logits, "logits")
+        if logits.ndim not in (2, 3) or logits.dtype not in _ROW_CODES:
             raise TypeError("logits are [N, V] or [B, L, V] in fp32, bf16 or fp16")
         if logits.shape[-1] < 1:
             raise ValueError("logits without columns")
@@ -130,11 +133,12 @@ class _Call:
         self._rows(logits)
 
     def _rows(self, logits: torch.Tensor) -> None:
-        a, shape, strides = self.args, logits.shape, logits.stride()
+        a, shape, strides, data = self.args, logits.shape, logits.stride(), logits.data_ptr()
         if strides[-1] != 1 and shape[-1] > 1:
             raise ValueError("logits need rows with unit stride")
-        a.dtype = nat.dtype_code(logits.dtype)
-        a.logits, a.vocab_size, a.stride = logits.data_ptr(), shape[-1], strides[-2]
+        self.layout = data, strides
+        a.dtype = _ROW_CODES[logits.dtype]
+        a.logits, a.vocab_size, a.stride = data, shape[-1], strides[-2]
         if len(shape) == 3:
             a.num_rows = shape[0] * shape[1]
             a.inner_rows, a.outer_stride = max(shape[1], 1), strides[0]
@@ -144,7 +148,7 @@ class _Call:
 
     def take_ids(self, ids: torch.Tensor) -> None:
         self.ids = ids
-        self.args.token_ids, self.args.ids_dtype = ids.data_ptr(), nat.dtype_code(ids.dtype)
+        self.args.token_ids, self.args.ids_dtype = ids.data_ptr(), _ID_CODES[ids.dtype]
 
     def take(self, name: str, t: torch.Tensor | None, shape) -> None:
         if t is not None:
@@ -167,15 +171,21 @@ class _Call:
         ref = ctypes.byref(a)
         if handle.mvsd_loss_plan(ref) != 0:
             raise ValueError(f"logits {tuple(self.logits.shape)} are more than one call takes")
-        device = self.device
+        device, scratch = self.device, a.workspace_bytes
         if train:
-            self.saved = torch.empty(a.saved_bytes, dtype=torch.uint8, device=device)
+            # what is saved, with a small call's scratch behind it
+            kept = (a.saved_bytes + 15) // 16 * 16
+            with_it = scratch <= _SMALL_SCRATCH
+            self.saved = torch.empty(kept + scratch if with_it else kept, dtype=torch.uint8, device=device)
             a.saved = self.saved.data_ptr() or None
             if a.one_pass:
                 self.grad = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=device)
                 a.grad = self.grad.data_ptr()
-        workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=device)
-        a.workspace = workspace.data_ptr()
+            if with_it:
+                a.workspace = (a.saved or 0) + kept
+        if not a.workspace:
+            workspace = torch.empty(scratch, dtype=torch.uint8, device=device)
+            a.workspace = workspace.data_ptr()
         status = handle.mvsd_row_loss(ref, nat.stream_of(device))
         if status != 0:
             nat.check(status, "mvsd_row_loss")
@@ -184,7 +194,8 @@ class _Call:
     def gradient(self, logits, ids, saved, upstream, upstream_entropy) -> torch.Tensor:
         """The logits' gradient for the outputs' (a tensor may lie elsewhere than when it was saved)."""
         a = self.args
-        self._rows(logits)
+        if self.layout != (logits.data_ptr(), logits.stride()):
+            self._rows(logits)
         a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr() or None
         # that of an upstream of 1, which is there already, goes out once: a kept graph's next is made anew
         grad, self.grad = self.grad, None
