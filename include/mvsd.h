@@ -770,13 +770,15 @@ int mvsd_beam_finish(const mvsd_beam_finish_args* args, mvsd_stream_t stream);
 /*     (m - margin - 1 / (2 beta))^2.  logprobs [2 num_pairs] = S.                             */
 /* token_ids (int32 or int64 by ids_dtype): a row with an id below 0 (distillation: without    */
 /* an entry) or of weight 0 is left out: its logits are not read, its values and its gradient  */
-/* are 0 (a pair of weight 0 adds nothing).  An id of vocab_size or more, a NaN, a +inf or nothing but -inf in a row: NaN.       */
+/* are 0 (a pair of weight 0 adds nothing).  An id of vocab_size or more, a NaN, a +inf or      */
+/* nothing but -inf in a row: NaN.                                                            */
 /* weights: fp32 [N] (preference: [num_pairs]) or NULL (1).  reduction: MVSD_REDUCE_SUM        */
 /* loss[0] = sum w l, MVSD_REDUCE_MEAN over sum w of the rows that are not left out (0: 0),    */
 /* MVSD_REDUCE_NONE loss[n] = w l.                                                            */
 /* saved: mvsd_loss_saved_bytes() bytes for mvsd_loss_gradient, or NULL.                       */
 /* workspace: mvsd_loss_workspace_bytes() bytes, no initial contents needed, one per call in    */
-/* flight.  Both are 16-byte aligned; a size of 0 or below: arguments that no call takes.      */
+/* flight.  Both are 16-byte aligned; a size below 0: arguments that no call takes.  At most   */
+/* 2^23 / (vocab_size / 2^18 + 1) rows and 2^23 pairs (MVSD_E_RANGE).                          */
 /* ------------------------------------------------------------------------------------ */
 enum { MVSD_LOSS_LOGPROBS = 0, MVSD_LOSS_DISTILL = 1, MVSD_LOSS_POLICY = 2, MVSD_LOSS_PREFERENCE = 3 };
 enum { MVSD_REDUCE_SUM = 0, MVSD_REDUCE_MEAN = 1, MVSD_REDUCE_NONE = 2 };
@@ -843,7 +845,8 @@ int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
 /* grad [N, V] contiguous in the logits' dtype, every row written.  upstream[n * up_stride]  */
 /* is the gradient of loss (LOGPROBS: of logprobs; PREFERENCE: index the pair;               */
 /* up_stride 0: one value), upstream_entropy that of LOGPROBS' entropy; NULL: 0.              */
-/* unit_gradient (with one upstream): grad holds the gradient for 1 already.                  */
+/* unit_gradient (with one upstream; only where mvsd_loss_one_pass gives 1, MVSD_E_INVALID    */
+/* otherwise): mvsd_row_loss has written grad, which stays as it is if the upstream is 1.      */
 /* ------------------------------------------------------------------------------------ */
 int mvsd_loss_gradient(const mvsd_loss_args* args, const float* upstream, int64_t up_stride,
                        const float* upstream_entropy, int64_t up_entropy_stride,

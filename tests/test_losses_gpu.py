@@ -374,6 +374,17 @@ def test_policy(device, dtype, N, V, ent):
     check_policy(x, tokens, old, A, ref, kl=0.1, ent=ent, weights=w, reduction="none")
 
 
+@pytest.mark.parametrize("N,V", [(1, 3), (127, 255), (512, 100), (513, 100), (700, 255), (128, 255)])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_policy_of_short_rows(device, N, V, reduction):
+    """Rows of one chunk, with their weights added by whom it concerns and by a launch of its own."""
+    x, tokens, old, A, ref = policy_inputs(device, (N,), V, "bf16", N + V)
+    tokens[N // 3] = -1 if N > 1 else tokens[0]
+    w = torch.rand(N, device=device) + 0.5
+    check_policy(x, tokens, old, A, ref, kl=0.1, ent=0.01, weights=w, reduction=reduction)
+    check_policy(x, tokens, old, A, reduction=reduction)
+
+
 def test_policy_clips(device):
     """Every side of the clip for both signs; a zero advantage; a border itself."""
     V = 64
@@ -507,6 +518,32 @@ def test_preference_padded(device, shape):
     ref = make(device, shape[:1], "fp32", 34) - 6.0 * shape[1]
     check_preference(x, tokens, ref)
     check_preference(x, tokens, ref, average=True, kind="squared", beta=0.5)
+
+
+@pytest.mark.parametrize("B", [2048, 2049, 5000])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_many_pairs(device, B, weighted):
+    """Whose weights are added once for all of them.  Between the inputs and a value lie at most 20 roundings
+    in the sum of the weights, 20 in that of the losses (20 terms a thread, 8 levels of a tree, within a bound
+    of 2^-24 each) and 24 others: 2^-18, of which the bars are twice; and a margin is off by four bounds of a
+    log-probability."""
+    V, beta = 9, 0.2
+    x = leaf(make(device, (2 * B, 1, V), "fp32", 35))
+    gen = torch.Generator(device=device).manual_seed(36)
+    tokens = torch.randint(0, V, (2 * B, 1), device=device, generator=gen)
+    w = torch.rand(B, device=device, generator=gen) + 0.1 if weighted else None
+    got = preference_loss(x, tokens, beta=beta, weights=w)
+    grad, = torch.autograd.grad(got.loss, x)
+    y = leaf(x.detach().double())
+    lp = torch.log_softmax(y, -1).gather(-1, tokens[..., None])[:, 0, 0]
+    f = torch.ones(B, device=device, dtype=torch.float64) if w is None else w.double()
+    f = f / f.sum()
+    loss = (f * torch.nn.functional.softplus(-beta * (lp[:B] - lp[B:]))).sum()
+    slope, = torch.autograd.grad(loss, y)
+    off = float(np.max(lp_bound(host(lp.detach()))))
+    assert abs(float(got.loss) - float(loss)) <= 2.0 ** -17 * float(loss) + 4 * beta * off
+    bar = beta * f.repeat(2)[:, None, None] * (2.0 ** -17 + 4 * beta * off + 2 * off)
+    assert ((grad.double() - slope).abs() <= bar).all()
 
 
 def test_preference_far_margins(device):
@@ -654,6 +691,34 @@ def test_backward_twice_and_scaled(device, N, V):
         loss.backward(retain_graph=True)
         loss.backward()
         assert ((y.grad - 2 * kept).abs() <= kept.abs() * 2.0 ** -20 + tiny).all(), name
+
+
+@pytest.mark.parametrize("N,V", SHAPES)
+def test_saved_tensors_that_move(device, N, V):
+    """What the backward pass needs may be kept elsewhere and come back to another place."""
+    x, ops = calls(device, N, V)
+    for name, op in ops.items():
+        y, z = leaf(x), leaf(x)
+        want, = torch.autograd.grad(op(y), y)
+        with torch.autograd.graph.save_on_cpu():
+            loss = op(z)
+        got, = torch.autograd.grad(loss, z, retain_graph=True)
+        assert torch.equal(got, want), name
+        again, = torch.autograd.grad(loss, z)
+        assert torch.equal(again, want), name
+
+
+@pytest.mark.parametrize("N,V", SHAPES)
+def test_recomputed(device, N, V):
+    """Forgotten in the forward pass and formed again in the backward pass."""
+    from torch.utils.checkpoint import checkpoint
+    x, ops = calls(device, N, V)
+    for name, op in ops.items():
+        for reentrant in (False, True):
+            y, z = leaf(x), leaf(x)
+            op(y).backward()
+            checkpoint(op, z, use_reentrant=reentrant).backward()
+            assert torch.equal(y.grad, z.grad), name
 
 
 def test_through_a_graph_of_layers(device):

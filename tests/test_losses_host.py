@@ -90,6 +90,16 @@ def test_refusals_of_the_gradient(kind, change, up, status):
     assert nat.lib().mvsd_loss_gradient(ctypes.byref(args(kind, **change)), *up, None) == status
 
 
+@pytest.mark.parametrize("kind,change", [
+    (POLICY, {}), (POLICY, {"num_rows": 4096, "reduction": 2}), (DISTILL, {}), (PREFERENCE, {}),
+    (LOGPROBS, {"num_rows": 4096, "vocab_size": 50257})])
+def test_a_gradient_that_no_call_wrote(kind, change):
+    """Only values of one pass write the gradient of an upstream of 1."""
+    a = args(kind, unit_gradient=1, **change)
+    assert nat.lib().mvsd_loss_one_pass(ctypes.byref(a)) == 0
+    assert nat.lib().mvsd_loss_gradient(ctypes.byref(a), P, 0, None, 0, None) == INVALID
+
+
 def test_null_arguments():
     lib = nat.lib()
     assert lib.mvsd_row_loss(None, None) == INVALID

@@ -207,7 +207,8 @@ __device__ inline void sum_losses(const LossParams& p, int64_t n) {
 __device__ inline void sum_by_the_last(const LossParams& p, int64_t n) {
   if (p.a.reduction == MVSD_REDUCE_NONE) return;
   __shared__ int s_last;
-  __syncthreads();  // all of the workgroup's losses are stored
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // each wave's losses have left it: a barrier waits for no stores
+  __syncthreads();
   if (threadIdx.x == 0) s_last = atomic_add_acq_rel(p.counters + 1, 1) == (int)gridDim.x - 1;
   __syncthreads();
   if (s_last) sum_losses(p, n);
@@ -219,14 +220,16 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(LossParams p, int64_t n)
 
 // ------------------------------------------------------------------ the mean's divisor ----------
 
-// Partial sums of the weights of the rows that are not left out.
+// Partial sums of the weights of the rows that are not left out, or of the pairs.
 __global__ __launch_bounds__(kLossThreads) void loss_norm_kernel(LossParams p) {
   __shared__ float scratch[kWaves];
-  const int64_t each = (p.a.num_rows + gridDim.x - 1) / gridDim.x;
-  const int64_t first = blockIdx.x * each, last = min(p.a.num_rows, first + each);
+  const bool pairs = p.a.kind == MVSD_LOSS_PREFERENCE;
+  const int64_t n = pairs ? p.a.num_pairs : p.a.num_rows;
+  const int64_t each = (n + gridDim.x - 1) / gridDim.x;
+  const int64_t first = blockIdx.x * each, last = min(n, first + each);
   float sum[1] = {0.f};
-  for (int64_t row = first + threadIdx.x; row < last; row += kLossThreads)
-    if (token_at(p.a, row, p.V) >= 0) sum[0] += row_weight(p.a, row);
+  for (int64_t i = first + threadIdx.x; i < last; i += kLossThreads)
+    if (pairs || token_at(p.a, i, p.V) >= 0) sum[0] += p.a.weights ? p.a.weights[i] : 1.f;
   block_sum<1>(sum, scratch);
   if (threadIdx.x == 0) p.norm[blockIdx.x] = sum[0];
   if (blockIdx.x == 0) clear_counters(p);
@@ -471,9 +474,12 @@ __global__ __launch_bounds__(kLossThreads) void loss_pairs_kernel(LossParams p) 
   const int64_t pair = blockIdx.x, B = a.num_pairs, N = a.num_rows;
   float w = a.weights ? a.weights[pair] : 1.f;
   if (a.reduction == MVSD_REDUCE_MEAN) {
-    float all[1] = {0.f};
-    for (int64_t i = threadIdx.x; i < B; i += kLossThreads) all[0] += a.weights ? a.weights[i] : 1.f;
+    float all[1] = {0.f};  // of many pairs, loss_norm_kernel's sums
+    const float* some = p.norm_parts ? p.norm : a.weights;
+    const int n = p.norm_parts ? p.norm_parts : (int)B;
+    for (int i = threadIdx.x; some && i < n; i += kLossThreads) all[0] += some[i];
     block_sum<1>(all, scratch);
+    if (!some) all[0] = (float)B;
     w = all[0] == 0.f ? 0.f : w / all[0];
   }
   int64_t begin[2], end[2];
@@ -1310,7 +1316,8 @@ int64_t aside_bytes(const mvsd_loss_args& a) {
 
 constexpr int64_t kMaxMarked = 3 << 16;  // columns whose two sets of marks are 48 KiB
 
-constexpr int64_t kFewRows = 512;  // whose weights every wave adds by itself (a launch less)
+constexpr int64_t kFewRows = 512;    // whose weights every wave adds by itself (a launch less)
+constexpr int64_t kFewPairs = 2048;  // the same of pairs and workgroups
 constexpr int64_t kCacheBytes = 256ll << 20;  // of the last level
 
 LossParams make_params(const mvsd_loss_args& a) {
@@ -1349,6 +1356,8 @@ LossParams make_params(const mvsd_loss_args& a) {
     p.norm_parts = (int)std::min((N + kWaves - 1) / kWaves, (int64_t)kNormParts);
   else if (a.kind == MVSD_LOSS_POLICY && a.reduction != MVSD_REDUCE_NONE && (N > kFewRows || loss_one_pass(a)))
     p.norm_parts = (int)std::min(N / 64 + 1, (int64_t)kNormParts);
+  else if (a.kind == MVSD_LOSS_PREFERENCE && a.reduction == MVSD_REDUCE_MEAN && a.weights && a.num_pairs > kFewPairs)
+    p.norm_parts = (int)std::min(a.num_pairs / 1024 + 1, (int64_t)kNormParts);
   // a workgroup that counts itself needs counters that an earlier launch cleared
   p.whole = p.nch == 1 && (a.kind != MVSD_LOSS_POLICY || a.reduction == MVSD_REDUCE_NONE || p.norm_parts > 0);
   return p;
@@ -1378,7 +1387,7 @@ template <int DT>
 hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
   const mvsd_loss_args& a = p.a;
   const dim3 grid((unsigned)(a.num_rows * p.nch)), block(kLossThreads);
-  if (p.norm_parts) {
+  if (p.norm_parts && a.kind != MVSD_LOSS_PREFERENCE) {
     if (has_list(a))
       hipLaunchKernelGGL(p.K <= kWave       ? loss_teacher_kernel<1>
                          : p.K <= 2 * kWave ? loss_teacher_kernel<2>
@@ -1468,6 +1477,8 @@ hipError_t launch_loss(const mvsd_loss_args& a, hipStream_t stream) {
     }
     if (err != hipSuccess) return err;
   }
+  if (a.kind == MVSD_LOSS_PREFERENCE && p.norm_parts)
+    hipLaunchKernelGGL(loss_norm_kernel, dim3(p.norm_parts), dim3(kLossThreads), 0, stream, p);
   if (a.kind == MVSD_LOSS_PREFERENCE && a.num_pairs > 0)
     hipLaunchKernelGGL(loss_pairs_kernel, dim3((unsigned)a.num_pairs), dim3(kLossThreads), 0, stream, p);
   const int64_t losses = a.kind == MVSD_LOSS_PREFERENCE ? a.num_pairs : a.num_rows;
@@ -1588,6 +1599,7 @@ int mvsd_loss_gradient(const mvsd_loss_args* args, const float* upstream, int64_
   const mvsd_loss_args& a = *args;
   if (a.num_rows == 0) return MVSD_OK;
   if (!a.grad || up_stride < 0 || up_entropy_stride < 0) return MVSD_E_INVALID;
+  if (a.unit_gradient && !mvsd::loss_one_pass(a)) return MVSD_E_INVALID;
   if (!upstream && a.kind != MVSD_LOSS_LOGPROBS) return MVSD_E_INVALID;
   if (!a.saved || misaligned(a.saved)) return MVSD_E_WORKSPACE;
   return mvsd::record_hip_error(mvsd::launch_loss_gradient(a, upstream, up_stride, upstream_entropy,
