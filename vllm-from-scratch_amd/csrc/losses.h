@@ -21,6 +21,19 @@ struct LossRecord {
 };
 static_assert(sizeof(LossRecord) == kRecord * sizeof(float));
 
+// What a row's entries give without the rest of the row: their maximum, and sums of e_k = exp((x_k - top) / T)
+// and of what the divergence needs.
+struct EntrySums {
+  float top, z, s1, s2;
+};
+
+struct LossTeacher {
+  EntrySums sums;
+  float value;   // the mass of the rest, or without a tail the log of the entries' sum
+  float weight;  // 0: the row is left out
+  float unused[2];
+};
+
 struct LossParams {
   mvsd_loss_args a;
   float c1;     // log2(e) / temperature
@@ -38,7 +51,8 @@ struct LossParams {
   int* counters;      // [2], see losses.hip
   float* row_loss;    // [N] (preference: [pairs]), weighted
   float* row_lp;      // preference: [N]
-  float2* teach;      // distillation: [N] what the teacher's kernel gives of a row, its weight (0: left out)
+  LossTeacher* teach;   // distillation: [N]
+  float* entry_logits;  // [N, K]
   LossRecord* records;    // [N] or null
   float* over;            // distillation: [N, K] gradients of the given tokens for unit upstream
   int32_t* over_ids;      // [N, K] the entries that count, -1: none

@@ -391,7 +391,7 @@ __global__ __launch_bounds__(kLossThreads) void loss_stats_kernel(LossParams p) 
   int token = -1;
   if (!LIST && p.norm_parts == 0 && blockIdx.x == 0) clear_counters(p);  // a later kernel counts
   if constexpr (LIST) {
-    if (p.teach[row].y == 0.f) return;
+    if (p.teach[row].weight == 0.f) return;
     for (int i = threadIdx.x; i < (p.chunk + 31) / 32; i += kLossThreads) bits[i] = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < p.K; k += kLossThreads) {
@@ -554,10 +554,15 @@ __device__ inline double wave_sum_f64(double v) {
   return v;
 }
 
-// The teacher's side, a wave a row: which entries count (over_ids, -1: not), the mass of the rest (0 where
-// the rest is no outcome) or, without a tail, the log of the entries' sum, the row's weight (0: left out),
-// and the partial sums of the weights.
-template <int E>  // entries a lane
+__device__ inline void teacher_of(const LossParams& p, float v, float teacher, float& q, float& log_q) {
+  log_q = p.a.tail ? v : v * p.inv_t - teacher;
+  q = expf(log_q);
+}
+
+// What needs the row's given tokens alone, a wave a row: which entries count (over_ids, -1: not) and their
+// logits; the mass of the rest (0 where the rest is no outcome) or, without a tail, the log of the entries'
+// sum; the row's weight (0: left out) and the partial sums of the weights; the entries' sums.
+template <int DT, int E>  // entries a lane
 __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p) {
   __shared__ __attribute__((aligned(16))) int s_ids[kWaves][E * kWave];
   __shared__ float scratch[kWaves];
@@ -623,8 +628,42 @@ __global__ __launch_bounds__(kLossThreads) void loss_teacher_kernel(LossParams p
       value = top * p.inv_t + logf(wave_sum(sum));
     }
     const float w = count == 0 ? 0.f : row_weight(a, row);
-    if (lane == 0) p.teach[row] = make_float2(value, w);
     weights[0] += w;
+    EntrySums sums = {0.f, 0.f, 0.f, 0.f};
+    if (w != 0.f) {
+      const auto* x = logits_row<DT>(a, row);
+      float g[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (i * kWave < K) g[i] = id[i] >= 0 && id[i] < p.V ? Elem<DT>::cvt(x[id[i]]) : id[i] < 0 ? -INFINITY : NAN;
+      top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (i * kWave >= K) break;
+        if (g[i] == INFINITY) g[i] = NAN;
+        top = fmaxf(top, g[i]);
+      }
+      sums.top = top = base_of(wave_max(top));
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (i * kWave >= K) break;
+        const int k = i * kWave + lane;
+        if (k < K) p.entry_logits[row * K + k] = g[i];
+        const float d = (g[i] - top) * p.inv_t, e = expf(d);
+        float q, log_q;
+        teacher_of(p, v[i], value, q, log_q);
+        if (id[i] < 0) continue;
+        sums.z += e;
+        if (a.divergence == MVSD_KL_FORWARD) {
+          sums.s1 += q == 0.f ? 0.f : q * (log_q - d);
+          sums.s2 += q;
+        } else {
+          sums.s1 += e == 0.f ? 0.f : e * (d - log_q);
+        }
+      }
+      sums = {top, wave_sum(sums.z), wave_sum(sums.s1), wave_sum(sums.s2)};
+    }
+    if (lane == 0) p.teach[row] = {sums, value, w, 0.f, 0.f};
   }
   if (lane != 0) weights[0] = 0.f;
   block_sum<1>(weights, scratch);
@@ -640,23 +679,17 @@ struct Entries {
 };
 
 template <int E>
-__device__ inline void load_entries(const LossParams& p, int64_t row, int T, Entries<E>& in) {
+__device__ inline void load_entry_values(const LossParams& p, int64_t row, int T, Entries<E>& in) {
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int k = i * T + (int)threadIdx.x;
-    in.id[i] = -1;
     in.v[i] = 0.f;
+    in.x[i] = -INFINITY;
     if (k < p.K) {
-      in.id[i] = p.over_ids[row * p.K + k];
       in.v[i] = p.a.teacher_logprobs[row * p.K + k];
+      in.x[i] = p.entry_logits[row * p.K + k];
     }
   }
-}
-template <int DT, int E>
-__device__ inline void load_entry_logits(const LossParams& p, int64_t row, Entries<E>& in) {
-  const auto* x = logits_row<DT>(p.a, row);
-#pragma unroll
-  for (int i = 0; i < E; ++i) in.x[i] = in.id[i] >= 0 && in.id[i] < p.V ? Elem<DT>::cvt(x[in.id[i]]) : NAN;
 }
 
 __device__ inline float sum16(float v) {
@@ -666,7 +699,7 @@ __device__ inline float sum16(float v) {
   return v + dpp_f32<kDppMirror>(v);
 }
 
-// Sums (or maxima) over the NW waves of a workgroup, in one order; two barriers.
+// Sums over the NW waves of a workgroup, in one order; two barriers.
 template <int N>
 __device__ inline void waves_sum(float (&v)[N], float* red, int NW) {
 #pragma unroll
@@ -681,60 +714,6 @@ __device__ inline void waves_sum(float (&v)[N], float* red, int NW) {
   for (int g = 0; g < N; ++g) v[g] = readlane_f32(sum16(part < NW ? red[g * NW + part] : 0.f), 0);
   __syncthreads();
 }
-__device__ inline float waves_max(float v, float* red, int NW) {
-  v = wave_max(v);
-  if (lane_id() == 0) red[wave_id()] = v;
-  __syncthreads();
-  const int part = lane_id() % 16;
-  v = readlane_f32(max16(part < NW ? red[part] : -INFINITY), 0);
-  __syncthreads();
-  return v;
-}
-
-// What a row's entries give without the rest of the row, over a workgroup: their maximum, and sums of
-// e_k = exp((x_k - top) / T) and of what the divergence needs.
-struct EntrySums {
-  float top, z, s1, s2;
-};
-
-template <int E>
-__device__ inline void teacher_of(const LossParams& p, const Entries<E>& in, int i, float teacher, float& q,
-                                  float& log_q) {
-  log_q = p.a.tail ? in.v[i] : in.v[i] * p.inv_t - teacher;
-  q = expf(log_q);
-}
-
-// red holds 3 NW floats.
-template <int E>
-__device__ inline EntrySums sum_entries(const LossParams& p, float teacher, float* red, int NW, Entries<E>& in) {
-  const mvsd_loss_args& a = p.a;
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    if (in.id[i] < 0) in.x[i] = -INFINITY;
-    if (in.x[i] == INFINITY) in.x[i] = NAN;
-    top = fmaxf(top, in.x[i]);
-  }
-  top = base_of(waves_max(top, red, NW));
-  float v[3] = {0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float d = (in.x[i] - top) * p.inv_t, e = expf(d);
-    float q, log_q;
-    teacher_of(p, in, i, teacher, q, log_q);
-    if (in.id[i] < 0) continue;
-    v[0] += e;
-    if (a.divergence == MVSD_KL_FORWARD) {
-      v[1] += q == 0.f ? 0.f : q * (log_q - d);
-      v[2] += q;
-    } else {
-      v[1] += e == 0.f ? 0.f : e * (d - log_q);
-    }
-  }
-  waves_sum<3>(v, red, NW);
-  return {top, v[0], v[1], v[2]};
-}
-
 // One row's loss by a workgroup of NW waves, from the statistics of its rest, its entries and what the
 // teacher's kernel gave of it.  Gives the gradients of the given tokens (over, at id, -1: none) and returns
 // the loss; *k is the record's.  `weight` is the row's, after the mean.  With d_k = (x_k - top) / T and lz the
@@ -766,7 +745,7 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
   for (int i = 0; i < E; ++i) {
     const float lp = (in.x[i] - k.top) * p.inv_t - lz;
     float q, log_q, term = 0.f;
-    teacher_of(p, in, i, teacher, q, log_q);
+    teacher_of(p, in.v[i], teacher, q, log_q);
     pr[i] = expf(lp);
     pd[i] = 0.f;
     if (in.id[i] >= 0) outcome(q, log_q, pr[i], lp, term, pd[i]);
@@ -808,18 +787,21 @@ __device__ inline void save_over(const LossParams& p, int64_t row, int T, const 
 }
 
 // A workgroup a row.
-template <int DT>
 __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossParams p) {
   constexpr int E = kMaxTeacher / kLossThreads;
-  __shared__ float red[3 * kWaves];
+  __shared__ float red[2 * kWaves];
   const int64_t row = blockIdx.x;
-  const float2 teacher = p.teach[row];
+  const LossTeacher teacher = p.teach[row];
   float loss = 0.f;
   LossRecord rec = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0};
-  if (teacher.y != 0.f) {
+  if (teacher.weight != 0.f) {
     Entries<E> in;
-    load_entries<E>(p, row, kLossThreads, in);
-    load_entry_logits<DT>(p, row, in);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int k = i * kLossThreads + (int)threadIdx.x;
+      in.id[i] = k < p.K ? p.over_ids[row * p.K + k] : -1;
+    }
+    load_entry_values<E>(p, row, kLossThreads, in);
     Stat st = {-INFINITY, 0.f, 0.f};
     for (int i = lane_id(); i < p.nch; i += kWave) {
       const float4 v = p.parts[row * p.nch + i];
@@ -829,8 +811,8 @@ __global__ __launch_bounds__(kLossThreads) void loss_distill_rows_kernel(LossPar
     rec.M = base_of(st.m);
     rec.c = 1.f;
     float over[E];
-    const EntrySums sums = sum_entries<E>(p, teacher.x, red, kWaves, in);
-    loss = distill_row<E>(p, st, sums, teacher.x, teacher.y * mean_factor(p), red, kWaves, in, over, &rec.k);
+    loss = distill_row<E>(p, st, teacher.sums, teacher.value, teacher.weight * mean_factor(p), red, kWaves, in, over,
+                          &rec.k);
     if (p.records) save_over<E>(p, row, kLossThreads, over);
   }
   if (threadIdx.x == 0) {
@@ -979,7 +961,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   constexpr int VEC = Elem<DT>::kVec, E = 1, kDelay = NV > 4 ? 4 : 2;
   extern __shared__ uint32_t bits[];
   __shared__ float4 s_part[2][kRowThreads / kWave];
-  __shared__ float red[3 * kRowThreads / kWave];
+  __shared__ float red[2 * kRowThreads / kWave];
   __shared__ int s_ticket[2], s_next;  // two of what is read behind a turn's one barrier: a wave may be a turn ahead
   const mvsd_loss_args& a = p.a;
   const int tid = threadIdx.x, V = p.V, N = (int)a.num_rows, T = blockDim.x, NW = T / kWave;
@@ -997,10 +979,10 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
 
   // What a row is given beside its logits, and what its gradient is formed from.
   int row = blockIdx.x, ticket = 0, token = -1, parity = 0;
-  float w = 0.f, teacher = 0.f, xt = NAN;
+  float w = 0.f, xt = NAN;
   PolicyIn given = {0.f, 0.f, 0.f};
   Entries<E> in = {};
-  EntrySums sums = {0.f, 0.f, 0.f, 0.f};
+  LossTeacher teacher = {};
   const S* x = nullptr;
   int cur = -1, cur_token = -1, pend_id[E];
   float pend[E], cur_M = 0.f, at_token = 0.f;
@@ -1010,15 +992,13 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
 #pragma unroll
   for (int i = 0; i < E; ++i) pend_id[i] = -1;
   // of the row after it, loaded while this one's loss is formed
-  Entries<E> after = {};
-  float2 teach = {0.f, 0.f};
-  int next_token = -1;
+  int next_token = -1, next_id = -1;
   float next_w = 0.f;
   auto announce = [&](int n) {
     if (n >= N) return;
     if constexpr (LIST) {
-      load_entries<E>(p, n, T, after);
-      teach = p.teach[n];
+      if (tid < p.K) next_id = p.over_ids[(int64_t)n * p.K + tid];
+      next_w = p.teach[n].weight;
     } else {
       next_token = token_at(a, n, V);
       next_w = row_weight(a, n);
@@ -1028,13 +1008,11 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
   auto advance = [&]() {
     for (; row < N; announce(row)) {
       if constexpr (LIST) {
-        in = after;
-        teacher = scalar(teach.x);
-        w = scalar(teach.y);
+        in.id[0] = next_id;
       } else {
         token = __builtin_amdgcn_readfirstlane(next_token);
-        w = scalar(next_w);
       }
+      w = scalar(next_w);
       if (w != 0.f && (LIST || token >= 0)) break;
       if (tid == 0) {
         p.row_loss[row] = 0.f;
@@ -1137,14 +1115,13 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
 #pragma unroll
       for (int n = 0; n < E; ++n)
         if (in.id[n] >= 0 && in.id[n] < V) atomicOr(&marked[in.id[n] >> 5], 1u << (in.id[n] & 31));
-      load_entry_logits<DT>(p, row, in);
       __syncthreads();
     }
 #pragma unroll
     for (int i = kDelay; i < NV; ++i) vector(i);
-    if (LIST && more) {  // while the last ones come
-      sums = sum_entries<E>(p, teacher, red, NW, in);
-      sums = {scalar(sums.top), scalar(sums.z), scalar(sums.s1), scalar(sums.s2)};
+    if (LIST && more) {  // what finish() needs, behind the vectors
+      teacher = p.teach[row];
+      load_entry_values<E>(p, row, T, in);
     }
 #pragma unroll
     for (int i = NV; i < NV + kDelay; ++i) vector(i);
@@ -1205,7 +1182,7 @@ __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p)
       marked = marked == bits ? bits + words : bits;
       rec.M = base_of(st.m);
       rec.c = 1.f;
-      loss = distill_row<E>(p, st, sums, teacher, w * mean, red, NW, in, pend, &rec.k);
+      loss = distill_row<E>(p, st, teacher.sums, teacher.value, w * mean, red, NW, in, pend, &rec.k);
       if (p.records) save_over<E>(p, row, T, pend);
 #pragma unroll
       for (int i = 0; i < E; ++i) pend_id[i] = in.id[i];
@@ -1343,8 +1320,10 @@ LossParams make_params(const mvsd_loss_args& a) {
   p.row_loss = a.reduction == MVSD_REDUCE_NONE && a.loss ? a.loss : reinterpret_cast<float*>(w);
   w += up16(std::max(N, a.num_pairs) * 4);
   p.row_lp = reinterpret_cast<float*>(w);
-  p.teach = reinterpret_cast<float2*>(w);  // of a distillation, which has no row_lp
-  w += up16(N * 8);
+  p.teach = reinterpret_cast<LossTeacher*>(w);  // of a distillation, which has no row_lp
+  w += up16(N * (has_list(a) ? (int64_t)sizeof(LossTeacher) : 4));
+  p.entry_logits = reinterpret_cast<float*>(w);
+  if (has_list(a)) w += up16(N * p.K * 4);
   p.over_ids = reinterpret_cast<int32_t*>(w);
   if (a.saved) {
     p.records = static_cast<LossRecord*>(a.saved);
@@ -1389,9 +1368,9 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)(a.num_rows * p.nch)), block(kLossThreads);
   if (p.norm_parts && a.kind != MVSD_LOSS_PREFERENCE) {
     if (has_list(a))
-      hipLaunchKernelGGL(p.K <= kWave       ? loss_teacher_kernel<1>
-                         : p.K <= 2 * kWave ? loss_teacher_kernel<2>
-                                            : loss_teacher_kernel<kMaxTeacher / kWave>,
+      hipLaunchKernelGGL((p.K <= kWave       ? loss_teacher_kernel<DT, 1>
+                          : p.K <= 2 * kWave ? loss_teacher_kernel<DT, 2>
+                                             : loss_teacher_kernel<DT, kMaxTeacher / kWave>),
                          dim3(p.norm_parts), block, 0, stream, p);
     else
       hipLaunchKernelGGL(loss_norm_kernel, dim3(p.norm_parts), block, 0, stream, p);
@@ -1413,7 +1392,7 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
   if (has_list(a)) {
     const unsigned lds = (unsigned)((p.chunk + 31) / 32 * 4);
     hipLaunchKernelGGL((loss_stats_kernel<DT, true, false>), grid, block, lds, stream, p);
-    hipLaunchKernelGGL(loss_distill_rows_kernel<DT>, dim3((unsigned)a.num_rows), block, 0, stream, p);
+    hipLaunchKernelGGL(loss_distill_rows_kernel, dim3((unsigned)a.num_rows), block, 0, stream, p);
   } else {
     if (p.entropy)
       hipLaunchKernelGGL((loss_stats_kernel<DT, false, true>), grid, block, 0, stream, p);
@@ -1458,8 +1437,8 @@ int64_t loss_workspace_bytes(const mvsd_loss_args& a) {
   const int64_t chunk = chunk_of(a.num_rows, (int)a.vocab_size, a.dtype);
   const int64_t nch = (a.vocab_size + chunk - 1) / chunk;
   return aside_bytes(a) + a.num_rows * nch * (int64_t)sizeof(float4) + kNormParts * 4 + 16 +
-         up16(std::max(a.num_rows, a.num_pairs) * 4) + up16(a.num_rows * 8) +
-         (has_list(a) ? a.num_rows * a.num_teacher * 4 : 0);
+         up16(std::max(a.num_rows, a.num_pairs) * 4) + up16(a.num_rows * (has_list(a) ? (int64_t)sizeof(LossTeacher) : 4)) +
+         (has_list(a) ? 2 * up16(a.num_rows * a.num_teacher * 4) : 0);
 }
 
 int64_t loss_saved_bytes(const mvsd_loss_args& a) {
