@@ -22,6 +22,11 @@ in their own dtype; every other argument is a constant.  Values and losses are f
 Reductions: "mean" is sum(w * l) / sum(w) over the rows that are not left out (0 if there are none),
 "sum" is sum(w * l), so weights carry any other normalisation and loss scales, "none" the w * l.
 
+A policy or distillation loss that is a scalar over many rows forms the logits' gradient for an upstream
+of 1 in the forward pass, where it reads them, and keeps it until the backward pass; for another upstream
+the rows are read again (a scale in ``weights`` with "sum" avoids that).  Leave rows out by their ids
+instead of indexing the logits, which copies them.
+
 Nothing here synchronises the host; work is enqueued on the current stream of the logits' device and may
 be captured into a graph.  Before a backward pass is captured, release graphs of the same leaves that ran
 eagerly (torch ends the process otherwise).
