@@ -974,7 +974,7 @@ __device__ inline float scalar(float v) { return readlane_f32(v, 0); }
 // Bytes read and written a second (a copy: 5.25 TB/s): 2048 policy rows of 151936 bf16 248 us, 4.8 TB/s; 2000 of
 // 32001 fp32 with entropies 117 us, 4.4; distillation, 1024 rows of 151936 bf16 and 33 entries, 149 us, 4.2, 2048
 // of 128 entries 277 us, 4.4; 4096 of 32000 fp16 133 us, 4.0.  What is lost: the gap between two turns, and in a
-// distillation the marks (5 us of 160) and the entries' own values, which follow the row's stores.
+// distillation the marks (4 us of 160) and the entries' own values, which follow the row's stores (3; 17 of 298).
 template <int DT, int NV, bool LIST, bool ENT, bool WANT>
 __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p) {
   using S = typename Elem<DT>::storage;
