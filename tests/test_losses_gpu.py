@@ -929,3 +929,38 @@ def test_refusals(device):
         with pytest.raises(error):
             call()
             print("accepted:", k)
+
+
+# --------------------------------------------------------------------------- masked entries
+
+DIVERGENCES = [("forward", True), ("forward", False), ("reverse", True), ("js", True)]
+
+
+def masked_entries(device, dtype, N, base, T, value=-math.inf):
+    """Rows around `base` whose entries have the logit `value`: all of them in every third row (the first
+    one among them), two of four in the next, none in the last."""
+    x = make(device, (N, 600), dtype, 101, spread=3.0 * min(T, 1.0)).float() + base
+    gen = torch.Generator(device=device).manual_seed(102)
+    ids = torch.rand((N, 600), device=device, generator=gen).argsort(dim=1)[:, :4].int()
+    gone = torch.ones(N, 4, dtype=torch.bool, device=device)
+    gone[1::3, 2:] = False
+    gone[2::3] = False
+    x.scatter_(1, ids.long(), torch.where(gone, value, x.gather(1, ids.long())))
+    teacher = torch.log_softmax(make(device, (N, 5), "fp32", 103, spread=1.0), dim=1)[:, :4].contiguous()
+    return x.to(DTYPES[dtype]), ids, teacher
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("how,tail", DIVERGENCES)
+@pytest.mark.parametrize("N", [3, 100])
+def test_distillation_entries_without_mass(device, dtype, how, tail, N):
+    """The student gives none of a row's entries any mass; its other logits lie anywhere.  By workgroups that
+    share a row, and in one pass."""
+    for base, T in ((0.0, 1.0), (-60.0, 1.0), (-110.0, 1.0), (-300.0, 1.0), (300.0, 1.0), (-40.0, 0.3),
+                    (-10.0, 0.1), (10.0, 0.1)):
+        x, ids, teacher = masked_entries(device, dtype, N, base, T)
+        for reduction in ("mean", "none"):
+            loss, grad = check_distill(x, ids, teacher, how, tail, T, reduction=reduction)
+            assert torch.isfinite(grad).all()
+            assert not torch.isnan(loss).any()
+            assert bool(torch.isfinite(loss).all()) == (how != "forward")

@@ -738,7 +738,9 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
                                     float* red, int NW, Entries<E>& in, float (&over)[E], float* k_out) {
   const mvsd_loss_args& a = p.a;
   const bool tail = a.tail && teacher != 0.f;
-  const float rest_d = st.m == -INFINITY ? 0.f : (st.m - k.top) * p.inv_t, far = fmaxf(rest_d, 0.f);
+  // entries that are all masked have no maximum: the rest's is the row's
+  const float top = k.z == 0.f ? base_of(st.m) : k.top;
+  const float rest_d = st.m == -INFINITY ? 0.f : (st.m - top) * p.inv_t, far = fmaxf(rest_d, 0.f);
   const float lz = far + logf(k.z * expf(-far) + st.s * expf(rest_d - far));
   const float rest_lp = rest_d + logf(st.s) - lz, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
   // the divergence's term, and p dL/dp, of an outcome
@@ -757,7 +759,7 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
   float both[2] = {0.f, 0.f}, pr[E], pd[E];  // the sums of terms, and of p dL/dp
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    const float lp = (in.x[i] - k.top) * p.inv_t - lz;
+    const float lp = (in.x[i] - top) * p.inv_t - lz;
     float q, log_q, term = 0.f;
     teacher_of(p, in.v[i], teacher, q, log_q);
     pr[i] = expf(lp);
