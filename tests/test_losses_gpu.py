@@ -964,3 +964,17 @@ def test_distillation_entries_without_mass(device, dtype, how, tail, N):
             assert torch.isfinite(grad).all()
             assert not torch.isnan(loss).any()
             assert bool(torch.isfinite(loss).all()) == (how != "forward")
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("how", ["reverse", "js"])
+@pytest.mark.parametrize("N", [3, 100])
+def test_distillation_entries_far_below(device, dtype, how, N):
+    """Entries of a probability that is 0 in 64 bits too, one of which the teacher rules out: they add nothing
+    where the student's mass is the weight."""
+    for gap, T in ((1000.0, 1.0), (120.0, 0.1)):
+        x, ids, teacher = masked_entries(device, dtype, N, 0.0, T, -gap)
+        teacher[:, 1] = -math.inf
+        keep = torch.arange(N, device=device) % 3 == 0  # in the others an entry has mass
+        loss, grad = check_distill(x, torch.where(keep[:, None], ids, -1), teacher, how, True, T)
+        assert torch.isfinite(loss) and torch.isfinite(grad).all()

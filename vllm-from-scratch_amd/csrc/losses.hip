@@ -772,7 +772,9 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
     both[0] = k.s1 + lz * k.s2;
     both[1] = -k.s2;
   } else if (a.divergence == MVSD_KL_REVERSE) {
-    both[0] = both[1] = (k.s1 - lz * k.z) * expf(-lz);
+    // entries whose probabilities are all below fp32's range are 0, also where the teacher has none
+    const float scale = expf(-lz);
+    both[0] = both[1] = scale == 0.f && k.s1 == k.s1 ? 0.f : (k.s1 - lz * k.z) * scale;
   } else {
     waves_sum<2>(both, red, NW);
   }
