@@ -978,3 +978,32 @@ def test_distillation_entries_far_below(device, dtype, how, N):
         keep = torch.arange(N, device=device) % 3 == 0  # in the others an entry has mass
         loss, grad = check_distill(x, torch.where(keep[:, None], ids, -1), teacher, how, True, T)
         assert torch.isfinite(loss) and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("how,tail", DIVERGENCES)
+@pytest.mark.parametrize("N", [3, 100])
+def test_distillation_entries_masked_by_the_lowest_value(device, dtype, how, tail, N):
+    """Over a temperature below 1 it is beyond fp32, as -inf is: the same bits.  (-inf itself against the
+    oracle: above.)"""
+    low = torch.finfo(DTYPES[dtype]).min
+    for T in (0.9, 0.5, 0.01):
+        got = []
+        for value in (-math.inf, low):
+            x, ids, teacher = masked_entries(device, dtype, N, -5.0 * T, T, value)
+            x = leaf(x)
+            loss = distillation_loss(x, ids, teacher, divergence=how, tail=tail, temperature=T)
+            got.append((loss.detach(), torch.autograd.grad(loss, x)[0]))
+        assert torch.equal(got[0][0], got[1][0]) and not torch.isnan(got[1][0])
+        assert torch.equal(got[0][1], got[1][1]) and torch.isfinite(got[1][1]).all()
+
+
+def test_distillation_of_what_the_teacher_rules_out(device):
+    """Entries without a teacher's mass that the student masks by the lowest value: the tail alone counts."""
+    x, ids, _ = masked_entries(device, "fp32", 3, 0.0, 0.5, torch.finfo(torch.float32).min)
+    for N in (1, 100):
+        y = x[:1].expand(N, -1).contiguous()
+        for how in ("forward", "js"):
+            teacher = torch.full((N, 4), -math.inf, device=device)
+            loss, grad = check_distill(y, ids[:1].expand(N, 4).contiguous(), teacher, how, True, 0.5)
+            assert torch.isfinite(loss) and torch.isfinite(grad).all()

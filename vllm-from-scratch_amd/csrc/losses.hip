@@ -740,9 +740,11 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
   const bool tail = a.tail && teacher != 0.f;
   // entries that are all masked have no maximum: the rest's is the row's
   const float top = k.z == 0.f ? base_of(st.m) : k.top;
+  // infinite where a mask of the type's lowest value over T leaves fp32: the sum is against the larger maximum, and
+  // the rest's log-probability is formed without lz
   const float rest_d = st.m == -INFINITY ? 0.f : (st.m - top) * p.inv_t, far = fmaxf(rest_d, 0.f);
-  const float lz = far + logf(k.z * expf(-far) + st.s * expf(rest_d - far));
-  const float rest_lp = rest_d + logf(st.s) - lz, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
+  const float near = fminf(rest_d, 0.f), log_sum = logf(k.z * expf(-far) + st.s * expf(near)), lz = far + log_sum;
+  const float rest_lp = near + logf(st.s) - log_sum, rest_p = st.s > 0.f ? expf(rest_lp) : st.s;
   // the divergence's term, and p dL/dp, of an outcome
   auto outcome = [&](float q, float log_q, float pr, float lp, float& term, float& pd) {
     if (a.divergence == MVSD_KL_FORWARD) {
@@ -769,7 +771,7 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
     both[1] += pd[i];
   }
   if (a.divergence == MVSD_KL_FORWARD) {
-    both[0] = k.s1 + lz * k.s2;
+    both[0] = k.s2 == 0.f && lz == INFINITY ? k.s1 : k.s1 + lz * k.s2;
     both[1] = -k.s2;
   } else if (a.divergence == MVSD_KL_REVERSE) {
     // entries whose probabilities are all below fp32's range are 0, also where the teacher has none
