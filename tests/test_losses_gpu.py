@@ -1007,3 +1007,29 @@ def test_distillation_of_what_the_teacher_rules_out(device):
             teacher = torch.full((N, 4), -math.inf, device=device)
             loss, grad = check_distill(y, ids[:1].expand(N, 4).contiguous(), teacher, how, True, 0.5)
             assert torch.isfinite(loss) and torch.isfinite(grad).all()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("how,tail", DIVERGENCES)
+@pytest.mark.parametrize("N", [7, 100])
+def test_distillation_rows_without_a_distribution(device, dtype, how, tail, N):
+    """Their values and the whole of their gradients are NaN, whatever else is masked; the other rows' are not."""
+    V, inf = 600, math.inf
+    x, ids, teacher = masked_entries(device, dtype, N, 0.0, 1.0, -1.0)
+    first = ids[:, 0].long()
+    bad = x[1:6]
+    bad[:4].fill_(-inf)
+    bad[1, first[2]] = math.nan
+    bad[2, first[3]] = inf
+    bad[3, first[4]] = 0.0
+    ids[4, 1] = V              # an entry that is no token
+    bad[4, 5] = math.nan
+    x = leaf(x)
+    got = distillation_loss(x, ids, teacher, divergence=how, tail=tail, reduction="none")
+    none, = torch.autograd.grad(got.sum(), x)
+    each, = torch.autograd.grad(distillation_loss(x, ids, teacher, divergence=how, tail=tail, reduction="sum"), x)
+    rows = torch.arange(N, device=device)
+    wrong = (rows >= 1) & (rows < 6)
+    assert torch.equal(torch.isnan(got), wrong)
+    for grad in (none, each):
+        assert torch.isnan(grad[wrong]).all() and torch.isfinite(grad[~wrong]).all()

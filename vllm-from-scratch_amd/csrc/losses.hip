@@ -788,7 +788,10 @@ __device__ inline float distill_row(const LossParams& p, Stat st, const EntrySum
     both[1] += rest_pd;
   }
   const float f = weight * p.inv_t;
-  *k_out = st.s == 0.f ? 0.f : -f * (rest_pd - rest_p * both[1]) / st.s;
+  if (lz != lz || log_sum == -INFINITY)  // a NaN in the row, or nothing but -inf
+    *k_out = NAN;
+  else
+    *k_out = st.s == 0.f ? 0.f : -f * (rest_pd - rest_p * both[1]) / st.s;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     over[i] = f * (pd[i] - pr[i] * both[1]);
