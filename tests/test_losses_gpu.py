@@ -1033,3 +1033,32 @@ def test_distillation_rows_without_a_distribution(device, dtype, how, tail, N):
     assert torch.equal(torch.isnan(got), wrong)
     for grad in (none, each):
         assert torch.isnan(grad[wrong]).all() and torch.isfinite(grad[~wrong]).all()
+
+
+# --------------------------------------------------------------------------- tokens without others
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("V", [1, 2, 300])
+def test_a_token_alone_at_any_height(device, dtype, V):
+    """Nothing beside it: a log-probability and an entropy of 0, no gradient, also where its logit over the
+    temperature is beyond fp32; -inf itself is no distribution.  A mean of 120 values of -1 has the rounding of
+    1 / 120 and at most nine of a sum over 256 threads: within 10 * 2^-24 < 2^-20."""
+    low = torch.finfo(DTYPES[dtype]).min
+    heights = torch.tensor([low, -low, low / 2, 0.0, -1e4, 1e4, -math.inf], device=device).to(DTYPES[dtype])
+    N = 140
+    for T in (1e-6, 0.5, 1.0, 10.0):
+        x = torch.full((N, V), -math.inf, device=device, dtype=DTYPES[dtype])
+        x[:, V - 1] = heights.repeat(N // 7)
+        nothing = torch.isinf(x[:, V - 1])
+        tokens = torch.full((N,), V - 1, device=device)
+        y = leaf(x)
+        lp, H = token_logprobs(y, tokens, temperature=T, return_entropy=True)
+        grad, = torch.autograd.grad([lp, H], y, [torch.ones_like(lp), torch.ones_like(H)])
+        for rows in (lp, H, grad):
+            assert torch.isnan(rows[nothing]).all() and (rows[~nothing] == 0).all()
+        y = leaf(x)
+        got = policy_loss(y, tokens, None, torch.ones(N, device=device), entropy_coef=0.1, temperature=T,
+                          weights=~nothing)
+        grad, = torch.autograd.grad(got.loss, y)
+        assert abs(got.loss.item() + 1) <= 2.0 ** -20 and (grad == 0).all()

@@ -269,7 +269,8 @@ __device__ inline TokenRow token_row(const LossParams& p, Stat st, float x) {
   const float base = base_of(st.m);
   if (x == INFINITY) x = NAN;  // as inf - inf
   const float log_s = logf(st.s);
-  const float odds = log_s + (base - x) * p.inv_t;  // of all others against the token
+  // of all others against the token; one operation, so that an x / T beyond fp32 is finite beside a log_s of -inf
+  const float odds = fmaf(base - x, p.inv_t, log_s);
   const float z = expf(-fabsf(odds)), soft = log1pf(z);
   r.lp = -(fmaxf(odds, 0.f) + soft);
   const float log_q = -(fmaxf(-odds, 0.f) + soft);  // q = 1 - p
