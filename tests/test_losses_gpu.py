@@ -1062,3 +1062,35 @@ def test_a_token_alone_at_any_height(device, dtype, V):
                           weights=~nothing)
         grad, = torch.autograd.grad(got.loss, y)
         assert abs(got.loss.item() + 1) <= 2.0 ** -20 and (grad == 0).all()
+
+
+# --------------------------------------------------------------------------- memory
+
+
+def test_memory_between_the_passes(device):
+    """Recomputation and saved tensors on the host leave nothing of the logits' size on the device, and after a
+    backward pass nothing of it is left but the gradient."""
+    from torch.utils.checkpoint import checkpoint
+    N, V = 600, 5000
+    x, ops = calls(device, N, V, "fp32")
+    size = x.numel() * 4
+
+    def held(make):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        kept = make()
+        return torch.cuda.memory_allocated() - before, kept
+
+    for name, op in ops.items():
+        y = leaf(x)
+        more, loss = held(lambda: checkpoint(op, y, use_reentrant=False))
+        assert more < size / 4, name
+        assert held(loss.backward)[0] < size * 1.25, name
+        y = leaf(x)
+        with torch.autograd.graph.save_on_cpu():
+            more, loss = held(lambda: op(y))
+        assert more < size / 4, name
+        assert held(loss.backward)[0] < size * 1.25, name
+        y = leaf(x)
+        more, loss = held(lambda: op(y))
+        assert more + held(loss.backward)[0] < size * 1.25, name

@@ -118,8 +118,8 @@ def _values(t: torch.Tensor, name: str, shape, device) -> torch.Tensor:
 class _Call:
     """One call: its arguments and the tensors they point to."""
 
-    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "grad", "device",
-                 "layout")
+    __slots__ = ("args", "kind", "logits", "ids", "keep", "outputs", "saved", "grad", "fresh",
+                 "device", "layout")
 
     def __init__(self, kind: int, logits: torch.Tensor, temperature: float, reduction: int):
         if not logits.is_cuda:
@@ -132,7 +132,7 @@ class _Call:
         if not 1e-6 <= temperature <= 1e6:
             raise ValueError(f"temperature={temperature}")
         self.kind, self.logits, self.device = kind, logits, logits.device
-        self.keep, self.saved, self.grad = [], None, None
+        self.keep, self.saved, self.grad, self.fresh = [], None, None, True
         a = self.args = nat.LossArgs()
         a.kind, a.reduction, a.temperature = kind, reduction, temperature
         self._rows(logits)
@@ -196,17 +196,17 @@ class _Call:
             nat.check(status, "mvsd_row_loss")
         self.keep = None
 
-    def gradient(self, logits, ids, saved, upstream, upstream_entropy) -> torch.Tensor:
-        """The logits' gradient for the outputs' (a tensor may lie elsewhere than when it was saved)."""
+    def gradient(self, logits, ids, saved, unit, upstream, upstream_entropy) -> torch.Tensor:
+        """The logits' gradient for the outputs' (a tensor may lie elsewhere than when it was saved);
+        ``unit``: that of an upstream of 1, where it is there already, or None."""
         a = self.args
         if self.layout != (logits.data_ptr(), logits.stride()):
             self._rows(logits)
         a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr() or None
-        # that of an upstream of 1, which is there already, goes out once: a kept graph's next is made anew
-        grad, self.grad = self.grad, None
-        a.unit_gradient = 0 if grad is None else 1
-        if grad is None:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        # it goes out once, free to be changed (an alias without its version): a kept graph's next is made anew
+        fresh, self.fresh = self.fresh and unit is not None, False
+        a.unit_gradient = 1 if fresh else 0
+        grad = unit.data if fresh else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if grad.numel() == 0:
             return grad
         a.grad = grad.data_ptr()
@@ -226,15 +226,15 @@ class _Call:
 
 
 def _backward(ctx, upstream, *others):
-    logits, ids, saved = ctx.saved_tensors
-    call = ctx.call
+    logits, ids, saved, *unit = ctx.saved_tensors
+    call, unit = ctx.call, unit[0] if unit else None
     entropy = others[0] if call.kind == _LOGPROBS and others else None
     if upstream is None and entropy is None:
         return None, None
     if logits.device.index == torch.cuda.current_device():
-        return call.gradient(logits, ids, saved, upstream, entropy), None
+        return call.gradient(logits, ids, saved, unit, upstream, entropy), None
     with torch.cuda.device(logits.device):
-        return call.gradient(logits, ids, saved, upstream, entropy), None
+        return call.gradient(logits, ids, saved, unit, upstream, entropy), None
 
 
 class _RowLoss(torch.autograd.Function):
@@ -244,8 +244,13 @@ class _RowLoss(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if call.kind != _LOGPROBS and len(call.outputs) > 1:
             ctx.mark_non_differentiable(*call.outputs[1:])
-        ctx.save_for_backward(logits, call.ids, call.saved)
-        outputs, call.outputs, call.logits, call.ids, call.saved = call.outputs, (), None, None, None
+        # the gradient that is there already among them, so that hooks and recomputation see it
+        if call.grad is None:
+            ctx.save_for_backward(logits, call.ids, call.saved)
+        else:
+            ctx.save_for_backward(logits, call.ids, call.saved, call.grad)
+        outputs, call.outputs = call.outputs, ()
+        call.logits = call.ids = call.saved = call.grad = None
         ctx.call = call
         return outputs
 
