@@ -10,6 +10,7 @@ A log-probability -log(1 + e^odds) changes by 1 - p times that, and has a few ul
 are sums of such values times at most log V.  A gradient is rounded to its dtype once: half a step."""
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -1094,3 +1095,33 @@ def test_memory_between_the_passes(device):
         y = leaf(x)
         more, loss = held(lambda: op(y))
         assert more + held(loss.backward)[0] < size * 1.25, name
+
+
+# --------------------------------------------------------------------------- several threads
+
+
+@pytest.mark.parametrize("N,V", SHAPES)
+def test_threads_go_back_through_one_graph(device, N, V):
+    """With no thread of the engine's between them, each with an upstream of its own (powers of two: exact)."""
+    x, ops = calls(device, N, V, "fp32")
+    for name, op in ops.items():
+        y = leaf(x)
+        loss = op(y)
+        want, = torch.autograd.grad(loss, y, retain_graph=True)
+        loss = op(y)
+        got, scales = {}, [1.0, 2.0, 0.5, -1.0]
+
+        def back(n):
+            with torch.autograd.set_multithreading_enabled(False):
+                got[n] = [torch.autograd.grad(loss, y, torch.full_like(loss, scales[n]), retain_graph=True)[0]
+                          for _ in range(5)]
+
+        threads = [threading.Thread(target=back, args=(n,)) for n in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        tiny = torch.finfo(torch.float32).smallest_normal
+        for n, grads in got.items():
+            for grad in grads:
+                assert ((grad - scales[n] * want).abs() <= want.abs() * 2.0 ** -20 + 2 * tiny).all(), (name, n)

@@ -2,13 +2,14 @@
 
 import ctypes
 import subprocess
+import threading
 from pathlib import Path
 
 import pytest
 import torch
 
 from mvsd import _native as nat
-from mvsd.sample import distillation_loss, policy_loss, preference_loss, token_logprobs
+from mvsd.sample import distillation_loss, losses, policy_loss, preference_loss, token_logprobs
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "mvsd.h"
 INVALID, WORKSPACE, RANGE = -1, -3, -5
@@ -145,3 +146,48 @@ def test_cpu_tensors_are_refused(call):
 def test_unknown_reductions_are_refused(call):
     with pytest.raises(ValueError, match="reduction"):
         call()
+
+
+# --------------------------------------------------------------------------- backward passes
+
+
+class Entry:
+    """Stands in for the gradient's C entry: two calls at once, each of which writes its upstream's index
+    where its own arguments point to when both are inside."""
+
+    def __init__(self):
+        self.both = threading.Barrier(2, timeout=20)
+
+    def mvsd_loss_gradient(self, ref, up, *more):
+        a = ref._obj
+        self.both.wait()
+        value = ctypes.c_float.from_address(up).value
+        ctypes.c_float.from_address(a.grad).value = value
+        ctypes.c_float.from_address(a.grad + 4).value = float(a.unit_gradient)
+        self.both.wait()
+        return 0
+
+
+def test_two_backward_passes_at_once(monkeypatch):
+    """Over one kept graph, as threads make them where the engine has none of its own: each writes its own
+    gradient, and only one of them has the one that is there already."""
+    entry = Entry()
+    monkeypatch.setattr(nat, "lib", lambda: entry)
+    monkeypatch.setattr(nat, "stream_of", lambda device: 0)
+    call = losses._Call.__new__(losses._Call)
+    x, ids, saved = torch.zeros(2, 3), torch.zeros(2, dtype=torch.int32), torch.zeros(8)
+    call.args, call.kind, call.layout, call.fresh = args(), POLICY, (x.data_ptr(), x.stride()), [True]
+    unit = torch.zeros(2, 3)
+    for units in ([0.0, 1.0], [0.0, 0.0]):
+        got = {}
+
+        def back(n):
+            got[n] = call.gradient(x, ids, saved, unit, torch.tensor(float(n)), None)
+
+        threads = [threading.Thread(target=back, args=(n,)) for n in (1, 2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert [float(got[n][0, 0]) for n in (1, 2)] == [1.0, 2.0]
+        assert sorted(float(got[n][0, 1]) for n in (1, 2)) == units

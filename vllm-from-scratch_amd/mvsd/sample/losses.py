@@ -132,16 +132,16 @@ class _Call:
         if not 1e-6 <= temperature <= 1e6:
             raise ValueError(f"temperature={temperature}")
         self.kind, self.logits, self.device = kind, logits, logits.device
-        self.keep, self.saved, self.grad, self.fresh = [], None, None, True
+        self.keep, self.saved, self.grad, self.fresh = [], None, None, [True]
         a = self.args = nat.LossArgs()
         a.kind, a.reduction, a.temperature = kind, reduction, temperature
-        self._rows(logits)
+        self.layout = self._rows(a, logits)
 
-    def _rows(self, logits: torch.Tensor) -> None:
-        a, shape, strides, data = self.args, logits.shape, logits.stride(), logits.data_ptr()
+    @staticmethod
+    def _rows(a: nat.LossArgs, logits: torch.Tensor) -> tuple:
+        shape, strides, data = logits.shape, logits.stride(), logits.data_ptr()
         if strides[-1] != 1 and shape[-1] > 1:
             raise ValueError("logits need rows with unit stride")
-        self.layout = data, strides
         a.dtype = _ROW_CODES[logits.dtype]
         a.logits, a.vocab_size, a.stride = data, shape[-1], strides[-2]
         if len(shape) == 3:
@@ -150,6 +150,7 @@ class _Call:
         else:
             a.num_rows = shape[0]
             a.inner_rows, a.outer_stride = max(shape[0], 1), 0
+        return data, strides
 
     def take_ids(self, ids: torch.Tensor) -> None:
         self.ids = ids
@@ -199,12 +200,16 @@ class _Call:
     def gradient(self, logits, ids, saved, unit, upstream, upstream_entropy) -> torch.Tensor:
         """The logits' gradient for the outputs' (a tensor may lie elsewhere than when it was saved);
         ``unit``: that of an upstream of 1, where it is there already, or None."""
-        a = self.args
+        # several threads may go back through a kept graph at once: a pass's own arguments
+        a = nat.LossArgs.from_buffer_copy(self.args)
         if self.layout != (logits.data_ptr(), logits.stride()):
-            self._rows(logits)
+            self._rows(a, logits)
         a.token_ids, a.saved = ids.data_ptr(), saved.data_ptr() or None
         # it goes out once, free to be changed (an alias without its version): a kept graph's next is made anew
-        fresh, self.fresh = self.fresh and unit is not None, False
+        try:
+            fresh = unit is not None and self.fresh.pop()
+        except IndexError:
+            fresh = False
         a.unit_gradient = 1 if fresh else 0
         grad = unit.data if fresh else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if grad.numel() == 0:
