@@ -1125,3 +1125,23 @@ def test_threads_go_back_through_one_graph(device, N, V):
         for n, grads in got.items():
             for grad in grads:
                 assert ((grad - scales[n] * want).abs() <= want.abs() * 2.0 ** -20 + 2 * tiny).all(), (name, n)
+
+
+# --------------------------------------------------------------------------- forward mode
+
+
+@pytest.mark.parametrize("N,V", SHAPES)
+def test_forward_mode_is_refused(device, N, V):
+    """With and without a gradient wanted beside it; logits cut from their tangent are taken."""
+    import torch.autograd.forward_ad as forward_ad
+    x, ops = calls(device, N, V)
+    for name, op in ops.items():
+        want = op(x)
+        with forward_ad.dual_level():
+            for y in (x.detach().clone(), leaf(x.clone())):
+                dual = forward_ad.make_dual(y, torch.ones_like(x))
+                with pytest.raises(NotImplementedError):
+                    op(dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    op(dual)
+                assert torch.equal(op(dual.detach()), want), name

@@ -191,3 +191,24 @@ def test_two_backward_passes_at_once(monkeypatch):
             t.join()
         assert [float(got[n][0, 0]) for n in (1, 2)] == [1.0, 2.0]
         assert sorted(float(got[n][0, 1]) for n in (1, 2)) == units
+
+
+def test_forward_mode_is_refused():
+    """A tangent of the logits is not dropped, whether or not they want a gradient as well."""
+    import torch.autograd.forward_ad as forward_ad
+
+    class Stub:
+        def __init__(self, logits):
+            self.logits, self.outputs = logits, (logits.detach(),)
+
+        def run(self, train):
+            pass
+
+    assert losses._finish(Stub(X))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(X.clone(), torch.ones_like(X))
+        with pytest.raises(NotImplementedError):
+            losses._finish(Stub(dual))
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            losses._finish(Stub(dual))
+        assert losses._finish(Stub(dual.detach()))

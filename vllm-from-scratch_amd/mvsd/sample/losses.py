@@ -16,8 +16,8 @@ samplers, the verification and beam search give.  The reference has none of them
 one.  Values of a row have the leading shape, fp32; what has fewer dimensions or ones is expanded.  Token
 ids are int32 or int64.  A row whose id is negative (distillation: that has no entry) or whose weight is
 0 is left out: its logits are not read, its values and its gradient are 0.  An id of V or more, or a row
-with a NaN, a +inf or nothing but -inf in it, gives NaN.  The logits get gradients, once differentiable,
-in their own dtype; every other argument is a constant.  Values and losses are fp32.
+with a NaN, a +inf or nothing but -inf in it, gives NaN.  The logits get gradients, once differentiable
+and not in forward mode, in their own dtype; every other argument is a constant.  Values and losses are fp32.
 
 Reductions: "mean" is sum(w * l) / sum(w) over the rows that are not left out (0 if there are none),
 "sum" is sum(w * l), so weights carry any other normalisation and loss scales, "none" the w * l.
@@ -39,6 +39,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 
@@ -271,6 +272,8 @@ _refusing_backward = torch.autograd.function.once_differentiable(_backward)
 
 def _finish(call: _Call):
     """The call's outputs, part of the graph where the logits want a gradient."""
+    if forward_ad.unpack_dual(call.logits).tangent is not None:
+        raise NotImplementedError("the losses have no forward-mode derivatives: detach the logits")
     if call.logits.requires_grad and torch.is_grad_enabled():
         return _RowLoss.apply(call.logits, call)
     call.run(False)
