@@ -844,7 +844,8 @@ int mvsd_row_loss(const mvsd_loss_args* args, mvsd_stream_t stream);
 /* loss_gradient — the gradient of the logits from the saved of mvsd_row_loss (same args), */
 /* grad [N, V] contiguous in the logits' dtype, every row written.  upstream[n * up_stride]  */
 /* is the gradient of loss (LOGPROBS: of logprobs; PREFERENCE: index the pair;               */
-/* up_stride 0: one value), upstream_entropy that of LOGPROBS' entropy; NULL: 0.              */
+/* up_stride 0: one value; without pairs it may be NULL), upstream_entropy that of LOGPROBS'   */
+/* entropy; of LOGPROBS either may be NULL (0).                                               */
 /* unit_gradient (with one upstream; only where mvsd_loss_one_pass gives 1, MVSD_E_INVALID    */
 /* otherwise): mvsd_row_loss has written grad, which stays as it is if the upstream is 1.      */
 /* ------------------------------------------------------------------------------------ */

@@ -1145,3 +1145,22 @@ def test_forward_mode_is_refused(device, N, V):
                 with torch.no_grad(), pytest.raises(NotImplementedError):
                     op(dual)
                 assert torch.equal(op(dual.detach()), want), name
+
+
+# --------------------------------------------------------------------------- rows of no pair
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("N,V", [(5, 700), (1500, 300)])
+def test_rows_without_pairs(device, reduction, N, V):
+    """A packed batch of no sequences with rows behind them."""
+    x = leaf(make(device, (N, V), "bf16", 111))
+    x.data[0] = math.nan
+    tokens = torch.zeros(N, dtype=torch.int32, device=device)
+    cu = torch.zeros(0, dtype=torch.int32, device=device)
+    got = preference_loss(x, tokens, torch.zeros(0, device=device), cu_num_tokens=cu, reduction=reduction,
+                          weights=torch.zeros(0, device=device))
+    assert got.logprobs.shape == (0,) and got.loss.shape == ((0,) if reduction == "none" else ())
+    assert got.loss.sum().item() == 0
+    grad, = torch.autograd.grad(got.loss.sum(), x)
+    assert grad.shape == x.shape and (grad == 0).all()

@@ -1609,7 +1609,8 @@ int mvsd_loss_gradient(const mvsd_loss_args* args, const float* upstream, int64_
   if (a.num_rows == 0) return MVSD_OK;
   if (!a.grad || up_stride < 0 || up_entropy_stride < 0) return MVSD_E_INVALID;
   if (a.unit_gradient && !mvsd::loss_one_pass(a)) return MVSD_E_INVALID;
-  if (!upstream && a.kind != MVSD_LOSS_LOGPROBS) return MVSD_E_INVALID;
+  const bool none = a.kind == MVSD_LOSS_PREFERENCE && a.num_pairs == 0;  // rows of no pair: zeros
+  if (!upstream && a.kind != MVSD_LOSS_LOGPROBS && !none) return MVSD_E_INVALID;
   if (!a.saved || misaligned(a.saved)) return MVSD_E_WORKSPACE;
   return mvsd::record_hip_error(mvsd::launch_loss_gradient(a, upstream, up_stride, upstream_entropy,
                                                            up_entropy_stride, (hipStream_t)stream));
