@@ -779,6 +779,7 @@ int mvsd_beam_finish(const mvsd_beam_finish_args* args, mvsd_stream_t stream);
 /* workspace: mvsd_loss_workspace_bytes() bytes, no initial contents needed, one per call in    */
 /* flight.  Both are 16-byte aligned; a size below 0: arguments that no call takes.  At most   */
 /* 2^23 / (vocab_size / 2^18 + 1) rows and 2^23 pairs (MVSD_E_RANGE).                          */
+/* The kind's numbers are finite (MVSD_E_INVALID).                                            */
 /* ------------------------------------------------------------------------------------ */
 enum { MVSD_LOSS_LOGPROBS = 0, MVSD_LOSS_DISTILL = 1, MVSD_LOSS_POLICY = 2, MVSD_LOSS_PREFERENCE = 3 };
 enum { MVSD_REDUCE_SUM = 0, MVSD_REDUCE_MEAN = 1, MVSD_REDUCE_NONE = 2 };

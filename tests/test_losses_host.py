@@ -212,3 +212,18 @@ def test_forward_mode_is_refused():
         with torch.no_grad(), pytest.raises(NotImplementedError):
             losses._finish(Stub(dual))
         assert losses._finish(Stub(dual.detach()))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("kind,name", [
+    (POLICY, "clip_low"), (POLICY, "clip_high"), (POLICY, "kl_coef"), (POLICY, "entropy_coef"),
+    (PREFERENCE, "beta"), (PREFERENCE, "margin"), (PREFERENCE, "label_smoothing")])
+@pytest.mark.parametrize("loss_type", [0, 1, 2])
+def test_numbers_that_are_not_finite(kind, name, value, loss_type):
+    """Refused before anything is launched: the workspace is one that no call takes."""
+    a = args(kind, loss_type=loss_type, workspace=None, saved=None)
+    assert nat.lib().mvsd_row_loss(ctypes.byref(a), None) == WORKSPACE
+    assert nat.lib().mvsd_loss_gradient(ctypes.byref(a), P, 0, None, 0, None) == WORKSPACE
+    setattr(a, name, value)
+    assert nat.lib().mvsd_row_loss(ctypes.byref(a), None) == INVALID
+    assert nat.lib().mvsd_loss_gradient(ctypes.byref(a), P, 0, None, 0, None) == INVALID

@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "losses.h"
 #include "mvsd_device.h"
@@ -1547,8 +1548,14 @@ int check_call(const mvsd_loss_args* a) {
     if (a->divergence != MVSD_KL_FORWARD && !a->tail) return MVSD_E_INVALID;
     if (rows && !a->teacher_logprobs) return MVSD_E_INVALID;
   }
-  if (a->kind == MVSD_LOSS_POLICY && rows && !a->advantages) return MVSD_E_INVALID;
+  if (a->kind == MVSD_LOSS_POLICY) {
+    if (rows && !a->advantages) return MVSD_E_INVALID;
+    for (const double v : {a->clip_low, a->clip_high, a->kl_coef, a->entropy_coef})
+      if (!std::isfinite(v)) return MVSD_E_INVALID;
+  }
   if (a->kind == MVSD_LOSS_PREFERENCE) {
+    for (const double v : {a->beta, a->margin, a->label_smoothing})
+      if (!std::isfinite(v)) return MVSD_E_INVALID;
     if (a->loss_type < MVSD_PREF_SIGMOID || a->loss_type > MVSD_PREF_SQUARED) return MVSD_E_INVALID;
     if (a->num_pairs == 0 && a->reduction == MVSD_REDUCE_NONE && !rows) return MVSD_OK;
     if (!a->cu_num_tokens && a->num_pairs > 0 && a->num_rows % (2 * a->num_pairs)) return MVSD_E_INVALID;
