@@ -1164,3 +1164,76 @@ def test_rows_without_pairs(device, reduction, N, V):
     assert got.loss.sum().item() == 0
     grad, = torch.autograd.grad(got.loss.sum(), x)
     assert grad.shape == x.shape and (grad == 0).all()
+
+
+# --------------------------------------------------------------------------- plans of the kernels
+
+
+@pytest.mark.parametrize("how,tail", DIVERGENCES)
+@pytest.mark.parametrize("V,K,dtype", [(256, 512, "fp32"), (256, 512, "bf16"), (257, 64, "fp16"), (1000, 256, "fp32"),
+                                       (1000, 130, "bf16"), (4099, 65, "fp32"), (32000, 512, "bf16"),
+                                       (32000, 512, "fp32")])
+def test_distillation_entries_of_several_waves(device, V, K, dtype, how, tail):
+    """In one pass: more entries than a wave has lanes, or than threads hold the row; rows left out, by their
+    entries and by their weight; entries of all rows' ends."""
+    N = 90
+    x = make(device, (N, V), dtype, V + K)
+    ids, teacher = teacher_of(x, K, V + K + 1, sampled=True, gaps=0.05)
+    ids[:, -1] = V - 1
+    ids[1::5] = -1
+    w = torch.rand(N, device=device) + 0.1
+    w[2::7] = 0.0
+    check_distill(x, ids, teacher, how, tail, 0.8, weights=w)
+    check_distill(x, ids, teacher, how, tail, weights=w, reduction="sum", up=0.5)
+
+
+@pytest.mark.parametrize("how", ["forward", "js"])
+@pytest.mark.parametrize("V,dtype", [(196608, "bf16"), (196609, "bf16"), (80000, "fp32")])
+def test_distillation_of_long_rows(device, V, dtype, how):
+    """Columns beyond what a workgroup's registers hold, and one more than those whose entries it marks.  A lane
+    adds 192 terms at most, so that a sum is good to 202 * 2^-24 + 5e-6 < 1.8e-5; the bars have 3e-5."""
+    N = 81
+    x = make(device, (N, V), dtype, V)
+    ids, teacher = teacher_of(x[:12], 33, V, sampled=True)
+    ids = torch.cat([ids, ids.new_full((N - 12, 33), -1)]).roll(40, 0)
+    ids[45, 3], ids[45, 4] = V - 1, V - 8
+    teacher = torch.cat([teacher, teacher.new_zeros(N - 12, 33)]).roll(40, 0)
+    check_distill(x, ids, teacher, how)
+
+
+@pytest.mark.parametrize("V,dtype", [(151936, "fp32"), (262144, "bf16"), (262145, "fp16")])
+@pytest.mark.parametrize("ent", [0.0, 0.02])
+def test_policy_of_long_rows(device, V, dtype, ent):
+    """The same of a policy loss, which has no limit there: 256 terms a lane, good to 266 * 2^-24 + 5e-6 < 2.2e-5."""
+    N = 130
+    x, tokens, old, A, ref = policy_inputs(device, (N,), V, dtype, V)
+    keep = torch.arange(N, device=device) % 9 == 0
+    tokens[0], tokens[9], tokens[18] = V - 1, 0, V - 9
+    old[:19:9] = -13.0
+    ref[:19:9] = -12.0
+    check_policy(x, torch.where(keep, tokens, -1), old, A, ref, kl=0.1, ent=ent)
+
+
+@pytest.mark.parametrize("V", [151936, 300000])
+def test_logprobs_of_many_long_rows(device, V):
+    """A workgroup adds a chunk of up to 2^18 columns: 1024 terms a lane, a sum within 1034 * 2^-24 + 5e-6 < 6.7e-5, a
+    log-probability within that and 1e-6, a gradient's term within that and its own exponential's 5e-6."""
+    N, bound = 1030, 7.5e-5
+    x = torch.zeros(N, V, dtype=torch.bfloat16, device=device)
+    live = torch.arange(3, N, 97, device=device)
+    x[live] = make(device, (len(live), V), "bf16", V)
+    tokens = torch.full((N,), -1, dtype=torch.int32, device=device)
+    tokens[live] = torch.randint(0, V, (len(live),), device=device, dtype=torch.int32,
+                                 generator=torch.Generator(device=device).manual_seed(7))
+    x = leaf(x)
+    lp, H = token_logprobs(x, tokens, return_entropy=True)
+    grad, = torch.autograd.grad([lp, H], x, [torch.ones_like(lp), torch.full_like(H, 0.5)])
+    for n in live.tolist():
+        t = int(tokens[n])
+        want, entropy, logp = oracle.token_row(host(x[n]), t)
+        close(host(lp[n]), want, bound * -np.expm1(want) + 2.0 ** -21 * abs(want))
+        close(host(H[n]), entropy, bound * (1 + math.log(V)))
+        slope, bar = oracle.token_gradient(logp, t, 1.0, 0.5)
+        close_gradient(grad[n], slope, bar * 2 * bound)
+    assert (lp[tokens < 0] == 0).all() and (H[tokens < 0] == 0).all()
+    assert int(grad[tokens < 0].count_nonzero()) == 0
