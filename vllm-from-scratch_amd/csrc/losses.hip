@@ -977,15 +977,17 @@ __device__ inline float scalar(float v) { return readlane_f32(v, 0); }
 // Rows by a workgroup, one after the other (by tickets: some are left out), every row in its registers: read
 // once, written once.  A turn of the loop writes the gradient of one row and, vector by vector, loads the next
 // one in its place and adds it to its statistics kDelay vectors later (4, 6, 8, 10 and 12 are within 4 %), so
-// that memory is busy except in the reductions and the row's own loss between two turns.  `active` threads hold NV vectors each, those of one i side by side (a span, a multiple
-// of 32 columns); the columns behind the spans (few, or what the registers do not hold) are read again.
+// that memory is busy except in the reductions and the row's own loss between two turns.  `active` threads hold NV
+// vectors each, those of one i side by side (a span, a multiple of 32 columns); the columns behind the spans (few, or
+// what the registers do not hold: 78208 of 151936 fp32) are read again, a vector at a time.
 // A turn's loads and stores are unconditional, with a first turn that only loads and a last one that only
 // stores (a conditional load makes the compiler wait for all of them at once); rows that are left out are
 // passed by, their gradient written on the way.
 // Bytes read and written a second (a copy: 5.25 TB/s): 2048 policy rows of 151936 bf16 248 us, 4.8 TB/s; 2000 of
 // 32001 fp32 with entropies 117 us, 4.4; distillation, 1024 rows of 151936 bf16 and 33 entries, 149 us, 4.2, 2048
-// of 128 entries 277 us, 4.4; 4096 of 32000 fp16 133 us, 4.0.  What is lost: the gap between two turns, and in a
-// distillation the marks (4 us of 160) and the entries' own values, which follow the row's stores (3; 17 of 298).
+// of 128 entries 277 us, 4.4; 4096 of 32000 fp16 133 us, 4.0; 2048 policy rows of 151936 fp32 624 us, 4.0, or 5.0 with
+// what is read again.  What is lost: the gap between two turns, and in a distillation the marks (4 us of 160) and the
+// entries' own values, which follow the row's stores (3; 17 of 298).
 template <int DT, int NV, bool LIST, bool ENT, bool WANT>
 __global__ __launch_bounds__(kRowThreads, 4) void loss_rows_kernel(LossParams p) {
   using S = typename Elem<DT>::storage;
@@ -1439,7 +1441,8 @@ hipError_t launch_dt(const LossParams& p, hipStream_t stream) {
 template <int DT>
 hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, const float* up_h, int64_t uhs,
                               hipStream_t stream) {
-  // mostly the gradient is there where a value of 1 is expected: few workgroups look for it
+  // Mostly the gradient is there where a value of 1 is expected: few workgroups look for it (4.6 us).  For another
+  // upstream these few form it, at 2.8 TB/s (2048 rows of 151936 bf16: 445 us, distillation of 1024: 233).
   const int64_t chunks = p.a.num_rows * p.nch;
   const dim3 grid((unsigned)(p.a.unit_gradient ? std::min(chunks, (int64_t)num_cus()) : chunks)), block(kLossThreads);
   const bool past = p.a.num_rows * p.V * (DT == MVSD_F32 ? 4 : 2) > kCacheBytes;
@@ -1458,9 +1461,15 @@ hipError_t launch_gradient_dt(const LossParams& p, const float* up, int64_t us, 
 bool loss_one_pass(const mvsd_loss_args& a) {
   if ((a.kind != MVSD_LOSS_DISTILL && a.kind != MVSD_LOSS_POLICY) || a.reduction == MVSD_REDUCE_NONE) return false;
   if (a.vocab_size < 256 || (has_list(a) && a.vocab_size > kMaxMarked)) return false;
-  // Where rows are few, workgroups that share a row are faster (bf16, kernels' us, one pass against split:
-  // policy loss, V = 151936: 96 rows 35.5 / 31.6, 160 rows 37.8 / 39.3; V = 32000: 96 rows 21.7 / 19.2, 256 rows
-  // 25.5 / 25.8; distillation, V = 151936: 96 rows 44.1 / 42.3, 160 rows 47.1 / 54.4; V = 32000: 48 rows 25.7 / 25.7)
+  // Where rows are few, workgroups that share a row are faster.  Forward and backward pass, us, one pass / split:
+  //   policy, bf16, V = 151936: 96 rows 35.1 / 28.5, 128 36.3 / 31.3, 160 38.4 / 36.0, 256 43.1 / 51.5;
+  //     V = 32000: 96 19.0 / 16.7, 128 19.5 / 18.0, 160 20.0 / 20.0, 256 22.7 / 23.1;
+  //   distillation, bf16, V = 151936: 64 39.3 / 35.1, 80 40.6 / 39.8, 96 41.5 / 43.3, 160 44.4 / 57.0;
+  //     V = 32000: 48 22.9 / 24.1, 80 25.0 / 27.4;
+  //   rows of which the registers hold a half, fp32, V = 151936: policy 128 59.4 / 46.8, 512 184 / 180, 2048 656 / 755,
+  //     distillation 128 65.8 / 70.8, 2048 655 / 815;
+  //   values alone, policy, bf16, V = 151936: 128 22.6 / 20.5, 2048 144 / 221.
+  // One border for all of a kind, although a policy's 128 to some 180 rows would be faster split.
   return a.num_rows >= (has_list(a) ? 80 : 128);
 }
 
