@@ -1237,3 +1237,23 @@ def test_logprobs_of_many_long_rows(device, V):
         close_gradient(grad[n], slope, bar * 2 * bound)
     assert (lp[tokens < 0] == 0).all() and (H[tokens < 0] == 0).all()
     assert int(grad[tokens < 0].count_nonzero()) == 0
+
+
+# --------------------------------------------------------------------------- ratios beyond fp32
+
+
+@pytest.mark.parametrize("N", [6, 132])
+def test_policy_ratios_beyond_fp32(device, N):
+    """e^150 times an advantage of 0 is 0, and a positive advantage's ratio is clipped; a NaN stays one."""
+    V = 500
+    x, tokens, old, _, ref = policy_inputs(device, (N,), V, "fp32", 121)
+    old[::2] -= 150.0
+    A = torch.tensor([0.0, 0.0, 1.5, -1.0, 0.0, 0.5], device=device).repeat(N // 6)
+    for ent in (0.0, 0.02):
+        got, grad = check_policy(x, tokens, old, A, ref, kl=0.1, ent=ent)
+        assert torch.isfinite(got.loss) and torch.isfinite(grad).all()
+        check_policy(x, tokens, old, A, reduction="none", ent=ent)
+    x[0, 3] = math.nan
+    got = policy_loss(x, tokens, old, A, reduction="none")
+    assert torch.isnan(got.loss).nonzero().flatten().tolist() == [0]
+    assert torch.isnan(policy_loss(leaf(x), tokens, old, A).loss)

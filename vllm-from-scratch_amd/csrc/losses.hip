@@ -307,8 +307,9 @@ __device__ inline PolicyIn policy_in(const mvsd_loss_args& a, int64_t row) {
 __device__ inline PolicyRow policy_row(const mvsd_loss_args& a, const PolicyIn& in, float lp, float H) {
   PolicyRow o;
   const float A = in.A;
-  const float r = a.old_logprobs ? expf(lp - in.old) : lp == lp ? 1.f : lp;
-  const float free = r * A;
+  const float gap = lp - in.old;
+  const float r = a.old_logprobs ? expf(gap) : lp == lp ? 1.f : lp;
+  const float free = A == 0.f && gap < INFINITY ? 0.f : r * A;  // 0 too where the ratio is beyond fp32
   const float bound = fminf(fmaxf(r, (float)(1.0 - a.clip_low)), (float)(1.0 + a.clip_high)) * A;
   const bool clipped = free > bound;
   o.loss = clipped ? -bound : -free;
